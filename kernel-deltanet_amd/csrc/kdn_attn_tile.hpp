@@ -1,0 +1,239 @@
+// Tiles and fragments of the softmax attention kernels (kdn_attn*.hip), all on the 32x32 output-tile MFMAs of CDNA4:
+//   v_mfma_f32_32x32x16_bf16 : lane l holds A[l%32][8*(l/32)+s], B[8*(l/32)+s][l%32], s = 0..7
+//   v_mfma_f32_32x32x2_f32   : lane l holds A[l%32][l/32],       B[l/32][l%32]
+//   D (both)                 : lane l holds D[rho(l, i)][l%32], rho(l, i) = 8*(i/4) + 4*(l/32) + i%4, i = 0..15
+// A fragment is eight values a lane, a 16-deep operand: one bf16 MFMA, or eight fp32 ones (slot s of every lane feeds the
+// s-th).  A and B take the same (lane, slot) -> depth map, so any order of the depth will do.  The attention kernels use
+// that: the accumulator of a product, its rows rho, is the B operand of the next one register for register (slots 8m ..
+// 8m + 7 are one fragment), if that product's A operand reads depth 16m + 8*(s/4) + 4*(l/32) + s%4 at slot s (col_frag).
+// So the scores never leave their registers.  32x32 tiles take half the LDS bytes per product of 16x16 ones: a wave reads
+// 1 KB of A per 32 cycles of its matrix core, the four waves of a CU 128 bytes a cycle, all that LDS gives; two 16x16
+// tiles would take twice that.
+#pragma once
+#include "kdn_frag.hpp"
+#include "kdn_internal.hpp"
+#include "../../include/kdn_anchor.h"
+
+namespace kdn {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+__device__ __forceinline__ int rho(int half, int i) { return 8 * (i >> 2) + 4 * half + (i & 3); }
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// Rows of D elements in LDS, in 16-byte pieces: piece c of row r lies at c ^ piece_swizzle(r).  Of the accesses:
+//   row_frag: 16 lanes read one piece c of 16 consecutive rows; the swizzle is a permutation of the row's low four bits
+//     (128-byte rows: of bits 1-3, bit 0 being the half of the 256 bytes), so that they take all 64 banks once;
+//   col_frag (bf16): 32 lanes read 8-byte runs of four rows r0 .. r0+3 (r0 a multiple of 4) and 32 columns; the row's low
+//     two bits are on bits 2-3 of the piece, its pieces c .. c+3 on bits 0-1: 64 banks once again.
+template <int PIECES>
+__device__ __host__ __forceinline__ constexpr int piece_swizzle(int r) {
+  return PIECES == 8 ? ((r >> 1) & 1) << 2 | ((r >> 2) & 3) : (r & 3) << 2 | ((r >> 2) & 3);
+}
+
+template <int D_>
+struct AttnBF16 {
+  typedef __bf16 elem;
+  typedef bf16x8 frag;
+  static constexpr int D = D_, ROW = 2 * D, PIECES = ROW / 16;
+  __device__ __forceinline__ static f32x16 mma(const f32x16& acc, const frag& a, const frag& b) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
+  }
+  __device__ __forceinline__ static frag load(const elem* p) { return *reinterpret_cast<const frag*>(p); }
+  // values 8m .. 8m + 7 of an accumulator as a fragment (rounded to bf16: what the matrix cores take; the sums stay fp32)
+  __device__ __forceinline__ static frag from_acc(const f32x16& v, int m) {
+    frag r;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) r[s] = (__bf16)v[8 * m + s];
+    return r;
+  }
+  // lane l slot s = T[row][16 ks + 8 (l/32) + s], row the lane's own
+  __device__ __forceinline__ static frag row_frag(const unsigned char* t, int row, int ks, int half) {
+    return *reinterpret_cast<const frag*>(t + row * ROW + 16 * ((2 * ks + half) ^ piece_swizzle<PIECES>(row)));
+  }
+  // lane l slot s = T[r0 + 8 (s/4) + 4 (l/32) + s%4][32 ct + l%32]: two transposing reads of four rows each.  In a
+  // 16-lane group lane j addresses the 8-byte run of row j/4 and columns 4 (j%4) ..+3 of the group's 16.
+  __device__ __forceinline__ static frag col_frag(const unsigned char* t, int r0, int ct, int lane) {
+    const int j = lane & 15, half = lane >> 5, c = 4 * ct + 2 * ((lane >> 4) & 1) + ((j & 3) >> 1);
+    bf16x4 part[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int row = r0 + 8 * p + 4 * half + (j >> 2);
+      const unsigned char* a = t + row * ROW + 16 * (c ^ piece_swizzle<PIECES>(row)) + 8 * (j & 1);
+      part[p] = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a)));
+    }
+    return __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
+
+template <int D_>
+struct AttnF32 {
+  typedef float elem;
+  typedef f32x8 frag;
+  static constexpr int D = D_, ROW = 4 * D, PIECES = ROW / 16;
+  __device__ __forceinline__ static f32x16 mma(f32x16 acc, const frag& a, const frag& b) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s], b[s], acc, 0, 0, 0);
+    return acc;
+  }
+  __device__ __forceinline__ static frag load(const elem* p) {
+    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+    return pair_to8(a, b);
+  }
+  __device__ __forceinline__ static frag from_acc(const f32x16& v, int m) {
+    frag r;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) r[s] = v[8 * m + s];
+    return r;
+  }
+  __device__ __forceinline__ static frag row_frag(const unsigned char* t, int row, int ks, int half) {
+    const int c = 4 * ks + 2 * half, f = piece_swizzle<PIECES>(row);
+    return pair_to8(*reinterpret_cast<const f32x4*>(t + row * ROW + 16 * (c ^ f)),
+                    *reinterpret_cast<const f32x4*>(t + row * ROW + 16 * ((c + 1) ^ f)));
+  }
+  __device__ __forceinline__ static frag col_frag(const unsigned char* t, int r0, int ct, int lane) {
+    const int half = lane >> 5, col = 32 * ct + (lane & 31);
+    frag r;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const int row = r0 + 8 * (s >> 2) + 4 * half + (s & 3);
+      r[s] = *reinterpret_cast<const float*>(t + row * ROW + 16 * ((col >> 2) ^ piece_swizzle<PIECES>(row)) + 4 * (col & 3));
+    }
+    return r;
+  }
+};
+
+// The copy of `ROWS` rows of D elements, row r at base + min(r, last) * stride, into an LDS tile by the load unit itself
+// (16 bytes a lane, 1 KB an instruction, nothing in registers): the WAVES waves of a workgroup share it.  The rows past
+// `last` repeat it, so that every address is inside the tensor and every value one that is there.
+template <class P, int ROWS, int WAVES>
+__device__ __forceinline__ void stage_rows(const typename P::elem* base, int64_t stride, int last, unsigned char* tile,
+                                           int wave, int lane) {
+  constexpr int N = ROWS * P::PIECES / 64;
+#pragma unroll
+  for (int i = 0; i < N / WAVES; ++i) {
+    const int at = (i * WAVES + wave) * 64 + lane, row = at / P::PIECES;
+    const int piece = (at % P::PIECES) ^ piece_swizzle<P::PIECES>(row);
+    const typename P::elem* src = base + (int64_t)min(row, last) * stride + piece * (16 / (int)sizeof(typename P::elem));
+    __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(src),
+                                     (__attribute__((address_space(3))) void*)(tile + (i * WAVES + wave) * 1024), 16, 0, 0);
+  }
+}
+
+// This wave's staged copies have arrived; after the barrier, every wave's have, and every wave has read the tile that the
+// next copies overwrite.
+__device__ __forceinline__ void staged_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// The values of lanes l % 32 and l % 32 + 32, in both.  (The elements are copied out before they are cast: a bit cast of an
+// element of the builtin's result takes element 0 whichever it names.)
+__device__ __forceinline__ void halves(float v, float& lower, float& upper) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+  const unsigned a = r[0], b = r[1];
+  lower = __builtin_bit_cast(float, a);
+  upper = __builtin_bit_cast(float, b);
+}
+__device__ __forceinline__ float half_max(float v) {
+  float a, b;
+  halves(v, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float half_sum(float v) {
+  float a, b;
+  halves(v, a, b);
+  return a + b;
+}
+
+// One 32-wide tile of a transposed accumulator (lane: row of the tensor; registers: 32 of its columns) times `f`, as the
+// columns 0 .. 31 of a row.  bf16: the halves of the wave exchange their 4-column runs, 16 bytes a store.
+__device__ __forceinline__ void store_row32(__bf16* row, const f32x16& v, float f, int half, bool live) {
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    unsigned a[2], b[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+      bf16x2 lo = {(__bf16)(v[8 * m + 2 * e] * f), (__bf16)(v[8 * m + 2 * e + 1] * f)};
+      bf16x2 hi = {(__bf16)(v[8 * m + 4 + 2 * e] * f), (__bf16)(v[8 * m + 5 + 2 * e] * f)};
+      const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi), false, false);
+      a[e] = r[0];
+      b[e] = r[1];
+    }
+    const u32x4 out = {a[0], a[1], b[0], b[1]};
+    if (live) *reinterpret_cast<u32x4*>(row + 16 * m + 8 * half) = out;
+  }
+}
+__device__ __forceinline__ void store_row32(float* row, const f32x16& v, float f, int half, bool live) {
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const f32x4 out = {v[4 * m] * f, v[4 * m + 1] * f, v[4 * m + 2] * f, v[4 * m + 3] * f};
+    if (live) *reinterpret_cast<f32x4*>(row + 8 * m + 4 * half) = out;
+  }
+}
+
+// Tile slots over a packed batch: sequence b has the slots [cu[b] / ROWS + b, cu[b + 1] / ROWS + b + 1), at least as many
+// as it has tiles of ROWS rows, so that a grid of total / ROWS + sequences slots covers every batch without its lengths
+// being known to the host.  The rows past the last sequence's end (a batch padded to a fixed size) are one sequence more,
+// number nseq, that sees nothing and that nothing sees.  The sequence of a slot is found 64 offsets at a time by the whole
+// wave.  Offsets are clamped to the tensor: a wrong one gives wrong rows, never an access outside.
+struct SeqTile {
+  int seq, row0;    // row0: first row of the tile in the sequence; negative: no tile
+  int64_t lo, len;  // the sequence's first row and length
+};
+__device__ __forceinline__ int64_t seq_start(const int64_t* cu, int64_t total, int64_t b) {
+  return min(max(cu[b], (int64_t)0), total);
+}
+template <int ROWS>
+__device__ __forceinline__ SeqTile find_tile(const int64_t* cu, int64_t nseq, int64_t total, int64_t slot, int lane) {
+  int64_t lo = 0, n = nseq + 1;
+  while (n > 1) {
+    const int64_t step = (n + 63) / 64, at = lo + lane * step;
+    const bool before = lane * step < n && seq_start(cu, total, min(at, nseq)) / ROWS + at <= slot;
+    const int hits = __popcll(__ballot(before));
+    const int64_t skip = (hits > 0 ? hits - 1 : 0) * step;
+    lo += skip;
+    n = min(step, n - skip);
+  }
+  SeqTile t;
+  t.seq = (int)lo;
+  t.lo = seq_start(cu, total, lo);
+  t.len = (lo < nseq ? max(seq_start(cu, total, lo + 1), t.lo) : total) - t.lo;
+  const int64_t tile = slot - (t.lo / ROWS + lo);
+  t.row0 = tile < 0 || tile * ROWS >= t.len ? -1 : (int)(tile * ROWS);
+  return t;
+}
+// The other tensor's rows of a tile's sequence: none for the rows past the last one.
+__device__ __forceinline__ void other_rows(const int64_t* cu, int64_t nseq, int64_t total, int seq, int64_t& lo, int64_t& len) {
+  lo = seq < nseq ? seq_start(cu, total, seq) : 0;
+  len = seq < nseq ? max(seq_start(cu, total, seq + 1), lo) - lo : 0;
+}
+
+// Device-side arguments of the attention kernels (kdn_attn_args with the defaults filled in).
+struct AttnParams {
+  const void *q, *k, *v, *y, *dy;
+  void *out, *dq, *dk, *dv;
+  int64_t qs[2], ks[2], vs[2], ys[2], dys[2], dqs[2], dks[2], dvs[2];  // element strides [token][head]
+  float* lse;          // [H][total_q]
+  const float* delta;  // [H][total_q]: dy . y of each row (backward)
+  const int64_t *cu_q, *cu_k;
+  int64_t nseq, total_q, total_k;
+  int H, KV, G;
+  float scale;
+};
+
+int attn_check(const kdn_attn_args* a);          // sizes
+int attn_check_tensors(const kdn_attn_args* a);  // pointers, strides, alignment
+bool attn_strides_ok(const int64_t s[2], int dtype);
+AttnParams attn_params(const kdn_attn_args* a);
+
+}  // namespace kdn

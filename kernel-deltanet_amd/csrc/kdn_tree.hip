@@ -1,0 +1,468 @@
+// Attention of each sequence's new tokens over its pages and over themselves: one token of a decode step, a run of them, or
+// a tree of drafts.  Token t of a sequence sees the whole context, itself, its parent and what that sees.
+//
+// The keys and values are what has to be read, each once: a sequence's context is cut into chunks, a workgroup per chunk
+// and key head, and the rows of all query heads that share the key head (G heads of every new token) go through the matrix
+// cores together, 32 to a tile.  A chunk leaves its rows' maximum, sum and unnormalised sum of values; a second launch joins
+// them in the chunks' order.  Sequences of one chunk are written at once.
+//   - up to 32 rows: the waves of a workgroup share the rows and take every fourth tile of 32 keys each, through two LDS
+//     slots of their own with no barrier; they meet once at the end;
+//   - more: each wave has 32 rows of its own, and all read the same tiles of 64 keys, as in the prompt's kernel.
+#include <algorithm>
+#include <cmath>
+#include "kdn_attn_tile.hpp"
+
+namespace kdn {
+
+struct TreeParams {
+  const void *q, *k, *v, *kp, *vp;
+  void* y;
+  int64_t qs[2], ks[2], vs[2], ys[2], kps[3], vps[3];  // [token][head]; pages [page][head][token]
+  const int64_t* cu;
+  const int32_t *lens, *table, *parents;
+  float *po, *pml;  // partial sums [sequence][key head][chunk][row][D] and maxima / sums [..][2]
+  int64_t table_stride, num_pages, total, max_context;
+  int H, KV, G, max_new, max_chunks, chunk, shift, nseq;
+  float scale;
+};
+
+// What a workgroup works on.
+struct TreeWork {
+  int64_t lo;          // first new token
+  int n, c0, c1;       // new tokens; the chunk's keys
+  int chunks, ctx;     // chunks of the sequence; its context
+};
+
+__device__ __forceinline__ TreeWork tree_work(const TreeParams& p, int b, int ch) {
+  TreeWork t;
+  t.lo = min(max(p.cu[b], (int64_t)0), p.total);
+  t.n = (int)min(min(max(p.cu[b + 1], t.lo), p.total) - t.lo, (int64_t)p.max_new);
+  t.ctx = (int)min((int64_t)max(p.lens[b], 0), p.max_context);
+  t.chunks = max(1, (t.ctx + p.chunk - 1) / p.chunk);
+  t.c0 = ch * p.chunk;
+  t.c1 = min(t.c0 + p.chunk, t.ctx);
+  return t;
+}
+
+// Bit u of a token's mask: it sees new token u.  Lane t of a wave has token t's; doubling along the parents, six steps for
+// up to 64 tokens.  A parent that is not an earlier token of the sequence hangs the token on the context alone.
+__device__ __forceinline__ uint64_t ancestors(const TreeParams& p, const TreeWork& t, int lane) {
+  if (!p.parents) return lane >= 63 ? ~0ull : (2ull << lane) - 1;
+  int up = lane < t.n ? p.parents[t.lo + lane] : -1;
+  if (up < 0 || up >= lane) up = -1;
+  uint64_t sees = 1ull << lane;
+#pragma unroll
+  for (int step = 0; step < 6; ++step) {
+    const int from = up < 0 ? lane : up;
+    const uint32_t lo = __shfl((uint32_t)sees, from), hi = __shfl((uint32_t)(sees >> 32), from);
+    const int next = __shfl(up, from);
+    sees |= (uint64_t)hi << 32 | lo;
+    up = up < 0 ? -1 : next;
+  }
+  return sees;
+}
+
+// ROWS keys from key k0 on into an LDS tile, by the instructions first, first + step, ... of it: from the pages (each
+// instruction's rows lie on one page, pages having at least 16), or from the new tokens' own tensor.  Rows past `last`
+// repeat it; a page number outside the pool reads its nearest page.
+template <class P, int ROWS, bool PAGED>
+__device__ __forceinline__ void stage_keys(const TreeParams& p, const void* base, const int64_t* stride, int b, int e,
+                                           int64_t lo, int k0, int last, unsigned char* tile, int first, int step, int lane) {
+  typedef typename P::elem E;
+  constexpr int N = ROWS * P::PIECES / 64, RPI = 64 / P::PIECES;
+  static_assert(RPI <= 16, "an instruction's rows lie on one page");
+  const int r = lane / P::PIECES;
+  typedef const __attribute__((address_space(4))) int32_t* Table;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (step > 1 && i >= N / step) break;
+    const int n = first + i * step, row = n * RPI + r;
+    const int piece = (lane % P::PIECES) ^ piece_swizzle<P::PIECES>(row);
+    const int key = min(k0 + row, last);
+    const E* src;
+    if constexpr (PAGED) {
+      const int at = __builtin_amdgcn_readfirstlane(min(k0 + n * RPI, last) >> p.shift);
+      const int64_t page = min(max(((Table)(p.table + (int64_t)b * p.table_stride))[at], 0), (int)p.num_pages - 1);
+      src = reinterpret_cast<const E*>(base) + page * stride[0] + (int64_t)e * stride[1] +
+            (int64_t)(key & ((1 << p.shift) - 1)) * stride[2];
+    } else {
+      src = reinterpret_cast<const E*>(base) + (lo + key) * stride[0] + (int64_t)e * stride[1];
+    }
+    __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(src + piece * (16 / (int)sizeof(E))),
+                                     (__attribute__((address_space(3))) void*)(tile + n * 1024), 16, 0, 0);
+  }
+}
+
+// The running softmax of one 32-row tile over 32 more keys: scores -> weights in `s`, the sums rescaled where the maximum
+// moved (by more than 2^6, as in the prompt's kernel).
+template <int CT>
+__device__ __forceinline__ void softmax_step(f32x16& s, float& m, float& l, f32x16 (&o)[CT], float c) {
+  float top = s[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+  top = half_max(top);
+  if (__any((top - m) * c > 6.f || (m == -INFINITY && top > m))) {
+    const float next = fmaxf(m, top);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - next) * c);
+    m = next;
+    l *= f;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[ct][i] *= f;
+  }
+  const float mc = m == -INFINITY ? 0.f : m * c;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -mc));
+    l += s[i];
+  }
+}
+
+template <class P>
+struct TreeFew {
+  static constexpr int STAGE = 2 * 32 * P::ROW;  // 32 keys and their values
+  static constexpr int WAVES = STAGE > 16384 ? 2 : 4;
+  static constexpr int LDS = WAVES * 2 * STAGE;
+  static_assert(STAGE == 8192 || STAGE == 16384 || STAGE == 32768, "the waits below count the copies of one stage");
+};
+
+template <class P>
+__global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreeParams p) {
+  typedef typename P::elem E;
+  constexpr int D = P::D, KS = D / 16, CT = D / 32, W = TreeFew<P>::WAVES, STAGE = TreeFew<P>::STAGE;
+  __shared__ __attribute__((aligned(256))) unsigned char lds[TreeFew<P>::LDS];
+  __shared__ float wm[W][32], wl[W][32];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ch = blockIdx.x % p.max_chunks, be = blockIdx.x / p.max_chunks, b = be / p.KV, e = be % p.KV;
+  const TreeWork t = tree_work(p, b, ch);
+  if (t.n <= 0 || ch >= t.chunks) return;
+  const int rows = t.n * p.G, row = min(lane & 31, rows - 1), tok = row / p.G, h = e * p.G + row % p.G;
+  const bool drafts = ch == t.chunks - 1;  // the last chunk has the new tokens too
+  const int nt = t.c1 > t.c0 ? (t.c1 - t.c0 + 31) / 32 : 0, total = nt + (drafts ? (t.n + 31) / 32 : 0);
+  uint64_t sees = 0;
+  if (drafts) {
+    const uint64_t all = ancestors(p, t, lane);
+    sees = (uint64_t)__shfl((uint32_t)(all >> 32), tok) << 32 | __shfl((uint32_t)all, tok);
+  }
+  typename P::frag q[KS];
+  {
+    const E* src = reinterpret_cast<const E*>(p.q) + (t.lo + tok) * p.qs[0] + (int64_t)h * p.qs[1];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) q[ks] = P::load(src + 16 * ks + 8 * half);
+  }
+  unsigned char* mine = lds + w * 2 * STAGE;
+  auto stage = [&](int at, int buf) {
+    unsigned char* to = mine + buf * STAGE;
+    if (at < nt) {
+      stage_keys<P, 32, true>(p, p.kp, p.kps, b, e, 0, t.c0 + 32 * at, t.c1 - 1, to, 0, 1, lane);
+      stage_keys<P, 32, true>(p, p.vp, p.vps, b, e, 0, t.c0 + 32 * at, t.c1 - 1, to + STAGE / 2, 0, 1, lane);
+    } else {
+      stage_keys<P, 32, false>(p, p.k, p.ks, b, e, t.lo, 32 * (at - nt), t.n - 1, to, 0, 1, lane);
+      stage_keys<P, 32, false>(p, p.v, p.vs, b, e, t.lo, 32 * (at - nt), t.n - 1, to + STAGE / 2, 0, 1, lane);
+    }
+  };
+  f32x16 o[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) o[ct] = zero16();
+  float m = -INFINITY, l = 0.f;
+  const float c = p.scale * LOG2E;
+  int buf = 0;
+  if (w < total) stage(w, 0);
+  for (int at = w; at < total; at += W, buf ^= 1) {
+    if (at + W < total) {
+      stage(at + W, buf ^ 1);
+      // everything but the last STAGE / 1024 copies, the next tile's, has arrived
+      if constexpr (STAGE == 8192) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      else if constexpr (STAGE == 16384) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(32)" ::: "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    const unsigned char *kt = mine + buf * STAGE, *vt = kt + STAGE / 2;
+    f32x16 s = zero16();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = P::mma(s, P::row_frag(kt, lane & 31, ks, half), q[ks]);
+    if (at >= nt) {
+      const uint32_t bits = (uint32_t)(sees >> (32 * (at - nt)));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = bits >> rho(half, i) & 1 ? s[i] : -INFINITY;
+    } else if (t.c0 + 32 * at + 32 > t.c1) {
+      const int limit = t.c1 - t.c0 - 32 * at;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = rho(half, i) < limit ? s[i] : -INFINITY;
+    }
+    softmax_step(s, m, l, o, c);
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      const typename P::frag pf = P::from_acc(s, kk);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, 16 * kk, ct, lane), pf);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its slot may be written again
+  }
+  // the waves' sums, each scaled to the common maximum, added in the waves' order
+  l = half_sum(l);
+  if (half == 0) wm[w][lane] = m, wl[w][lane] = l;
+  __syncthreads();
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int x = 0; x < W; ++x) top = fmaxf(top, wm[x][lane & 31]);
+  const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * c);
+  constexpr int PITCH = D + 4;
+  float* ob = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const f32x4 x = {o[ct][4 * a] * f, o[ct][4 * a + 1] * f, o[ct][4 * a + 2] * f, o[ct][4 * a + 3] * f};
+      *reinterpret_cast<f32x4*>(ob + (w * 32 + (lane & 31)) * PITCH + 32 * ct + 8 * a + 4 * half) = x;
+    }
+#pragma unroll
+  for (int x = 0; x < W; ++x)
+    sum += wm[x][lane & 31] == -INFINITY ? 0.f : wl[x][lane & 31] * __builtin_amdgcn_exp2f((wm[x][lane & 31] - top) * c);
+  __syncthreads();
+  if (w == 0 && half == 0) wl[0][lane] = sum, wm[0][lane] = top;
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (D / 4); i += 64 * W) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    f32x4 x = *reinterpret_cast<const f32x4*>(ob + r * PITCH + d);
+#pragma unroll
+    for (int y = 1; y < W; ++y) x += *reinterpret_cast<const f32x4*>(ob + (y * 32 + r) * PITCH + d);
+    if (t.chunks == 1) {
+      const float g = wl[0][r] == 0.f ? 0.f : 1.f / wl[0][r];
+      float out[4] = {x[0] * g, x[1] * g, x[2] * g, x[3] * g};
+      E* dst = reinterpret_cast<E*>(p.y) + (t.lo + r / p.G) * p.ys[0] + (int64_t)(e * p.G + r % p.G) * p.ys[1] + d;
+      if constexpr (sizeof(E) == 2) {
+        const bf16x4 v = {(__bf16)out[0], (__bf16)out[1], (__bf16)out[2], (__bf16)out[3]};
+        *reinterpret_cast<bf16x4*>(dst) = v;
+      } else {
+        *reinterpret_cast<f32x4*>(dst) = f32x4{out[0], out[1], out[2], out[3]};
+      }
+    } else {
+      const int64_t at = ((int64_t)be * p.max_chunks + ch) * p.max_new * p.G + r;
+      *reinterpret_cast<f32x4*>(p.po + at * D + d) = x;
+      if (d == 0) p.pml[2 * at] = wm[0][r] * c, p.pml[2 * at + 1] = wl[0][r];
+    }
+  }
+}
+
+// More than 32 rows: 128 rows a workgroup.
+template <class P>
+__global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tree_many_kernel(TreeParams p, int blocks) {
+  typedef typename P::elem E;
+  constexpr int D = P::D, KS = D / 16, CT = D / 32, TILE = 64 * P::ROW;
+  __shared__ __attribute__((aligned(256))) unsigned char lds[4 * TILE];
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // the row blocks of one chunk on one XCD, one after another: its L2 has the keys from the second on
+  const int unit = blockIdx.x / 8 / blocks * 8 + blockIdx.x % 8, rb = blockIdx.x / 8 % blocks;
+  const int ch = unit % p.max_chunks, be = unit / p.max_chunks, b = be / p.KV, e = be % p.KV;
+  if (b >= p.nseq) return;
+  const TreeWork t = tree_work(p, b, ch);
+  const int rows = t.n * p.G;
+  if (t.n <= 0 || ch >= t.chunks || 128 * rb >= rows) return;
+  const int mine = 128 * rb + 32 * w + (lane & 31);
+  const bool live = mine < rows, busy = 128 * rb + 32 * w < rows;
+  const int row = min(mine, rows - 1), tok = row / p.G, h = e * p.G + row % p.G;
+  const bool drafts = ch == t.chunks - 1;
+  const int nt = t.c1 > t.c0 ? (t.c1 - t.c0 + 63) / 64 : 0, total = nt + (drafts ? 1 : 0);
+  uint64_t sees = 0;
+  if (drafts) {
+    const uint64_t all = ancestors(p, t, lane);
+    sees = (uint64_t)__shfl((uint32_t)(all >> 32), tok) << 32 | __shfl((uint32_t)all, tok);
+  }
+  typename P::frag q[KS];
+  {
+    const E* src = reinterpret_cast<const E*>(p.q) + (t.lo + tok) * p.qs[0] + (int64_t)h * p.qs[1];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) q[ks] = P::load(src + 16 * ks + 8 * half);
+  }
+  auto stage = [&](int at, int buf) {
+    unsigned char *kt = lds + buf * TILE, *vt = lds + (2 + buf) * TILE;
+    if (at < nt) {
+      stage_keys<P, 64, true>(p, p.kp, p.kps, b, e, 0, t.c0 + 64 * at, t.c1 - 1, kt, w, 4, lane);
+      stage_keys<P, 64, true>(p, p.vp, p.vps, b, e, 0, t.c0 + 64 * at, t.c1 - 1, vt, w, 4, lane);
+    } else {
+      stage_keys<P, 64, false>(p, p.k, p.ks, b, e, t.lo, 0, t.n - 1, kt, w, 4, lane);
+      stage_keys<P, 64, false>(p, p.v, p.vs, b, e, t.lo, 0, t.n - 1, vt, w, 4, lane);
+    }
+  };
+  f32x16 o[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) o[ct] = zero16();
+  float m = -INFINITY, l = 0.f;
+  const float c = p.scale * LOG2E;
+  if (total > 0) stage(0, 0);
+  for (int at = 0; at < total; ++at) {
+    staged_barrier();
+    if (at + 1 < total) stage(at + 1, (at + 1) & 1);
+    if (!busy) continue;
+    const unsigned char *kt = lds + (at & 1) * TILE, *vt = lds + (2 + (at & 1)) * TILE;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      f32x16 s = zero16();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s = P::mma(s, P::row_frag(kt, 32 * u + (lane & 31), ks, half), q[ks]);
+      if (at >= nt) {
+        const uint32_t bits = (uint32_t)(sees >> (32 * u));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = bits >> rho(half, i) & 1 ? s[i] : -INFINITY;
+      } else if (t.c0 + 64 * at + 32 * u + 32 > t.c1) {
+        const int limit = t.c1 - t.c0 - 64 * at - 32 * u;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = rho(half, i) < limit ? s[i] : -INFINITY;
+      }
+      softmax_step(s, m, l, o, c);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const typename P::frag pf = P::from_acc(s, kk);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, 32 * u + 16 * kk, ct, lane), pf);
+      }
+    }
+  }
+  l = half_sum(l);
+  if (t.chunks == 1) {
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    E* dst = reinterpret_cast<E*>(p.y) + (t.lo + tok) * p.ys[0] + (int64_t)h * p.ys[1];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) store_row32(dst + 32 * ct, o[ct], f, half, live);
+  } else {
+    const int64_t at = ((int64_t)be * p.max_chunks + ch) * p.max_new * p.G + row;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) store_row32(p.po + at * D + 32 * ct, o[ct], 1.f, half, live);
+    if (live && half == 0) p.pml[2 * at] = m * c, p.pml[2 * at + 1] = l;
+  }
+}
+
+// The chunks of one row joined in their order: a wave a row, D / 64 values a lane.
+template <class E, int D>
+__global__ void __launch_bounds__(256) tree_join_kernel(TreeParams p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int most = p.max_new * p.G, r = (int)(id % most);
+  const int64_t be = id / most;
+  if (be >= (int64_t)p.nseq * p.KV) return;
+  const int b = (int)(be / p.KV), e = (int)(be % p.KV);
+  const TreeWork t = tree_work(p, b, 0);
+  if (r >= t.n * p.G || t.chunks == 1) return;
+  const int64_t first = be * p.max_chunks * most + r;
+  float top = -INFINITY;
+  for (int x = lane; x < t.chunks; x += 64) top = fmaxf(top, p.pml[2 * (first + (int64_t)x * most)]);
+#pragma unroll
+  for (int s = 1; s < 64; s *= 2) top = fmaxf(top, __shfl_xor(top, s));
+  constexpr int V = D / 64;
+  float sum = 0.f, o[V] = {};
+#pragma unroll 4
+  for (int x = 0; x < t.chunks; ++x) {
+    const int64_t at = first + (int64_t)x * most;
+    const float m = p.pml[2 * at], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    sum += p.pml[2 * at + 1] * f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = __builtin_fmaf(p.po[at * D + V * lane + i], f, o[i]);
+  }
+  const float g = sum == 0.f ? 0.f : 1.f / sum;
+  E* dst = reinterpret_cast<E*>(p.y) + (t.lo + r / p.G) * p.ys[0] + (int64_t)(e * p.G + r % p.G) * p.ys[1] + V * lane;
+#pragma unroll
+  for (int i = 0; i < V; ++i) dst[i] = (E)(o[i] * g);
+}
+
+// Keys of a chunk: 256 to 1024, the fewest with which the grid stays within 2048 workgroups (a chunk's own cost, its
+// queries and its partial sums, is that of a few dozen keys; short chunks even out unequal contexts).
+static int tree_chunk(const kdn_tree_attn_args* a) {
+  const int64_t rows = a->max_new * (a->H / a->H_kv), blocks = rows <= 32 ? 1 : (rows + 127) / 128;
+  int chunk = 256;
+  while (chunk < 1024 && a->num_seqs * a->H_kv * blocks * ((a->max_context + chunk - 1) / chunk) > 2048) chunk *= 2;
+  return chunk;
+}
+static int64_t tree_chunks(const kdn_tree_attn_args* a) {
+  const int chunk = tree_chunk(a);
+  return a->max_context > 0 ? (a->max_context + chunk - 1) / chunk : 1;
+}
+
+static int tree_check(const kdn_tree_attn_args* a) {
+  if (!a || a->num_seqs < 0 || a->total_new < 0 || a->H <= 0 || a->H_kv <= 0 || a->H > (1 << 20) || a->H % a->H_kv != 0 ||
+      !valid_dtype(a->dtype) || !(a->scale > 0.f) || !std::isfinite(a->scale) || a->max_context < 0 || a->max_new <= 0 ||
+      a->page_tokens <= 0 || a->num_pages < 0 || a->table_width < 0)
+    return KDN_ERR_INVALID_ARGUMENT;
+  if ((a->d != 64 && a->d != 128) || a->max_new > 64 || a->page_tokens < 16 || (a->page_tokens & (a->page_tokens - 1)) != 0 ||
+      a->total_new > INT32_MAX || a->num_seqs > INT32_MAX || a->num_pages > INT32_MAX || a->max_context > (1 << 30))
+    return KDN_ERR_UNSUPPORTED;
+  if (a->max_context > 0 && (a->num_pages == 0 || a->max_context > a->table_width * a->page_tokens)) return KDN_ERR_INVALID_ARGUMENT;
+  return KDN_OK;
+}
+
+template <class P>
+static int launch_tree(const TreeParams& p, hipStream_t st) {
+  const int rows = p.max_new * p.G;
+  const int64_t units = (int64_t)p.nseq * p.KV * p.max_chunks;
+  if (rows <= 32) {
+    hipLaunchKernelGGL(tree_few_kernel<P>, dim3((unsigned)units), dim3(64 * TreeFew<P>::WAVES), 0, st, p);
+  } else {
+    const int blocks = (rows + 127) / 128;
+    hipLaunchKernelGGL(tree_many_kernel<P>, dim3((unsigned)((units + 7) / 8 * 8 * blocks)), dim3(256), 0, st, p, blocks);
+  }
+  if (p.max_chunks > 1) {
+    const int64_t joins = (int64_t)p.nseq * p.KV * rows;
+    hipLaunchKernelGGL((tree_join_kernel<typename P::elem, P::D>), dim3((unsigned)((joins + 3) / 4)), dim3(256), 0, st, p);
+  }
+  return launch_status();
+}
+
+}  // namespace kdn
+
+using namespace kdn;
+
+// Bytes of the partial sums of `units` chunks.
+static size_t tree_partial_bytes(const kdn_tree_attn_args* a, int64_t units) {
+  return (size_t)units * (size_t)(a->max_new * (a->H / a->H_kv)) * (size_t)(a->d + 2) * 4 + 16;
+}
+
+// Not the call's own number of chunks but a bound that grows with every size, so that a workspace for the largest call
+// holds for the others: the rule for a chunk's length gives a smaller call shorter chunks, and at times more of them.
+extern "C" size_t kdn_tree_attn_workspace_bytes(const kdn_tree_attn_args* a) {
+  if (tree_check(a) != KDN_OK) return 0;
+  const int64_t heads = a->num_seqs * a->H_kv, fine = heads * ((a->max_context + 255) / 256), coarse = heads * ((a->max_context + 1023) / 1024);
+  return a->max_context <= 256 ? 16 : tree_partial_bytes(a, std::min(fine, std::max<int64_t>(2048, coarse)));
+}
+
+extern "C" int kdn_tree_attn(const kdn_tree_attn_args* a, void* stream) {
+  int rc = tree_check(a);
+  if (rc != KDN_OK) return rc;
+  if (a->num_seqs == 0 || a->total_new == 0) return KDN_OK;
+  if (!a->cu_new || !a->context_lens || !a->q || !a->k || !a->v || !a->y ||
+      (a->max_context > 0 && (!a->page_table || !a->k_pages || !a->v_pages)))
+    return KDN_ERR_INVALID_ARGUMENT;
+  const int64_t per = 16 / (int64_t)dtype_size(a->dtype);
+  bool fits = aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) && aligned(a->y, 16) && aligned(a->k_pages, 16) &&
+              aligned(a->v_pages, 16) && aligned(a->workspace, 16) && attn_strides_ok(a->q_stride, a->dtype) &&
+              attn_strides_ok(a->k_stride, a->dtype) && attn_strides_ok(a->v_stride, a->dtype) && attn_strides_ok(a->y_stride, a->dtype);
+  for (int i = 0; i < 3; ++i)
+    fits = fits && a->k_pages_stride[i] >= 0 && a->v_pages_stride[i] >= 0 && a->k_pages_stride[i] % per == 0 && a->v_pages_stride[i] % per == 0;
+  if (!fits) return KDN_ERR_MISALIGNED;
+  const int64_t chunks = tree_chunks(a), rows = a->max_new * (a->H / a->H_kv), blocks = rows <= 32 ? 1 : (rows + 127) / 128;
+  if (a->num_seqs * a->H_kv * chunks * blocks > INT32_MAX - 8 * blocks || a->num_seqs * a->H_kv * rows > INT32_MAX)
+    return KDN_ERR_UNSUPPORTED;
+  if (chunks > 1 && (!a->workspace || a->workspace_bytes < tree_partial_bytes(a, a->num_seqs * a->H_kv * chunks))) return KDN_ERR_WORKSPACE_TOO_SMALL;
+  TreeParams p = {};
+  p.q = a->q; p.k = a->k; p.v = a->v; p.kp = a->k_pages; p.vp = a->v_pages; p.y = a->y;
+  for (int i = 0; i < 2; ++i) {
+    p.qs[i] = a->q_stride[i]; p.ks[i] = a->k_stride[i]; p.vs[i] = a->v_stride[i]; p.ys[i] = a->y_stride[i];
+  }
+  for (int i = 0; i < 3; ++i) {
+    p.kps[i] = a->k_pages_stride[i]; p.vps[i] = a->v_pages_stride[i];
+  }
+  p.cu = a->cu_new; p.lens = a->context_lens; p.table = a->page_table; p.parents = a->parents;
+  p.table_stride = a->table_stride; p.num_pages = a->num_pages; p.total = a->total_new; p.max_context = a->max_context;
+  p.H = (int)a->H; p.KV = (int)a->H_kv; p.G = (int)(a->H / a->H_kv);
+  p.max_new = (int)a->max_new; p.max_chunks = (int)chunks; p.chunk = tree_chunk(a); p.nseq = (int)a->num_seqs;
+  p.shift = __builtin_ctz((unsigned)a->page_tokens);
+  p.scale = a->scale;
+  p.po = reinterpret_cast<float*>(a->workspace);
+  p.pml = p.po + (size_t)a->num_seqs * a->H * chunks * a->max_new * a->d;
+  hipStream_t st = as_stream(stream);
+  if (a->dtype == KDN_DTYPE_BF16) return a->d == 64 ? launch_tree<AttnBF16<64>>(p, st) : launch_tree<AttnBF16<128>>(p, st);
+  return a->d == 64 ? launch_tree<AttnF32<64>>(p, st) : launch_tree<AttnF32<128>>(p, st);
+}

@@ -60,6 +60,32 @@ EXPORTED = (
     "kdn_fwht_lift_factored_bwd",
 )
 
+# Exported symbols of include/kdn_anchor.h (checked by tests/test_anchor_abi.py).
+ANCHOR_EXPORTED = (
+    "kdn_anchor_version",
+    "kdn_attn_fwd",
+    "kdn_attn_bwd_workspace_bytes",
+    "kdn_attn_bwd",
+    "kdn_rotary",
+    "kdn_page_copy",
+    "kdn_page_append",
+    "kdn_page_pool_create",
+    "kdn_page_pool_destroy",
+    "kdn_page_pool_open",
+    "kdn_page_pool_fork",
+    "kdn_page_pool_close",
+    "kdn_page_pool_extend",
+    "kdn_page_pool_truncate",
+    "kdn_page_pool_length",
+    "kdn_page_pool_table",
+    "kdn_page_pool_rows",
+    "kdn_page_pool_compact",
+    "kdn_page_pool_used",
+    "kdn_page_pool_free",
+    "kdn_tree_attn_workspace_bytes",
+    "kdn_tree_attn",
+)
+
 KDN_ERR_CAPACITY = -6
 KDN_ERR_WORKSPACE_TOO_SMALL = -3
 NOALLOC_SCRATCH_BYTES = 256 << 20   # KDN_NOALLOC_SCRATCH_BYTES of include/kdn.h
@@ -172,6 +198,113 @@ class ScanBwdArgs(ctypes.Structure):
     ]
 
 
+class AttnArgs(ctypes.Structure):
+    """Mirror of struct kdn_attn_args (include/kdn_anchor.h)."""
+
+    _fields_ = [
+        ("num_seqs", _i64), ("total_q", _i64), ("total_k", _i64), ("H", _i64), ("H_kv", _i64),
+        ("d", ctypes.c_int), ("dtype", ctypes.c_int), ("scale", ctypes.c_float),
+        ("cu_q", ctypes.c_void_p), ("cu_k", ctypes.c_void_p),
+        ("q", ctypes.c_void_p), ("q_stride", _i64x2),
+        ("k", ctypes.c_void_p), ("k_stride", _i64x2),
+        ("v", ctypes.c_void_p), ("v_stride", _i64x2),
+        ("y", ctypes.c_void_p), ("y_stride", _i64x2),
+        ("lse", ctypes.c_void_p),
+    ]
+
+
+class AttnBwdArgs(ctypes.Structure):
+    """Mirror of struct kdn_attn_bwd_args (include/kdn_anchor.h)."""
+
+    _fields_ = [
+        ("fwd", ctypes.c_void_p),
+        ("dy", ctypes.c_void_p), ("dy_stride", _i64x2),
+        ("dq", ctypes.c_void_p), ("dq_stride", _i64x2),
+        ("dk", ctypes.c_void_p), ("dk_stride", _i64x2),
+        ("dv", ctypes.c_void_p), ("dv_stride", _i64x2),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    """Mirror of struct kdn_rotary_args (include/kdn_anchor.h)."""
+
+    _fields_ = [
+        ("tokens", _i64), ("H", _i64), ("H_kv", _i64),
+        ("d", ctypes.c_int), ("rotary_dim", ctypes.c_int), ("dtype", ctypes.c_int), ("interleaved", ctypes.c_int),
+        ("inverse", ctypes.c_int), ("magnitude", ctypes.c_float),
+        ("positions", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
+        ("q", ctypes.c_void_p), ("q_stride", _i64x2),
+        ("k", ctypes.c_void_p), ("k_stride", _i64x2),
+        ("q_out", ctypes.c_void_p), ("q_out_stride", _i64x2),
+        ("k_out", ctypes.c_void_p), ("k_out_stride", _i64x2),
+    ]
+
+
+class PageAppendArgs(ctypes.Structure):
+    """Mirror of struct kdn_page_append_args (include/kdn_anchor.h)."""
+
+    _fields_ = [
+        ("tokens", _i64), ("H_kv", _i64),
+        ("d", ctypes.c_int), ("dtype", ctypes.c_int),
+        ("page_tokens", _i64), ("num_pages", _i64),
+        ("rows", ctypes.c_void_p),
+        ("k", ctypes.c_void_p), ("k_stride", _i64x2),
+        ("v", ctypes.c_void_p), ("v_stride", _i64x2),
+        ("k_pages", ctypes.c_void_p), ("k_pages_stride", _i64x3),
+        ("v_pages", ctypes.c_void_p), ("v_pages_stride", _i64x3),
+    ]
+
+
+class TreeAttnArgs(ctypes.Structure):
+    """Mirror of struct kdn_tree_attn_args (include/kdn_anchor.h)."""
+
+    _fields_ = [
+        ("num_seqs", _i64), ("total_new", _i64), ("max_new", _i64), ("max_context", _i64), ("H", _i64), ("H_kv", _i64),
+        ("d", ctypes.c_int), ("dtype", ctypes.c_int), ("scale", ctypes.c_float),
+        ("page_tokens", _i64), ("num_pages", _i64), ("table_width", _i64), ("table_stride", _i64),
+        ("cu_new", ctypes.c_void_p), ("context_lens", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+        ("parents", ctypes.c_void_p),
+        ("q", ctypes.c_void_p), ("q_stride", _i64x2),
+        ("k", ctypes.c_void_p), ("k_stride", _i64x2),
+        ("v", ctypes.c_void_p), ("v_stride", _i64x2),
+        ("k_pages", ctypes.c_void_p), ("k_pages_stride", _i64x3),
+        ("v_pages", ctypes.c_void_p), ("v_pages_stride", _i64x3),
+        ("y", ctypes.c_void_p), ("y_stride", _i64x2),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+def _declare_anchor(L: ctypes.CDLL) -> None:
+    """Argument and result types of include/kdn_anchor.h."""
+    vp, i64, ci, sz, ptr = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.POINTER
+    for name, args, res in (
+            ("kdn_anchor_version", [], ci),
+            ("kdn_attn_fwd", [ptr(AttnArgs), vp], ci),
+            ("kdn_attn_bwd_workspace_bytes", [ptr(AttnBwdArgs)], sz),
+            ("kdn_attn_bwd", [ptr(AttnBwdArgs), vp], ci),
+            ("kdn_rotary", [ptr(RotaryArgs), vp], ci),
+            ("kdn_page_copy", [vp, i64, i64, vp, i64, vp], ci),
+            ("kdn_page_append", [ptr(PageAppendArgs), vp], ci),
+            ("kdn_page_pool_create", [i64, i64, i64, ptr(vp)], ci),
+            ("kdn_page_pool_destroy", [vp], None),
+            ("kdn_page_pool_open", [vp], ci),
+            ("kdn_page_pool_fork", [vp, ci], ci),
+            ("kdn_page_pool_close", [vp, ci], ci),
+            ("kdn_page_pool_extend", [vp, ci, i64, vp], ci),
+            ("kdn_page_pool_truncate", [vp, ci, i64], ci),
+            ("kdn_page_pool_length", [vp, ci], i64),
+            ("kdn_page_pool_table", [vp, ci, vp, i64], i64),
+            ("kdn_page_pool_rows", [vp, ci, i64, i64, vp], ci),
+            ("kdn_page_pool_compact", [vp, vp, i64], i64),
+            ("kdn_page_pool_used", [vp], i64),
+            ("kdn_page_pool_free", [vp], i64),
+            ("kdn_tree_attn_workspace_bytes", [ptr(TreeAttnArgs)], sz),
+            ("kdn_tree_attn", [ptr(TreeAttnArgs), vp], ci)):
+        fn = getattr(L, name)
+        fn.argtypes, fn.restype = args, res
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -263,6 +396,7 @@ def lib() -> ctypes.CDLL:
             L.kdn_scan_bwd_phase.restype = ci
             L.kdn_scan_bwd_segments.argtypes = [ctypes.POINTER(ScanBwdArgs), ctypes.POINTER(ctypes.c_int64)]
             L.kdn_scan_bwd_segments.restype = i64
+            _declare_anchor(L)
             _lib = L
     return _lib
 

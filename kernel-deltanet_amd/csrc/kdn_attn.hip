@@ -12,7 +12,7 @@
 
 namespace kdn {
 
-constexpr int FWD_ROWS = 128, FWD_KEYS = 64;
+constexpr int FWD_ROWS = 128, FWD_KEYS = 64, FWD_BLOCKS = FWD_KEYS / 32;
 
 template <class P>
 __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) attn_fwd_kernel(AttnParams p, int64_t slots) {
@@ -57,38 +57,38 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   const int64_t sees = min(lenk, t.row0 + FWD_ROWS + off);  // keys that any row of the workgroup sees
   const int ntiles = sees > 0 ? (int)((sees + FWD_KEYS - 1) / FWD_KEYS) : 0;
   const int64_t wfirst = t.row0 + 32 * w + off, wlast = wfirst + 31;  // last key the wave's first / last row sees
-  if (ntiles > 0) {
-    stage_rows<P, FWD_KEYS, 4>(kb, p.ks[0], (int)min(lenk - 1, (int64_t)FWD_KEYS - 1), lds, w, lane);
-    stage_rows<P, FWD_KEYS, 4>(vb, p.vs[0], (int)min(lenk - 1, (int64_t)FWD_KEYS - 1), lds + 2 * TILE, w, lane);
-  }
-  for (int j = 0; j < ntiles; ++j) {
-    staged_barrier();
+  auto stage = [&](int j, unsigned char* to) {
     const int64_t k0 = (int64_t)j * FWD_KEYS;
-    if (j + 1 < ntiles) {
-      const int64_t k1 = k0 + FWD_KEYS;
-      const int last = (int)min(lenk - 1 - k1, (int64_t)FWD_KEYS - 1);
-      stage_rows<P, FWD_KEYS, 4>(kb + k1 * p.ks[0], p.ks[0], last, lds + ((j + 1) & 1) * TILE, w, lane);
-      stage_rows<P, FWD_KEYS, 4>(vb + k1 * p.vs[0], p.vs[0], last, lds + (2 + ((j + 1) & 1)) * TILE, w, lane);
-    }
-    if (k0 > wlast) continue;  // nothing of this tile is visible to the wave
-    const unsigned char *kt = lds + (j & 1) * TILE, *vt = lds + (2 + (j & 1)) * TILE;
-    f32x16 s[2] = {zero16(), zero16()};
+    const int last = (int)min(lenk - 1 - k0, (int64_t)FWD_KEYS - 1);
+    stage_rows<P, FWD_KEYS, 4>(kb + k0 * p.ks[0], p.ks[0], last, to, w, lane);
+    stage_rows<P, FWD_KEYS, 4>(vb + k0 * p.vs[0], p.vs[0], last, to + TILE, w, lane);
+  };
+  // One tile, read from `kt`, while the next one's copies go to `next`.  That the two do not overlap is said to the compiler
+  // (__restrict): it would wait for the copies before it reads V otherwise.
+  auto step = [&](int j, const unsigned char* __restrict kt, unsigned char* __restrict next) {
+    if (j + 1 < ntiles) stage(j + 1, next);
+    const int64_t k0 = (int64_t)j * FWD_KEYS;
+    if (k0 > wlast) return;  // nothing of this tile is visible to the wave
+    const unsigned char* vt = kt + TILE;
+    f32x16 s[FWD_BLOCKS];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < FWD_BLOCKS; ++b) {
+      s[b] = zero16();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) s[b] = P::mma(s[b], P::row_frag(kt, 32 * b + (lane & 31), ks, half), q[ks]);
+    }
     if (k0 + FWD_KEYS - 1 > wfirst) {
       const int limit = (int)min(max((int64_t)row + off - k0, (int64_t)-1), (int64_t)FWD_KEYS);
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < FWD_BLOCKS; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[b][i] = 32 * b + rho(half, i) <= limit ? s[b][i] : -INFINITY;
     }
     float top = s[0][0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[0][i]);
+    for (int b = 0; b < FWD_BLOCKS; ++b)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[1][i]);
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
     top = half_max(top);
     // the maximum moves only where it grows by more than 2^6 (the sums stay far inside fp32): most tiles rescale nothing
     if (__any((top - m) * c > 6.f || (m == -INFINITY && top > m))) {
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
     const float mc = m == -INFINITY ? 0.f : m * c;
     float sum = 0.f;
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < FWD_BLOCKS; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, -mc));
@@ -112,11 +112,16 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
       }
     l += sum;
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
+    for (int kk = 0; kk < 2 * FWD_BLOCKS; ++kk) {
       const typename P::frag pf = P::from_acc(s[kk >> 1], kk & 1);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, 16 * kk, ct, lane), pf);
     }
+  };
+  if (ntiles > 0) stage(0, lds);
+  for (int j = 0; j < ntiles; ++j) {
+    staged_barrier();
+    step(j, lds + (j & 1) * 2 * TILE, lds + (~j & 1) * 2 * TILE);
   }
   l = half_sum(l);
   const float f = l == 0.f ? 0.f : 1.f / l;

@@ -45,9 +45,9 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 && P::D == 
     attn_dkdv_kernel(AttnParams p, int64_t slots) {
   typedef typename P::elem E;
   constexpr int D = P::D, KS = D / 16, CT = D / 32, TILE = BWD_TILE * P::ROW;
-  constexpr int NBUF = 4 * TILE + 4 * 256 <= 160 * 1024 ? 2 : 1;
-  __shared__ __attribute__((aligned(256))) unsigned char lds[2 * NBUF * TILE];
-  __shared__ __attribute__((aligned(256))) float stat[2 * NBUF][BWD_TILE];
+  constexpr int SLOT = 2 * TILE + 2 * BWD_TILE * 4;  // Q and dY rows, their lse and delta
+  constexpr int NBUF = 2 * SLOT <= 160 * 1024 ? 2 : 1;
+  __shared__ __attribute__((aligned(256))) unsigned char lds[NBUF * SLOT];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t id = blockIdx.x;
@@ -80,34 +80,25 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 && P::D == 
   const int64_t q0 = max(t.row0 - off, (int64_t)0) / BWD_TILE * BWD_TILE;
   const int per = q0 < lenq ? (int)((lenq - q0 + BWD_TILE - 1) / BWD_TILE) : 0;
   const int ntiles = per * p.G;
-  auto stage = [&](int j, int b) {
+  auto stage = [&](int j, unsigned char* to) {
     const int h = e * p.G + j / per;
     const int64_t r0 = q0 + (int64_t)(j % per) * BWD_TILE;
     const int last = (int)min(lenq - 1 - r0, (int64_t)BWD_TILE - 1);
     const E* qb = reinterpret_cast<const E*>(p.q) + (qlo + r0) * p.qs[0] + (int64_t)h * p.qs[1];
     const E* yb = reinterpret_cast<const E*>(p.dy) + (qlo + r0) * p.dys[0] + (int64_t)h * p.dys[1];
-    stage_rows<P, BWD_TILE, 4>(qb, p.qs[0], last, lds + 2 * b * TILE, w, lane);
-    stage_rows<P, BWD_TILE, 4>(yb, p.dys[0], last, lds + (2 * b + 1) * TILE, w, lane);
+    stage_rows<P, BWD_TILE, 4>(qb, p.qs[0], last, to, w, lane);
+    stage_rows<P, BWD_TILE, 4>(yb, p.dys[0], last, to + TILE, w, lane);
     if (w < 2) {
       const float* src = (w == 0 ? p.lse : p.delta) + (int64_t)h * p.total_q + qlo + r0 + min(lane, last);
       __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(src),
-                                       (__attribute__((address_space(3))) void*)(&stat[2 * b + w][0]), 4, 0, 0);
+                                       (__attribute__((address_space(3))) void*)(to + 2 * TILE + w * BWD_TILE * 4), 4, 0, 0);
     }
   };
-  if (NBUF == 2 && ntiles > 0) stage(0, 0);
-  for (int j = 0; j < ntiles; ++j) {
-    int b = 0;
-    if (NBUF == 2) {
-      b = j & 1;
-      staged_barrier();
-      if (j + 1 < ntiles) stage(j + 1, b ^ 1);
-    } else {
-      staged_barrier();
-      stage(j, 0);
-      staged_barrier();
-    }
+  // as in the forward: the next tile's copies and this one's reads do not overlap
+  auto step = [&](int j, const unsigned char* __restrict qt, unsigned char* __restrict next) {
+    if (NBUF == 2 && j + 1 < ntiles) stage(j + 1, next);
     const int64_t r0 = q0 + (int64_t)(j % per) * BWD_TILE;
-    const unsigned char *qt = lds + 2 * b * TILE, *yt = lds + (2 * b + 1) * TILE;
+    const unsigned char *yt = qt + TILE, *stat = qt + 2 * TILE;
 #pragma unroll(sizeof(E) == 2 ? 2 : 1)
     for (int u = 0; u < BWD_TILE / 32; ++u) {
       const int64_t i0 = r0 + 32 * u;  // rows i0 .. i0 + 31
@@ -122,8 +113,8 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 && P::D == 
       const int lo = (int)min(first, (int64_t)32), hi = (int)min(lenq - i0, (int64_t)32);
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(&stat[2 * b][32 * u + 8 * a + 4 * half]);
-        const f32x4 de = *reinterpret_cast<const f32x4*>(&stat[2 * b + 1][32 * u + 8 * a + 4 * half]);
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(stat + 4 * (32 * u + 8 * a + 4 * half));
+        const f32x4 de = *reinterpret_cast<const f32x4*>(stat + 4 * (BWD_TILE + 32 * u + 8 * a + 4 * half));
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int i = 4 * a + x, r = rho(half, i);
@@ -148,6 +139,16 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 && P::D == 
         }
       }
     }
+  };
+  if (NBUF == 2 && ntiles > 0) stage(0, lds);
+  for (int j = 0; j < ntiles; ++j) {
+    if (NBUF == 1) {
+      staged_barrier();
+      stage(j, lds);
+    }
+    staged_barrier();
+    if constexpr (NBUF == 2) step(j, lds + (j & 1) * SLOT, lds + (~j & 1) * SLOT);
+    else step(j, lds, lds);
   }
   E* dkr = reinterpret_cast<E*>(p.dk) + (t.lo + key) * p.dks[0] + (int64_t)e * p.dks[1];
   E* dvr = reinterpret_cast<E*>(p.dv) + (t.lo + key) * p.dvs[0] + (int64_t)e * p.dvs[1];
@@ -205,21 +206,16 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   const int64_t sees = min(lenk, t.row0 + BWD_ROWS + off);
   const int ntiles = sees > 0 ? (int)((sees + BWD_TILE - 1) / BWD_TILE) : 0;
   const int64_t wfirst = t.row0 + 32 * w + off, wlast = wfirst + 31;
-  if (ntiles > 0) {
-    const int last = (int)min(lenk - 1, (int64_t)BWD_TILE - 1);
-    stage_rows<P, BWD_TILE, 4>(kb, p.ks[0], last, lds, w, lane);
-    stage_rows<P, BWD_TILE, 4>(vb, p.vs[0], last, lds + 2 * TILE, w, lane);
-  }
-  for (int j = 0; j < ntiles; ++j) {
-    staged_barrier();
+  auto stage = [&](int j, unsigned char* to) {
     const int64_t k0 = (int64_t)j * BWD_TILE;
-    if (j + 1 < ntiles) {
-      const int64_t k1 = k0 + BWD_TILE;
-      const int last = (int)min(lenk - 1 - k1, (int64_t)BWD_TILE - 1);
-      stage_rows<P, BWD_TILE, 4>(kb + k1 * p.ks[0], p.ks[0], last, lds + ((j + 1) & 1) * TILE, w, lane);
-      stage_rows<P, BWD_TILE, 4>(vb + k1 * p.vs[0], p.vs[0], last, lds + (2 + ((j + 1) & 1)) * TILE, w, lane);
-    }
-    const unsigned char *kt = lds + (j & 1) * TILE, *vt = lds + (2 + (j & 1)) * TILE;
+    const int last = (int)min(lenk - 1 - k0, (int64_t)BWD_TILE - 1);
+    stage_rows<P, BWD_TILE, 4>(kb + k0 * p.ks[0], p.ks[0], last, to, w, lane);
+    stage_rows<P, BWD_TILE, 4>(vb + k0 * p.vs[0], p.vs[0], last, to + TILE, w, lane);
+  };
+  auto step = [&](int j, const unsigned char* __restrict kt, unsigned char* __restrict next) {
+    if (j + 1 < ntiles) stage(j + 1, next);
+    const int64_t k0 = (int64_t)j * BWD_TILE;
+    const unsigned char* vt = kt + TILE;
 #pragma unroll
     for (int u = 0; u < BWD_TILE / 32; ++u) {
       const int64_t j0 = k0 + 32 * u;
@@ -244,6 +240,11 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
         for (int ct = 0; ct < CT; ++ct) dq[ct] = P::mma(dq[ct], P::col_frag(kt, 32 * u + 16 * m, ct, lane), df);
       }
     }
+  };
+  if (ntiles > 0) stage(0, lds);
+  for (int j = 0; j < ntiles; ++j) {
+    staged_barrier();
+    step(j, lds + (j & 1) * 2 * TILE, lds + (~j & 1) * 2 * TILE);
   }
   E* dst = reinterpret_cast<E*>(p.dq) + (t.lo + row) * p.dqs[0] + (int64_t)h * p.dqs[1];
 #pragma unroll

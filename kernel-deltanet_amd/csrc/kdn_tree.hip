@@ -62,35 +62,51 @@ __device__ __forceinline__ uint64_t ancestors(const TreeParams& p, const TreeWor
   return sees;
 }
 
-// ROWS keys from key k0 on into an LDS tile, by the instructions first, first + step, ... of it: from the pages (each
-// instruction's rows lie on one page, pages having at least 16), or from the new tokens' own tensor.  Rows past `last`
-// repeat it; a page number outside the pool reads its nearest page.
-template <class P, int ROWS, bool PAGED>
-__device__ __forceinline__ void stage_keys(const TreeParams& p, const void* base, const int64_t* stride, int b, int e,
-                                           int64_t lo, int k0, int last, unsigned char* tile, int first, int step, int lane) {
-  typedef typename P::elem E;
-  constexpr int N = ROWS * P::PIECES / 64, RPI = 64 / P::PIECES;
-  static_assert(RPI <= 16, "an instruction's rows lie on one page");
-  const int r = lane / P::PIECES;
-  typedef const __attribute__((address_space(4))) int32_t* Table;
+// Sixteen keys (or values) into rows 16 g .. of an LDS tile: row r from base + min(r, last) * row_bytes, the base the same
+// in all lanes, so that a copy takes one 32-bit offset a lane.
+template <class P>
+__device__ __forceinline__ void stage_group(const unsigned char* base, uint32_t row_bytes, int last, unsigned char* tile, int g, int lane) {
+  constexpr int N = 16 * P::PIECES / 64, RPI = 64 / P::PIECES;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    if (step > 1 && i >= N / step) break;
-    const int n = first + i * step, row = n * RPI + r;
-    const int piece = (lane % P::PIECES) ^ piece_swizzle<P::PIECES>(row);
-    const int key = min(k0 + row, last);
-    const E* src;
-    if constexpr (PAGED) {
-      const int at = __builtin_amdgcn_readfirstlane(min(k0 + n * RPI, last) >> p.shift);
-      const int64_t page = min(max(((Table)(p.table + (int64_t)b * p.table_stride))[at], 0), (int)p.num_pages - 1);
-      src = reinterpret_cast<const E*>(base) + page * stride[0] + (int64_t)e * stride[1] +
-            (int64_t)(key & ((1 << p.shift) - 1)) * stride[2];
-    } else {
-      src = reinterpret_cast<const E*>(base) + (lo + key) * stride[0] + (int64_t)e * stride[1];
-    }
-    __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(src + piece * (16 / (int)sizeof(E))),
-                                     (__attribute__((address_space(3))) void*)(tile + n * 1024), 16, 0, 0);
+    const int row = i * RPI + lane / P::PIECES, piece = (lane % P::PIECES) ^ piece_swizzle<P::PIECES>(row);
+    const uint32_t off = (uint32_t)min(row, last) * row_bytes + 16 * piece;
+    __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(base + off),
+                                     (__attribute__((address_space(3))) void*)(tile + (g * N + i) * 1024), 16, 0, 0);
   }
+}
+
+// Which sixteen keys a group has: its own, or where none of them is there, the last ones that are; `last` the last of them.
+struct Group {
+  int key, last;
+};
+__device__ __forceinline__ Group key_group(int key, int last_key) {
+  Group g;
+  g.key = key <= last_key ? key : last_key & ~15;
+  g.last = min(last_key - g.key, 15);
+  return g;
+}
+// The page of a key; a number outside the pool is its nearest page's.
+__device__ __forceinline__ int page_of(const TreeParams& p, int b, int key) {
+  typedef const __attribute__((address_space(4))) int32_t* Table;  // nothing writes it meanwhile: scalar loads
+  return min(max(((Table)(p.table + (int64_t)b * p.table_stride))[__builtin_amdgcn_readfirstlane(key >> p.shift)], 0), (int)p.num_pages - 1);
+}
+template <class P>
+__device__ __forceinline__ void stage_paged(const TreeParams& p, int page, int e, Group g, unsigned char* kt, unsigned char* vt, int at, int lane) {
+  constexpr int64_t S = sizeof(typename P::elem);
+  const int off = g.key & ((1 << p.shift) - 1);
+  stage_group<P>(reinterpret_cast<const unsigned char*>(p.kp) + S * (page * p.kps[0] + e * p.kps[1] + off * p.kps[2]),
+                 (uint32_t)(S * p.kps[2]), g.last, kt, at, lane);
+  stage_group<P>(reinterpret_cast<const unsigned char*>(p.vp) + S * (page * p.vps[0] + e * p.vps[1] + off * p.vps[2]),
+                 (uint32_t)(S * p.vps[2]), g.last, vt, at, lane);
+}
+template <class P>
+__device__ __forceinline__ void stage_new(const TreeParams& p, int64_t lo, int e, Group g, unsigned char* kt, unsigned char* vt, int at, int lane) {
+  constexpr int64_t S = sizeof(typename P::elem);
+  stage_group<P>(reinterpret_cast<const unsigned char*>(p.k) + S * ((lo + g.key) * p.ks[0] + e * p.ks[1]), (uint32_t)(S * p.ks[0]), g.last,
+                 kt, at, lane);
+  stage_group<P>(reinterpret_cast<const unsigned char*>(p.v) + S * ((lo + g.key) * p.vs[0] + e * p.vs[1]), (uint32_t)(S * p.vs[0]), g.last,
+                 vt, at, lane);
 }
 
 // The running softmax of one 32-row tile over 32 more keys: scores -> weights in `s`, the sums rescaled where the maximum
@@ -121,26 +137,50 @@ __device__ __forceinline__ void softmax_step(f32x16& s, float& m, float& l, f32x
 
 template <class P>
 struct TreeFew {
-  static constexpr int STAGE = 2 * 32 * P::ROW;  // 32 keys and their values
-  static constexpr int WAVES = STAGE > 16384 ? 2 : 4;
+  static constexpr int STAGE = 2 * 32 * P::ROW;          // 32 keys and their values
+  static constexpr int WAVES = 65536 / (2 * STAGE);      // two workgroups a CU: one starts or ends while the other reads
   static constexpr int LDS = WAVES * 2 * STAGE;
+  static constexpr int PITCH = P::D + 4;
   static_assert(STAGE == 8192 || STAGE == 16384 || STAGE == 32768, "the waits below count the copies of one stage");
+  static_assert(WAVES * 32 * PITCH * 4 <= LDS, "the waves' sums meet in the stages' place");
 };
 
 template <class P>
 __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreeParams p) {
   typedef typename P::elem E;
   constexpr int D = P::D, KS = D / 16, CT = D / 32, W = TreeFew<P>::WAVES, STAGE = TreeFew<P>::STAGE;
-  __shared__ __attribute__((aligned(256))) unsigned char lds[TreeFew<P>::LDS];
-  __shared__ float wm[W][32], wl[W][32];
+  __shared__ __attribute__((aligned(256))) unsigned char lds[TreeFew<P>::LDS + 2 * W * 32 * 4];
+  float(*wm)[32] = reinterpret_cast<float(*)[32]>(lds + TreeFew<P>::LDS), (*wl)[32] = wm + W;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int ch = blockIdx.x % p.max_chunks, be = blockIdx.x / p.max_chunks, b = be / p.KV, e = be % p.KV;
+  // chunk by chunk of all sequences: workgroups go round the XCDs in order, and were a sequence's chunks next to one another,
+  // the first chunks, which every sequence has, would fall on a few of them
+  const int heads = p.nseq * p.KV, ch = blockIdx.x / heads, be = blockIdx.x % heads, b = be / p.KV, e = be % p.KV;
   const TreeWork t = tree_work(p, b, ch);
   if (t.n <= 0 || ch >= t.chunks) return;
   const int rows = t.n * p.G, row = min(lane & 31, rows - 1), tok = row / p.G, h = e * p.G + row % p.G;
   const bool drafts = ch == t.chunks - 1;  // the last chunk has the new tokens too
   const int nt = t.c1 > t.c0 ? (t.c1 - t.c0 + 31) / 32 : 0, total = nt + (drafts ? (t.n + 31) / 32 : 0);
+  unsigned char* mine = lds + w * 2 * STAGE;
+  // the pages of a tile's two groups, known a tile ahead of its copies
+  int page0 = 0, page1 = 0;
+  auto pages = [&](int at) {
+    if (at >= nt) return;
+    page0 = page_of(p, b, key_group(t.c0 + 32 * at, t.c1 - 1).key);
+    page1 = page_of(p, b, key_group(t.c0 + 32 * at + 16, t.c1 - 1).key);
+  };
+  auto stage = [&](int at, unsigned char* to) {
+    if (at < nt) {
+      stage_paged<P>(p, page0, e, key_group(t.c0 + 32 * at, t.c1 - 1), to, to + STAGE / 2, 0, lane);
+      stage_paged<P>(p, page1, e, key_group(t.c0 + 32 * at + 16, t.c1 - 1), to, to + STAGE / 2, 1, lane);
+    } else {
+      stage_new<P>(p, t.lo, e, key_group(32 * (at - nt), t.n - 1), to, to + STAGE / 2, 0, lane);
+      stage_new<P>(p, t.lo, e, key_group(32 * (at - nt) + 16, t.n - 1), to, to + STAGE / 2, 1, lane);
+    }
+  };
+  pages(w);
+  if (w < total) stage(w, mine);
+  pages(w + W);
   uint64_t sees = 0;
   if (drafts) {
     const uint64_t all = ancestors(p, t, lane);
@@ -152,27 +192,16 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) q[ks] = P::load(src + 16 * ks + 8 * half);
   }
-  unsigned char* mine = lds + w * 2 * STAGE;
-  auto stage = [&](int at, int buf) {
-    unsigned char* to = mine + buf * STAGE;
-    if (at < nt) {
-      stage_keys<P, 32, true>(p, p.kp, p.kps, b, e, 0, t.c0 + 32 * at, t.c1 - 1, to, 0, 1, lane);
-      stage_keys<P, 32, true>(p, p.vp, p.vps, b, e, 0, t.c0 + 32 * at, t.c1 - 1, to + STAGE / 2, 0, 1, lane);
-    } else {
-      stage_keys<P, 32, false>(p, p.k, p.ks, b, e, t.lo, 32 * (at - nt), t.n - 1, to, 0, 1, lane);
-      stage_keys<P, 32, false>(p, p.v, p.vs, b, e, t.lo, 32 * (at - nt), t.n - 1, to + STAGE / 2, 0, 1, lane);
-    }
-  };
   f32x16 o[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) o[ct] = zero16();
   float m = -INFINITY, l = 0.f;
   const float c = p.scale * LOG2E;
-  int buf = 0;
-  if (w < total) stage(w, 0);
-  for (int at = w; at < total; at += W, buf ^= 1) {
+  // one tile, read from `kt` while the next one's copies go to `next` (as in the prompt's kernel)
+  auto step = [&](int at, const unsigned char* __restrict kt, unsigned char* __restrict next) {
     if (at + W < total) {
-      stage(at + W, buf ^ 1);
+      stage(at + W, next);
+      pages(at + 2 * W);
       // everything but the last STAGE / 1024 copies, the next tile's, has arrived
       if constexpr (STAGE == 8192) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
       else if constexpr (STAGE == 16384) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
@@ -180,7 +209,7 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    const unsigned char *kt = mine + buf * STAGE, *vt = kt + STAGE / 2;
+    const unsigned char* vt = kt + STAGE / 2;
     f32x16 s = zero16();
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) s = P::mma(s, P::row_frag(kt, lane & 31, ks, half), q[ks]);
@@ -201,7 +230,8 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
       for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, 16 * kk, ct, lane), pf);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its slot may be written again
-  }
+  };
+  for (int at = w, buf = 0; at < total; at += W, buf ^= 1) step(at, mine + buf * STAGE, mine + (buf ^ 1) * STAGE);
   // the waves' sums, each scaled to the common maximum, added in the waves' order
   l = half_sum(l);
   if (half == 0) wm[w][lane] = m, wl[w][lane] = l;
@@ -210,7 +240,7 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
 #pragma unroll
   for (int x = 0; x < W; ++x) top = fmaxf(top, wm[x][lane & 31]);
   const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * c);
-  constexpr int PITCH = D + 4;
+  constexpr int PITCH = TreeFew<P>::PITCH;
   float* ob = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct)
@@ -258,8 +288,8 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // the row blocks of one chunk on one XCD, one after another: its L2 has the keys from the second on
   const int unit = blockIdx.x / 8 / blocks * 8 + blockIdx.x % 8, rb = blockIdx.x / 8 % blocks;
-  const int ch = unit % p.max_chunks, be = unit / p.max_chunks, b = be / p.KV, e = be % p.KV;
-  if (b >= p.nseq) return;
+  const int heads = p.nseq * p.KV, ch = unit / heads, be = unit % heads, b = be / p.KV, e = be % p.KV;
+  if (ch >= p.max_chunks) return;
   const TreeWork t = tree_work(p, b, ch);
   const int rows = t.n * p.G;
   if (t.n <= 0 || ch >= t.chunks || 128 * rb >= rows) return;
@@ -268,6 +298,18 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
   const int row = min(mine, rows - 1), tok = row / p.G, h = e * p.G + row % p.G;
   const bool drafts = ch == t.chunks - 1;
   const int nt = t.c1 > t.c0 ? (t.c1 - t.c0 + 63) / 64 : 0, total = nt + (drafts ? 1 : 0);
+  // wave w copies keys 16 w .. of each tile; their page is known a tile ahead
+  int page = 0;
+  auto pages = [&](int at) {
+    if (at < nt) page = page_of(p, b, key_group(t.c0 + 64 * at + 16 * w, t.c1 - 1).key);
+  };
+  auto stage = [&](int at, unsigned char* to) {
+    if (at < nt) stage_paged<P>(p, page, e, key_group(t.c0 + 64 * at + 16 * w, t.c1 - 1), to, to + TILE, w, lane);
+    else stage_new<P>(p, t.lo, e, key_group(16 * w, t.n - 1), to, to + TILE, w, lane);
+  };
+  pages(0);
+  stage(0, lds);
+  pages(1);
   uint64_t sees = 0;
   if (drafts) {
     const uint64_t all = ancestors(p, t, lane);
@@ -279,27 +321,18 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) q[ks] = P::load(src + 16 * ks + 8 * half);
   }
-  auto stage = [&](int at, int buf) {
-    unsigned char *kt = lds + buf * TILE, *vt = lds + (2 + buf) * TILE;
-    if (at < nt) {
-      stage_keys<P, 64, true>(p, p.kp, p.kps, b, e, 0, t.c0 + 64 * at, t.c1 - 1, kt, w, 4, lane);
-      stage_keys<P, 64, true>(p, p.vp, p.vps, b, e, 0, t.c0 + 64 * at, t.c1 - 1, vt, w, 4, lane);
-    } else {
-      stage_keys<P, 64, false>(p, p.k, p.ks, b, e, t.lo, 0, t.n - 1, kt, w, 4, lane);
-      stage_keys<P, 64, false>(p, p.v, p.vs, b, e, t.lo, 0, t.n - 1, vt, w, 4, lane);
-    }
-  };
   f32x16 o[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) o[ct] = zero16();
   float m = -INFINITY, l = 0.f;
   const float c = p.scale * LOG2E;
-  if (total > 0) stage(0, 0);
-  for (int at = 0; at < total; ++at) {
-    staged_barrier();
-    if (at + 1 < total) stage(at + 1, (at + 1) & 1);
-    if (!busy) continue;
-    const unsigned char *kt = lds + (at & 1) * TILE, *vt = lds + (2 + (at & 1)) * TILE;
+  auto step = [&](int at, const unsigned char* __restrict kt, unsigned char* __restrict next) {
+    if (at + 1 < total) {
+      stage(at + 1, next);
+      pages(at + 2);
+    }
+    if (!busy) return;
+    const unsigned char* vt = kt + TILE;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       f32x16 s = zero16();
@@ -322,6 +355,10 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
         for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, 32 * u + 16 * kk, ct, lane), pf);
       }
     }
+  };
+  for (int at = 0; at < total; ++at) {
+    staged_barrier();
+    step(at, lds + (at & 1) * 2 * TILE, lds + (~at & 1) * 2 * TILE);
   }
   l = half_sum(l);
   if (t.chunks == 1) {
@@ -445,6 +482,9 @@ extern "C" int kdn_tree_attn(const kdn_tree_attn_args* a, void* stream) {
   const int64_t chunks = tree_chunks(a), rows = a->max_new * (a->H / a->H_kv), blocks = rows <= 32 ? 1 : (rows + 127) / 128;
   if (a->num_seqs * a->H_kv * chunks * blocks > INT32_MAX - 8 * blocks || a->num_seqs * a->H_kv * rows > INT32_MAX)
     return KDN_ERR_UNSUPPORTED;
+  // a copy's lanes have 32-bit offsets from its first row
+  const int64_t size = (int64_t)dtype_size(a->dtype), far = INT32_MAX / (16 * size);
+  if (a->k_stride[0] > far || a->v_stride[0] > far || a->k_pages_stride[2] > far || a->v_pages_stride[2] > far) return KDN_ERR_UNSUPPORTED;
   if (chunks > 1 && (!a->workspace || a->workspace_bytes < tree_partial_bytes(a, a->num_seqs * a->H_kv * chunks))) return KDN_ERR_WORKSPACE_TOO_SMALL;
   TreeParams p = {};
   p.q = a->q; p.k = a->k; p.v = a->v; p.kp = a->k_pages; p.vp = a->v_pages; p.y = a->y;

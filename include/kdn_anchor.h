@@ -37,11 +37,12 @@ typedef struct kdn_attn_args {
   const void* v; int64_t v_stride[2];
   void* y;       int64_t y_stride[2];
   float* lse;                   /* [H][total_q]: log of the sum of exp(scale q.k), or NULL */
+  void* y_low;   int64_t y_low_stride[2];   /* what rounding to bf16 took from y, for the backward, or NULL (unused with fp32) */
 } kdn_attn_args;
 int kdn_attn_fwd(const kdn_attn_args* a, void* stream);
 
 /* Gradients of a loss through kdn_attn_fwd, given dy = dL/dy: `fwd` holds the forward's arguments with its y and lse
- * (both required).  dq, dk, dv in the inputs' dtype, each rounded once from fp32 sums, summed in a fixed order (the same
+ * (both required) and y_low (if the forward wrote it: dy . y is formed from both; without it from the rounded y).  dq, dk, dv in the inputs' dtype, each rounded once from fp32 sums, summed in a fixed order (the same
  * bits every time); every row of a sequence is written.  workspace: kdn_attn_bwd_workspace_bytes, 16-byte aligned. */
 typedef struct kdn_attn_bwd_args {
   const kdn_attn_args* fwd;

@@ -12,15 +12,26 @@
 
 namespace kdn {
 
-constexpr int FWD_ROWS = 128, FWD_KEYS = 64, FWD_BLOCKS = FWD_KEYS / 32;
+// What bounds it: with one wave of 32 rows a SIMD's matrix core is busy half of the time at best (a tile's softmax is as
+// many cycles as its products), with two about as much as a large matrix product keeps it.  The walk over the keys is one
+// chain, so that a batch with few rows takes the time of its longest row, however idle the GPU: then SPLIT waves share 32
+// rows and take every SPLIT-th block of 32 keys of a tile each, and their sums meet at the end.
+template <class P, int SPLIT>
+struct Fwd {
+  static constexpr int ROWS = 128 / SPLIT, KEYS = SPLIT == 4 ? 128 : 64, BLOCKS = KEYS / 32 / SPLIT;
+  static constexpr int TILE = KEYS * P::ROW, BUFS = 4 * TILE <= 128 * 1024 ? 2 : 1;
+  static constexpr int JOIN = SPLIT > 1 ? 4 * (P::D / 32) * 4096 + 4 * 64 * 8 : 0;
+  static constexpr int LDS = 2 * BUFS * TILE > JOIN ? 2 * BUFS * TILE : JOIN;
+};
 
-template <class P>
+template <class P, int SPLIT>
 __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) attn_fwd_kernel(AttnParams p, int64_t slots) {
   typedef typename P::elem E;
-  constexpr int D = P::D, KS = D / 16, CT = D / 32, TILE = FWD_KEYS * P::ROW;
-  __shared__ __attribute__((aligned(256))) unsigned char lds[4 * TILE];
+  typedef Fwd<P, SPLIT> S;
+  constexpr int KS = P::D / 16, CT = P::D / 32, KEYS = S::KEYS, TILE = S::TILE;
+  __shared__ __attribute__((aligned(256))) unsigned char lds[S::LDS];
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = w % SPLIT;
   // the last tiles (the longest rows) first, and an XCD's heads next to one another so that its L2 holds their keys
   int64_t id = blockIdx.x;
   int h;
@@ -31,20 +42,21 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
     h = (int)(id % p.H);
   }
   const int64_t slot = slots - 1 - id / p.H;
-  const SeqTile t = find_tile<FWD_ROWS>(p.cu_q, p.nseq, p.total_q, slot, lane);
+  const SeqTile t = find_tile<S::ROWS>(p.cu_q, p.nseq, p.total_q, slot, lane);
   if (t.row0 < 0) return;
-  const int64_t lenq = t.len;
-  int64_t klo, lenk;
+  const int lenq = t.len;
+  int64_t klo;
+  int lenk;
   other_rows(p.cu_k, p.nseq, p.total_k, t.seq, klo, lenk);
-  const int64_t off = lenk - lenq;  // query i sees keys 0 .. i + off
-  const int row = t.row0 + 32 * w + (lane & 31);
+  const int off = lenk - lenq;  // query i sees keys 0 .. i + off
+  const int first_row = t.row0 + 32 * (w / SPLIT), row = first_row + (lane & 31);
   const bool live = row < lenq;
   const E* kb = reinterpret_cast<const E*>(p.k) + klo * p.ks[0] + (int64_t)(h / p.G) * p.ks[1];
   const E* vb = reinterpret_cast<const E*>(p.v) + klo * p.vs[0] + (int64_t)(h / p.G) * p.vs[1];
 
   typename P::frag q[KS];
   {
-    const E* src = reinterpret_cast<const E*>(p.q) + (t.lo + min((int64_t)row, lenq - 1)) * p.qs[0] + (int64_t)h * p.qs[1];
+    const E* src = reinterpret_cast<const E*>(p.q) + (t.lo + min(row, lenq - 1)) * p.qs[0] + (int64_t)h * p.qs[1];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) q[ks] = P::load(src + 16 * ks + 8 * half);
   }
@@ -54,47 +66,47 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   float m = -INFINITY, l = 0.f;
   const float c = p.scale * LOG2E;
 
-  const int64_t sees = min(lenk, t.row0 + FWD_ROWS + off);  // keys that any row of the workgroup sees
-  const int ntiles = sees > 0 ? (int)((sees + FWD_KEYS - 1) / FWD_KEYS) : 0;
-  const int64_t wfirst = t.row0 + 32 * w + off, wlast = wfirst + 31;  // last key the wave's first / last row sees
+  const int sees = min(lenk, t.row0 + S::ROWS + off);  // keys that any row of the workgroup sees
+  const int ntiles = sees > 0 ? (sees + KEYS - 1) / KEYS : 0;
+  const int wfirst = first_row + off, wlast = wfirst + 31;  // last key the wave's first / last row sees
+  const Stager<P, KEYS, 4> stage_k(p.ks[0], w, lane), stage_v(p.vs[0], w, lane);
   auto stage = [&](int j, unsigned char* to) {
-    const int64_t k0 = (int64_t)j * FWD_KEYS;
-    const int last = (int)min(lenk - 1 - k0, (int64_t)FWD_KEYS - 1);
-    stage_rows<P, FWD_KEYS, 4>(kb + k0 * p.ks[0], p.ks[0], last, to, w, lane);
-    stage_rows<P, FWD_KEYS, 4>(vb + k0 * p.vs[0], p.vs[0], last, to + TILE, w, lane);
+    const int k0 = j * KEYS, last = min(lenk - 1 - k0, KEYS - 1);
+    stage_k(kb + k0 * p.ks[0], last, to);
+    stage_v(vb + k0 * p.vs[0], last, to + TILE);
   };
   // One tile, read from `kt`, while the next one's copies go to `next`.  That the two do not overlap is said to the compiler
   // (__restrict): it would wait for the copies before it reads V otherwise.
   auto step = [&](int j, const unsigned char* __restrict kt, unsigned char* __restrict next) {
-    if (j + 1 < ntiles) stage(j + 1, next);
-    const int64_t k0 = (int64_t)j * FWD_KEYS;
+    if (S::BUFS == 2 && j + 1 < ntiles) stage(j + 1, next);
+    const int r0 = 32 * S::BLOCKS * part, k0 = j * KEYS + r0;  // the wave's keys of the tile
     if (k0 > wlast) return;  // nothing of this tile is visible to the wave
     const unsigned char* vt = kt + TILE;
-    f32x16 s[FWD_BLOCKS];
+    f32x16 s[S::BLOCKS];
 #pragma unroll
-    for (int b = 0; b < FWD_BLOCKS; ++b) {
-      s[b] = zero16();
+    for (int b = 0; b < S::BLOCKS; ++b) s[b] = zero16();
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s[b] = P::mma(s[b], P::row_frag(kt, 32 * b + (lane & 31), ks, half), q[ks]);
-    }
-    if (k0 + FWD_KEYS - 1 > wfirst) {
-      const int limit = (int)min(max((int64_t)row + off - k0, (int64_t)-1), (int64_t)FWD_KEYS);
+    for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int b = 0; b < FWD_BLOCKS; ++b)
+      for (int b = 0; b < S::BLOCKS; ++b) s[b] = P::mma(s[b], P::row_frag(kt, r0 + 32 * b + (lane & 31), ks, half), q[ks]);
+    if (k0 + 32 * S::BLOCKS - 1 > wfirst) {
+      const int limit = row + off - k0;
+#pragma unroll
+      for (int b = 0; b < S::BLOCKS; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[b][i] = 32 * b + rho(half, i) <= limit ? s[b][i] : -INFINITY;
     }
     float top = s[0][0];
 #pragma unroll
-    for (int b = 0; b < FWD_BLOCKS; ++b)
+    for (int b = 0; b < S::BLOCKS; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
     top = half_max(top);
     // the maximum moves only where it grows by more than 2^6 (the sums stay far inside fp32): most tiles rescale nothing
     if (__any((top - m) * c > 6.f || (m == -INFINITY && top > m))) {
-      const float next = fmaxf(m, top);
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - next) * c);
-      m = next;
+      const float next_m = fmaxf(m, top);
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - next_m) * c);
+      m = next_m;
       l *= f;
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
@@ -104,7 +116,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
     const float mc = m == -INFINITY ? 0.f : m * c;
     float sum = 0.f;
 #pragma unroll
-    for (int b = 0; b < FWD_BLOCKS; ++b)
+    for (int b = 0; b < S::BLOCKS; ++b)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         s[b][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, -mc));
@@ -112,23 +124,57 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
       }
     l += sum;
 #pragma unroll
-    for (int kk = 0; kk < 2 * FWD_BLOCKS; ++kk) {
+    for (int kk = 0; kk < 2 * S::BLOCKS; ++kk) {
       const typename P::frag pf = P::from_acc(s[kk >> 1], kk & 1);
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, 16 * kk, ct, lane), pf);
+      for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, r0 + 16 * kk, ct, lane), pf);
     }
   };
-  if (ntiles > 0) stage(0, lds);
+  if (S::BUFS == 2 && ntiles > 0) stage(0, lds);
   for (int j = 0; j < ntiles; ++j) {
+    if (S::BUFS == 1) {
+      staged_barrier();
+      stage(j, lds);
+    }
     staged_barrier();
-    step(j, lds + (j & 1) * 2 * TILE, lds + (~j & 1) * 2 * TILE);
+    step(j, lds + (S::BUFS == 2 ? (j & 1) * 2 * TILE : 0), lds + (S::BUFS == 2 ? (~j & 1) * 2 * TILE : 0));
   }
   l = half_sum(l);
-  const float f = l == 0.f ? 0.f : 1.f / l;
   E* dst = reinterpret_cast<E*>(p.out) + (t.lo + row) * p.ys[0] + (int64_t)h * p.ys[1];
+  E* low = p.low ? reinterpret_cast<E*>(p.low) + (t.lo + row) * p.lows[0] + (int64_t)h * p.lows[1] : nullptr;
+  auto ends = [&](int ct, const f32x16& v, float f) {
+    store_row32(dst + 32 * ct, v, f, half, live);
+    if (sizeof(E) == 2 && low) {
+      f32x16 rest;
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) store_row32(dst + 32 * ct, o[ct], f, half, live);
-  if (p.lse && live && half == 0) p.lse[(int64_t)h * p.total_q + t.lo + row] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
+      for (int i = 0; i < 16; ++i) rest[i] = v[i] * f - (float)(E)(v[i] * f);
+      store_row32(low + 32 * ct, rest, 1.f, half, live);
+    }
+  };
+  if constexpr (SPLIT == 1) {
+    const float f = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) ends(ct, o[ct], f);
+  } else {
+    float* stat = reinterpret_cast<float*>(lds + 4 * CT * 4096);  // each wave's maxima and sums
+    __syncthreads();
+    stat[w * 64 + lane] = m;
+    stat[256 + w * 64 + lane] = l;
+    __syncthreads();
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < SPLIT; ++x) top = fmaxf(top, stat[(w - part + x) * 64 + lane]);
+#pragma unroll
+    for (int x = 0; x < SPLIT; ++x) {
+      const float mx = stat[(w - part + x) * 64 + lane];
+      sum += mx == -INFINITY ? 0.f : stat[256 + (w - part + x) * 64 + lane] * __builtin_amdgcn_exp2f((mx - top) * c);
+    }
+    const float mine = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * c), f = sum == 0.f ? 0.f : 1.f / sum;
+    join_sums<SPLIT>(o, mine, lds, w, lane, [&](int ct, const f32x16& v) { ends(ct, v, f); });
+    m = top;
+    l = sum;
+  }
+  if (p.lse && live && half == 0 && part == 0) p.lse[(int64_t)h * p.total_q + t.lo + row] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
 }
 
 bool attn_strides_ok(const int64_t s[2], int dtype) {
@@ -141,7 +187,7 @@ int attn_check(const kdn_attn_args* a) {
       a->H % a->H_kv != 0 || !valid_dtype(a->dtype) || !(a->scale > 0.f) || !std::isfinite(a->scale))
     return KDN_ERR_INVALID_ARGUMENT;
   if (a->d != 64 && a->d != 128) return KDN_ERR_UNSUPPORTED;
-  if (a->total_q > INT32_MAX || a->total_k > INT32_MAX || a->num_seqs > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  if (a->total_q > (1 << 30) || a->total_k > (1 << 30) || a->num_seqs > (1 << 30)) return KDN_ERR_UNSUPPORTED;
   if (!a->cu_k && a->total_k != a->total_q) return KDN_ERR_INVALID_ARGUMENT;
   return KDN_OK;
 }
@@ -149,11 +195,19 @@ int attn_check(const kdn_attn_args* a) {
 int attn_check_tensors(const kdn_attn_args* a) {
   if (!a->cu_q || !a->q || !a->y) return KDN_ERR_INVALID_ARGUMENT;
   if (a->total_k > 0 && (!a->k || !a->v)) return KDN_ERR_INVALID_ARGUMENT;
-  if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->y, 16) || !aligned(a->lse, 4) ||
+  if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->v, 16) || !aligned(a->y, 16) || !aligned(a->y_low, 16) || !aligned(a->lse, 4) ||
       !attn_strides_ok(a->q_stride, a->dtype) || !attn_strides_ok(a->k_stride, a->dtype) ||
-      !attn_strides_ok(a->v_stride, a->dtype) || !attn_strides_ok(a->y_stride, a->dtype))
+      !attn_strides_ok(a->v_stride, a->dtype) || !attn_strides_ok(a->y_stride, a->dtype) ||
+      (a->y_low && !attn_strides_ok(a->y_low_stride, a->dtype)))
     return KDN_ERR_MISALIGNED;
+  if (!stage_reach(a->q_stride[0], a->dtype) || !stage_reach(a->k_stride[0], a->dtype) || !stage_reach(a->v_stride[0], a->dtype))
+    return KDN_ERR_UNSUPPORTED;
   return KDN_OK;
+}
+
+int attn_split(int64_t rows, int64_t heads) {
+  const int64_t tiles = rows / 128 * heads;
+  return tiles < 256 ? 4 : tiles < 512 ? 2 : 1;
 }
 
 AttnParams attn_params(const kdn_attn_args* a) {
@@ -162,6 +216,8 @@ AttnParams attn_params(const kdn_attn_args* a) {
   for (int i = 0; i < 2; ++i) {
     p.qs[i] = a->q_stride[i]; p.ks[i] = a->k_stride[i]; p.vs[i] = a->v_stride[i]; p.ys[i] = a->y_stride[i];
   }
+  p.low = a->y_low;
+  for (int i = 0; i < 2; ++i) p.lows[i] = a->y_low_stride[i];
   p.lse = a->lse;
   p.cu_q = a->cu_q;
   p.cu_k = a->cu_k ? a->cu_k : a->cu_q;
@@ -177,22 +233,30 @@ using namespace kdn;
 
 extern "C" int kdn_anchor_version(void) { return 1 << 16; }
 
+template <class P, int SPLIT>
+static int launch_fwd(const AttnParams& p, hipStream_t st) {
+  const int64_t slots = p.total_q / Fwd<P, SPLIT>::ROWS + p.nseq + 1, grid = slots * p.H;
+  if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((attn_fwd_kernel<P, SPLIT>), dim3((unsigned)grid), dim3(256), 0, st, p, slots);
+  return launch_status();
+}
+
+template <class P>
+static int launch_fwd(const AttnParams& p, hipStream_t st) {
+  switch (attn_split(p.total_q, p.H)) {
+    case 4: return launch_fwd<P, 4>(p, st);
+    case 2: return launch_fwd<P, 2>(p, st);
+    default: return launch_fwd<P, 1>(p, st);
+  }
+}
+
 extern "C" int kdn_attn_fwd(const kdn_attn_args* a, void* stream) {
   int rc = attn_check(a);
   if (rc != KDN_OK) return rc;
   if (a->total_q == 0) return KDN_OK;
   if ((rc = attn_check_tensors(a)) != KDN_OK) return rc;
   const AttnParams p = attn_params(a);
-  const int64_t slots = a->total_q / FWD_ROWS + a->num_seqs + 1, grid = slots * a->H;
-  if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
-  const dim3 g((unsigned)grid), b(256);
   hipStream_t st = as_stream(stream);
-  if (a->dtype == KDN_DTYPE_BF16) {
-    if (a->d == 64) hipLaunchKernelGGL(attn_fwd_kernel<AttnBF16<64>>, g, b, 0, st, p, slots);
-    else hipLaunchKernelGGL(attn_fwd_kernel<AttnBF16<128>>, g, b, 0, st, p, slots);
-  } else {
-    if (a->d == 64) hipLaunchKernelGGL(attn_fwd_kernel<AttnF32<64>>, g, b, 0, st, p, slots);
-    else hipLaunchKernelGGL(attn_fwd_kernel<AttnF32<128>>, g, b, 0, st, p, slots);
-  }
-  return launch_status();
+  if (a->dtype == KDN_DTYPE_BF16) return a->d == 64 ? launch_fwd<AttnBF16<64>>(p, st) : launch_fwd<AttnBF16<128>>(p, st);
+  return a->d == 64 ? launch_fwd<AttnF32<64>>(p, st) : launch_fwd<AttnF32<128>>(p, st);
 }

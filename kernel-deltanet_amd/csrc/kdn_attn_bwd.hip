@@ -8,11 +8,11 @@
 // workgroup per 128 query rows of a head walking its keys.  The scores are formed twice (seven products for the five that
 // one pass with atomic sums of dq would take): every sum then has one owner and one order, so that the gradients are the
 // same bits every time.  As in the forward a product's accumulator is the next one's B operand in registers.
+#include <algorithm>
 #include "kdn_attn_tile.hpp"
+#include "kdn_io.hpp"
 
 namespace kdn {
-
-constexpr int BWD_ROWS = 128, BWD_TILE = 64;
 
 // delta: sixteen lanes a row, eight values each at a time.
 template <class P>
@@ -27,8 +27,16 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnParams p, float* de
   float sum = 0.f;
   if (8 * j < P::D) {
     const typename P::frag a = P::load(y + 8 * j), b = P::load(dy + 8 * j);
+    float x[8];
 #pragma unroll
-    for (int s = 0; s < 8; ++s) sum = __builtin_fmaf((float)a[s], (float)b[s], sum);
+    for (int s = 0; s < 8; ++s) x[s] = (float)a[s];
+    if (sizeof(E) == 2 && p.low) {
+      const typename P::frag rest = P::load(reinterpret_cast<const E*>(p.low) + row * p.lows[0] + h * p.lows[1] + 8 * j);
+#pragma unroll
+      for (int s = 0; s < 8; ++s) x[s] += (float)rest[s];
+    }
+#pragma unroll
+    for (int s = 0; s < 8; ++s) sum = __builtin_fmaf(x[s], (float)b[s], sum);
   }
   sum += xor_shuffle<1>(sum);
   sum += xor_shuffle<2>(sum);
@@ -37,84 +45,94 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnParams p, float* de
   if (j == 0) delta[h * p.total_q + row] = sum;
 }
 
-// dk, dv of 128 keys: a wave owns 32 keys (a lane one), their K and V fragments and the transposed sums in registers.
-// The query rows pass in tiles of 64 with their lse and delta; S = Q K^T and dP = dY V^T have the queries in registers,
-// so that P and dS are the B operands of dV^T += dY^T P and dK^T += Q^T dS.
-template <class P>
-__global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 && P::D == 64 ? 2 : 1)
-    attn_dkdv_kernel(AttnParams p, int64_t slots) {
+// dk and dv of 128 / SPLIT keys: a wave owns 32 keys (a lane one), their K and V fragments and the transposed sums in
+// registers.  The query rows pass in tiles with their lse and delta; S = Q K^T and dP = dY V^T have the queries in
+// registers, so that P and dS are the B operands of dV^T += dY^T P and dK^T += Q^T dS.
+//   With 128 features both sums and the operands do not fit the registers of two waves a SIMD, and one wave, whose softmax
+// nothing overlaps, takes 2.13 ms at 8192 rows, 32 heads: there dv and dk are two launches (DV, DK), S formed in both.
+template <class P, int SPLIT>
+struct Dkdv {
+  static constexpr int KEYS = 128 / SPLIT, ROWS = SPLIT == 4 ? 128 : 64, BLOCKS = ROWS / 32 / SPLIT;
+  static constexpr int TILE = ROWS * P::ROW, SLOT = 2 * TILE + 2 * ROWS * 4, BUFS = 2 * SLOT <= 160 * 1024 ? 2 : 1;
+  static constexpr int JOIN = SPLIT > 1 ? 4 * (P::D / 32) * 4096 : 0;
+  static constexpr int LDS = BUFS * SLOT > JOIN ? BUFS * SLOT : JOIN;
+};
+
+template <class P, int SPLIT, bool DV, bool DK>
+__global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) attn_dkdv_kernel(AttnParams p, int64_t slots) {
   typedef typename P::elem E;
-  constexpr int D = P::D, KS = D / 16, CT = D / 32, TILE = BWD_TILE * P::ROW;
-  constexpr int SLOT = 2 * TILE + 2 * BWD_TILE * 4;  // Q and dY rows, their lse and delta
-  constexpr int NBUF = 2 * SLOT <= 160 * 1024 ? 2 : 1;
-  __shared__ __attribute__((aligned(256))) unsigned char lds[NBUF * SLOT];
+  typedef Dkdv<P, SPLIT> S;
+  constexpr int KS = P::D / 16, CT = P::D / 32, TILE = S::TILE, ROWS = S::ROWS;
+  __shared__ __attribute__((aligned(256))) unsigned char lds[S::LDS];
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t id = blockIdx.x;
-  const int e = (int)(id % p.KV);
-  const SeqTile t = find_tile<BWD_ROWS>(p.cu_k, p.nseq, p.total_k, id / p.KV, lane);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = w % SPLIT;
+  const int64_t id = blockIdx.x;  // the first keys, which the most rows see, first
+  const int e = (int)(id % p.KV), sub = (int)(id / p.KV % p.subsets), heads = p.G / p.subsets;
+  const SeqTile t = find_tile<S::KEYS>(p.cu_k, p.nseq, p.total_k, id / p.KV / p.subsets, lane);
   if (t.row0 < 0) return;
-  const int64_t lenk = t.len;
-  int64_t qlo, lenq;
+  const int lenk = t.len;
+  int64_t qlo;
+  int lenq;
   other_rows(p.cu_q, p.nseq, p.total_q, t.seq, qlo, lenq);
-  const int64_t off = lenk - lenq;
-  const int key = t.row0 + 32 * w + (lane & 31);
+  const int off = lenk - lenq;
+  const int first_key = t.row0 + 32 * (w / SPLIT), key = first_key + (lane & 31);
   const bool live = key < lenk;
-  typename P::frag k[KS], v[KS];
+  typename P::frag k[KS], v[DK ? KS : 1];
   {
-    const int64_t at = t.lo + min((int64_t)key, lenk - 1);
+    const int64_t at = t.lo + min(key, lenk - 1);
     const E* ksrc = reinterpret_cast<const E*>(p.k) + at * p.ks[0] + (int64_t)e * p.ks[1];
     const E* vsrc = reinterpret_cast<const E*>(p.v) + at * p.vs[0] + (int64_t)e * p.vs[1];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       k[ks] = P::load(ksrc + 16 * ks + 8 * half);
-      v[ks] = P::load(vsrc + 16 * ks + 8 * half);
+      if constexpr (DK) v[ks] = P::load(vsrc + 16 * ks + 8 * half);
     }
   }
-  f32x16 dk[CT], dv[CT];
+  f32x16 dk[DK ? CT : 1], dv[DV ? CT : 1];
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) dk[ct] = dv[ct] = zero16();
+  for (int ct = 0; ct < CT; ++ct) {
+    if constexpr (DK) dk[ct] = zero16();
+    if constexpr (DV) dv[ct] = zero16();
+  }
   const float c = p.scale * LOG2E;
 
-  // the query tiles that see key row0: rows from row0 - off on, of each head of the group
-  const int64_t q0 = max(t.row0 - off, (int64_t)0) / BWD_TILE * BWD_TILE;
-  const int per = q0 < lenq ? (int)((lenq - q0 + BWD_TILE - 1) / BWD_TILE) : 0;
-  const int ntiles = per * p.G;
+  // the query tiles that see key row0: rows from row0 - off on, of each head of the subset
+  const int q0 = max(t.row0 - off, 0) / ROWS * ROWS;
+  const int per = q0 < lenq ? (lenq - q0 + ROWS - 1) / ROWS : 0;
+  const int ntiles = per * heads;
+  const Stager<P, ROWS, 4> stage_q(p.qs[0], w, lane), stage_y(p.dys[0], w, lane);
   auto stage = [&](int j, unsigned char* to) {
-    const int h = e * p.G + j / per;
-    const int64_t r0 = q0 + (int64_t)(j % per) * BWD_TILE;
-    const int last = (int)min(lenq - 1 - r0, (int64_t)BWD_TILE - 1);
-    const E* qb = reinterpret_cast<const E*>(p.q) + (qlo + r0) * p.qs[0] + (int64_t)h * p.qs[1];
-    const E* yb = reinterpret_cast<const E*>(p.dy) + (qlo + r0) * p.dys[0] + (int64_t)h * p.dys[1];
-    stage_rows<P, BWD_TILE, 4>(qb, p.qs[0], last, to, w, lane);
-    stage_rows<P, BWD_TILE, 4>(yb, p.dys[0], last, to + TILE, w, lane);
-    if (w < 2) {
-      const float* src = (w == 0 ? p.lse : p.delta) + (int64_t)h * p.total_q + qlo + r0 + min(lane, last);
+    const int h = e * p.G + sub * heads + j / per, r0 = q0 + j % per * ROWS, last = min(lenq - 1 - r0, ROWS - 1);
+    stage_q(reinterpret_cast<const E*>(p.q) + (qlo + r0) * p.qs[0] + (int64_t)h * p.qs[1], last, to);
+    stage_y(reinterpret_cast<const E*>(p.dy) + (qlo + r0) * p.dys[0] + (int64_t)h * p.dys[1], last, to + TILE);
+    const int x = 64 * w + lane;  // lse of the rows, then delta
+    if (64 * w < 2 * ROWS) {
+      const float* src = (x < ROWS ? p.lse : p.delta) + (int64_t)h * p.total_q + qlo + r0 + min(x % ROWS, last);
       __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(src),
-                                       (__attribute__((address_space(3))) void*)(to + 2 * TILE + w * BWD_TILE * 4), 4, 0, 0);
+                                       (__attribute__((address_space(3))) void*)(to + 2 * TILE + 256 * w), 4, 0, 0);
     }
   };
   // as in the forward: the next tile's copies and this one's reads do not overlap
   auto step = [&](int j, const unsigned char* __restrict qt, unsigned char* __restrict next) {
-    if (NBUF == 2 && j + 1 < ntiles) stage(j + 1, next);
-    const int64_t r0 = q0 + (int64_t)(j % per) * BWD_TILE;
+    if (S::BUFS == 2 && j + 1 < ntiles) stage(j + 1, next);
     const unsigned char *yt = qt + TILE, *stat = qt + 2 * TILE;
-#pragma unroll(sizeof(E) == 2 ? 2 : 1)
-    for (int u = 0; u < BWD_TILE / 32; ++u) {
-      const int64_t i0 = r0 + 32 * u;  // rows i0 .. i0 + 31
-      if (i0 >= lenq || i0 + 31 + off < t.row0 + 32 * w) continue;  // none of them sees a key of this wave
+#pragma unroll sizeof(E) == 2 ? S::BLOCKS : 1
+    for (int u = 0; u < S::BLOCKS; ++u) {
+      const int tr = 32 * (S::BLOCKS * part + u), i0 = q0 + j % per * ROWS + tr;  // the wave's rows of the tile: i0 .. i0 + 31
+      if (i0 >= lenq || i0 + 31 + off < first_key) continue;                      // none of them sees a key of this wave
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = P::mma(s, P::row_frag(qt, 32 * u + (lane & 31), ks, half), k[ks]);
+      for (int ks = 0; ks < KS; ++ks) s = P::mma(s, P::row_frag(qt, tr + (lane & 31), ks, half), k[ks]);
+      if constexpr (DK) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) dp = P::mma(dp, P::row_frag(yt, 32 * u + (lane & 31), ks, half), v[ks]);
-      const bool whole = i0 + off >= t.row0 + 32 * w + 31 && i0 + 32 <= lenq;
-      const int64_t first = max((int64_t)key - off, (int64_t)0) - i0;  // rows of the tile from `first` to `end` see the key
-      const int lo = (int)min(first, (int64_t)32), hi = (int)min(lenq - i0, (int64_t)32);
+        for (int ks = 0; ks < KS; ++ks) dp = P::mma(dp, P::row_frag(yt, tr + (lane & 31), ks, half), v[ks]);
+      }
+      const bool whole = i0 + off >= first_key + 31 && i0 + 32 <= lenq;
+      const int lo = max(key - off, 0) - i0, hi = lenq - i0;  // rows lo .. hi - 1 of the block see the key
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(stat + 4 * (32 * u + 8 * a + 4 * half));
-        const f32x4 de = *reinterpret_cast<const f32x4*>(stat + 4 * (BWD_TILE + 32 * u + 8 * a + 4 * half));
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(stat + 4 * (tr + 8 * a + 4 * half));
+        const f32x4 de = *reinterpret_cast<const f32x4*>(stat + 4 * (ROWS + tr + 8 * a + 4 * half));
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int i = 4 * a + x, r = rho(half, i);
@@ -134,40 +152,78 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 && P::D == 
         const typename P::frag pf = P::from_acc(s, m), df = P::from_acc(dp, m);
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-          dv[ct] = P::mma(dv[ct], P::col_frag(yt, 32 * u + 16 * m, ct, lane), pf);
-          dk[ct] = P::mma(dk[ct], P::col_frag(qt, 32 * u + 16 * m, ct, lane), df);
+          if constexpr (DV) dv[ct] = P::mma(dv[ct], P::col_frag(yt, tr + 16 * m, ct, lane), pf);
+          if constexpr (DK) dk[ct] = P::mma(dk[ct], P::col_frag(qt, tr + 16 * m, ct, lane), df);
         }
       }
     }
   };
-  if (NBUF == 2 && ntiles > 0) stage(0, lds);
+  if (S::BUFS == 2 && ntiles > 0) stage(0, lds);
   for (int j = 0; j < ntiles; ++j) {
-    if (NBUF == 1) {
+    if (S::BUFS == 1) {
       staged_barrier();
       stage(j, lds);
     }
     staged_barrier();
-    if constexpr (NBUF == 2) step(j, lds + (j & 1) * SLOT, lds + (~j & 1) * SLOT);
-    else step(j, lds, lds);
+    step(j, lds + (S::BUFS == 2 ? (j & 1) * S::SLOT : 0), lds + (S::BUFS == 2 ? (~j & 1) * S::SLOT : 0));
   }
-  E* dkr = reinterpret_cast<E*>(p.dk) + (t.lo + key) * p.dks[0] + (int64_t)e * p.dks[1];
-  E* dvr = reinterpret_cast<E*>(p.dv) + (t.lo + key) * p.dvs[0] + (int64_t)e * p.dvs[1];
+  const int64_t at = t.lo + key, part_at = (((int64_t)sub * p.total_k + at) * p.KV + e) * P::D;
+  auto store_k = [&](int ct, const f32x16& x, float f) {
+    if (p.subsets > 1) store_row32(p.part_dk + part_at + 32 * ct, x, f, half, live);
+    else store_row32(reinterpret_cast<E*>(p.dk) + at * p.dks[0] + (int64_t)e * p.dks[1] + 32 * ct, x, f, half, live);
+  };
+  auto store_v = [&](int ct, const f32x16& x) {
+    if (p.subsets > 1) store_row32(p.part_dv + part_at + 32 * ct, x, 1.f, half, live);
+    else store_row32(reinterpret_cast<E*>(p.dv) + at * p.dvs[0] + (int64_t)e * p.dvs[1] + 32 * ct, x, 1.f, half, live);
+  };
+  if constexpr (SPLIT == 1) {
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    store_row32(dkr + 32 * ct, dk[ct], p.scale, half, live);
-    store_row32(dvr + 32 * ct, dv[ct], 1.f, half, live);
+    for (int ct = 0; ct < CT; ++ct) {
+      if constexpr (DK) store_k(ct, dk[ct], p.scale);
+      if constexpr (DV) store_v(ct, dv[ct]);
+    }
+  } else {
+    staged_barrier();
+    if constexpr (DK) join_sums<SPLIT>(dk, p.scale, lds, w, lane, [&](int ct, const f32x16& x) { store_k(ct, x, 1.f); });
+    if constexpr (DV) join_sums<SPLIT>(dv, 1.f, lds, w, lane, store_v);
   }
 }
 
-// dq of 128 query rows of a head: the forward's walk over the keys with S^T = K Q^T and dP^T = V dY^T, and
-// dQ^T += K^T dS^T.
+// The subsets' sums added in order and rounded: four values of dk and of dv a lane.
 template <class P>
+__global__ void __launch_bounds__(256) attn_subsets_kernel(AttnParams p) {
+  typedef typename P::elem E;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = p.total_k * p.KV * (P::D / 4);
+  if (i >= n) return;
+  const int64_t row = i / (P::D / 4), d = 4 * (i % (P::D / 4)), at = row / p.KV, e = row % p.KV;
+  f32x4 dk = zero4(), dv = zero4();
+  for (int s = 0; s < p.subsets; ++s) {
+    dk += reinterpret_cast<const f32x4*>(p.part_dk)[s * n + i];
+    dv += reinterpret_cast<const f32x4*>(p.part_dv)[s * n + i];
+  }
+  const float x[4] = {dk[0], dk[1], dk[2], dk[3]}, y[4] = {dv[0], dv[1], dv[2], dv[3]};
+  store4(reinterpret_cast<E*>(p.dk) + at * p.dks[0] + e * p.dks[1] + d, x);
+  store4(reinterpret_cast<E*>(p.dv) + at * p.dvs[0] + e * p.dvs[1] + d, y);
+}
+
+// dq of 128 / SPLIT query rows of a head: the forward's walk over the keys with S^T = K Q^T and dP^T = V dY^T, and
+// dQ^T += K^T dS^T.
+template <class P, int SPLIT>
+struct Dq {
+  static constexpr int ROWS = 128 / SPLIT, KEYS = SPLIT == 4 ? 128 : 64, BLOCKS = KEYS / 32 / SPLIT;
+  static constexpr int TILE = KEYS * P::ROW, BUFS = 4 * TILE <= 128 * 1024 ? 2 : 1;
+  static constexpr int JOIN = SPLIT > 1 ? 4 * (P::D / 32) * 4096 : 0;
+  static constexpr int LDS = 2 * BUFS * TILE > JOIN ? 2 * BUFS * TILE : JOIN;
+};
+
+template <class P, int SPLIT>
 __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) attn_dq_kernel(AttnParams p, int64_t slots) {
   typedef typename P::elem E;
-  constexpr int D = P::D, KS = D / 16, CT = D / 32, TILE = BWD_TILE * P::ROW;
-  __shared__ __attribute__((aligned(256))) unsigned char lds[4 * TILE];
+  typedef Dq<P, SPLIT> S;
+  constexpr int KS = P::D / 16, CT = P::D / 32, KEYS = S::KEYS, TILE = S::TILE;
+  __shared__ __attribute__((aligned(256))) unsigned char lds[S::LDS];
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = w % SPLIT;
   int64_t id = blockIdx.x;
   int h;
   if (p.H % 8 == 0) {
@@ -176,15 +232,16 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   } else {
     h = (int)(id % p.H);
   }
-  const SeqTile t = find_tile<BWD_ROWS>(p.cu_q, p.nseq, p.total_q, slots - 1 - id / p.H, lane);
+  const SeqTile t = find_tile<S::ROWS>(p.cu_q, p.nseq, p.total_q, slots - 1 - id / p.H, lane);
   if (t.row0 < 0) return;
-  const int64_t lenq = t.len;
-  int64_t klo, lenk;
+  const int lenq = t.len;
+  int64_t klo;
+  int lenk;
   other_rows(p.cu_k, p.nseq, p.total_k, t.seq, klo, lenk);
-  const int64_t off = lenk - lenq;
-  const int row = t.row0 + 32 * w + (lane & 31);
+  const int off = lenk - lenq;
+  const int first_row = t.row0 + 32 * (w / SPLIT), row = first_row + (lane & 31);
   const bool live = row < lenq;
-  const int64_t at = t.lo + min((int64_t)row, lenq - 1);
+  const int64_t at = t.lo + min(row, lenq - 1);
   const E* kb = reinterpret_cast<const E*>(p.k) + klo * p.ks[0] + (int64_t)(h / p.G) * p.ks[1];
   const E* vb = reinterpret_cast<const E*>(p.v) + klo * p.vs[0] + (int64_t)(h / p.G) * p.vs[1];
   typename P::frag q[KS], dy[KS];
@@ -203,30 +260,29 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) dq[ct] = zero16();
 
-  const int64_t sees = min(lenk, t.row0 + BWD_ROWS + off);
-  const int ntiles = sees > 0 ? (int)((sees + BWD_TILE - 1) / BWD_TILE) : 0;
-  const int64_t wfirst = t.row0 + 32 * w + off, wlast = wfirst + 31;
+  const int sees = min(lenk, t.row0 + S::ROWS + off);
+  const int ntiles = sees > 0 ? (sees + KEYS - 1) / KEYS : 0;
+  const int wfirst = first_row + off, wlast = wfirst + 31;
+  const Stager<P, KEYS, 4> stage_k(p.ks[0], w, lane), stage_v(p.vs[0], w, lane);
   auto stage = [&](int j, unsigned char* to) {
-    const int64_t k0 = (int64_t)j * BWD_TILE;
-    const int last = (int)min(lenk - 1 - k0, (int64_t)BWD_TILE - 1);
-    stage_rows<P, BWD_TILE, 4>(kb + k0 * p.ks[0], p.ks[0], last, to, w, lane);
-    stage_rows<P, BWD_TILE, 4>(vb + k0 * p.vs[0], p.vs[0], last, to + TILE, w, lane);
+    const int k0 = j * KEYS, last = min(lenk - 1 - k0, KEYS - 1);
+    stage_k(kb + k0 * p.ks[0], last, to);
+    stage_v(vb + k0 * p.vs[0], last, to + TILE);
   };
   auto step = [&](int j, const unsigned char* __restrict kt, unsigned char* __restrict next) {
-    if (j + 1 < ntiles) stage(j + 1, next);
-    const int64_t k0 = (int64_t)j * BWD_TILE;
+    if (S::BUFS == 2 && j + 1 < ntiles) stage(j + 1, next);
     const unsigned char* vt = kt + TILE;
 #pragma unroll
-    for (int u = 0; u < BWD_TILE / 32; ++u) {
-      const int64_t j0 = k0 + 32 * u;
+    for (int u = 0; u < S::BLOCKS; ++u) {
+      const int r0 = 32 * (S::BLOCKS * part + u), j0 = j * KEYS + r0;  // the wave's keys of the tile
       if (j0 > wlast || j0 >= lenk) continue;
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = P::mma(s, P::row_frag(kt, 32 * u + (lane & 31), ks, half), q[ks]);
+      for (int ks = 0; ks < KS; ++ks) s = P::mma(s, P::row_frag(kt, r0 + (lane & 31), ks, half), q[ks]);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) dp = P::mma(dp, P::row_frag(vt, 32 * u + (lane & 31), ks, half), dy[ks]);
+      for (int ks = 0; ks < KS; ++ks) dp = P::mma(dp, P::row_frag(vt, r0 + (lane & 31), ks, half), dy[ks]);
       const bool whole = j0 + 31 <= wfirst;
-      const int limit = (int)min(max((int64_t)row + off - j0, (int64_t)-1), (int64_t)32);
+      const int limit = row + off - j0;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls)) * (dp[i] - de);
@@ -237,33 +293,87 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
       for (int m = 0; m < 2; ++m) {
         const typename P::frag df = P::from_acc(dp, m);
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) dq[ct] = P::mma(dq[ct], P::col_frag(kt, 32 * u + 16 * m, ct, lane), df);
+        for (int ct = 0; ct < CT; ++ct) dq[ct] = P::mma(dq[ct], P::col_frag(kt, r0 + 16 * m, ct, lane), df);
       }
     }
   };
-  if (ntiles > 0) stage(0, lds);
+  if (S::BUFS == 2 && ntiles > 0) stage(0, lds);
   for (int j = 0; j < ntiles; ++j) {
+    if (S::BUFS == 1) {
+      staged_barrier();
+      stage(j, lds);
+    }
     staged_barrier();
-    step(j, lds + (j & 1) * 2 * TILE, lds + (~j & 1) * 2 * TILE);
+    step(j, lds + (S::BUFS == 2 ? (j & 1) * 2 * TILE : 0), lds + (S::BUFS == 2 ? (~j & 1) * 2 * TILE : 0));
   }
   E* dst = reinterpret_cast<E*>(p.dq) + (t.lo + row) * p.dqs[0] + (int64_t)h * p.dqs[1];
+  if constexpr (SPLIT == 1) {
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) store_row32(dst + 32 * ct, dq[ct], p.scale, half, live);
+    for (int ct = 0; ct < CT; ++ct) store_row32(dst + 32 * ct, dq[ct], p.scale, half, live);
+  } else {
+    staged_barrier();
+    join_sums<SPLIT>(dq, p.scale, lds, w, lane, [&](int ct, const f32x16& x) { store_row32(dst + 32 * ct, x, 1.f, half, live); });
+  }
+}
+
+template <class P, int SPLIT>
+static int launch_dkdv(const AttnParams& p, hipStream_t st) {
+  const int64_t slots = p.total_k / Dkdv<P, SPLIT>::KEYS + p.nseq + 1, grid = slots * p.KV * p.subsets;
+  if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  const dim3 g((unsigned)grid), b(256);
+  if constexpr (P::D == 64) {
+    hipLaunchKernelGGL((attn_dkdv_kernel<P, SPLIT, true, true>), g, b, 0, st, p, slots);
+  } else {
+    hipLaunchKernelGGL((attn_dkdv_kernel<P, SPLIT, true, false>), g, b, 0, st, p, slots);
+    hipLaunchKernelGGL((attn_dkdv_kernel<P, SPLIT, false, true>), g, b, 0, st, p, slots);
+  }
+  if (p.subsets > 1) {
+    const int64_t blocks = (p.total_k * p.KV * (P::D / 4) + 255) / 256;
+    if (blocks > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(attn_subsets_kernel<P>, dim3((unsigned)blocks), b, 0, st, p);
+  }
+  return launch_status();
+}
+
+template <class P, int SPLIT>
+static int launch_dq(const AttnParams& p, hipStream_t st) {
+  const int64_t slots = p.total_q / Dq<P, SPLIT>::ROWS + p.nseq + 1, grid = slots * p.H;
+  if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((attn_dq_kernel<P, SPLIT>), dim3((unsigned)grid), dim3(256), 0, st, p, slots);
+  return launch_status();
 }
 
 template <class P>
 static int launch_bwd(const AttnParams& p, float* delta, hipStream_t st) {
-  const int64_t rows = p.total_q * p.H;
-  const int64_t kslots = p.total_k / BWD_ROWS + p.nseq + 1, qslots = p.total_q / BWD_ROWS + p.nseq + 1;
-  if ((rows + 15) / 16 > INT32_MAX || kslots * p.KV > INT32_MAX || qslots * p.H > INT32_MAX) return KDN_ERR_UNSUPPORTED;
-  if (p.total_q > 0)
+  int rc = KDN_OK;
+  if (p.total_q > 0) {
+    const int64_t rows = p.total_q * p.H;
+    if ((rows + 15) / 16 > INT32_MAX) return KDN_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(attn_delta_kernel<P>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, p, delta);
-  if (p.total_k > 0)
-    hipLaunchKernelGGL(attn_dkdv_kernel<P>, dim3((unsigned)(kslots * p.KV)), dim3(256), 0, st, p, kslots);
-  if (p.total_q > 0)
-    hipLaunchKernelGGL(attn_dq_kernel<P>, dim3((unsigned)(qslots * p.H)), dim3(256), 0, st, p, qslots);
-  return launch_status();
+    if ((rc = launch_status()) != KDN_OK) return rc;
+  }
+  if (p.total_k > 0) {
+    const int split = attn_split(p.total_k, (int64_t)p.KV * p.subsets);
+    rc = split == 4 ? launch_dkdv<P, 4>(p, st) : split == 2 ? launch_dkdv<P, 2>(p, st) : launch_dkdv<P, 1>(p, st);
+  }
+  if (rc == KDN_OK && p.total_q > 0) {
+    const int split = attn_split(p.total_q, p.H);
+    rc = split == 4 ? launch_dq<P, 4>(p, st) : split == 2 ? launch_dq<P, 2>(p, st) : launch_dq<P, 1>(p, st);
+  }
+  return rc;
 }
+
+// Subsets of the query heads that share a key head whose dk and dv are summed apart: as many as it takes to have four
+// workgroups of 128 keys for each CU (two run there at a time, and the first keys have twice the average's work).
+static int bwd_subsets(const kdn_attn_args* f) {
+  const int G = (int)(f->H / f->H_kv);
+  const int64_t tiles = f->total_k / 128 * f->H_kv;
+  int n = 1;
+  while (n < G && (tiles * n < 1024 || G % n != 0)) ++n;
+  return n;
+}
+static size_t bwd_delta_bytes(const kdn_attn_args* f) { return ((size_t)f->H * (size_t)f->total_q * 4 + 255) / 256 * 256 + 256; }
+static size_t bwd_part_bytes(const kdn_attn_args* f) { return (size_t)f->total_k * (size_t)f->H_kv * (size_t)f->d * 4; }
 
 }  // namespace kdn
 
@@ -271,8 +381,8 @@ using namespace kdn;
 
 extern "C" size_t kdn_attn_bwd_workspace_bytes(const kdn_attn_bwd_args* a) {
   if (!a || attn_check(a->fwd) != KDN_OK) return 0;
-  const size_t bytes = (size_t)a->fwd->H * (size_t)a->fwd->total_q * 4;
-  return bytes < 16 ? 16 : bytes;
+  const int subsets = bwd_subsets(a->fwd);
+  return bwd_delta_bytes(a->fwd) + (subsets > 1 ? 2 * subsets * bwd_part_bytes(a->fwd) : 0);
 }
 
 extern "C" int kdn_attn_bwd(const kdn_attn_bwd_args* a, void* stream) {
@@ -283,7 +393,7 @@ extern "C" int kdn_attn_bwd(const kdn_attn_bwd_args* a, void* stream) {
   if (f->total_q == 0 && f->total_k == 0) return KDN_OK;
   if (f->total_q > 0) {
     if ((rc = attn_check_tensors(f)) != KDN_OK) return rc;
-    if (!f->lse || !a->dy || !a->dq || !a->workspace) return KDN_ERR_INVALID_ARGUMENT;
+    if (!f->lse || !a->dy || !a->dq) return KDN_ERR_INVALID_ARGUMENT;
   }
   if (!f->cu_q || (f->total_k > 0 && (!f->k || !f->v || !a->dk || !a->dv))) return KDN_ERR_INVALID_ARGUMENT;
   if (!aligned(a->dy, 16) || !aligned(a->dq, 16) || !aligned(a->dk, 16) || !aligned(a->dv, 16) || !aligned(a->workspace, 16) ||
@@ -291,10 +401,14 @@ extern "C" int kdn_attn_bwd(const kdn_attn_bwd_args* a, void* stream) {
       !attn_strides_ok(a->dk_stride, f->dtype) || !attn_strides_ok(a->dv_stride, f->dtype) ||
       !attn_strides_ok(f->k_stride, f->dtype) || !attn_strides_ok(f->v_stride, f->dtype) || !aligned(f->k, 16) || !aligned(f->v, 16))
     return KDN_ERR_MISALIGNED;
-  if (f->total_q > 0 && a->workspace_bytes < kdn_attn_bwd_workspace_bytes(a)) return KDN_ERR_WORKSPACE_TOO_SMALL;
+  if (!stage_reach(a->dy_stride[0], f->dtype)) return KDN_ERR_UNSUPPORTED;
+  if (!a->workspace || a->workspace_bytes < kdn_attn_bwd_workspace_bytes(a)) return KDN_ERR_WORKSPACE_TOO_SMALL;
   AttnParams p = attn_params(f);
   p.dy = a->dy; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
   p.delta = reinterpret_cast<const float*>(a->workspace);
+  p.subsets = bwd_subsets(f);
+  p.part_dk = reinterpret_cast<float*>((unsigned char*)a->workspace + bwd_delta_bytes(f));
+  p.part_dv = p.part_dk + (size_t)p.subsets * bwd_part_bytes(f) / 4;
   for (int i = 0; i < 2; ++i) {
     p.dys[i] = a->dy_stride[i]; p.dqs[i] = a->dq_stride[i]; p.dks[i] = a->dk_stride[i]; p.dvs[i] = a->dv_stride[i];
   }

@@ -114,22 +114,42 @@ struct AttnF32 {
   }
 };
 
-// The copy of `ROWS` rows of D elements, row r at base + min(r, last) * stride, into an LDS tile by the load unit itself
-// (16 bytes a lane, 1 KB an instruction, nothing in registers): the WAVES waves of a workgroup share it.  The rows past
-// `last` repeat it, so that every address is inside the tensor and every value one that is there.
+// The copy of ROWS rows of D elements into an LDS tile by the load unit itself (16 bytes a lane, 1 KB an instruction,
+// nothing in registers): the WAVES waves of a workgroup share it.  The first row's address is the same in all lanes, a lane's
+// offset from it the same for every tile, so that a whole tile's copies take no vector arithmetic.  (With each lane's own
+// 64-bit address formed for each copy, the multiplications were a fifth of the forward's vector cycles.)  Rows past `last`
+// repeat it, so that every address is inside the tensor and every value one that is there.
 template <class P, int ROWS, int WAVES>
-__device__ __forceinline__ void stage_rows(const typename P::elem* base, int64_t stride, int last, unsigned char* tile,
-                                           int wave, int lane) {
-  constexpr int N = ROWS * P::PIECES / 64;
+struct Stager {
+  static constexpr int RPI = 64 / P::PIECES, N = ROWS * P::PIECES / 64 / WAVES, STEP = WAVES * RPI, NV = STEP >= 16 ? 1 : 16 / STEP;
+  static_assert(N * WAVES * RPI == ROWS, "the waves share the copies evenly");
+  uint32_t row_bytes, off[NV];
+  int wave, lane;
+  __device__ __forceinline__ Stager(int64_t stride, int wave_, int lane_) : wave(wave_), lane(lane_) {
+    row_bytes = (uint32_t)(stride * (int64_t)sizeof(typename P::elem));
 #pragma unroll
-  for (int i = 0; i < N / WAVES; ++i) {
-    const int at = (i * WAVES + wave) * 64 + lane, row = at / P::PIECES;
-    const int piece = (at % P::PIECES) ^ piece_swizzle<P::PIECES>(row);
-    const typename P::elem* src = base + (int64_t)min(row, last) * stride + piece * (16 / (int)sizeof(typename P::elem));
-    __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(src),
-                                     (__attribute__((address_space(3))) void*)(tile + (i * WAVES + wave) * 1024), 16, 0, 0);
+    for (int v = 0; v < NV; ++v) off[v] = (uint32_t)(wave * RPI + lane / P::PIECES) * row_bytes + 16 * piece(v);
   }
-}
+  __device__ __forceinline__ int piece(int i) const {
+    return (lane % P::PIECES) ^ piece_swizzle<P::PIECES>(i * STEP + wave * RPI + lane / P::PIECES);
+  }
+  __device__ __forceinline__ static void copy(const unsigned char* from, unsigned char* to) {
+    __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(from), (__attribute__((address_space(3))) void*)(to), 16, 0, 0);
+  }
+  __device__ __forceinline__ void operator()(const typename P::elem* first, int last, unsigned char* tile) const {
+    const unsigned char* base = reinterpret_cast<const unsigned char*>(first);
+    if (last >= ROWS - 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) copy(base + (uint64_t)(i * STEP) * row_bytes + off[i % NV], tile + (i * WAVES + wave) * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        copy(base + ((uint32_t)min(i * STEP + wave * RPI + lane / P::PIECES, last) * row_bytes + 16 * piece(i % NV)), tile + (i * WAVES + wave) * 1024);
+    }
+  }
+};
+// Strides that a copy's 32-bit offsets reach over.
+inline bool stage_reach(int64_t stride, int dtype) { return stride <= INT32_MAX / (64 * (int64_t)dtype_size(dtype)); }
 
 // This wave's staged copies have arrived; after the barrier, every wave's have, and every wave has read the tile that the
 // next copies overwrite.
@@ -181,14 +201,50 @@ __device__ __forceinline__ void store_row32(float* row, const f32x16& v, float f
   }
 }
 
+// The waves of a workgroup that share rows (SPLIT of them; the workgroup's four waves are 4 / SPLIT groups) add their sums
+// in the waves' order: each wave puts the column tiles it does not finish into LDS, as they lie in its registers, and adds
+// the others' to those it does (column tile ct is finished by wave ct % SPLIT).  `mine` scales a wave's own sums first.
+// `ends` runs for the tiles that the wave finishes.  4 KB of LDS a wave and column tile; ends with all waves having read.
+template <int SPLIT, int CT, class F>
+__device__ __forceinline__ void join_sums(f32x16 (&o)[CT], float mine, unsigned char* lds, int w, int lane, F ends) {
+  const int part = w % SPLIT, group = w / SPLIT;
+  f32x4* box = reinterpret_cast<f32x4*>(lds) + lane;
+  auto at = [&](int ct, int from) { return (((group * CT + ct) * SPLIT + from) * 4) * 64; };
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[ct][i] *= mine;
+    if (ct % SPLIT != part)
+#pragma unroll
+      for (int a = 0; a < 4; ++a) box[at(ct, part) + 64 * a] = f32x4{o[ct][4 * a], o[ct][4 * a + 1], o[ct][4 * a + 2], o[ct][4 * a + 3]};
+  }
+  __syncthreads();
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+    if (ct % SPLIT == part) {
+      f32x16 sum = zero16();
+#pragma unroll
+      for (int from = 0; from < SPLIT; ++from)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const f32x4 x = from == ct % SPLIT ? f32x4{o[ct][4 * a], o[ct][4 * a + 1], o[ct][4 * a + 2], o[ct][4 * a + 3]} : box[at(ct, from) + 64 * a];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) sum[4 * a + y] += x[y];
+        }
+      ends(ct, sum);
+    }
+  __syncthreads();
+}
+
 // Tile slots over a packed batch: sequence b has the slots [cu[b] / ROWS + b, cu[b + 1] / ROWS + b + 1), at least as many
 // as it has tiles of ROWS rows, so that a grid of total / ROWS + sequences slots covers every batch without its lengths
 // being known to the host.  The rows past the last sequence's end (a batch padded to a fixed size) are one sequence more,
 // number nseq, that sees nothing and that nothing sees.  The sequence of a slot is found 64 offsets at a time by the whole
 // wave.  Offsets are clamped to the tensor: a wrong one gives wrong rows, never an access outside.
 struct SeqTile {
-  int seq, row0;    // row0: first row of the tile in the sequence; negative: no tile
-  int64_t lo, len;  // the sequence's first row and length
+  int seq, row0;  // row0: first row of the tile in the sequence; negative: no tile
+  int64_t lo;     // the sequence's first row
+  int len;        // and length
 };
 __device__ __forceinline__ int64_t seq_start(const int64_t* cu, int64_t total, int64_t b) {
   return min(max(cu[b], (int64_t)0), total);
@@ -207,27 +263,30 @@ __device__ __forceinline__ SeqTile find_tile(const int64_t* cu, int64_t nseq, in
   SeqTile t;
   t.seq = (int)lo;
   t.lo = seq_start(cu, total, lo);
-  t.len = (lo < nseq ? max(seq_start(cu, total, lo + 1), t.lo) : total) - t.lo;
+  t.len = (int)((lo < nseq ? max(seq_start(cu, total, lo + 1), t.lo) : total) - t.lo);
   const int64_t tile = slot - (t.lo / ROWS + lo);
   t.row0 = tile < 0 || tile * ROWS >= t.len ? -1 : (int)(tile * ROWS);
   return t;
 }
 // The other tensor's rows of a tile's sequence: none for the rows past the last one.
-__device__ __forceinline__ void other_rows(const int64_t* cu, int64_t nseq, int64_t total, int seq, int64_t& lo, int64_t& len) {
+__device__ __forceinline__ void other_rows(const int64_t* cu, int64_t nseq, int64_t total, int seq, int64_t& lo, int& len) {
   lo = seq < nseq ? seq_start(cu, total, seq) : 0;
-  len = seq < nseq ? max(seq_start(cu, total, seq + 1), lo) - lo : 0;
+  len = seq < nseq ? (int)(max(seq_start(cu, total, seq + 1), lo) - lo) : 0;
 }
 
 // Device-side arguments of the attention kernels (kdn_attn_args with the defaults filled in).
 struct AttnParams {
   const void *q, *k, *v, *y, *dy;
   void *out, *dq, *dk, *dv;
+  void* low;           // what rounding took from y, or NULL
+  int64_t lows[2];
   int64_t qs[2], ks[2], vs[2], ys[2], dys[2], dqs[2], dks[2], dvs[2];  // element strides [token][head]
   float* lse;          // [H][total_q]
   const float* delta;  // [H][total_q]: dy . y of each row (backward)
   const int64_t *cu_q, *cu_k;
   int64_t nseq, total_q, total_k;
-  int H, KV, G;
+  float *part_dk, *part_dv;  // [subset][total_k][KV][D] sums of dk and dv over a subset of a key head's query heads (subsets > 1)
+  int H, KV, G, subsets;
   float scale;
 };
 
@@ -235,5 +294,6 @@ int attn_check(const kdn_attn_args* a);          // sizes
 int attn_check_tensors(const kdn_attn_args* a);  // pointers, strides, alignment
 bool attn_strides_ok(const int64_t s[2], int dtype);
 AttnParams attn_params(const kdn_attn_args* a);
+int attn_split(int64_t rows, int64_t heads);     // waves that share 32 rows
 
 }  // namespace kdn

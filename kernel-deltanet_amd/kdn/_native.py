@@ -210,6 +210,7 @@ class AttnArgs(ctypes.Structure):
         ("v", ctypes.c_void_p), ("v_stride", _i64x2),
         ("y", ctypes.c_void_p), ("y_stride", _i64x2),
         ("lse", ctypes.c_void_p),
+        ("y_low", ctypes.c_void_p), ("y_low_stride", _i64x2),
     ]
 
 

@@ -176,7 +176,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
 # ------------------------------------------------------------------------------------------------- prompt attention
 
 
-def _attn_args(q, k, v, cu_q, cu_k, scale, y, lse) -> N.AttnArgs:
+def _attn_args(q, k, v, cu_q, cu_k, scale, y, lse, low=None) -> N.AttnArgs:
     a = N.AttnArgs()
     a.num_seqs, a.total_q, a.total_k = cu_q.shape[0] - 1, q.shape[0], k.shape[0]
     a.H, a.H_kv, a.d, a.dtype, a.scale = q.shape[1], k.shape[1], q.shape[2], _tag(q.dtype, "attention"), scale
@@ -184,6 +184,8 @@ def _attn_args(q, k, v, cu_q, cu_k, scale, y, lse) -> N.AttnArgs:
     for name, t in (("q", q), ("k", k), ("v", v), ("y", y)):
         _set(a, name, t)
     a.lse = None if lse is None else lse.data_ptr()
+    if low is not None:
+        _set(a, "y_low", low)
     return a
 
 
@@ -201,27 +203,35 @@ def _attn_inputs(q, k, v, cu_q, cu_k):
 
 
 def attention_forward(q, k, v, cu_seqlens, cu_seqlens_k=None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
-                      return_lse: bool = False):
-    """`attention` without autograd: y, or (y, lse (H, tokens) float32)."""
+                      return_lse: bool = False, return_low: bool = False):
+    """`attention` without autograd: y; or with return_lse (y, lse (H, tokens) float32); or with return_low too (y, lse, low),
+    low what rounding took from y (None in float32), which makes the gradients' dy . y exact."""
     q, k, v, cu_q, cu_k = _attn_inputs(q, k, v, cu_seqlens, cu_seqlens_k)
     y = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else _out(out, "attention out", q.shape, q)
     lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device) if return_lse else None
-    a = _attn_args(q, k, v, cu_q, cu_k, _scale(scale, q.shape[-1], "attention"), y, lse)
+    low = torch.empty(q.shape, dtype=q.dtype, device=q.device) if return_low and q.dtype is torch.bfloat16 else None
+    a = _attn_args(q, k, v, cu_q, cu_k, _scale(scale, q.shape[-1], "attention"), y, lse, low)
     with _on(q.device):
         N.check(N.lib().kdn_attn_fwd(_ref(a), _stream(q.device)), "kdn_attn_fwd")
-    return (y, lse) if return_lse else y
+    return (y, lse, low) if return_low else (y, lse) if return_lse else y
 
 
-def attention_backward(q, k, v, y, lse, dy, cu_seqlens, cu_seqlens_k=None, scale: Optional[float] = None):
-    """(dq, dk, dv) of `attention_forward`'s y and lse for dL/dy, in the inputs' dtype, the same bits every time."""
+def attention_backward(q, k, v, y, lse, dy, cu_seqlens, cu_seqlens_k=None, scale: Optional[float] = None,
+                       low: Optional[torch.Tensor] = None):
+    """(dq, dk, dv) of `attention_forward`'s y, lse and low (optional) for dL/dy, in the inputs' dtype, the same bits every
+    time."""
     q, k, v, cu_q, cu_k = _attn_inputs(q, k, v, cu_seqlens, cu_seqlens_k)
     y, dy = _heads(y, "attention y", q), _heads(dy, "attention dy", q)
     if y.shape != q.shape or dy.shape != q.shape or tuple(lse.shape) != (q.shape[1], q.shape[0]) or lse.dtype != torch.float32 or \
             lse.device != q.device:
         raise ValueError(f"attention backward: y and dy have q's shape {tuple(q.shape)}, lse is (H, tokens) float32 on {q.device}")
     lse = lse.contiguous()
+    if low is not None:
+        low = _heads(low, "attention low", q)
+        if low.shape != q.shape:
+            raise ValueError(f"attention backward: low has q's shape {tuple(q.shape)}")
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    f = _attn_args(q, k, v, cu_q, cu_k, _scale(scale, q.shape[-1], "attention"), y, lse)
+    f = _attn_args(q, k, v, cu_q, cu_k, _scale(scale, q.shape[-1], "attention"), y, lse, low)
     a = N.AttnBwdArgs()
     a.fwd = ctypes.addressof(f)
     for name, t in (("dy", dy), ("dq", dq), ("dk", dk), ("dv", dv)):
@@ -237,15 +247,15 @@ def attention_backward(q, k, v, y, lse, dy, cu_seqlens, cu_seqlens_k=None, scale
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, scale):
-        y, lse = attention_forward(q, k, v, cu_q, cu_k, scale, return_lse=True)
-        ctx.save_for_backward(q, k, v, y, lse, cu_q, cu_k)
+        y, lse, low = attention_forward(q, k, v, cu_q, cu_k, scale, return_lse=True, return_low=True)
+        ctx.save_for_backward(q, k, v, y, lse, cu_q, cu_k, low)
         ctx.scale = scale
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        q, k, v, y, lse, cu_q, cu_k = ctx.saved_tensors
-        return (*attention_backward(q, k, v, y, lse, dy, cu_q, cu_k, ctx.scale), None, None, None)
+        q, k, v, y, lse, cu_q, cu_k, low = ctx.saved_tensors
+        return (*attention_backward(q, k, v, y, lse, dy, cu_q, cu_k, ctx.scale, low), None, None, None)
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,

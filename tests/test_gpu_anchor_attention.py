@@ -36,12 +36,12 @@ def close(got, want, bound, f, what):
     assert float(over.max() if over.numel() else 0) <= 0, (what, float(((got - want).abs() / slack).max()))
 
 
-def check(lens_q, lens_k=None, H=4, KV=2, d=64, dtype=torch.bfloat16, spread=1.0, scale=None, seed=0):
+def check(lens_q, lens_k=None, H=4, KV=2, d=64, dtype=torch.bfloat16, spread=1.0, scale=None, seed=0, low=True):
     q, k, v, dy, cq, ck = make(lens_q, lens_q if lens_k is None else lens_k, H, KV, d, dtype, seed, spread)
     dev = [t.to(DEV) for t in (q, k, v, dy, cq, ck)]
     cks = None if lens_k is None else dev[5]
-    y, lse = anchor.attention_forward(*dev[:3], dev[4], cks, scale, return_lse=True)
-    dq, dk, dv = anchor.attention_backward(*dev[:3], y, lse, dev[3], dev[4], cks, scale)
+    y, lse, rest = anchor.attention_forward(*dev[:3], dev[4], cks, scale, return_lse=True, return_low=True)
+    dq, dk, dv = anchor.attention_backward(*dev[:3], y, lse, dev[3], dev[4], cks, scale, rest if low else None)
     want = oa.attention(q, k, v, cq, None if lens_k is None else ck, scale, dy)
     n = max([1, *lens_q]) * (H // KV) + max([1, *(lens_k or lens_q)])
     f = unit(dtype, d, n, want["most"])
@@ -85,6 +85,15 @@ def test_many_short_sequences():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [60, 115])
+def test_enough_rows_for_fewer_waves_a_row(n, d, dtype):
+    """8700 and 17000 rows of 4 heads: two waves a row, and one (the others here have too few rows for that)."""
+    check([(37 * i) % 301 for i in range(n)], H=4, KV=4, d=d, dtype=dtype)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("d", [64, 128])
 def test_longer(d):
     check([1111], H=2, KV=1, d=d)
@@ -100,6 +109,24 @@ def test_wide_scores(dtype):
 @pytest.mark.gpu
 def test_scale():
     check([100], scale=0.5)
+
+
+@pytest.mark.gpu
+def test_without_the_low_part():
+    check([100, 3], low=False)
+
+
+@pytest.mark.gpu
+def test_low_part():
+    """y and its low part together are the unrounded result, to the low part's own rounding, 2^-16 of y: what is left is the
+    weights' rounding, 2^-8 sum p |v|."""
+    q, k, v, dy, cu, _ = make([90], [90], 4, 2, 64, torch.bfloat16)
+    y, lse, low = anchor.attention_forward(*(t.to(DEV) for t in (q, k, v)), cu.to(DEV), return_lse=True, return_low=True)
+    assert float((low.float().abs() - 2.0 ** -8 * y.float().abs()).max()) <= 0
+    want = oa.attention(q, k, v, cu)
+    off = (y.double() + low.double()).cpu() - want["y"]
+    assert float((off.abs() - (2.0 ** -8 + 2.0 ** -18) * want["bounds"]["y"] - 2.0 ** -15 * want["y"].abs()).max()) <= 0
+    assert anchor.attention_forward(*(t.float().to(DEV) for t in (q, k, v)), cu.to(DEV), return_lse=True, return_low=True)[2] is None
 
 
 @pytest.mark.gpu
@@ -187,8 +214,8 @@ def test_autograd_and_uniform_batches():
     y.backward(dy)
     cu = torch.arange(0, 4 * 45, 45, device=DEV)
     flat = [t.detach().reshape(-1, *t.shape[2:]) for t in (q, k, v)]
-    y2, lse = anchor.attention_forward(*flat, cu.int(), return_lse=True)
-    grads = anchor.attention_backward(*flat, y2, lse, dy.reshape(y2.shape), cu)
+    y2, lse, low = anchor.attention_forward(*flat, cu.int(), return_lse=True, return_low=True)
+    grads = anchor.attention_backward(*flat, y2, lse, dy.reshape(y2.shape), cu, low=low)
     assert torch.equal(y.detach().reshape(y2.shape), y2)
     for t, want in zip((q, k, v), grads):
         assert torch.equal(t.grad.reshape(want.shape), want)

@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int b = 0; b < S::BLOCKS; ++b) s[b] = P::mma(s[b], P::row_frag(kt, r0 + 32 * b + (lane & 31), ks, half), q[ks]);
+    sched_products<P, KS * S::BLOCKS, P::ROW_READS>();
     if (k0 + 32 * S::BLOCKS - 1 > wfirst) {
       const int limit = row + off - k0;
 #pragma unroll
@@ -129,6 +130,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, r0 + 16 * kk, ct, lane), pf);
     }
+    sched_products<P, 2 * S::BLOCKS * CT, P::COL_READS>();
   };
   if (S::BUFS == 2 && ntiles > 0) stage(0, lds);
   for (int j = 0; j < ntiles; ++j) {
@@ -207,7 +209,7 @@ int attn_check_tensors(const kdn_attn_args* a) {
 
 int attn_split(int64_t rows, int64_t heads) {
   const int64_t tiles = rows / 128 * heads;
-  return tiles < 256 ? 4 : tiles < 512 ? 2 : 1;
+  return tiles < 512 ? 4 : tiles < 1024 ? 2 : 1;
 }
 
 AttnParams attn_params(const kdn_attn_args* a) {

@@ -105,11 +105,9 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
     const int h = e * p.G + sub * heads + j / per, r0 = q0 + j % per * ROWS, last = min(lenq - 1 - r0, ROWS - 1);
     stage_q(reinterpret_cast<const E*>(p.q) + (qlo + r0) * p.qs[0] + (int64_t)h * p.qs[1], last, to);
     stage_y(reinterpret_cast<const E*>(p.dy) + (qlo + r0) * p.dys[0] + (int64_t)h * p.dys[1], last, to + TILE);
-    const int x = 64 * w + lane;  // lse of the rows, then delta
-    if (64 * w < 2 * ROWS) {
-      const float* src = (x < ROWS ? p.lse : p.delta) + (int64_t)h * p.total_q + qlo + r0 + min(x % ROWS, last);
-      __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(src),
-                                       (__attribute__((address_space(3))) void*)(to + 2 * TILE + 256 * w), 4, 0, 0);
+    if (64 * w < 2 * ROWS) {  // lse of the rows, then delta, 64 a wave
+      const float* src = (64 * w < ROWS ? p.lse : p.delta) + (int64_t)h * p.total_q + qlo + r0;
+      copy4_to_lds(buffer_at(src), 4 * min(64 * w % ROWS + lane, last), to + 2 * TILE + 256 * w);
     }
   };
   // as in the forward: the next tile's copies and this one's reads do not overlap
@@ -123,9 +121,11 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) s = P::mma(s, P::row_frag(qt, tr + (lane & 31), ks, half), k[ks]);
+      if constexpr (!DK) sched_products<P, KS, P::ROW_READS>();
       if constexpr (DK) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) dp = P::mma(dp, P::row_frag(yt, tr + (lane & 31), ks, half), v[ks]);
+        sched_products<P, 2 * KS, P::ROW_READS>();
       }
       const bool whole = i0 + off >= first_key + 31 && i0 + 32 <= lenq;
       const int lo = max(key - off, 0) - i0, hi = lenq - i0;  // rows lo .. hi - 1 of the block see the key
@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
           if constexpr (DK) dk[ct] = P::mma(dk[ct], P::col_frag(qt, tr + 16 * m, ct, lane), df);
         }
       }
+      sched_products<P, 2 * CT * (DV + DK), P::COL_READS>();
     }
   };
   if (S::BUFS == 2 && ntiles > 0) stage(0, lds);
@@ -281,6 +282,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
       for (int ks = 0; ks < KS; ++ks) s = P::mma(s, P::row_frag(kt, r0 + (lane & 31), ks, half), q[ks]);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) dp = P::mma(dp, P::row_frag(vt, r0 + (lane & 31), ks, half), dy[ks]);
+      sched_products<P, 2 * KS, P::ROW_READS>();
       const bool whole = j0 + 31 <= wfirst;
       const int limit = row + off - j0;
 #pragma unroll
@@ -295,6 +297,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) dq[ct] = P::mma(dq[ct], P::col_frag(kt, r0 + 16 * m, ct, lane), df);
       }
+      sched_products<P, 2 * CT, P::COL_READS>();
     }
   };
   if (S::BUFS == 2 && ntiles > 0) stage(0, lds);

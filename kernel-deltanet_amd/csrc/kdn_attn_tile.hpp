@@ -47,6 +47,7 @@ struct AttnBF16 {
   typedef __bf16 elem;
   typedef bf16x8 frag;
   static constexpr int D = D_, ROW = 2 * D, PIECES = ROW / 16;
+  static constexpr int MFMAS = 1, ROW_READS = 1, COL_READS = 2, AHEAD = 4;  // of a product; operands read ahead
   __device__ __forceinline__ static f32x16 mma(const f32x16& acc, const frag& a, const frag& b) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
   }
@@ -82,6 +83,7 @@ struct AttnF32 {
   typedef float elem;
   typedef f32x8 frag;
   static constexpr int D = D_, ROW = 4 * D, PIECES = ROW / 16;
+  static constexpr int MFMAS = 8, ROW_READS = 2, COL_READS = 8, AHEAD = 2;
   __device__ __forceinline__ static f32x16 mma(f32x16 acc, const frag& a, const frag& b) {
 #pragma unroll
     for (int s = 0; s < 8; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s], b[s], acc, 0, 0, 0);
@@ -114,6 +116,23 @@ struct AttnF32 {
   }
 };
 
+// A copy by the load unit from memory to LDS, 16 or 4 bytes a lane: from the buffer's start + lane_off + off to `to`, the
+// lanes one after another.
+// The buffer form of it: the compiler takes the global one for an access that may be to either memory, and waits for all
+// of a wave's LDS reads wherever it needs one while such a copy is on its way.
+// `start` is the same in all lanes: said to the compiler, which goes through the lanes' values one by one otherwise.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* start) {
+  const uint64_t at = reinterpret_cast<uint64_t>(start);
+  const uint64_t one = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(one), 0, -1, 0x00027000);  // raw bytes, no bound of its own
+}
+__device__ __forceinline__ void copy16_to_lds(__amdgpu_buffer_rsrc_t from, uint32_t lane_off, uint32_t off, unsigned char* to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)(to), 16, (int)lane_off, (int)off, 0, 0);
+}
+__device__ __forceinline__ void copy4_to_lds(__amdgpu_buffer_rsrc_t from, uint32_t lane_off, unsigned char* to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)(to), 4, (int)lane_off, 0, 0, 0);
+}
+
 // The copy of ROWS rows of D elements into an LDS tile by the load unit itself (16 bytes a lane, 1 KB an instruction,
 // nothing in registers): the WAVES waves of a workgroup share it.  The first row's address is the same in all lanes, a lane's
 // offset from it the same for every tile, so that a whole tile's copies take no vector arithmetic.  (With each lane's own
@@ -133,27 +152,43 @@ struct Stager {
   __device__ __forceinline__ int piece(int i) const {
     return (lane % P::PIECES) ^ piece_swizzle<P::PIECES>(i * STEP + wave * RPI + lane / P::PIECES);
   }
-  __device__ __forceinline__ static void copy(const unsigned char* from, unsigned char* to) {
-    __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(from), (__attribute__((address_space(3))) void*)(to), 16, 0, 0);
-  }
   __device__ __forceinline__ void operator()(const typename P::elem* first, int last, unsigned char* tile) const {
-    const unsigned char* base = reinterpret_cast<const unsigned char*>(first);
+    const __amdgpu_buffer_rsrc_t rows = buffer_at(first);
     if (last >= ROWS - 1) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) copy(base + (uint64_t)(i * STEP) * row_bytes + off[i % NV], tile + (i * WAVES + wave) * 1024);
+      for (int i = 0; i < N; ++i) copy16_to_lds(rows, off[i % NV], i * STEP * row_bytes, tile + (i * WAVES + wave) * 1024);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        copy(base + ((uint32_t)min(i * STEP + wave * RPI + lane / P::PIECES, last) * row_bytes + 16 * piece(i % NV)), tile + (i * WAVES + wave) * 1024);
+        copy16_to_lds(rows, (uint32_t)min(i * STEP + wave * RPI + lane / P::PIECES, last) * row_bytes + 16 * piece(i % NV), 0,
+                        tile + (i * WAVES + wave) * 1024);
     }
   }
 };
 // Strides that a copy's 32-bit offsets reach over.
 inline bool stage_reach(int64_t stride, int dtype) { return stride <= INT32_MAX / (64 * (int64_t)dtype_size(dtype)); }
 
-// This wave's staged copies have arrived; after the barrier, every wave's have, and every wave has read the tile that the
-// next copies overwrite.
-__device__ __forceinline__ void staged_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// All but this wave's last N copies have arrived; after the barrier, so have every wave's, and every wave has read the tile
+// that the next copies overwrite.
+template <int N = 0>
+__device__ __forceinline__ void staged_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// The order of N products and of the LDS reads of their operands (READS each) in the instructions around this: the first
+// AHEAD operands, then a product and the operand of the one AHEAD after it, in turn.  Left to itself the compiler keeps one
+// operand's registers and waits for LDS, 100 cycles and more, before each product of 32.
+template <class P, int N, int READS>
+__device__ __forceinline__ void sched_products() {
+  constexpr int AHEAD = N < P::AHEAD ? N : P::AHEAD;
+  __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * READS, 0);
+#pragma unroll
+  for (int i = 0; i < N - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, P::MFMAS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * P::MFMAS, 0);
+}
 
 // The values of lanes l % 32 and l % 32 + 32, in both.  (The elements are copied out before they are cast: a bit cast of an
 // element of the builtin's result takes element 0 whichever it names.)

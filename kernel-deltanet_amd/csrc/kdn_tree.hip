@@ -26,22 +26,67 @@ struct TreeParams {
   float scale;
 };
 
-// What a workgroup works on.
+// What a workgroup works on: chunk `ch` of sequence b.
 struct TreeWork {
   int64_t lo;          // first new token
   int n, c0, c1;       // new tokens; the chunk's keys
   int chunks, ctx;     // chunks of the sequence; its context
+  int b, ch;           // b negative: nothing
 };
 
-__device__ __forceinline__ TreeWork tree_work(const TreeParams& p, int b, int ch) {
+__device__ __forceinline__ TreeWork tree_seq(const TreeParams& p, int b) {
   TreeWork t;
   t.lo = min(max(p.cu[b], (int64_t)0), p.total);
   t.n = (int)min(min(max(p.cu[b + 1], t.lo), p.total) - t.lo, (int64_t)p.max_new);
   t.ctx = (int)min((int64_t)max(p.lens[b], 0), p.max_context);
-  t.chunks = max(1, (t.ctx + p.chunk - 1) / p.chunk);
-  t.c0 = ch * p.chunk;
-  t.c1 = min(t.c0 + p.chunk, t.ctx);
+  t.chunks = t.n > 0 ? max(1, (t.ctx + p.chunk - 1) / p.chunk) : 0;
   return t;
+}
+
+// Lane `at`'s value (`at` the same in all lanes), as a scalar.
+__device__ __forceinline__ int lane_value(int v, int at) { return __builtin_amdgcn_readlane(v, __builtin_amdgcn_readfirstlane(at)); }
+
+// The u-th chunk of all the sequences' chunks, one sequence's after another's.  The grid is sized from the longest context
+// that the host allows for; the chunks that are there come first in it and the rest of the grid ends at once.  (Numbered by
+// sequence and place, the workgroups without a chunk came between the others, each holding a CU for its start: 16 trees
+// over 6000 tokens took 244 us, the CUs two thirds busy.)  Every lane counts the chunks of its share of the sequences, 64
+// shares make a prefix sum, and the share that has chunk u is looked through in the same way.
+__device__ __forceinline__ TreeWork tree_work(const TreeParams& p, int u, int lane) {
+  TreeWork mine = {};
+  int first = 0, n = p.nseq;  // the sequences still in question
+  for (;;) {
+    const int share = (n + 63) / 64, begin = first + min(lane * share, n), end = first + min(lane * share + share, n);
+    int count = 0;
+    for (int b = begin; b < end; ++b) {
+      mine = tree_seq(p, b);
+      count += mine.chunks;
+    }
+    int upto = count;
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) {
+      const int x = __shfl_up(upto, s);
+      if (lane >= s) upto += x;
+    }
+    const int at = __popcll(__ballot(upto <= u));  // shares that lie wholly before chunk u
+    if (at == 64) {
+      mine.b = -1;
+      return mine;
+    }
+    u -= lane_value(upto - count, at);
+    first = lane_value(begin, at);
+    n = lane_value(end, at) - first;
+    if (share > 1) continue;
+    TreeWork t;
+    t.b = first;
+    t.ch = u;
+    t.lo = (int64_t)lane_value((int)(mine.lo >> 32), at) << 32 | (uint32_t)lane_value((int)mine.lo, at);
+    t.n = lane_value(mine.n, at);
+    t.ctx = lane_value(mine.ctx, at);
+    t.chunks = lane_value(mine.chunks, at);
+    t.c0 = t.ch * p.chunk;
+    t.c1 = min(t.c0 + p.chunk, t.ctx);
+    return t;
+  }
 }
 
 // Bit u of a token's mask: it sees new token u.  Lane t of a wave has token t's; doubling along the parents, six steps for
@@ -67,12 +112,13 @@ __device__ __forceinline__ uint64_t ancestors(const TreeParams& p, const TreeWor
 template <class P>
 __device__ __forceinline__ void stage_group(const unsigned char* base, uint32_t row_bytes, int last, unsigned char* tile, int g, int lane) {
   constexpr int N = 16 * P::PIECES / 64, RPI = 64 / P::PIECES;
+  const __amdgpu_buffer_rsrc_t from = buffer_at(base);
+  // the offsets are formed here: kept from one tile to the next they take registers that the products need
+  asm volatile("" : "+s"(row_bytes), "+v"(lane));
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int row = i * RPI + lane / P::PIECES, piece = (lane % P::PIECES) ^ piece_swizzle<P::PIECES>(row);
-    const uint32_t off = (uint32_t)min(row, last) * row_bytes + 16 * piece;
-    __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(base + off),
-                                     (__attribute__((address_space(3))) void*)(tile + (g * N + i) * 1024), 16, 0, 0);
+    copy16_to_lds(from, (uint32_t)min(row, last) * row_bytes + 16 * piece, 0, tile + (g * N + i) * 1024);
   }
 }
 
@@ -86,36 +132,39 @@ __device__ __forceinline__ Group key_group(int key, int last_key) {
   g.last = min(last_key - g.key, 15);
   return g;
 }
-// The page of a key; a number outside the pool is its nearest page's.
+// The page number of a key, as the table has it: it is used (stage_paged) a tile later, and anything done to it here would
+// wait for it here.
 __device__ __forceinline__ int page_of(const TreeParams& p, int b, int key) {
   typedef const __attribute__((address_space(4))) int32_t* Table;  // nothing writes it meanwhile: scalar loads
-  return min(max(((Table)(p.table + (int64_t)b * p.table_stride))[__builtin_amdgcn_readfirstlane(key >> p.shift)], 0), (int)p.num_pages - 1);
+  return ((Table)(p.table + (int64_t)b * p.table_stride))[__builtin_amdgcn_readfirstlane(key >> p.shift)];
 }
+// A group's keys (or with `v` its values) from the pages, or from the new tokens' own tensor, into group `at` of a tile.
 template <class P>
-__device__ __forceinline__ void stage_paged(const TreeParams& p, int page, int e, Group g, unsigned char* kt, unsigned char* vt, int at, int lane) {
+__device__ __forceinline__ void stage_paged(const TreeParams& p, int page, int e, Group g, bool v, unsigned char* tile, int at, int lane) {
   constexpr int64_t S = sizeof(typename P::elem);
   const int off = g.key & ((1 << p.shift) - 1);
-  stage_group<P>(reinterpret_cast<const unsigned char*>(p.kp) + S * (page * p.kps[0] + e * p.kps[1] + off * p.kps[2]),
-                 (uint32_t)(S * p.kps[2]), g.last, kt, at, lane);
-  stage_group<P>(reinterpret_cast<const unsigned char*>(p.vp) + S * (page * p.vps[0] + e * p.vps[1] + off * p.vps[2]),
-                 (uint32_t)(S * p.vps[2]), g.last, vt, at, lane);
+  page = min(max(page, 0), (int)p.num_pages - 1);  // a number outside the pool is its nearest page's
+  const int64_t* s = v ? p.vps : p.kps;
+  stage_group<P>(reinterpret_cast<const unsigned char*>(v ? p.vp : p.kp) + S * (page * s[0] + e * s[1] + off * s[2]), (uint32_t)(S * s[2]), g.last,
+                 tile, at, lane);
 }
 template <class P>
-__device__ __forceinline__ void stage_new(const TreeParams& p, int64_t lo, int e, Group g, unsigned char* kt, unsigned char* vt, int at, int lane) {
+__device__ __forceinline__ void stage_new(const TreeParams& p, int64_t lo, int e, Group g, bool v, unsigned char* tile, int at, int lane) {
   constexpr int64_t S = sizeof(typename P::elem);
-  stage_group<P>(reinterpret_cast<const unsigned char*>(p.k) + S * ((lo + g.key) * p.ks[0] + e * p.ks[1]), (uint32_t)(S * p.ks[0]), g.last,
-                 kt, at, lane);
-  stage_group<P>(reinterpret_cast<const unsigned char*>(p.v) + S * ((lo + g.key) * p.vs[0] + e * p.vs[1]), (uint32_t)(S * p.vs[0]), g.last,
-                 vt, at, lane);
+  const int64_t* s = v ? p.vs : p.ks;
+  stage_group<P>(reinterpret_cast<const unsigned char*>(v ? p.v : p.k) + S * ((lo + g.key) * s[0] + e * s[1]), (uint32_t)(S * s[0]), g.last, tile,
+                 at, lane);
 }
 
-// The running softmax of one 32-row tile over 32 more keys: scores -> weights in `s`, the sums rescaled where the maximum
+// The running softmax of one 32-row tile over 32 N more keys: scores -> weights in `s`, the sums rescaled where the maximum
 // moved (by more than 2^6, as in the prompt's kernel).
-template <int CT>
-__device__ __forceinline__ void softmax_step(f32x16& s, float& m, float& l, f32x16 (&o)[CT], float c) {
-  float top = s[0];
+template <int N, int CT>
+__device__ __forceinline__ void softmax_step(f32x16 (&s)[N], float& m, float& l, f32x16 (&o)[CT], float c) {
+  float top = s[0][0];
 #pragma unroll
-  for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
   top = half_max(top);
   if (__any((top - m) * c > 6.f || (m == -INFINITY && top > m))) {
     const float next = fmaxf(m, top);
@@ -129,10 +178,12 @@ __device__ __forceinline__ void softmax_step(f32x16& s, float& m, float& l, f32x
   }
   const float mc = m == -INFINITY ? 0.f : m * c;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -mc));
-    l += s[i];
-  }
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], c, -mc));
+      l += s[u][i];
+    }
 }
 
 template <class P>
@@ -153,11 +204,10 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
   float(*wm)[32] = reinterpret_cast<float(*)[32]>(lds + TreeFew<P>::LDS), (*wl)[32] = wm + W;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // chunk by chunk of all sequences: workgroups go round the XCDs in order, and were a sequence's chunks next to one another,
-  // the first chunks, which every sequence has, would fall on a few of them
-  const int heads = p.nseq * p.KV, ch = blockIdx.x / heads, be = blockIdx.x % heads, b = be / p.KV, e = be % p.KV;
-  const TreeWork t = tree_work(p, b, ch);
-  if (t.n <= 0 || ch >= t.chunks) return;
+  const int e = blockIdx.x % p.KV;  // the key heads of a chunk next to one another: they go round the XCDs
+  const TreeWork t = tree_work(p, blockIdx.x / p.KV, lane);
+  if (t.b < 0) return;
+  const int b = t.b, ch = t.ch, be = b * p.KV + e;
   const int rows = t.n * p.G, row = min(lane & 31, rows - 1), tok = row / p.G, h = e * p.G + row % p.G;
   const bool drafts = ch == t.chunks - 1;  // the last chunk has the new tokens too
   const int nt = t.c1 > t.c0 ? (t.c1 - t.c0 + 31) / 32 : 0, total = nt + (drafts ? (t.n + 31) / 32 : 0);
@@ -171,11 +221,13 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
   };
   auto stage = [&](int at, unsigned char* to) {
     if (at < nt) {
-      stage_paged<P>(p, page0, e, key_group(t.c0 + 32 * at, t.c1 - 1), to, to + STAGE / 2, 0, lane);
-      stage_paged<P>(p, page1, e, key_group(t.c0 + 32 * at + 16, t.c1 - 1), to, to + STAGE / 2, 1, lane);
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        stage_paged<P>(p, x & 1 ? page1 : page0, e, key_group(t.c0 + 32 * at + 16 * (x & 1), t.c1 - 1), x >> 1, to + (x >> 1) * STAGE / 2, x & 1, lane);
     } else {
-      stage_new<P>(p, t.lo, e, key_group(32 * (at - nt), t.n - 1), to, to + STAGE / 2, 0, lane);
-      stage_new<P>(p, t.lo, e, key_group(32 * (at - nt) + 16, t.n - 1), to, to + STAGE / 2, 1, lane);
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        stage_new<P>(p, t.lo, e, key_group(32 * (at - nt) + 16 * (x & 1), t.n - 1), x >> 1, to + (x >> 1) * STAGE / 2, x & 1, lane);
     }
   };
   pages(w);
@@ -210,25 +262,27 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
     const unsigned char* vt = kt + STAGE / 2;
-    f32x16 s = zero16();
+    f32x16 s[1] = {zero16()};
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = P::mma(s, P::row_frag(kt, lane & 31, ks, half), q[ks]);
+    for (int ks = 0; ks < KS; ++ks) s[0] = P::mma(s[0], P::row_frag(kt, lane & 31, ks, half), q[ks]);
+    sched_products<P, KS, P::ROW_READS>();
     if (at >= nt) {
       const uint32_t bits = (uint32_t)(sees >> (32 * (at - nt)));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = bits >> rho(half, i) & 1 ? s[i] : -INFINITY;
+      for (int i = 0; i < 16; ++i) s[0][i] = bits >> rho(half, i) & 1 ? s[0][i] : -INFINITY;
     } else if (t.c0 + 32 * at + 32 > t.c1) {
       const int limit = t.c1 - t.c0 - 32 * at;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = rho(half, i) < limit ? s[i] : -INFINITY;
+      for (int i = 0; i < 16; ++i) s[0][i] = rho(half, i) < limit ? s[0][i] : -INFINITY;
     }
-    softmax_step(s, m, l, o, c);
+    softmax_step<1>(s, m, l, o, c);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
-      const typename P::frag pf = P::from_acc(s, kk);
+      const typename P::frag pf = P::from_acc(s[0], kk);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, 16 * kk, ct, lane), pf);
     }
+    sched_products<P, 2 * CT, P::COL_READS>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its slot may be written again
   };
   for (int at = w, buf = 0; at < total; at += W, buf ^= 1) step(at, mine + buf * STAGE, mine + (buf ^ 1) * STAGE);
@@ -278,38 +332,55 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
   }
 }
 
-// More than 32 rows: 128 rows a workgroup.
+// More than 32 rows: workgroups of four waves, `per` of them with 32 rows each, as even as they come (160 rows: three and
+// two; the others only copy).
 template <class P>
-__global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tree_many_kernel(TreeParams p, int blocks) {
+struct TreeMany {
+  static constexpr int TILE = 64 * P::ROW;
+  // tiles in LDS, all but the one in use on their way; two workgroups a CU
+  static constexpr int BUFS = 8 * TILE <= 64 * 1024 ? 4 : 2, COPIES = 2 * 16 * P::PIECES / 64;  // copies of a wave and tile
+  static int blocks(int rows) { return (rows + 127) / 128; }
+  static int per(int rows) { return ((rows + 31) / 32 + blocks(rows) - 1) / blocks(rows); }
+};
+
+template <class P>
+__global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tree_many_kernel(TreeParams p, int blocks, int per) {
   typedef typename P::elem E;
-  constexpr int D = P::D, KS = D / 16, CT = D / 32, TILE = 64 * P::ROW;
-  __shared__ __attribute__((aligned(256))) unsigned char lds[4 * TILE];
+  constexpr int D = P::D, KS = D / 16, CT = D / 32, TILE = TreeMany<P>::TILE;
+  constexpr int BUFS = TreeMany<P>::BUFS, COPIES = TreeMany<P>::COPIES;
+  __shared__ __attribute__((aligned(256))) unsigned char lds[2 * BUFS * TILE];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // the row blocks of one chunk on one XCD, one after another: its L2 has the keys from the second on
   const int unit = blockIdx.x / 8 / blocks * 8 + blockIdx.x % 8, rb = blockIdx.x / 8 % blocks;
-  const int heads = p.nseq * p.KV, ch = unit / heads, be = unit % heads, b = be / p.KV, e = be % p.KV;
-  if (ch >= p.max_chunks) return;
-  const TreeWork t = tree_work(p, b, ch);
-  const int rows = t.n * p.G;
-  if (t.n <= 0 || ch >= t.chunks || 128 * rb >= rows) return;
-  const int mine = 128 * rb + 32 * w + (lane & 31);
-  const bool live = mine < rows, busy = 128 * rb + 32 * w < rows;
-  const int row = min(mine, rows - 1), tok = row / p.G, h = e * p.G + row % p.G;
+  const int e = unit % p.KV;
+  const TreeWork t = tree_work(p, unit / p.KV, lane);
+  if (t.b < 0) return;
+  const int b = t.b, ch = t.ch, be = b * p.KV + e;
+  const int rows = t.n * p.G, first = 32 * (per * rb + w);
+  if (32 * per * rb >= rows) return;
+  const bool busy = w < per && first < rows, live = busy && first + (lane & 31) < rows;
+  const int row = min(first + (lane & 31), rows - 1), tok = row / p.G, h = e * p.G + row % p.G;
   const bool drafts = ch == t.chunks - 1;
   const int nt = t.c1 > t.c0 ? (t.c1 - t.c0 + 63) / 64 : 0, total = nt + (drafts ? 1 : 0);
-  // wave w copies keys 16 w .. of each tile; their page is known a tile ahead
+  // wave w copies keys 16 w .. of each tile and their values; their page is known a tile ahead
   int page = 0;
   auto pages = [&](int at) {
     if (at < nt) page = page_of(p, b, key_group(t.c0 + 64 * at + 16 * w, t.c1 - 1).key);
   };
   auto stage = [&](int at, unsigned char* to) {
-    if (at < nt) stage_paged<P>(p, page, e, key_group(t.c0 + 64 * at + 16 * w, t.c1 - 1), to, to + TILE, w, lane);
-    else stage_new<P>(p, t.lo, e, key_group(16 * w, t.n - 1), to, to + TILE, w, lane);
+    const Group g = at < nt ? key_group(t.c0 + 64 * at + 16 * w, t.c1 - 1) : key_group(16 * w, t.n - 1);
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+      if (at < nt) stage_paged<P>(p, page, e, g, v, to + v * TILE, w, lane);
+      else stage_new<P>(p, t.lo, e, g, v, to + v * TILE, w, lane);
   };
-  pages(0);
-  stage(0, lds);
-  pages(1);
+#pragma unroll
+  for (int x = 0; x < BUFS - 1; ++x) {
+    pages(x);
+    if (x < total) stage(x, lds + x * 2 * TILE);
+  }
+  pages(BUFS - 1);
   uint64_t sees = 0;
   if (drafts) {
     const uint64_t all = ancestors(p, t, lane);
@@ -327,38 +398,45 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
   float m = -INFINITY, l = 0.f;
   const float c = p.scale * LOG2E;
   auto step = [&](int at, const unsigned char* __restrict kt, unsigned char* __restrict next) {
-    if (at + 1 < total) {
-      stage(at + 1, next);
-      pages(at + 2);
+    if (at + BUFS - 1 < total) {
+      stage(at + BUFS - 1, next);
+      pages(at + BUFS);
     }
     if (!busy) return;
     const unsigned char* vt = kt + TILE;
+    f32x16 s[2] = {zero16(), zero16()};
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      f32x16 s = zero16();
+    for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = P::mma(s, P::row_frag(kt, 32 * u + (lane & 31), ks, half), q[ks]);
-      if (at >= nt) {
-        const uint32_t bits = (uint32_t)(sees >> (32 * u));
+      for (int u = 0; u < 2; ++u) s[u] = P::mma(s[u], P::row_frag(kt, 32 * u + (lane & 31), ks, half), q[ks]);
+    sched_products<P, 2 * KS, P::ROW_READS>();
+    if (at >= nt) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = bits >> rho(half, i) & 1 ? s[i] : -INFINITY;
-      } else if (t.c0 + 64 * at + 32 * u + 32 > t.c1) {
-        const int limit = t.c1 - t.c0 - 64 * at - 32 * u;
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = rho(half, i) < limit ? s[i] : -INFINITY;
-      }
-      softmax_step(s, m, l, o, c);
+        for (int i = 0; i < 16; ++i) s[u][i] = (uint32_t)(sees >> (32 * u)) >> (4 * half) >> rho(0, i) & 1 ? s[u][i] : -INFINITY;
+    } else if (t.c0 + 64 * at + 64 > t.c1) {
+      const int limit = t.c1 - t.c0 - 64 * at;
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        const typename P::frag pf = P::from_acc(s, kk);
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, 32 * u + 16 * kk, ct, lane), pf);
-      }
+        for (int i = 0; i < 16; ++i) s[u][i] = 32 * u + rho(half, i) < limit ? s[u][i] : -INFINITY;
     }
+    softmax_step<2>(s, m, l, o, c);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      const typename P::frag pf = P::from_acc(s[kk >> 1], kk & 1);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, 16 * kk, ct, lane), pf);
+    }
+    sched_products<P, 4 * CT, P::COL_READS>();
   };
-  for (int at = 0; at < total; ++at) {
-    staged_barrier();
-    step(at, lds + (at & 1) * 2 * TILE, lds + (~at & 1) * 2 * TILE);
+  for (int at = 0, now = 0; at < total; ++at) {
+    if (at + BUFS - 2 >= total) staged_barrier();
+    else staged_barrier<(BUFS - 2) * COPIES>();
+    const int then = now == 0 ? BUFS - 1 : now - 1;  // the tile before: read by all
+    step(at, lds + now * 2 * TILE, lds + then * 2 * TILE);
+    now = now == BUFS - 1 ? 0 : now + 1;
   }
   l = half_sum(l);
   if (t.chunks == 1) {
@@ -383,7 +461,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeParams p) {
   const int64_t be = id / most;
   if (be >= (int64_t)p.nseq * p.KV) return;
   const int b = (int)(be / p.KV), e = (int)(be % p.KV);
-  const TreeWork t = tree_work(p, b, 0);
+  const TreeWork t = tree_seq(p, b);
   if (r >= t.n * p.G || t.chunks == 1) return;
   const int64_t first = be * p.max_chunks * most + r;
   float top = -INFINITY;
@@ -410,8 +488,8 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeParams p) {
 // queries and its partial sums, is that of a few dozen keys; short chunks even out unequal contexts).
 static int tree_chunk(const kdn_tree_attn_args* a) {
   const int64_t rows = a->max_new * (a->H / a->H_kv), blocks = rows <= 32 ? 1 : (rows + 127) / 128;
-  int chunk = 256;
-  while (chunk < 1024 && a->num_seqs * a->H_kv * blocks * ((a->max_context + chunk - 1) / chunk) > 2048) chunk *= 2;
+  int chunk = 128;
+  while (chunk < 1024 && a->num_seqs * a->H_kv * blocks * ((a->max_context + chunk - 1) / chunk) > (chunk < 256 ? 512 : 2048)) chunk *= 2;
   return chunk;
 }
 static int64_t tree_chunks(const kdn_tree_attn_args* a) {
@@ -438,8 +516,8 @@ static int launch_tree(const TreeParams& p, hipStream_t st) {
   if (rows <= 32) {
     hipLaunchKernelGGL(tree_few_kernel<P>, dim3((unsigned)units), dim3(64 * TreeFew<P>::WAVES), 0, st, p);
   } else {
-    const int blocks = (rows + 127) / 128;
-    hipLaunchKernelGGL(tree_many_kernel<P>, dim3((unsigned)((units + 7) / 8 * 8 * blocks)), dim3(256), 0, st, p, blocks);
+    const int blocks = TreeMany<P>::blocks(rows);
+    hipLaunchKernelGGL(tree_many_kernel<P>, dim3((unsigned)((units + 7) / 8 * 8 * blocks)), dim3(256), 0, st, p, blocks, TreeMany<P>::per(rows));
   }
   if (p.max_chunks > 1) {
     const int64_t joins = (int64_t)p.nseq * p.KV * rows;
@@ -461,8 +539,8 @@ static size_t tree_partial_bytes(const kdn_tree_attn_args* a, int64_t units) {
 // holds for the others: the rule for a chunk's length gives a smaller call shorter chunks, and at times more of them.
 extern "C" size_t kdn_tree_attn_workspace_bytes(const kdn_tree_attn_args* a) {
   if (tree_check(a) != KDN_OK) return 0;
-  const int64_t heads = a->num_seqs * a->H_kv, fine = heads * ((a->max_context + 255) / 256), coarse = heads * ((a->max_context + 1023) / 1024);
-  return a->max_context <= 256 ? 16 : tree_partial_bytes(a, std::min(fine, std::max<int64_t>(2048, coarse)));
+  const int64_t heads = a->num_seqs * a->H_kv, fine = heads * ((a->max_context + 127) / 128), coarse = heads * ((a->max_context + 1023) / 1024);
+  return a->max_context <= 128 ? 16 : tree_partial_bytes(a, std::min(fine, std::max<int64_t>(2048, coarse)));
 }
 
 extern "C" int kdn_tree_attn(const kdn_tree_attn_args* a, void* stream) {
@@ -479,7 +557,7 @@ extern "C" int kdn_tree_attn(const kdn_tree_attn_args* a, void* stream) {
   for (int i = 0; i < 3; ++i)
     fits = fits && a->k_pages_stride[i] >= 0 && a->v_pages_stride[i] >= 0 && a->k_pages_stride[i] % per == 0 && a->v_pages_stride[i] % per == 0;
   if (!fits) return KDN_ERR_MISALIGNED;
-  const int64_t chunks = tree_chunks(a), rows = a->max_new * (a->H / a->H_kv), blocks = rows <= 32 ? 1 : (rows + 127) / 128;
+  const int64_t chunks = tree_chunks(a), rows = a->max_new * (a->H / a->H_kv), blocks = rows <= 32 ? 1 : (rows + 127) / 128;  // at least as many as there will be
   if (a->num_seqs * a->H_kv * chunks * blocks > INT32_MAX - 8 * blocks || a->num_seqs * a->H_kv * rows > INT32_MAX)
     return KDN_ERR_UNSUPPORTED;
   // a copy's lanes have 32-bit offsets from its first row

@@ -280,13 +280,14 @@ def _declare_anchor(L: ctypes.CDLL) -> None:
     """Argument and result types of include/kdn_anchor.h."""
     vp, i64, ci, sz, ptr = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.POINTER
     for name, args, res in (
+            # the argument structs go over as their packed bytes (kdn/anchor.py) or as a mirror's address
             ("kdn_anchor_version", [], ci),
-            ("kdn_attn_fwd", [ptr(AttnArgs), vp], ci),
-            ("kdn_attn_bwd_workspace_bytes", [ptr(AttnBwdArgs)], sz),
-            ("kdn_attn_bwd", [ptr(AttnBwdArgs), vp], ci),
-            ("kdn_rotary", [ptr(RotaryArgs), vp], ci),
+            ("kdn_attn_fwd", [vp, vp], ci),
+            ("kdn_attn_bwd_workspace_bytes", [vp], sz),
+            ("kdn_attn_bwd", [vp, vp], ci),
+            ("kdn_rotary", [vp, vp], ci),
             ("kdn_page_copy", [vp, i64, i64, vp, i64, vp], ci),
-            ("kdn_page_append", [ptr(PageAppendArgs), vp], ci),
+            ("kdn_page_append", [vp, vp], ci),
             ("kdn_page_pool_create", [i64, i64, i64, ptr(vp)], ci),
             ("kdn_page_pool_destroy", [vp], None),
             ("kdn_page_pool_open", [vp], ci),
@@ -300,8 +301,8 @@ def _declare_anchor(L: ctypes.CDLL) -> None:
             ("kdn_page_pool_compact", [vp, vp, i64], i64),
             ("kdn_page_pool_used", [vp], i64),
             ("kdn_page_pool_free", [vp], i64),
-            ("kdn_tree_attn_workspace_bytes", [ptr(TreeAttnArgs)], sz),
-            ("kdn_tree_attn", [ptr(TreeAttnArgs), vp], ci)):
+            ("kdn_tree_attn_workspace_bytes", [vp], sz),
+            ("kdn_tree_attn", [vp, vp], ci)):
         fn = getattr(L, name)
         fn.argtypes, fn.restype = args, res
 

@@ -17,53 +17,76 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import List, Optional, Sequence, Tuple
 
 import torch
 
 from . import _native as N
-from .ops import _on, _stream, _tag, require_device
+from .ops import _HERE, _tag, require_device
 
 _ref = ctypes.byref
+_BF16, _F32 = torch.bfloat16, torch.float32
+_raw_stream, _this_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+# The argument structs of include/kdn_anchor.h as packed bytes, in C's own alignment: a decode step's calls are host-bound,
+# and a ctypes structure filled field by field takes as long as the rest of a call.  The order is that of the mirrors in
+# kdn/_native.py (tests/test_anchor_host.py holds them against each other).
+_ATTN = struct.Struct("@qqqqqiifPP" + 4 * "Pqq" + "P" + "Pqq")
+_ATTN_BWD = struct.Struct("@P" + 4 * "Pqq" + "PN")
+_ROTARY = struct.Struct("@qqqiiiiifPP" + 4 * "Pqq")
+_APPEND = struct.Struct("@qqiiqqP" + 2 * "Pqq" + 2 * "Pqqq")
+_TREE = struct.Struct("@qqqqqqiifqqqqPPPP" + 3 * "Pqq" + 2 * "Pqqq" + "Pqq" + "PN")
 
 
-def _heads(t: torch.Tensor, what: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """t as the library reads it: (tokens, heads, d), contiguous heads, rows on 16 bytes."""
-    require_device(t, what)
+def _device(index: int):
+    """The context of work on a device, as ops._on."""
+    return _HERE if index == _this_device() else torch.cuda.device(index)
+
+
+def _heads(t: torch.Tensor, what: str, like: Optional[torch.Tensor] = None):
+    """(t, its address, token stride, head stride), t as the library reads it: (tokens, heads, d), contiguous heads, rows on
+    16 bytes (copied if they are not)."""
+    if not t.is_cuda:
+        require_device(t, what)
     if t.dim() != 3:
         raise ValueError(f"{what}: expects (tokens, heads, d), got {tuple(t.shape)}")
-    if like is not None and (t.device != like.device or t.dtype != like.dtype or t.shape[-1] != like.shape[-1]):
-        raise ValueError(f"{what}: expects {like.dtype} with d = {like.shape[-1]} on {like.device}; got {t.dtype}, "
+    dt = t.dtype
+    if like is not None and (dt is not like.dtype or t.get_device() != like.get_device() or t.shape[2] != like.shape[2]):
+        raise ValueError(f"{what}: expects {like.dtype} with d = {like.shape[-1]} on {like.device}; got {dt}, "
                          f"{tuple(t.shape)} on {t.device}")
-    size = t.element_size()
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:2]):
+    a, b, c = t.stride()
+    p = t.data_ptr()
+    if c != 1 or p & 15 or (a | b) & (7 if dt is _BF16 else 3):
         t = t.contiguous()  # a view that starts off 16 bytes may be contiguous already
-        t = t.clone() if t.data_ptr() % 16 else t
-    return t
+        t = t.clone() if t.data_ptr() & 15 else t
+        a, b, c = t.stride()
+        p = t.data_ptr()
+    return t, p, a, b
 
 
-def _out(t: torch.Tensor, what: str, shape, like: torch.Tensor) -> torch.Tensor:
-    """An output that the caller gave: it is written where it is, so that it has to be in place."""
+def _out(t: torch.Tensor, what: str, shape, like: torch.Tensor):
+    """As _heads, of an output that the caller gave: it is written where it is, so that it has to be in place."""
     require_device(t, what)
-    if tuple(t.shape) != tuple(shape) or t.dtype != like.dtype or t.device != like.device:
+    if t.shape != shape or t.dtype is not like.dtype or t.device != like.device:
         raise ValueError(f"{what}: expects {tuple(shape)} {like.dtype} on {like.device}; got {tuple(t.shape)} {t.dtype} on {t.device}")
     if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s * t.element_size() % 16 for s in t.stride()[:2]):
         raise ValueError(f"{what}: needs contiguous heads whose rows start on 16 bytes")
-    return t
+    return t, t.data_ptr(), t.stride(0), t.stride(1)
 
 
-def _ints(t: torch.Tensor, what: str, dtype: torch.dtype, dev: torch.device, n: Optional[int] = None) -> torch.Tensor:
+def _new(like: torch.Tensor, shape):
+    t = like.new_empty(shape)
+    return t, t.data_ptr(), shape[1] * shape[2], shape[2]
+
+
+def _ints(t: torch.Tensor, what: str, dtype: torch.dtype, dev: int, n: Optional[int] = None) -> torch.Tensor:
+    if t.dtype is dtype and t.dim() == 1 and t.get_device() == dev and (n is None or t.shape[0] == n) and t.is_contiguous():
+        return t
     require_device(t, what)
-    if t.device != dev or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{what}: expects {'' if n is None else n} integers on {dev}; got {tuple(t.shape)} {t.dtype} on {t.device}")
+    if t.get_device() != dev or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: expects {'' if n is None else n} integers on GPU {dev}; got {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.to(dtype).contiguous()
-
-
-def _set(a: ctypes.Structure, name: str, t: torch.Tensor) -> None:
-    setattr(a, name, t.data_ptr())
-    field = getattr(a, name + "_stride")
-    for i in range(len(field)):
-        field[i] = t.stride(i)
 
 
 def _groups(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, what: str) -> None:
@@ -114,34 +137,29 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "n
 
 
 def _rotate(q, k, positions, inv_freq, interleaved, magnitude, inverse, in_place):
-    what = "rotary"
-    dev = q.device
     if in_place:
-        q, k = _out(q, "rotary q", q.shape, q), None if k is None else _out(k, "rotary k", k.shape, q)
+        q, qp, q0, q1 = _out(q, "rotary q", q.shape, q)
     else:
-        q, k = _heads(q, "rotary q"), None if k is None else _heads(k, "rotary k", q)
-    n = q.shape[0]
-    if k is not None and k.shape[0] != n:
-        raise ValueError(f"{what}: q and k have the same tokens; got {tuple(q.shape)}, {tuple(k.shape)}")
+        q, qp, q0, q1 = _heads(q, "rotary q")
+    n, H, d = q.shape
+    dev = q.get_device()
+    KV, kp, k0, k1 = 0, 0, 0, 0
+    if k is not None:
+        k, kp, k0, k1 = _out(k, "rotary k", k.shape, q) if in_place else _heads(k, "rotary k", q)
+        KV = k.shape[1]
+        if k.shape[0] != n or k.shape[2] != d:
+            raise ValueError(f"rotary: q and k have the same tokens and d; got {tuple(q.shape)}, {tuple(k.shape)}")
     pos = _ints(positions, "rotary positions", torch.int64, dev, n)
-    if inv_freq.device != dev or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= q.shape[-1]:
-        raise ValueError(f"{what}: inv_freq is (rotary_dim / 2,) float64 on {dev} with rotary_dim <= {q.shape[-1]}; got "
+    if inv_freq.get_device() != dev or inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.shape[0] <= d:
+        raise ValueError(f"rotary: inv_freq is (rotary_dim / 2,) float64 on {q.device} with rotary_dim <= {d}; got "
                          f"{tuple(inv_freq.shape)} {inv_freq.dtype} on {inv_freq.device}")
     f = inv_freq.contiguous()
-    qo = q if in_place else torch.empty(q.shape, dtype=q.dtype, device=dev)
-    ko = k if in_place or k is None else torch.empty(k.shape, dtype=k.dtype, device=dev)
-    a = N.RotaryArgs()
-    a.tokens, a.H, a.H_kv, a.d = n, q.shape[1], 0 if k is None else k.shape[1], q.shape[2]
-    a.rotary_dim, a.dtype = 2 * f.shape[0], _tag(q.dtype, what)
-    a.interleaved, a.inverse, a.magnitude = int(bool(interleaved)), int(bool(inverse)), float(magnitude)
-    a.positions, a.inv_freq = pos.data_ptr(), f.data_ptr()
-    _set(a, "q", q)
-    _set(a, "q_out", qo)
-    if k is not None:
-        _set(a, "k", k)
-        _set(a, "k_out", ko)
-    with _on(dev):
-        N.check(N.lib().kdn_rotary(_ref(a), _stream(dev)), "kdn_rotary")
+    qo, qop, qo0, qo1 = (q, qp, q0, q1) if in_place else _new(q, (n, H, d))
+    ko, kop, ko0, ko1 = (k, kp, k0, k1) if in_place or k is None else _new(k, (n, KV, d))
+    with _device(dev):
+        N.check(N.lib().kdn_rotary(_ROTARY.pack(n, H, KV, d, 2 * f.shape[0], _tag(q.dtype, "rotary"), interleaved, inverse, magnitude,
+                                                pos.data_ptr(), f.data_ptr(), qp, q0, q1, kp, k0, k1, qop, qo0, qo1, kop, ko0, ko1),
+                                   _raw_stream(dev)), "kdn_rotary")
     return qo, ko
 
 
@@ -170,78 +188,74 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         if in_place:
             raise ValueError("rotary: in_place has no gradient")
         return _Rotary.apply(q, k, positions, inv_freq, bool(interleaved), float(magnitude), bool(inverse))
-    return _rotate(q, k, positions, inv_freq, interleaved, magnitude, inverse, in_place)
+    return _rotate(q, k, positions, inv_freq, bool(interleaved), float(magnitude), bool(inverse), in_place)
 
 
 # ------------------------------------------------------------------------------------------------- prompt attention
 
 
-def _attn_args(q, k, v, cu_q, cu_k, scale, y, lse, low=None) -> N.AttnArgs:
-    a = N.AttnArgs()
-    a.num_seqs, a.total_q, a.total_k = cu_q.shape[0] - 1, q.shape[0], k.shape[0]
-    a.H, a.H_kv, a.d, a.dtype, a.scale = q.shape[1], k.shape[1], q.shape[2], _tag(q.dtype, "attention"), scale
-    a.cu_q, a.cu_k = cu_q.data_ptr(), None if cu_k is None else cu_k.data_ptr()
-    for name, t in (("q", q), ("k", k), ("v", v), ("y", y)):
-        _set(a, name, t)
-    a.lse = None if lse is None else lse.data_ptr()
-    if low is not None:
-        _set(a, "y_low", low)
-    return a
-
-
 def _attn_inputs(q, k, v, cu_q, cu_k):
-    q = _heads(q, "attention q")
-    k, v = _heads(k, "attention k", q), _heads(v, "attention v", q)
+    """q, k, v as _heads gives them and the offsets, checked."""
+    qs = _heads(q, "attention q")
+    ks, vs = _heads(k, "attention k", q), _heads(v, "attention v", q)
     _groups(q, k, v, "attention")
-    dev = q.device
-    if cu_q.shape[0] < 1 or (cu_k is not None and cu_k.shape != cu_q.shape):
+    dev = q.get_device()
+    if cu_q.dim() != 1 or cu_q.shape[0] < 1 or (cu_k is not None and cu_k.shape != cu_q.shape):
         raise ValueError("attention: cu_seqlens are (sequences + 1,), the same number for queries and keys")
     if cu_k is None and k.shape[0] != q.shape[0]:
         raise ValueError(f"attention: {q.shape[0]} queries and {k.shape[0]} keys need cu_seqlens_k")
-    return (q, k, v, _ints(cu_q, "attention cu_seqlens", torch.int64, dev),
+    return (qs, ks, vs, _ints(cu_q, "attention cu_seqlens", torch.int64, dev),
             None if cu_k is None else _ints(cu_k, "attention cu_seqlens_k", torch.int64, dev))
+
+
+def _pack_attn(qs, ks, vs, cu_q, cu_k, scale, y, lse, low) -> bytes:
+    n, H, d = qs[0].shape
+    return _ATTN.pack(cu_q.shape[0] - 1, n, ks[0].shape[0], H, ks[0].shape[1], d, _tag(qs[0].dtype, "attention"), scale,
+                      cu_q.data_ptr(), 0 if cu_k is None else cu_k.data_ptr(), *qs[1:], *ks[1:], *vs[1:], *y[1:],
+                      0 if lse is None else lse.data_ptr(), *((0, 0, 0) if low is None else low[1:]))
 
 
 def attention_forward(q, k, v, cu_seqlens, cu_seqlens_k=None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
                       return_lse: bool = False, return_low: bool = False):
     """`attention` without autograd: y; or with return_lse (y, lse (H, tokens) float32); or with return_low too (y, lse, low),
     low what rounding took from y (None in float32), which makes the gradients' dy . y exact."""
-    q, k, v, cu_q, cu_k = _attn_inputs(q, k, v, cu_seqlens, cu_seqlens_k)
-    y = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else _out(out, "attention out", q.shape, q)
-    lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device) if return_lse else None
-    low = torch.empty(q.shape, dtype=q.dtype, device=q.device) if return_low and q.dtype is torch.bfloat16 else None
-    a = _attn_args(q, k, v, cu_q, cu_k, _scale(scale, q.shape[-1], "attention"), y, lse, low)
-    with _on(q.device):
-        N.check(N.lib().kdn_attn_fwd(_ref(a), _stream(q.device)), "kdn_attn_fwd")
-    return (y, lse, low) if return_low else (y, lse) if return_lse else y
+    qs, ks, vs, cu_q, cu_k = _attn_inputs(q, k, v, cu_seqlens, cu_seqlens_k)
+    n, H, d = q.shape
+    y = _new(q, (n, H, d)) if out is None else _out(out, "attention out", q.shape, q)
+    lse = q.new_empty((H, n), dtype=_F32) if return_lse or return_low else None
+    low = _new(q, (n, H, d)) if return_low and q.dtype is _BF16 else None
+    args = _pack_attn(qs, ks, vs, cu_q, cu_k, _scale(scale, d, "attention"), y, lse, low)
+    dev = q.get_device()
+    with _device(dev):
+        N.check(N.lib().kdn_attn_fwd(args, _raw_stream(dev)), "kdn_attn_fwd")
+    return (y[0], lse, None if low is None else low[0]) if return_low else (y[0], lse) if return_lse else y[0]
 
 
 def attention_backward(q, k, v, y, lse, dy, cu_seqlens, cu_seqlens_k=None, scale: Optional[float] = None,
                        low: Optional[torch.Tensor] = None):
     """(dq, dk, dv) of `attention_forward`'s y, lse and low (optional) for dL/dy, in the inputs' dtype, the same bits every
     time."""
-    q, k, v, cu_q, cu_k = _attn_inputs(q, k, v, cu_seqlens, cu_seqlens_k)
-    y, dy = _heads(y, "attention y", q), _heads(dy, "attention dy", q)
-    if y.shape != q.shape or dy.shape != q.shape or tuple(lse.shape) != (q.shape[1], q.shape[0]) or lse.dtype != torch.float32 or \
+    qs, ks, vs, cu_q, cu_k = _attn_inputs(q, k, v, cu_seqlens, cu_seqlens_k)
+    ys, dys = _heads(y, "attention y", q), _heads(dy, "attention dy", q)
+    if y.shape != q.shape or dy.shape != q.shape or tuple(lse.shape) != (q.shape[1], q.shape[0]) or lse.dtype is not _F32 or \
             lse.device != q.device:
         raise ValueError(f"attention backward: y and dy have q's shape {tuple(q.shape)}, lse is (H, tokens) float32 on {q.device}")
     lse = lse.contiguous()
+    lows = None
     if low is not None:
-        low = _heads(low, "attention low", q)
+        lows = _heads(low, "attention low", q)
         if low.shape != q.shape:
             raise ValueError(f"attention backward: low has q's shape {tuple(q.shape)}")
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    f = _attn_args(q, k, v, cu_q, cu_k, _scale(scale, q.shape[-1], "attention"), y, lse, low)
-    a = N.AttnBwdArgs()
-    a.fwd = ctypes.addressof(f)
-    for name, t in (("dy", dy), ("dq", dq), ("dk", dk), ("dv", dv)):
-        _set(a, name, t)
-    with _on(q.device):
-        nbytes = N.lib().kdn_attn_bwd_workspace_bytes(_ref(a))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-        N.check(N.lib().kdn_attn_bwd(_ref(a), _stream(q.device)), "kdn_attn_bwd")
-    return dq, dk, dv
+    dq, dk, dv = _new(q, tuple(q.shape)), _new(k, tuple(k.shape)), _new(v, tuple(v.shape))
+    fwd = ctypes.c_char_p(_pack_attn(qs, ks, vs, cu_q, cu_k, _scale(scale, q.shape[-1], "attention"), ys, lse, lows))
+    at = ctypes.cast(fwd, ctypes.c_void_p).value
+    dev = q.get_device()
+    with _device(dev):
+        nbytes = N.lib().kdn_attn_bwd_workspace_bytes(_ATTN_BWD.pack(at, *dys[1:], *dq[1:], *dk[1:], *dv[1:], 0, 0))
+        ws = q.new_empty(nbytes, dtype=torch.uint8)
+        N.check(N.lib().kdn_attn_bwd(_ATTN_BWD.pack(at, *dys[1:], *dq[1:], *dk[1:], *dv[1:], ws.data_ptr(), nbytes), _raw_stream(dev)),
+                "kdn_attn_bwd")
+    return dq[0], dk[0], dv[0]
 
 
 class _Attention(torch.autograd.Function):
@@ -289,30 +303,38 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Opt
 # ------------------------------------------------------------------------------------------------- pages
 
 
-def _pages(t: torch.Tensor, what: str, like: torch.Tensor) -> torch.Tensor:
+def _pages(t: torch.Tensor, what: str, like: torch.Tensor):
+    """(t, its address, page, head and token strides); a cache is used where it is, never copied."""
     require_device(t, what)
-    if t.dim() != 4 or t.dtype != like.dtype or t.device != like.device or t.shape[-1] != like.shape[-1]:
+    if t.dim() != 4 or t.dtype is not like.dtype or t.get_device() != like.get_device() or t.shape[3] != like.shape[2]:
         raise ValueError(f"{what}: expects (pages, heads, page_tokens, {like.shape[-1]}) {like.dtype} on {like.device}; got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s * t.element_size() % 16 for s in t.stride()[:3]):
+    a, b, c, e = t.stride()
+    p = t.data_ptr()
+    if e != 1 or p & 15 or (a | b | c) & (7 if t.dtype is _BF16 else 3):
         raise ValueError(f"{what}: needs contiguous rows that start on 16 bytes (a cache is used where it is, never copied)")
-    return t
+    return t, p, a, b, c
 
 
 def page_copy(slab: torch.Tensor, pairs) -> None:
     """Page pairs[i][0] of slab (pages, ...; contiguous) to page pairs[i][1], for host pairs (a CPU int32 tensor (n, 2) or
     pairs of numbers) as `PagePool` gives them: no page is the target of two pairs, or a target and a source."""
-    require_device(slab, "page_copy")
-    if not slab.is_contiguous() or slab.dim() < 2:
+    if not slab.is_cuda:
+        require_device(slab, "page_copy")
+    if slab.dim() < 2 or not slab.is_contiguous():
         raise ValueError("page_copy: the slab must be contiguous, pages first")
-    p = torch.as_tensor(pairs, dtype=torch.int32).reshape(-1, 2).contiguous()
+    p = pairs
+    if not isinstance(p, torch.Tensor) or p.dtype is not torch.int32 or p.dim() != 2 or p.shape[1] != 2 or not p.is_contiguous():
+        p = torch.as_tensor(pairs, dtype=torch.int32).reshape(-1, 2).contiguous()
     if p.is_cuda:
         raise ValueError("page_copy: pairs are host numbers")
-    if p.shape[0] == 0:
+    n = p.shape[0]
+    if n == 0:
         return
-    nbytes = slab[0].numel() * slab.element_size()
-    with _on(slab.device):
-        N.check(N.lib().kdn_page_copy(slab.data_ptr(), slab.shape[0], nbytes, p.data_ptr(), p.shape[0], _stream(slab.device)),
+    dev = slab.get_device()
+    pages = slab.shape[0]
+    with _device(dev):
+        N.check(N.lib().kdn_page_copy(slab.data_ptr(), pages, slab.nbytes // max(pages, 1), p.data_ptr(), n, _raw_stream(dev)),
                 "kdn_page_copy")
 
 
@@ -320,19 +342,16 @@ def page_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
     """k and v (tokens, H_kv, d) into k_pages and v_pages (pages, H_kv, page_tokens, d): token i to place
     rows[i] % page_tokens of page rows[i] / page_tokens (`PagePool.rows`); one whose row is negative or past the pages is
     skipped.  Rows are distinct."""
-    k = _heads(k, "page_append k")
-    v = _heads(v, "page_append v", k)
+    ks, vs = _heads(k, "page_append k"), _heads(v, "page_append v", k)
     kp, vp = _pages(k_pages, "page_append k_pages", k), _pages(v_pages, "page_append v_pages", k)
-    if k.shape != v.shape or kp.shape != vp.shape or kp.shape[1] != k.shape[1]:
-        raise ValueError(f"page_append: k, v {tuple(k.shape)}, {tuple(v.shape)} and pages {tuple(kp.shape)}, {tuple(vp.shape)} differ")
-    r = _ints(rows, "page_append rows", torch.int64, k.device, k.shape[0])
-    a = N.PageAppendArgs()
-    a.tokens, a.H_kv, a.d, a.dtype = k.shape[0], k.shape[1], k.shape[2], _tag(k.dtype, "page_append")
-    a.page_tokens, a.num_pages, a.rows = kp.shape[2], kp.shape[0], r.data_ptr()
-    for name, t in (("k", k), ("v", v), ("k_pages", kp), ("v_pages", vp)):
-        _set(a, name, t)
-    with _on(k.device):
-        N.check(N.lib().kdn_page_append(_ref(a), _stream(k.device)), "kdn_page_append")
+    n, KV, d = k.shape
+    if v.shape != k.shape or k_pages.shape != v_pages.shape or k_pages.shape[1] != KV:
+        raise ValueError(f"page_append: k, v {tuple(k.shape)}, {tuple(v.shape)} and pages {tuple(k_pages.shape)}, {tuple(v_pages.shape)} differ")
+    dev = k.get_device()
+    r = _ints(rows, "page_append rows", torch.int64, dev, n)
+    with _device(dev):
+        N.check(N.lib().kdn_page_append(_APPEND.pack(n, KV, d, _tag(k.dtype, "page_append"), k_pages.shape[2], k_pages.shape[0], r.data_ptr(),
+                                                     *ks[1:], *vs[1:], *kp[1:], *vp[1:]), _raw_stream(dev)), "kdn_page_append")
 
 
 class PagePool:
@@ -408,15 +427,6 @@ class PagePool:
 # ------------------------------------------------------------------------------------------------- attention over pages
 
 
-def _tree_args(q, k, v, k_pages, v_pages, page_table, num_seqs, max_context, max_new, scale) -> N.TreeAttnArgs:
-    a = N.TreeAttnArgs()
-    a.num_seqs, a.total_new, a.max_new, a.max_context = num_seqs, q.shape[0], max_new, max_context
-    a.H, a.H_kv, a.d, a.dtype, a.scale = q.shape[1], k.shape[1], q.shape[2], _tag(q.dtype, "tree_attention"), scale
-    a.page_tokens, a.num_pages = k_pages.shape[2], k_pages.shape[0]
-    a.table_width, a.table_stride = page_table.shape[1], page_table.stride(0)
-    return a
-
-
 def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                    page_table: torch.Tensor, context_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
                    parents: Optional[torch.Tensor] = None, scale: Optional[float] = None, max_context: Optional[int] = None,
@@ -432,49 +442,50 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: t
     At most 64 new tokens a stream; max_new (64, or 1 without cu_seqlens) and max_context (what page_table holds) bound
     them from the host, so that nothing is read back; the closer, the smaller the launch.  `workspace`: uint8, at least
     `tree_workspace_bytes`, for a caller that allocates once."""
-    q = _heads(q, "tree_attention q")
-    k, v = _heads(k, "tree_attention k", q), _heads(v, "tree_attention v", q)
-    _groups(q, k, v, "tree_attention")
-    dev = q.device
+    what = "tree_attention"
+    qs = _heads(q, "tree_attention q")
+    ks, vs = _heads(k, "tree_attention k", q), _heads(v, "tree_attention v", q)
+    _groups(q, k, v, what)
     kp, vp = _pages(k_pages, "tree_attention k_pages", q), _pages(v_pages, "tree_attention v_pages", q)
-    if k.shape[0] != q.shape[0] or kp.shape != vp.shape or kp.shape[1] != k.shape[1]:
-        raise ValueError(f"tree_attention: q {tuple(q.shape)}, k {tuple(k.shape)} and pages {tuple(kp.shape)}, {tuple(vp.shape)} do not go together")
-    require_device(page_table, "tree_attention page_table")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != dev or (page_table.shape[1] and page_table.stride(1) != 1):
-        raise ValueError(f"tree_attention: page_table is (streams, width) int32 on {dev}, got {tuple(page_table.shape)} {page_table.dtype}")
-    B = page_table.shape[0]
+    n, H, d = q.shape
+    KV, (pages, heads, P, _) = k.shape[1], k_pages.shape
+    if k.shape[0] != n or v_pages.shape != k_pages.shape or heads != KV:
+        raise ValueError(f"tree_attention: q {tuple(q.shape)}, k {tuple(k.shape)} and pages {tuple(k_pages.shape)}, {tuple(v_pages.shape)} "
+                         f"do not go together")
+    dev = q.get_device()
+    if page_table.get_device() != dev or page_table.dim() != 2 or page_table.dtype is not torch.int32 or \
+            (page_table.shape[1] and page_table.stride(1) != 1):
+        raise ValueError(f"tree_attention: page_table is (streams, width) int32 on {q.device}, got {tuple(page_table.shape)} "
+                         f"{page_table.dtype} on {page_table.device}")
+    B, width = page_table.shape
     lens = _ints(context_lens, "tree_attention context_lens", torch.int32, dev, B)
     if cu_seqlens is None:
-        if q.shape[0] != B:
-            raise ValueError(f"tree_attention: {q.shape[0]} new tokens of {B} streams need cu_seqlens")
-        cu, most = torch.arange(B + 1, device=dev), 1 if max_new is None else int(max_new)
+        if n != B:
+            raise ValueError(f"tree_attention: {n} new tokens of {B} streams need cu_seqlens")
+        cu, most = torch.arange(B + 1, device=q.device), 1 if max_new is None else int(max_new)
     else:
         cu, most = _ints(cu_seqlens, "tree_attention cu_seqlens", torch.int64, dev, B + 1), 64 if max_new is None else int(max_new)
-    par = None if parents is None else _ints(parents, "tree_attention parents", torch.int32, dev, q.shape[0])
-    room = page_table.shape[1] * kp.shape[2]
-    most_context = room if max_context is None else min(int(max_context), room)
-    y = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else _out(out, "tree_attention out", q.shape, q)
-    a = _tree_args(q, k, v, kp, vp, page_table, B, most_context, most, _scale(scale, q.shape[-1], "tree_attention"))
-    a.cu_new, a.context_lens, a.page_table = cu.data_ptr(), lens.data_ptr(), page_table.data_ptr()
-    a.parents = None if par is None else par.data_ptr()
-    for name, t in (("q", q), ("k", k), ("v", v), ("k_pages", kp), ("v_pages", vp), ("y", y)):
-        _set(a, name, t)
-    with _on(dev):
-        ws = workspace
-        if ws is None:
-            ws = torch.empty(N.lib().kdn_tree_attn_workspace_bytes(_ref(a)), dtype=torch.uint8, device=dev)
-        elif ws.device != dev or not ws.is_contiguous():
-            raise ValueError(f"tree_attention: the workspace is contiguous on {dev}")
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
-        N.check(N.lib().kdn_tree_attn(_ref(a), _stream(dev)), "kdn_tree_attn")
-    return y
+    par = None if parents is None else _ints(parents, "tree_attention parents", torch.int32, dev, n)
+    room = width * P
+    ctx = room if max_context is None else min(int(max_context), room)
+    y = _new(q, (n, H, d)) if out is None else _out(out, "tree_attention out", q.shape, q)
+    sizes = (B, n, most, ctx, H, KV, d, _tag(q.dtype, what), _scale(scale, d, what), P, pages, width, page_table.stride(0))
+    with _device(dev):
+        if workspace is None:
+            workspace = q.new_empty(N.lib().kdn_tree_attn_workspace_bytes(_TREE.pack(*sizes, *_NO_TENSORS)), dtype=torch.uint8)
+        elif workspace.get_device() != dev or not workspace.is_contiguous():
+            raise ValueError(f"tree_attention: the workspace is contiguous on {q.device}")
+        N.check(N.lib().kdn_tree_attn(_TREE.pack(*sizes, cu.data_ptr(), lens.data_ptr(), page_table.data_ptr(), 0 if par is None else par.data_ptr(),
+                                                 *qs[1:], *ks[1:], *vs[1:], *kp[1:], *vp[1:], *y[1:], workspace.data_ptr(), workspace.nbytes),
+                                      _raw_stream(dev)), "kdn_tree_attn")
+    return y[0]
+
+
+_NO_TENSORS = (0,) * 26  # the tensor fields of kdn_tree_attn_args, where only sizes are read
 
 
 def tree_workspace_bytes(streams: int, H: int, H_kv: int, d: int, dtype: torch.dtype, page_tokens: int, max_context: int,
                          max_new: int = 1) -> int:
     """Bytes of `tree_attention`'s workspace for up to these sizes (0: not supported)."""
-    a = N.TreeAttnArgs()
-    a.num_seqs, a.total_new, a.max_new, a.max_context = streams, streams, max_new, max_context
-    a.H, a.H_kv, a.d, a.dtype, a.scale = H, H_kv, d, _tag(dtype, "tree_attention"), 1.0
-    a.page_tokens, a.num_pages, a.table_width = page_tokens, 1, -(-max_context // page_tokens)
-    return int(N.lib().kdn_tree_attn_workspace_bytes(_ref(a)))
+    return int(N.lib().kdn_tree_attn_workspace_bytes(_TREE.pack(streams, streams, max_new, max_context, H, H_kv, d, _tag(dtype, "tree_attention"),
+                                                                1.0, page_tokens, 1, -(-max_context // page_tokens), 0, *_NO_TENSORS)))

@@ -38,6 +38,19 @@ def test_struct_layouts(cname, mirror, tmp_path):
     assert got == [ctypes.sizeof(mirror), *(getattr(mirror, f).offset for f in fields)]
 
 
+@pytest.mark.parametrize("packed,mirror", [(anchor._ATTN, N.AttnArgs), (anchor._ATTN_BWD, N.AttnBwdArgs), (anchor._ROTARY, N.RotaryArgs),
+                                           (anchor._APPEND, N.PageAppendArgs), (anchor._TREE, N.TreeAttnArgs)])
+def test_packed_arguments_are_the_mirrors(packed, mirror):
+    """Numbers 1, 2, ... packed in order read back from the mirror's fields in order (arrays flattened)."""
+    n = len(packed.unpack(bytes(packed.size)))
+    a = mirror.from_buffer_copy(packed.pack(*range(1, n + 1)).ljust(ctypes.sizeof(mirror), b"\0"))
+    got = []
+    for name, _ in mirror._fields_:
+        x = getattr(a, name)
+        got += list(x) if isinstance(x, ctypes.Array) else [x]
+    assert got == list(range(1, n + 1))
+
+
 def _attn(**kw):
     a = N.AttnArgs()
     a.num_seqs, a.total_q, a.total_k, a.H, a.H_kv, a.d, a.dtype, a.scale = 1, 8, 8, 4, 2, 64, 1, 0.125
@@ -129,7 +142,7 @@ def test_tree_arguments():
     assert call(args(num_seqs=0), None) == 0
     grows = [size(args(num_seqs=n, max_context=c)) for n in (1, 2, 7, 8, 9, 64, 300) for c in (4096,)]
     assert grows == sorted(grows)
-    grows = [size(args(max_context=c)) for c in (0, 1, 256, 257, 1000, 4096)]
+    grows = [size(args(max_context=c)) for c in (0, 1, 128, 129, 1000, 4096)]
     assert grows == sorted(grows) and grows[0] == 16
 
 

@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   __shared__ __attribute__((aligned(256))) unsigned char lds[S::LDS];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = w % SPLIT;
-  // the last tiles (the longest rows) first, and an XCD's heads next to one another so that its L2 holds their keys
+  // an XCD's heads next to one another, so that its L2 holds their keys
   int64_t id = blockIdx.x;
   int h;
   if (p.H % 8 == 0) {
@@ -41,8 +41,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   } else {
     h = (int)(id % p.H);
   }
-  const int64_t slot = slots - 1 - id / p.H;
-  const SeqTile t = find_tile<S::ROWS>(p.cu_q, p.nseq, p.total_q, slot, lane);
+  const SeqTile t = find_heavy<S::ROWS, false>(p.cu_q, p.nseq, p.total_q, id / p.H, slots, lane);
   if (t.row0 < 0) return;
   const int lenq = t.len;
   int64_t klo;

@@ -14,9 +14,9 @@
 
 namespace kdn {
 
-// delta: sixteen lanes a row, eight values each at a time.
+// delta, and lse times log2 e: sixteen lanes a row, eight values each at a time.
 template <class P>
-__global__ void __launch_bounds__(256) attn_delta_kernel(AttnParams p, float* delta) {
+__global__ void __launch_bounds__(256) attn_delta_kernel(AttnParams p, float* lse2, float* delta) {
   typedef typename P::elem E;
   const int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (row, head), heads fastest
   const int j = threadIdx.x & 15;
@@ -42,7 +42,10 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnParams p, float* de
   sum += xor_shuffle<2>(sum);
   sum += xor_shuffle<4>(sum);
   sum += xor_shuffle<8>(sum);
-  if (j == 0) delta[h * p.total_q + row] = sum;
+  if (j == 0) {
+    delta[h * p.total_q + row] = sum;
+    lse2[h * p.total_q + row] = p.lse[h * p.total_q + row] * LOG2E;
+  }
 }
 
 // dk and dv of 128 / SPLIT keys: a wave owns 32 keys (a lane one), their K and V fragments and the transposed sums in
@@ -66,9 +69,9 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   __shared__ __attribute__((aligned(256))) unsigned char lds[S::LDS];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = w % SPLIT;
-  const int64_t id = blockIdx.x;  // the first keys, which the most rows see, first
+  const int64_t id = blockIdx.x;
   const int e = (int)(id % p.KV), sub = (int)(id / p.KV % p.subsets), heads = p.G / p.subsets;
-  const SeqTile t = find_tile<S::KEYS>(p.cu_k, p.nseq, p.total_k, id / p.KV / p.subsets, lane);
+  const SeqTile t = find_heavy<S::KEYS, true>(p.cu_k, p.nseq, p.total_k, id / p.KV / p.subsets, slots, lane);
   if (t.row0 < 0) return;
   const int lenk = t.len;
   int64_t qlo;
@@ -106,7 +109,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
     stage_q(reinterpret_cast<const E*>(p.q) + (qlo + r0) * p.qs[0] + (int64_t)h * p.qs[1], last, to);
     stage_y(reinterpret_cast<const E*>(p.dy) + (qlo + r0) * p.dys[0] + (int64_t)h * p.dys[1], last, to + TILE);
     if (64 * w < 2 * ROWS) {  // lse of the rows, then delta, 64 a wave
-      const float* src = (64 * w < ROWS ? p.lse : p.delta) + (int64_t)h * p.total_q + qlo + r0;
+      const float* src = (64 * w < ROWS ? p.lse2 : p.delta) + (int64_t)h * p.total_q + qlo + r0;
       copy4_to_lds(buffer_at(src), 4 * min(64 * w % ROWS + lane, last), to + 2 * TILE + 256 * w);
     }
   };
@@ -136,7 +139,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int i = 4 * a + x, r = rho(half, i);
-          float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls[x] * LOG2E));
+          float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls[x]));
           float d = pr * (dp[i] - de[x]);
           if (!whole) {
             const bool sees = r >= lo && r < hi;
@@ -233,7 +236,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   } else {
     h = (int)(id % p.H);
   }
-  const SeqTile t = find_tile<S::ROWS>(p.cu_q, p.nseq, p.total_q, slots - 1 - id / p.H, lane);
+  const SeqTile t = find_heavy<S::ROWS, false>(p.cu_q, p.nseq, p.total_q, id / p.H, slots, lane);
   if (t.row0 < 0) return;
   const int lenq = t.len;
   int64_t klo;
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
     }
   }
   const float c = p.scale * LOG2E;
-  const float ls = p.lse[(int64_t)h * p.total_q + at] * LOG2E, de = p.delta[(int64_t)h * p.total_q + at];
+  const float ls = p.lse2[(int64_t)h * p.total_q + at], de = p.delta[(int64_t)h * p.total_q + at];
   f32x16 dq[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) dq[ct] = zero16();
@@ -347,12 +350,12 @@ static int launch_dq(const AttnParams& p, hipStream_t st) {
 }
 
 template <class P>
-static int launch_bwd(const AttnParams& p, float* delta, hipStream_t st) {
+static int launch_bwd(const AttnParams& p, float* lse2, float* delta, hipStream_t st) {
   int rc = KDN_OK;
   if (p.total_q > 0) {
     const int64_t rows = p.total_q * p.H;
     if ((rows + 15) / 16 > INT32_MAX) return KDN_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL(attn_delta_kernel<P>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, p, delta);
+    hipLaunchKernelGGL(attn_delta_kernel<P>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, p, lse2, delta);
     if ((rc = launch_status()) != KDN_OK) return rc;
   }
   if (p.total_k > 0) {
@@ -375,7 +378,7 @@ static int bwd_subsets(const kdn_attn_args* f) {
   while (n < G && (tiles * n < 1024 || G % n != 0)) ++n;
   return n;
 }
-static size_t bwd_delta_bytes(const kdn_attn_args* f) { return ((size_t)f->H * (size_t)f->total_q * 4 + 255) / 256 * 256 + 256; }
+static size_t bwd_row_bytes(const kdn_attn_args* f) { return ((size_t)f->H * (size_t)f->total_q * 4 + 255) / 256 * 256 + 256; }
 static size_t bwd_part_bytes(const kdn_attn_args* f) { return (size_t)f->total_k * (size_t)f->H_kv * (size_t)f->d * 4; }
 
 }  // namespace kdn
@@ -385,7 +388,7 @@ using namespace kdn;
 extern "C" size_t kdn_attn_bwd_workspace_bytes(const kdn_attn_bwd_args* a) {
   if (!a || attn_check(a->fwd) != KDN_OK) return 0;
   const int subsets = bwd_subsets(a->fwd);
-  return bwd_delta_bytes(a->fwd) + (subsets > 1 ? 2 * subsets * bwd_part_bytes(a->fwd) : 0);
+  return 2 * bwd_row_bytes(a->fwd) + (subsets > 1 ? 2 * subsets * bwd_part_bytes(a->fwd) : 0);
 }
 
 extern "C" int kdn_attn_bwd(const kdn_attn_bwd_args* a, void* stream) {
@@ -408,16 +411,17 @@ extern "C" int kdn_attn_bwd(const kdn_attn_bwd_args* a, void* stream) {
   if (!a->workspace || a->workspace_bytes < kdn_attn_bwd_workspace_bytes(a)) return KDN_ERR_WORKSPACE_TOO_SMALL;
   AttnParams p = attn_params(f);
   p.dy = a->dy; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
-  p.delta = reinterpret_cast<const float*>(a->workspace);
+  float *lse2 = reinterpret_cast<float*>(a->workspace), *delta = lse2 + bwd_row_bytes(f) / 4;
+  p.lse2 = lse2;
+  p.delta = delta;
   p.subsets = bwd_subsets(f);
-  p.part_dk = reinterpret_cast<float*>((unsigned char*)a->workspace + bwd_delta_bytes(f));
+  p.part_dk = reinterpret_cast<float*>((unsigned char*)a->workspace + 2 * bwd_row_bytes(f));
   p.part_dv = p.part_dk + (size_t)p.subsets * bwd_part_bytes(f) / 4;
   for (int i = 0; i < 2; ++i) {
     p.dys[i] = a->dy_stride[i]; p.dqs[i] = a->dq_stride[i]; p.dks[i] = a->dk_stride[i]; p.dvs[i] = a->dv_stride[i];
   }
-  float* delta = reinterpret_cast<float*>(a->workspace);
   hipStream_t st = as_stream(stream);
   if (f->dtype == KDN_DTYPE_BF16)
-    return f->d == 64 ? launch_bwd<AttnBF16<64>>(p, delta, st) : launch_bwd<AttnBF16<128>>(p, delta, st);
-  return f->d == 64 ? launch_bwd<AttnF32<64>>(p, delta, st) : launch_bwd<AttnF32<128>>(p, delta, st);
+    return f->d == 64 ? launch_bwd<AttnBF16<64>>(p, lse2, delta, st) : launch_bwd<AttnBF16<128>>(p, lse2, delta, st);
+  return f->d == 64 ? launch_bwd<AttnF32<64>>(p, lse2, delta, st) : launch_bwd<AttnF32<128>>(p, lse2, delta, st);
 }

@@ -303,6 +303,47 @@ __device__ __forceinline__ SeqTile find_tile(const int64_t* cu, int64_t nseq, in
   t.row0 = tile < 0 || tile * ROWS >= t.len ? -1 : (int)(tile * ROWS);
   return t;
 }
+// The tile that is the id-th in the order of most work first, a tile's work being its place in its sequence (its rows see
+// that many tiles of keys; counted from the sequence's end for the keys, whose first ones the most rows see): what runs
+// longest starts first, whichever sequence it is of.  Up to 63 sequences; with more, slot `slots` - 1 - id of find_tile (each
+// sequence's own tiles most work first).  Lane b has sequence b's tiles nt; N(t), the tiles at place t or behind it, is
+// the sum of max(nt - t, 0), and the tile's place the last t with N(t) > id.
+template <int ROWS, bool FROM_END>
+__device__ __forceinline__ SeqTile find_heavy(const int64_t* cu, int64_t nseq, int64_t total, int64_t id, int64_t slots, int lane) {
+  if (nseq >= 64) {
+    SeqTile t = find_tile<ROWS>(cu, nseq, total, slots - 1 - id, lane);
+    if (FROM_END && t.row0 >= 0) t.row0 = (t.len - 1) / ROWS * ROWS - t.row0;
+    return t;
+  }
+  const int n = (int)nseq + 1;
+  const int64_t lo = seq_start(cu, total, min((int64_t)lane, nseq));
+  const int64_t hi = lane < nseq ? max(seq_start(cu, total, lane + 1), lo) : total;
+  const int len = lane < n ? (int)(hi - lo) : 0, nt = (len + ROWS - 1) / ROWS;
+  auto behind = [&](int t) {
+    int sum = 0;
+    for (int b = 0; b < n; ++b) sum += max(__builtin_amdgcn_readlane(nt, b) - t, 0);
+    return sum;
+  };
+  int most = 0;
+  for (int b = 0; b < n; ++b) most = max(most, __builtin_amdgcn_readlane(nt, b));
+  SeqTile s;
+  s.row0 = -1;
+  if (id >= behind(0)) return s;
+  int t = 0;
+  for (int range = most; range > 1;) {
+    const int step = (range + 63) / 64, hits = __popcll(__ballot(lane * step < range && behind(t + lane * step) > id));
+    t += (hits - 1) * step;
+    range = min(step, range - (hits - 1) * step);
+  }
+  const int rank = (int)id - behind(t + 1);
+  const uint64_t there = __ballot(nt > t);
+  const int seq = __ffsll((unsigned long long)__ballot((there >> lane & 1) && __popcll(there & ((1ull << lane) - 1)) == rank)) - 1;
+  s.seq = __builtin_amdgcn_readfirstlane(seq);
+  s.len = __builtin_amdgcn_readlane(len, s.seq);
+  s.lo = (int64_t)__builtin_amdgcn_readlane((int)(lo >> 32), s.seq) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, s.seq);
+  s.row0 = (FROM_END ? __builtin_amdgcn_readlane(nt, s.seq) - 1 - t : t) * ROWS;
+  return s;
+}
 // The other tensor's rows of a tile's sequence: none for the rows past the last one.
 __device__ __forceinline__ void other_rows(const int64_t* cu, int64_t nseq, int64_t total, int seq, int64_t& lo, int& len) {
   lo = seq < nseq ? seq_start(cu, total, seq) : 0;
@@ -317,7 +358,7 @@ struct AttnParams {
   int64_t lows[2];
   int64_t qs[2], ks[2], vs[2], ys[2], dys[2], dqs[2], dks[2], dvs[2];  // element strides [token][head]
   float* lse;          // [H][total_q]
-  const float* delta;  // [H][total_q]: dy . y of each row (backward)
+  const float *lse2, *delta;  // [H][total_q]: lse in units of log 2, and dy . y of each row (backward)
   const int64_t *cu_q, *cu_k;
   int64_t nseq, total_q, total_k;
   float *part_dk, *part_dv;  // [subset][total_k][KV][D] sums of dk and dv over a subset of a key head's query heads (subsets > 1)

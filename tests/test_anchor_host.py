@@ -81,10 +81,10 @@ def test_backward_arguments():
     a = _attn(lse=1 << 12)
     b = N.AttnBwdArgs()
     b.fwd = ctypes.addressof(a)
-    assert N.lib().kdn_attn_bwd_workspace_bytes(ctypes.byref(b)) == 512 + 2 * 2 * 8 * 2 * 64 * 4  # delta; dk and dv of two heads each
+    assert N.lib().kdn_attn_bwd_workspace_bytes(ctypes.byref(b)) == 1024 + 2 * 2 * 8 * 2 * 64 * 4  # lse and delta; dk and dv of two heads each
     assert N.lib().kdn_attn_bwd(ctypes.byref(b), None) == -1  # no dy
     b.dy = b.dq = b.dk = b.dv = b.workspace = 1 << 12
-    b.workspace_bytes = 512 + 2 * 2 * 8 * 2 * 64 * 4 - 1
+    b.workspace_bytes = 1024 + 2 * 2 * 8 * 2 * 64 * 4 - 1
     assert N.lib().kdn_attn_bwd(ctypes.byref(b), None) == -3
     assert N.lib().kdn_attn_bwd(None, None) == -1
     b.fwd = None

@@ -240,3 +240,46 @@ def test_oracle_gradients_against_differences():
 def test_oracle_rows_that_see_nothing():
     r = oa.attention(torch.ones(4, 1, 4), torch.ones(1, 1, 4), torch.ones(1, 1, 4), [0, 4], [0, 1], dy=torch.ones(4, 1, 4))
     assert not r["y"][:3].any() and r["y"][3].eq(1).all() and torch.isneginf(r["lse"][0, :3]).all() and not r["dq"][:3].any()
+
+
+def test_hybrid_pool_bookkeeping_on_the_host():
+    from serving import HybridMemoryPool
+    pool = HybridMemoryPool(4, 64, num_layers=1, num_heads=1, val_dim=16, lifted_dim=64, device="cpu", anchor_layers=2, anchor_heads=1,
+                            anchor_pages=6)
+    a = pool.allocate_stream(20)
+    plan = pool.anchor_plan([a], [20])
+    assert plan.rows.tolist() == list(range(20)) and plan.positions.tolist() == list(range(20)) and plan.context_lens.tolist() == [0]
+    b = pool.fork_stream(a)
+    plan = pool.anchor_plan([b, a], [1, 2])
+    assert plan.rows.tolist() == [2 * P + 4, P + 4, P + 5] and plan.cu_seqlens.tolist() == [0, 1, 3] and plan.context_lens.tolist() == [20, 20]
+    assert plan.page_table.tolist() == [[0, 2], [0, 1]] and (plan.max_new, plan.max_context) == (2, 20)
+    plan = pool.anchor_plan([a, b], [2, 1], depths=[0, 1, 0])
+    assert plan.positions.tolist() == [22, 23, 21] and plan.rows is None and pool.anchor_tokens(a) == 22
+    with pytest.raises(RuntimeError):
+        pool.anchor_plan([a, b], [30, 40])  # five pages where three are free
+    assert (pool.anchor_tokens(a), pool.anchor_tokens(b), pool.anchor_pages_free) == (22, 21, 3)
+    with pytest.raises(ValueError):
+        pool.anchor_plan([a, a], [1, 1])
+    pool.release_stream(a)
+    assert pool.anchor_pages_used == 2 and pool.anchor_compact() == 1  # pages 0 and 2 are b's
+    assert pool.anchor_plan([b], [1]).page_table.tolist() == [[0, 1]]
+    assert HybridMemoryPool(2, 64, num_layers=1, num_heads=1, val_dim=16, lifted_dim=64, device="cpu").anchor_layers == 0
+
+
+@pytest.mark.timeout(900)
+def test_host_paths_clean_under_asan_and_ubsan(tmp_path):
+    """The argument checks and the pages' bookkeeping above, in a child process, against the library with its host code
+    instrumented (as tests/test_host_sanitizers.py does for the rest)."""
+    import sys
+    from kdn import build as kbuild
+    runtime = kbuild.asan_runtime()
+    if os.environ.get("KDN_LIBRARY") or not runtime or not os.path.exists(kbuild.hipcc()):
+        pytest.skip("hipcc's ASan runtime is not installed, or this is the child")
+    lib = kbuild.build_host_sanitized(str(tmp_path / "hostsan"))
+    env = dict(os.environ, KDN_LIBRARY=lib, LD_PRELOAD=runtime, UBSAN_OPTIONS="halt_on_error=1:print_stacktrace=1:exitcode=87",
+               ASAN_OPTIONS="detect_leaks=0:halt_on_error=1:abort_on_error=0:exitcode=86")
+    res = subprocess.run([sys.executable, "-m", "pytest", "-q", "-m", "not gpu", "-p", "no:cacheprovider", __file__], cwd=REPO, env=env,
+                         capture_output=True, text=True, timeout=600)
+    report = res.stdout[-3000:] + res.stderr[-3000:]
+    assert res.returncode == 0 and "ERROR: AddressSanitizer" not in report and "runtime error" not in report, report
+    assert " passed" in report or res.stdout.count(".") >= 30, report

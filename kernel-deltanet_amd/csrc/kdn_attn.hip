@@ -140,6 +140,68 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
     staged_barrier();
     step(j, lds + (S::BUFS == 2 ? (j & 1) * 2 * TILE : 0), lds + (S::BUFS == 2 ? (~j & 1) * 2 * TILE : 0));
   }
+  // A weight of zero times an infinity or NaN is no number: a tile that a row sees in part would give it what a key that it
+  // does not see holds.  Where the sums are not all numbers, the workgroup goes over its tiles once more, slowly and with
+  // the maxima known: V's numbers alone, weighted; then for each sum a count of the infinities, minus infinities and NaNs of
+  // seen keys.  (Selecting V's values in the loop itself costs its registers: 237 for 164 at 64 features, two waves for three.)
+  bool odd = false;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) odd |= !(__builtin_fabsf(o[ct][i]) < INFINITY);
+  __syncthreads();
+  int* flag = reinterpret_cast<int*>(lds);
+  if (lane == 0) flag[w] = 0;
+  if (live && odd) flag[w] = 1;  // (a wave's LDS accesses are in order)
+  __syncthreads();
+  const bool again = __builtin_amdgcn_readfirstlane(flag[0] | flag[1] | flag[2] | flag[3]);
+  if (again) {
+    const float mc = m == -INFINITY ? 0.f : m * c;
+    const E* src = reinterpret_cast<const E*>(p.q) + (t.lo + min(row, lenq - 1)) * p.qs[0] + (int64_t)h * p.qs[1];
+    f32x16 sum[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) o[ct] = zero16();
+#pragma unroll 1
+    for (int kind = 0; kind <= 3; ++kind) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) sum[ct] = zero16();
+#pragma unroll 1
+      for (int j = 0; j < ntiles; ++j) {
+        __syncthreads();
+        stage(j, lds);
+        staged_barrier();
+#pragma unroll 1
+        for (int b = 0; b < S::BLOCKS; ++b) {
+          const int r0 = 32 * (S::BLOCKS * part + b), limit = row + off - (j * KEYS + r0);  // keys of the block that the row sees
+          f32x16 x = zero16();
+#pragma unroll 1
+          for (int ks = 0; ks < KS; ++ks) x = P::mma(x, P::row_frag(lds, r0 + (lane & 31), ks, half), P::load(src + 16 * ks + 8 * half));
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const bool sees = rho(half, i) <= limit;
+            x[i] = !sees ? 0.f : kind == 0 ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -mc)) : 1.f;
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const typename P::frag xf = P::from_acc(x, u);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+              const typename P::frag v = P::col_frag(lds + TILE, r0 + 16 * u, ct, lane);
+              typename P::frag is;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) is[e] = P::is_kind(v, e, kind) ? (kind == 0 ? v[e] : (E)1.f) : (E)0.f;
+              sum[ct] = P::mma(sum[ct], is, xf);
+            }
+          }
+        }
+      }
+      const float value = kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[ct][i] += kind == 0 ? sum[ct][i] : sum[ct][i] > 0.f ? value : 0.f;
+    }
+  }
   l = half_sum(l);
   E* dst = reinterpret_cast<E*>(p.out) + (t.lo + row) * p.ys[0] + (int64_t)h * p.ys[1];
   E* low = p.low ? reinterpret_cast<E*>(p.low) + (t.lo + row) * p.lows[0] + (int64_t)h * p.lows[1] : nullptr;

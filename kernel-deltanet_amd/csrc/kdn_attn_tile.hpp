@@ -42,6 +42,9 @@ __device__ __host__ __forceinline__ constexpr int piece_swizzle(int r) {
   return PIECES == 8 ? ((r >> 1) & 1) << 2 | ((r >> 2) & 3) : (r & 3) << 2 | ((r >> 2) & 3);
 }
 
+// 0: a number, 1: infinity, 2: minus infinity, 3: no number.
+__device__ __forceinline__ int value_kind(float x) { return x != x ? 3 : x == INFINITY ? 1 : x == -INFINITY ? 2 : 0; }
+
 template <int D_>
 struct AttnBF16 {
   typedef __bf16 elem;
@@ -59,6 +62,16 @@ struct AttnBF16 {
     for (int s = 0; s < 8; ++s) r[s] = (__bf16)v[8 * m + s];
     return r;
   }
+  // the fragment with its infinities and NaNs as zeros; `rest` keeps whether there was one
+  __device__ __forceinline__ static frag finite(const frag& f, bool& rest) {
+    typedef __attribute__((ext_vector_type(8))) unsigned short u16x8;
+    const u16x8 x = __builtin_bit_cast(u16x8, f), gap = (x & (unsigned short)0x7f80) ^ (unsigned short)0x7f80;  // 0: no number
+    const u16x8 one = __builtin_elementwise_min(gap, (u16x8)(unsigned short)1);
+    const u32x4 all = __builtin_bit_cast(u32x4, one);
+    rest |= (all[0] & all[1] & all[2] & all[3]) != 0x00010001u;
+    return __builtin_bit_cast(frag, (u16x8)(x & (u16x8)((unsigned short)0 - one)));
+  }
+  __device__ __forceinline__ static bool is_kind(const frag& f, int s, int kind) { return value_kind((float)f[s]) == kind; }
   // lane l slot s = T[row][16 ks + 8 (l/32) + s], row the lane's own
   __device__ __forceinline__ static frag row_frag(const unsigned char* t, int row, int ks, int half) {
     return *reinterpret_cast<const frag*>(t + row * ROW + 16 * ((2 * ks + half) ^ piece_swizzle<PIECES>(row)));
@@ -99,6 +112,17 @@ struct AttnF32 {
     for (int s = 0; s < 8; ++s) r[s] = v[8 * m + s];
     return r;
   }
+  __device__ __forceinline__ static frag finite(const frag& f, bool& rest) {
+    frag r;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const bool number = __builtin_fabsf(f[s]) < INFINITY;
+      rest |= !number;
+      r[s] = number ? f[s] : 0.f;
+    }
+    return r;
+  }
+  __device__ __forceinline__ static bool is_kind(const frag& f, int s, int kind) { return value_kind(f[s]) == kind; }
   __device__ __forceinline__ static frag row_frag(const unsigned char* t, int row, int ks, int half) {
     const int c = 4 * ks + 2 * half, f = piece_swizzle<PIECES>(row);
     return pair_to8(*reinterpret_cast<const f32x4*>(t + row * ROW + 16 * (c ^ f)),
@@ -233,6 +257,46 @@ __device__ __forceinline__ void store_row32(float* row, const f32x16& v, float f
   for (int m = 0; m < 4; ++m) {
     const f32x4 out = {v[4 * m] * f, v[4 * m + 1] * f, v[4 * m + 2] * f, v[4 * m + 3] * f};
     if (live) *reinterpret_cast<f32x4*>(row + 8 * m + 4 * half) = out;
+  }
+}
+
+// o += V^T P over 16 KK keys of which rows see only some: `s` the weights (zero where unseen), seen(x) whether the lane's row
+// sees key x of them.  A weight of zero times an infinity is no number, and a row would get what a key that it
+// does not see holds: V goes into the products with such values as zeros, and where there are any, three more products count,
+// for each sum, the infinities, minus infinities and NaNs of seen keys alone.
+template <class P, int KK, int CT, class Seen>
+__device__ __forceinline__ void masked_values(f32x16 (&o)[CT], const unsigned char* vt, int r0, int lane, const f32x16* s, Seen seen) {
+  bool rest = false;
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) {
+    __builtin_amdgcn_sched_barrier(0);  // one block's operands at a time: registers
+    const typename P::frag pf = P::from_acc(s[kk >> 1], kk & 1);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::finite(P::col_frag(vt, r0 + 16 * kk, ct, lane), rest), pf);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  if (!__any(rest)) return;
+  const int half = lane >> 5;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll 1
+    for (int kind = 1; kind <= 3; ++kind) {
+      f32x16 count = zero16();
+#pragma unroll 1
+      for (int kk = 0; kk < KK; ++kk) {
+        const typename P::frag v = P::col_frag(vt, r0 + 16 * kk, ct, lane);
+        typename P::frag is, sees;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          is[x] = (typename P::elem)(P::is_kind(v, x, kind) ? 1.f : 0.f);
+          sees[x] = (typename P::elem)(seen(16 * kk + rho(half, x)) ? 1.f : 0.f);
+        }
+        count = P::mma(count, is, sees);
+      }
+      const float value = kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[ct][i] += count[i] > 0.f ? value : 0.f;
+    }
   }
 }
 

@@ -10,6 +10,7 @@
 //   - more: each wave has 32 rows of its own, and all read the same tiles of 64 keys, as in the prompt's kernel.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include "kdn_attn_tile.hpp"
 
 namespace kdn {
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
   const int b = t.b, ch = t.ch, be = b * p.KV + e;
   const int rows = t.n * p.G, row = min(lane & 31, rows - 1), tok = row / p.G, h = e * p.G + row % p.G;
   const bool drafts = ch == t.chunks - 1;  // the last chunk has the new tokens too
-  const int nt = t.c1 > t.c0 ? (t.c1 - t.c0 + 31) / 32 : 0, total = nt + (drafts ? (t.n + 31) / 32 : 0);
+  const int nt = t.c1 > t.c0 ? (t.c1 - t.c0 + 31) / 32 : 0, total = nt + (drafts ? 1 : 0);
   unsigned char* mine = lds + w * 2 * STAGE;
   // the pages of a tile's two groups, known a tile ahead of its copies
   int page0 = 0, page1 = 0;
@@ -219,16 +220,16 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
     page0 = page_of(p, b, key_group(t.c0 + 32 * at, t.c1 - 1).key);
     page1 = page_of(p, b, key_group(t.c0 + 32 * at + 16, t.c1 - 1).key);
   };
+  auto stage_drafts = [&](unsigned char* to) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      stage_new<P>(p, t.lo, e, key_group(16 * (x & 1), t.n - 1), x >> 1, to + (x >> 1) * STAGE / 2, x & 1, lane);
+  };
   auto stage = [&](int at, unsigned char* to) {
-    if (at < nt) {
+    if (at >= nt) return stage_drafts(to);
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        stage_paged<P>(p, x & 1 ? page1 : page0, e, key_group(t.c0 + 32 * at + 16 * (x & 1), t.c1 - 1), x >> 1, to + (x >> 1) * STAGE / 2, x & 1, lane);
-    } else {
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        stage_new<P>(p, t.lo, e, key_group(32 * (at - nt) + 16 * (x & 1), t.n - 1), x >> 1, to + (x >> 1) * STAGE / 2, x & 1, lane);
-    }
+    for (int x = 0; x < 4; ++x)
+      stage_paged<P>(p, x & 1 ? page1 : page0, e, key_group(t.c0 + 32 * at + 16 * (x & 1), t.c1 - 1), x >> 1, to + (x >> 1) * STAGE / 2, x & 1, lane);
   };
   pages(w);
   if (w < total) stage(w, mine);
@@ -249,11 +250,16 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
   for (int ct = 0; ct < CT; ++ct) o[ct] = zero16();
   float m = -INFINITY, l = 0.f;
   const float c = p.scale * LOG2E;
-  // one tile, read from `kt` while the next one's copies go to `next` (as in the prompt's kernel)
-  auto step = [&](int at, const unsigned char* __restrict kt, unsigned char* __restrict next) {
+  // one tile, read from `kt` while the next one's copies go to `next` (as in the prompt's kernel);
+  // `whole`: of the context, all 32 keys of it there
+  auto step = [&](auto whole, int at, const unsigned char* __restrict kt, unsigned char* __restrict next) {
     if (at + W < total) {
-      stage(at + W, next);
-      pages(at + 2 * W);
+      if constexpr (whole.value) {
+        stage(at + W, next);
+        pages(at + 2 * W);
+      } else {
+        stage_drafts(next);
+      }
       // everything but the last STAGE / 1024 copies, the next tile's, has arrived
       if constexpr (STAGE == 8192) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
       else if constexpr (STAGE == 16384) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
@@ -266,26 +272,31 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) s[0] = P::mma(s[0], P::row_frag(kt, lane & 31, ks, half), q[ks]);
     sched_products<P, KS, P::ROW_READS>();
-    if (at >= nt) {
-      const uint32_t bits = (uint32_t)(sees >> (32 * (at - nt)));
+    uint32_t bits = ~0u;  // the keys of the tile that the row sees
+    if constexpr (!whole.value) {
+      bits = at >= nt ? (uint32_t)sees : (uint32_t)((1ull << (t.c1 - t.c0 - 32 * at)) - 1);
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[0][i] = bits >> rho(half, i) & 1 ? s[0][i] : -INFINITY;
-    } else if (t.c0 + 32 * at + 32 > t.c1) {
-      const int limit = t.c1 - t.c0 - 32 * at;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[0][i] = rho(half, i) < limit ? s[0][i] : -INFINITY;
     }
     softmax_step<1>(s, m, l, o, c);
+    if constexpr (whole.value) {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      const typename P::frag pf = P::from_acc(s[0], kk);
+      for (int kk = 0; kk < 2; ++kk) {
+        const typename P::frag pf = P::from_acc(s[0], kk);
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, 16 * kk, ct, lane), pf);
+        for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, 16 * kk, ct, lane), pf);
+      }
+      sched_products<P, 2 * CT, P::COL_READS>();
+    } else {
+      masked_values<P, 2>(o, vt, 0, lane, s, [&](int x) { return bits >> x & 1; });
     }
-    sched_products<P, 2 * CT, P::COL_READS>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its slot may be written again
   };
-  for (int at = w, buf = 0; at < total; at += W, buf ^= 1) step(at, mine + buf * STAGE, mine + (buf ^ 1) * STAGE);
+  const int full = (t.c1 - t.c0) / 32;
+  int at = w, buf = 0;
+  for (; at < full; at += W, buf ^= 1) step(std::true_type{}, at, mine + buf * STAGE, mine + (buf ^ 1) * STAGE);
+#pragma unroll 1
+  for (; at < total; at += W, buf ^= 1) step(std::false_type{}, at, mine + buf * STAGE, mine + (buf ^ 1) * STAGE);
   // the waves' sums, each scaled to the common maximum, added in the waves' order
   l = half_sum(l);
   if (half == 0) wm[w][lane] = m, wl[w][lane] = l;
@@ -397,7 +408,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
   for (int ct = 0; ct < CT; ++ct) o[ct] = zero16();
   float m = -INFINITY, l = 0.f;
   const float c = p.scale * LOG2E;
-  auto step = [&](int at, const unsigned char* __restrict kt, unsigned char* __restrict next) {
+  auto step = [&](auto whole, int at, const unsigned char* __restrict kt, unsigned char* __restrict next) {
     if (at + BUFS - 1 < total) {
       stage(at + BUFS - 1, next);
       pages(at + BUFS);
@@ -410,34 +421,39 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
 #pragma unroll
       for (int u = 0; u < 2; ++u) s[u] = P::mma(s[u], P::row_frag(kt, 32 * u + (lane & 31), ks, half), q[ks]);
     sched_products<P, 2 * KS, P::ROW_READS>();
-    if (at >= nt) {
+    uint64_t bits = ~0ull;  // the keys of the tile that the row sees
+    if constexpr (!whole.value) {
+      bits = at >= nt ? sees : (1ull << (t.c1 - t.c0 - 64 * at)) - 1;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[u][i] = (uint32_t)(sees >> (32 * u)) >> (4 * half) >> rho(0, i) & 1 ? s[u][i] : -INFINITY;
-    } else if (t.c0 + 64 * at + 64 > t.c1) {
-      const int limit = t.c1 - t.c0 - 64 * at;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[u][i] = 32 * u + rho(half, i) < limit ? s[u][i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) s[u][i] = (uint32_t)(bits >> (32 * u)) >> (4 * half) >> rho(0, i) & 1 ? s[u][i] : -INFINITY;
     }
     softmax_step<2>(s, m, l, o, c);
+    if constexpr (whole.value) {
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      const typename P::frag pf = P::from_acc(s[kk >> 1], kk & 1);
+      for (int kk = 0; kk < 4; ++kk) {
+        const typename P::frag pf = P::from_acc(s[kk >> 1], kk & 1);
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, 16 * kk, ct, lane), pf);
+        for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, 16 * kk, ct, lane), pf);
+      }
+      sched_products<P, 4 * CT, P::COL_READS>();
+    } else {
+      masked_values<P, 4>(o, vt, 0, lane, s, [&](int x) { return bits >> x & 1; });
     }
-    sched_products<P, 4 * CT, P::COL_READS>();
   };
-  for (int at = 0, now = 0; at < total; ++at) {
+  int at = 0, now = 0;
+  auto turn = [&](auto whole) {
     if (at + BUFS - 2 >= total) staged_barrier();
     else staged_barrier<(BUFS - 2) * COPIES>();
     const int then = now == 0 ? BUFS - 1 : now - 1;  // the tile before: read by all
-    step(at, lds + now * 2 * TILE, lds + then * 2 * TILE);
+    step(whole, at, lds + now * 2 * TILE, lds + then * 2 * TILE);
     now = now == BUFS - 1 ? 0 : now + 1;
-  }
+  };
+  const int full = (t.c1 - t.c0) / 64;
+  for (; at < full; ++at) turn(std::true_type{});
+#pragma unroll 1
+  for (; at < total; ++at) turn(std::false_type{});
   l = half_sum(l);
   if (t.chunks == 1) {
     const float f = l == 0.f ? 0.f : 1.f / l;

@@ -172,6 +172,51 @@ def test_other_sequences_and_padding_do_not_reach_a_row():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [1, 100, 150])
+def test_values_of_unseen_keys_do_not_reach_a_row(n, d, dtype):
+    """A few values infinite or NaN: a row has them only where it sees their keys, everything else stays a number.  (n sequences
+    of 240 tokens and four heads: four, two and one wave to a row.)"""
+    q, k, v, dy, cu, _ = make([240] * n, [240] * n, 4, 2, d, dtype)
+    clean = v.clone()
+    inf, nan = float("inf"), float("nan")
+    rare = torch.zeros(240, 2, d, dtype=torch.float64)  # in the first and the last sequence
+    for at, e, x, value in ((37, 0, 3, inf), (70, 0, 3, inf), (70, 0, 40, -inf), (101, 0, 3, -inf), (130, 1, d - 1, nan), (239, 1, 0, inf), (0, 1, 7, -inf)):
+        rare[at, e, x] = value
+    dirty = torch.isnan(rare) | (rare != 0)
+    for b in {0, n - 1}:
+        v[240 * b:240 * (b + 1)][dirty] = rare[dirty].to(dtype)
+        clean[240 * b:240 * (b + 1)][dirty] = 0
+    y = anchor.attention_forward(*(t.to(DEV) for t in (q, k, v, cu))).cpu().double()
+    some = [0, n - 1, n // 2]
+    pick = lambda t: torch.cat([t[240 * b:240 * (b + 1)] for b in some])  # noqa: E731
+    got = pick(y).view(3, 240, 4, d)
+    want = oa.attention(pick(q), pick(k), pick(clean), torch.arange(4) * 240)
+    extra = rare.cumsum(0).repeat_interleave(2, 1)  # what a row has seen: infinities that meet are no number
+    reached = torch.isnan(extra) | (extra != 0)
+    for i, b in enumerate(some):
+        g = got[i].clone()
+        if b in (0, n - 1):
+            assert torch.equal(torch.isnan(g), torch.isnan(extra)) and torch.equal(torch.isinf(g), torch.isinf(extra))
+            assert torch.equal(g[torch.isinf(extra)], extra[torch.isinf(extra)])
+            g[reached] = want["y"].view(3, 240, 4, d)[i][reached]
+        close(g, want["y"].view(3, 240, 4, d)[i], want["bounds"]["y"].view(3, 240, 4, d)[i], unit(dtype, d, 480, want["most"]), b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_unseen_keys_that_are_no_numbers(dtype):
+    """NaN and infinite keys and values from token 100 on: the rows before are what they are without them, the rows after NaN."""
+    q, k, v, dy, cu, _ = make([180], [180], 4, 2, 64, dtype)
+    want = oa.attention(q[:100], k[:100], v[:100], torch.tensor([0, 100]))
+    k[100], k[101:], v[100:] = float("nan"), float("inf"), float("nan")
+    y, lse = anchor.attention_forward(*(t.to(DEV) for t in (q, k, v, cu)), return_lse=True)
+    close(y[:100], want["y"], want["bounds"]["y"], unit(dtype, 64, 200, want["most"]), "y")
+    assert torch.isfinite(lse[:, :100]).all() and torch.isnan(y[100:]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_same_bits_every_time(dtype):
     lens = [300, 17]
     q, k, v, dy, cu, _ = (t.to(DEV) for t in make(lens, lens, 8, 2, 128, dtype))

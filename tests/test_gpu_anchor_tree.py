@@ -121,6 +121,50 @@ def test_bad_parents_and_page_numbers_stay_inside():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("KV", [8, 2])
+def test_siblings_that_are_no_numbers(KV, d, dtype):
+    """Draft 3 with NaN keys and values, draft 4 with an infinite value: they reach themselves and what hangs on them, nobody else.
+    A context that ends with an infinite value gives its infinity.  (Few rows to a key head, and many.)"""
+    lens, new = [0, 33, 300], [12, 9, 12]
+    args = make(lens, new, 8, KV, d, 16, dtype)
+    q, k, v, kp, vp, table, cl, cu, _ = args
+    parents = torch.tensor([-1, 0, 0, 0, 1, 2, 3, 4, 5, 6, 2, 8] + [-1, 0, 0, 0, 1, 2, 3, 4, 5] + [-1, 0, 0, 0, 1, 2, 3, 4, 5, 6, 2, 8],
+                           dtype=torch.int32)
+    tree = lambda *a: anchor.tree_attention(*(t.to(DEV) for t in a), parents=parents.to(DEV)).cpu().double()  # noqa: E731
+    want, bound = oa.tree_attention(*args[:8], parents)
+    last = int(table[2, 299 // 16])
+    for b, lo in enumerate((0, 12, 21)):
+        k[lo + 3], v[lo + 3] = float("nan"), float("nan")
+        v[lo + 4, :, 5] = float("inf")
+    vp[last, :, 299 % 16, 6] = float("-inf")
+    got = tree(*args[:8])
+    f = 2 * 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24 * ((d + 4) * 41 + 300 + 72)
+    slack = f * (bound + want.abs()) + 2.0 ** -18 * bound
+    for lo, n in ((0, 12), (12, 9), (21, 12)):
+        for i in range(n):
+            up, j = set(), i
+            while j >= 0:
+                up.add(j)
+                j = int(parents[lo + j])
+            y, special = got[lo + i], {}
+            if 3 in up:
+                assert torch.isnan(y).all()
+                continue
+            if 4 in up:
+                special[5] = float("inf")
+            if lo == 21:
+                special[6] = float("-inf")
+            keep = torch.ones(d, dtype=torch.bool)
+            for x, value in special.items():
+                assert (y[:, x] == value).all(), (lo, i, x)
+                keep[x] = False
+            assert torch.isfinite(y[:, keep]).all(), (lo, i)
+            assert float(((y - want[lo + i]).abs() - slack[lo + i])[:, keep].max()) <= 0, (lo, i)
+
+
+@pytest.mark.gpu
 def test_far_pages_pass_32_bits():
     """A slab over 4 GiB: its last pages lie at offsets past 2^32 bytes and 2^31 elements."""
     P, KV, d = 64, 4, 128

@@ -95,6 +95,13 @@ def test_many_streams_use_one_launch_size():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 7])
+def test_longest_chunks(new):
+    """Streams enough for chunks of 2048 keys, one of them with three: one token, and 7 (56 rows to a key head)."""
+    check([4100, 2049, 2048] + [3] * 297, [new] * 300, H=16, KV=2, P=256)
+
+
+@pytest.mark.gpu
 def test_pages_in_other_layouts():
     lens, new = [100, 37], [1, 4]
     q, k, v, kp, vp, table, ctx, cu, par = (t.to(DEV) for t in make(lens, new, 8, 2, 64, 16, torch.bfloat16))

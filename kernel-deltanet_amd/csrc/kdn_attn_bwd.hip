@@ -14,9 +14,9 @@
 
 namespace kdn {
 
-// delta, and lse times log2 e: sixteen lanes a row, eight values each at a time.
+// minus delta, and minus lse / scale: what the products of dkdv's kernel start from.  Sixteen lanes a row, eight values each at a time.
 template <class P>
-__global__ void __launch_bounds__(256) attn_delta_kernel(AttnParams p, float* lse2, float* delta) {
+__global__ void __launch_bounds__(256) attn_delta_kernel(AttnParams p, float* stat, float* delta) {
   typedef typename P::elem E;
   const int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (row, head), heads fastest
   const int j = threadIdx.x & 15;
@@ -43,8 +43,8 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnParams p, float* ls
   sum += xor_shuffle<4>(sum);
   sum += xor_shuffle<8>(sum);
   if (j == 0) {
-    delta[h * p.total_q + row] = sum;
-    lse2[h * p.total_q + row] = p.lse[h * p.total_q + row] * LOG2E;
+    delta[h * p.total_q + row] = -sum;
+    stat[h * p.total_q + row] = -p.lse[h * p.total_q + row] / p.scale;
   }
 }
 
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
     stage_q(reinterpret_cast<const E*>(p.q) + (qlo + r0) * p.qs[0] + (int64_t)h * p.qs[1], last, to);
     stage_y(reinterpret_cast<const E*>(p.dy) + (qlo + r0) * p.dys[0] + (int64_t)h * p.dys[1], last, to + TILE);
     if (64 * w < 2 * ROWS) {  // lse of the rows, then delta, 64 a wave
-      const float* src = (64 * w < ROWS ? p.lse2 : p.delta) + (int64_t)h * p.total_q + qlo + r0;
+      const float* src = (64 * w < ROWS ? p.stat : p.delta) + (int64_t)h * p.total_q + qlo + r0;
       copy4_to_lds(buffer_at(src), 4 * min(64 * w % ROWS + lane, last), to + 2 * TILE + 256 * w);
     }
   };
@@ -121,7 +121,26 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
     for (int u = 0; u < S::BLOCKS; ++u) {
       const int tr = 32 * (S::BLOCKS * part + u), i0 = q0 + j % per * ROWS + tr;  // the wave's rows of the tile: i0 .. i0 + 31
       if (i0 >= lenq || i0 + 31 + off < first_key) continue;                      // none of them sees a key of this wave
+      // bf16: the sums start at minus lse / scale and minus delta of their rows.  fp32 adds these last: a sum that starts at
+      // 100 rounds each of its products at that size.
+      constexpr bool START = sizeof(E) == 2;
       f32x16 s = zero16(), dp = zero16();
+      auto add_stat = [&]() {
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const f32x4 ls = *reinterpret_cast<const f32x4*>(stat + 4 * (tr + 8 * a + 4 * half));
+          const f32x4 de = DK ? *reinterpret_cast<const f32x4*>(stat + 4 * (ROWS + tr + 8 * a + 4 * half)) : zero4();
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            s[4 * a + x] = START ? ls[x] : s[4 * a + x] + ls[x];
+            dp[4 * a + x] = START ? de[x] : dp[4 * a + x] + de[x];
+          }
+        }
+      };
+      if constexpr (START) {
+        add_stat();
+        __builtin_amdgcn_sched_group_barrier(0x100, DK ? 8 : 4, 0);
+      }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) s = P::mma(s, P::row_frag(qt, tr + (lane & 31), ks, half), k[ks]);
       if constexpr (!DK) sched_products<P, KS, P::ROW_READS>();
@@ -130,25 +149,21 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
         for (int ks = 0; ks < KS; ++ks) dp = P::mma(dp, P::row_frag(yt, tr + (lane & 31), ks, half), v[ks]);
         sched_products<P, 2 * KS, P::ROW_READS>();
       }
+      if constexpr (!START) add_stat();
       const bool whole = i0 + off >= first_key + 31 && i0 + 32 <= lenq;
       const int lo = max(key - off, 0) - i0, hi = lenq - i0;  // rows lo .. hi - 1 of the block see the key
 #pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(stat + 4 * (tr + 8 * a + 4 * half));
-        const f32x4 de = *reinterpret_cast<const f32x4*>(stat + 4 * (ROWS + tr + 8 * a + 4 * half));
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int i = 4 * a + x, r = rho(half, i);
-          float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls[x]));
-          float d = pr * (dp[i] - de[x]);
-          if (!whole) {
-            const bool sees = r >= lo && r < hi;
-            pr = sees ? pr : 0.f;
-            d = sees ? d : 0.f;
-          }
-          s[i] = pr;
-          dp[i] = d;
+      for (int i = 0; i < 16; ++i) {
+        const int r = rho(half, i);
+        float pr = __builtin_amdgcn_exp2f(s[i] * c);
+        float d = pr * dp[i];
+        if (!whole) {
+          const bool sees = r >= lo && r < hi;
+          pr = sees ? pr : 0.f;
+          d = sees ? d : 0.f;
         }
+        s[i] = pr;
+        dp[i] = d;
       }
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
@@ -259,7 +274,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
     }
   }
   const float c = p.scale * LOG2E;
-  const float ls = p.lse2[(int64_t)h * p.total_q + at], de = p.delta[(int64_t)h * p.total_q + at];
+  const float ls = p.stat[(int64_t)h * p.total_q + at] * c, de = p.delta[(int64_t)h * p.total_q + at];
   f32x16 dq[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) dq[ct] = zero16();
@@ -290,7 +305,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
       const int limit = row + off - j0;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        float d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -ls)) * (dp[i] - de);
+        float d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, ls)) * (dp[i] + de);
         if (!whole) d = rho(half, i) <= limit ? d : 0.f;
         dp[i] = d;
       }
@@ -350,12 +365,12 @@ static int launch_dq(const AttnParams& p, hipStream_t st) {
 }
 
 template <class P>
-static int launch_bwd(const AttnParams& p, float* lse2, float* delta, hipStream_t st) {
+static int launch_bwd(const AttnParams& p, float* stat, float* delta, hipStream_t st) {
   int rc = KDN_OK;
   if (p.total_q > 0) {
     const int64_t rows = p.total_q * p.H;
     if ((rows + 15) / 16 > INT32_MAX) return KDN_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL(attn_delta_kernel<P>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, p, lse2, delta);
+    hipLaunchKernelGGL(attn_delta_kernel<P>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, p, stat, delta);
     if ((rc = launch_status()) != KDN_OK) return rc;
   }
   if (p.total_k > 0) {
@@ -375,7 +390,7 @@ static int bwd_subsets(const kdn_attn_args* f) {
   const int G = (int)(f->H / f->H_kv);
   const int64_t tiles = f->total_k / 128 * f->H_kv;
   int n = 1;
-  while (n < G && (tiles * n < 1024 || G % n != 0)) ++n;
+  while (n < G && (tiles * n < 2048 || G % n != 0)) ++n;
   return n;
 }
 static size_t bwd_row_bytes(const kdn_attn_args* f) { return ((size_t)f->H * (size_t)f->total_q * 4 + 255) / 256 * 256 + 256; }
@@ -411,8 +426,8 @@ extern "C" int kdn_attn_bwd(const kdn_attn_bwd_args* a, void* stream) {
   if (!a->workspace || a->workspace_bytes < kdn_attn_bwd_workspace_bytes(a)) return KDN_ERR_WORKSPACE_TOO_SMALL;
   AttnParams p = attn_params(f);
   p.dy = a->dy; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
-  float *lse2 = reinterpret_cast<float*>(a->workspace), *delta = lse2 + bwd_row_bytes(f) / 4;
-  p.lse2 = lse2;
+  float *stat = reinterpret_cast<float*>(a->workspace), *delta = stat + bwd_row_bytes(f) / 4;
+  p.stat = stat;
   p.delta = delta;
   p.subsets = bwd_subsets(f);
   p.part_dk = reinterpret_cast<float*>((unsigned char*)a->workspace + 2 * bwd_row_bytes(f));
@@ -422,6 +437,6 @@ extern "C" int kdn_attn_bwd(const kdn_attn_bwd_args* a, void* stream) {
   }
   hipStream_t st = as_stream(stream);
   if (f->dtype == KDN_DTYPE_BF16)
-    return f->d == 64 ? launch_bwd<AttnBF16<64>>(p, lse2, delta, st) : launch_bwd<AttnBF16<128>>(p, lse2, delta, st);
-  return f->d == 64 ? launch_bwd<AttnF32<64>>(p, lse2, delta, st) : launch_bwd<AttnF32<128>>(p, lse2, delta, st);
+    return f->d == 64 ? launch_bwd<AttnBF16<64>>(p, stat, delta, st) : launch_bwd<AttnBF16<128>>(p, stat, delta, st);
+  return f->d == 64 ? launch_bwd<AttnF32<64>>(p, stat, delta, st) : launch_bwd<AttnF32<128>>(p, stat, delta, st);
 }

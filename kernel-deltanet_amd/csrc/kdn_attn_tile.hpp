@@ -422,7 +422,7 @@ struct AttnParams {
   int64_t lows[2];
   int64_t qs[2], ks[2], vs[2], ys[2], dys[2], dqs[2], dks[2], dvs[2];  // element strides [token][head]
   float* lse;          // [H][total_q]
-  const float *lse2, *delta;  // [H][total_q]: lse in units of log 2, and dy . y of each row (backward)
+  const float *stat, *delta;  // [H][total_q]: minus lse / scale, and minus dy . y of each row (backward)
   const int64_t *cu_q, *cu_k;
   int64_t nseq, total_q, total_k;
   float *part_dk, *part_dv;  // [subset][total_k][KV][D] sums of dk and dv over a subset of a key head's query heads (subsets > 1)

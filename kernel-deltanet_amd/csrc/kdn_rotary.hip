@@ -4,6 +4,8 @@
 // forms the sines and cosines of its tokens once, in LDS.  A position times a frequency needs more bits than fp32 has (at
 // position 131072 an fp32 product is off by up to 0.004 radians): it is formed in 64 bits, reduced to a turn, and only the
 // sine and cosine of the rest, within half a turn, are fp32.
+//   65536 tokens of 32 + 8 heads of 128, bf16 (1.34 GB): 253 us, 5.3 TB/s, where a large copy reaches 4.9.  Nine tokens of
+// 16 + 4 heads: 3.1 us, a launch's latency.
 #include <cmath>
 #include "kdn_io.hpp"
 #include "kdn_internal.hpp"

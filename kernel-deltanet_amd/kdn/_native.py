@@ -60,7 +60,7 @@ EXPORTED = (
     "kdn_fwht_lift_factored_bwd",
 )
 
-# Exported symbols of include/kdn_anchor.h (checked by tests/test_anchor_abi.py).
+# Exported symbols of include/kdn_anchor.h (checked by tests/test_anchor_host.py).
 ANCHOR_EXPORTED = (
     "kdn_anchor_version",
     "kdn_attn_fwd",

@@ -468,7 +468,7 @@ int kdn_slot_step(const kdn_slot_step_args* a, void* stream, void* aux_stream);
 /* ---- Slab state pool --------------------------------------------------------------------------
  * Slot bookkeeping over a caller-allocated slab of `max_slots` equal fp32 state slots of slot_bytes
  * each (for example [slot][layer][head][D][d_v]); the reference's HybridMemoryPool recurrent slab,
- * serving/hybrid_memory_pool.{h,cpp} (the softmax anchor pages of that class are not part of this path).
+ * serving/hybrid_memory_pool.{h,cpp} (the softmax anchor pages of that class: kdn_anchor.h).
  * Host-side and single-threaded per pool; functions that take a slab pointer also enqueue device work
  * on `stream` (zeroing a new slot, copying a forked one), and skip it when slab is NULL. */
 typedef struct kdn_pool kdn_pool;

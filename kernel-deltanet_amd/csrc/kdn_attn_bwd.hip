@@ -10,8 +10,8 @@
 // so that the gradients are the same bits every time.  As in the forward a product's accumulator is the next one's B
 // operand in registers.
 //   What bounds it: as in the forward, products and exponentials that overlap in part.  One sequence of 8192 rows, 32 heads
-// of 128 over 8, bf16: the forward 0.56 ms, the gradients 2.1 to 2.3 (1.76 TFLOP in eight products: 0.8 PFLOP/s; five of
-// them, those that the formulas need, 0.5), at 1.7 to 1.9 GHz.
+// of 128 over 8, bf16: the forward 0.56 ms, the gradients 2.1 to 2.4 (2.20 TFLOP in eight products: 0.9 to 1.0 PFLOP/s; five of
+// them, those that the formulas need, 0.6), at 1.7 to 1.9 GHz.
 #include <algorithm>
 #include "kdn_attn_tile.hpp"
 #include "kdn_io.hpp"

@@ -9,8 +9,8 @@
 //     slots of their own with no barrier; they meet once at the end;
 //   - more: each wave has 32 rows of its own, and all read the same tiles of 64 keys, as in the prompt's kernel.
 // What bounds them: few rows, HBM (one token of 224 streams, contexts of 512 to 16384, 16 heads of 128 over 4: 2.07 GB in 378 us,
-// 5.5 TB/s; a large copy 4.9, a read 4.0); many, the products and the softmax of rows that share each key (16 trees of 40 drafts,
-// contexts of 1500 to 16384, 32 heads over 8: 0.53 GB in 172 us, of which the join 10 to 18), as in the prompt's kernel.
+// 5.5 TB/s; a large copy 4.9, a read 4.0); many, the copies' latency, one tile of 64 keys ahead, and the unequal chunks' tail (16 trees
+// of 40 drafts, contexts of 1500 to 16384, 32 heads over 8: 0.53 GB in 170 us, of which the join 14; matrix cores busy 16 %).
 // One token of three streams, contexts of 700 to 2500, fp32: 14 us, a chunk's latency, and 4 for the join.
 #include <algorithm>
 #include <cmath>

@@ -16,6 +16,7 @@ serving/hybrid_memory_pool.{h,cpp}.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import struct
 from typing import List, Optional, Sequence, Tuple
@@ -231,6 +232,13 @@ def attention_forward(q, k, v, cu_seqlens, cu_seqlens_k=None, scale: Optional[fl
     return (y[0], lse, None if low is None else low[0]) if return_low else (y[0], lse) if return_lse else y[0]
 
 
+@functools.lru_cache(maxsize=64)
+def _bwd_bytes(nseq: int, nq: int, nk: int, H: int, KV: int, d: int, dtype: int) -> int:
+    """kdn_attn_bwd_workspace_bytes, which reads sizes only."""
+    fwd = ctypes.c_char_p(_ATTN.pack(nseq, nq, nk, H, KV, d, dtype, 1.0, 1, 1, *(0,) * 16))
+    return N.lib().kdn_attn_bwd_workspace_bytes(_ATTN_BWD.pack(ctypes.cast(fwd, ctypes.c_void_p).value, *(0,) * 14))
+
+
 def attention_backward(q, k, v, y, lse, dy, cu_seqlens, cu_seqlens_k=None, scale: Optional[float] = None,
                        low: Optional[torch.Tensor] = None):
     """(dq, dk, dv) of `attention_forward`'s y, lse and low (optional) for dL/dy, in the inputs' dtype, the same bits every
@@ -251,7 +259,7 @@ def attention_backward(q, k, v, y, lse, dy, cu_seqlens, cu_seqlens_k=None, scale
     at = ctypes.cast(fwd, ctypes.c_void_p).value
     dev = q.get_device()
     with _device(dev):
-        nbytes = N.lib().kdn_attn_bwd_workspace_bytes(_ATTN_BWD.pack(at, *dys[1:], *dq[1:], *dk[1:], *dv[1:], 0, 0))
+        nbytes = _bwd_bytes(cu_q.shape[0] - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], _tag(q.dtype, "attention"))
         ws = q.new_empty(nbytes, dtype=torch.uint8)
         N.check(N.lib().kdn_attn_bwd(_ATTN_BWD.pack(at, *dys[1:], *dq[1:], *dk[1:], *dv[1:], ws.data_ptr(), nbytes), _raw_stream(dev)),
                 "kdn_attn_bwd")

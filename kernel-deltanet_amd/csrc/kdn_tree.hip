@@ -351,9 +351,9 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
 // two; the others only copy).
 template <class P>
 struct TreeMany {
-  static constexpr int TILE = 64 * P::ROW;
-  // tiles in LDS, all but the one in use on their way; two workgroups a CU
-  static constexpr int BUFS = 8 * TILE <= 64 * 1024 ? 4 : 2, COPIES = 2 * 16 * P::PIECES / 64;  // copies of a wave and tile
+  static constexpr int KEYS = P::ROW <= 128 ? 64 : 32, TILE = KEYS * P::ROW;
+  // tiles in LDS, all but the one in use on their way; two workgroups a CU, or of fp32, whose registers allow one, one
+  static constexpr int BUFS = 4, COPIES = KEYS / 32 * 16 * P::PIECES / 64;  // copies of a wave and tile
   static int blocks(int rows) { return (rows + 127) / 128; }
   static int per(int rows) { return ((rows + 31) / 32 + blocks(rows) - 1) / blocks(rows); }
 };
@@ -361,7 +361,7 @@ struct TreeMany {
 template <class P>
 __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tree_many_kernel(TreeParams p, int blocks, int per) {
   typedef typename P::elem E;
-  constexpr int D = P::D, KS = D / 16, CT = D / 32, TILE = TreeMany<P>::TILE;
+  constexpr int D = P::D, KS = D / 16, CT = D / 32, KEYS = TreeMany<P>::KEYS, TILE = TreeMany<P>::TILE;
   constexpr int BUFS = TreeMany<P>::BUFS, COPIES = TreeMany<P>::COPIES;
   __shared__ __attribute__((aligned(256))) unsigned char lds[2 * BUFS * TILE];
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -378,18 +378,45 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
   const bool busy = w < per && first < rows, live = busy && first + (lane & 31) < rows;
   const int row = min(first + (lane & 31), rows - 1), tok = row / p.G, h = e * p.G + row % p.G;
   const bool drafts = ch == t.chunks - 1;
-  const int nt = t.c1 > t.c0 ? (t.c1 - t.c0 + 63) / 64 : 0, total = nt + (drafts ? 1 : 0);
-  // wave w copies keys 16 w .. of each tile and their values; their page is known a tile ahead
+  const int nt = t.c1 > t.c0 ? (t.c1 - t.c0 + KEYS - 1) / KEYS : 0, total = nt + (drafts ? (t.n + KEYS - 1) / KEYS : 0);
+  // of 64 keys wave w copies keys 16 w .. of each tile and their values, of 32 either; their page is known a tile ahead
+  const int mine = KEYS == 64 ? w : w & 1;
   int page = 0;
   auto pages = [&](int at) {
-    if (at < nt) page = page_of(p, b, key_group(t.c0 + 64 * at + 16 * w, t.c1 - 1).key);
+    if (at < nt) page = page_of(p, b, key_group(t.c0 + KEYS * at + 16 * mine, t.c1 - 1).key);
   };
-  auto stage = [&](int at, unsigned char* to) {
-    const Group g = at < nt ? key_group(t.c0 + 64 * at + 16 * w, t.c1 - 1) : key_group(16 * w, t.n - 1);
+  // where a lane's copies of sixteen keys that are all there come from, behind the first of them
+  constexpr int N = 16 * P::PIECES / 64, RPI = 64 / P::PIECES, OWN = KEYS == 64 ? 2 : 1;
+  uint32_t from[OWN][N];
 #pragma unroll
-    for (int v = 0; v < 2; ++v)
-      if (at < nt) stage_paged<P>(p, page, e, g, v, to + v * TILE, w, lane);
-      else stage_new<P>(p, t.lo, e, g, v, to + v * TILE, w, lane);
+  for (int x = 0; x < OWN; ++x)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = i * RPI + lane / P::PIECES, piece = (lane % P::PIECES) ^ piece_swizzle<P::PIECES>(r);
+      from[x][i] = (uint32_t)(r * sizeof(E)) * (uint32_t)(OWN == 2 ? (x ? p.vps[2] : p.kps[2]) : (w >> 1 ? p.vps[2] : p.kps[2])) + 16 * piece;
+    }
+  auto stage_whole = [&](int at, unsigned char* to) {
+    const int off = (t.c0 + KEYS * at + 16 * mine) & ((1 << p.shift) - 1), pg = min(max(page, 0), (int)p.num_pages - 1);
+    auto part = [&](bool v, const uint32_t (&lane_off)[N]) {
+      const int64_t* st = v ? p.vps : p.kps;
+      const __amdgpu_buffer_rsrc_t rsrc =
+          buffer_at(reinterpret_cast<const unsigned char*>(v ? p.vp : p.kp) + sizeof(E) * (pg * st[0] + e * st[1] + off * st[2]));
+#pragma unroll
+      for (int i = 0; i < N; ++i) copy16_to_lds(rsrc, lane_off[i], 0, to + v * TILE + (mine * N + i) * 1024);
+    };
+    if constexpr (KEYS == 64) part(false, from[0]), part(true, from[OWN - 1]);
+    else part(w >> 1, from[0]);
+  };
+  const int full = (t.c1 - t.c0) / KEYS;
+  auto stage = [&](int at, unsigned char* to) {
+    if (at < full) return stage_whole(at, to);
+    const Group g = at < nt ? key_group(t.c0 + KEYS * at + 16 * mine, t.c1 - 1) : key_group(KEYS * (at - nt) + 16 * mine, t.n - 1);
+    auto part = [&](bool v) {
+      if (at < nt) stage_paged<P>(p, page, e, g, v, to + v * TILE, mine, lane);
+      else stage_new<P>(p, t.lo, e, g, v, to + v * TILE, mine, lane);
+    };
+    if constexpr (KEYS == 64) part(false), part(true);
+    else part(w >> 1);
   };
 #pragma unroll
   for (int x = 0; x < BUFS - 1; ++x) {
@@ -420,31 +447,33 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
     }
     if (!busy) return;
     const unsigned char* vt = kt + TILE;
-    f32x16 s[2] = {zero16(), zero16()};
+    f32x16 s[KEYS / 32];
+#pragma unroll
+    for (int u = 0; u < KEYS / 32; ++u) s[u] = zero16();
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) s[u] = P::mma(s[u], P::row_frag(kt, 32 * u + (lane & 31), ks, half), q[ks]);
-    sched_products<P, 2 * KS, P::ROW_READS>();
+      for (int u = 0; u < KEYS / 32; ++u) s[u] = P::mma(s[u], P::row_frag(kt, 32 * u + (lane & 31), ks, half), q[ks]);
+    sched_products<P, KEYS / 32 * KS, P::ROW_READS>();
     uint64_t bits = ~0ull;  // the keys of the tile that the row sees
     if constexpr (!whole.value) {
-      bits = at >= nt ? sees : (1ull << (t.c1 - t.c0 - 64 * at)) - 1;
+      bits = at >= nt ? sees >> (KEYS * (at - nt)) : (1ull << (t.c1 - t.c0 - KEYS * at)) - 1;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < KEYS / 32; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[u][i] = (uint32_t)(bits >> (32 * u)) >> (4 * half) >> rho(0, i) & 1 ? s[u][i] : -INFINITY;
     }
-    softmax_step<2>(s, m, l, o, c);
+    softmax_step<KEYS / 32>(s, m, l, o, c);
     if constexpr (whole.value) {
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
+      for (int kk = 0; kk < KEYS / 16; ++kk) {
         const typename P::frag pf = P::from_acc(s[kk >> 1], kk & 1);
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, 16 * kk, ct, lane), pf);
       }
-      sched_products<P, 4 * CT, P::COL_READS>();
+      sched_products<P, KEYS / 16 * CT, P::COL_READS>();
     } else {
-      masked_values<P, 4>(o, vt, 0, lane, s, [&](int x) { return bits >> x & 1; });
+      masked_values<P, KEYS / 16>(o, vt, 0, lane, s, [&](int x) { return bits >> x & 1; });
     }
   };
   int at = 0, now = 0;
@@ -455,7 +484,6 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
     step(whole, at, lds + now * 2 * TILE, lds + then * 2 * TILE);
     now = now == BUFS - 1 ? 0 : now + 1;
   };
-  const int full = (t.c1 - t.c0) / 64;
   for (; at < full; ++at) turn(std::true_type{});
 #pragma unroll 1
   for (; at < total; ++at) turn(std::false_type{});

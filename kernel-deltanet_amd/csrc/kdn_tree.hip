@@ -7,10 +7,11 @@
 // them in the chunks' order.  Sequences of one chunk are written at once.
 //   - up to 32 rows: the waves of a workgroup share the rows and take every fourth tile of 32 keys each, through two LDS
 //     slots of their own with no barrier; they meet once at the end;
-//   - more: each wave has 32 rows of its own, and all read the same tiles of 64 keys, as in the prompt's kernel.
-// What bounds them: few rows, HBM (one token of 224 streams, contexts of 512 to 16384, 16 heads of 128 over 4: 2.07 GB in 378 us,
-// 5.5 TB/s; a large copy 4.9, a read 4.0); many, the copies' latency, one tile of 64 keys ahead, and the unequal chunks' tail (16 trees
-// of 40 drafts, contexts of 1500 to 16384, 32 heads over 8: 0.53 GB in 170 us, of which the join 14; matrix cores busy 16 %).
+//   - more: each wave has 32 rows of its own, and all read the same tiles of 64 or 32 keys, as in the prompt's kernel.
+// What bounds them: few rows, HBM (one token of 224 streams, contexts of 512 to 16384, 16 heads of 128 over 4: 2.07 GB in 373 us,
+// 5.5 TB/s; a large copy 4.9, a read 4.0); many, a wave's own chain of copies, products and softmax for each tile, two to a SIMD where
+// 160 rows are five waves on two workgroups, and the unequal chunks' tail (16 trees of 40 drafts, contexts of 1500 to 16384, 32 heads
+// over 8: 0.53 GB in 158 us, of which the join 14; matrix cores busy 17 %, CUs 78 %).
 // One token of three streams, contexts of 700 to 2500, fp32: 14 us, a chunk's latency, and 4 for the join.
 #include <algorithm>
 #include <cmath>
@@ -161,6 +162,29 @@ __device__ __forceinline__ void stage_new(const TreeParams& p, int64_t lo, int e
                  at, lane);
 }
 
+// The same of sixteen keys that are all there: where a lane's copies come from behind the first key, formed once.  (Formed for each
+// tile they were half of the vector instructions: 16 trees of drafts 170 us, 157 with these.)
+template <class P>
+struct WholeGroup {
+  static constexpr int N = 16 * P::PIECES / 64, RPI = 64 / P::PIECES;
+  uint32_t from[N];
+  __device__ __forceinline__ WholeGroup(int64_t stride, int lane) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = i * RPI + lane / P::PIECES, piece = (lane % P::PIECES) ^ piece_swizzle<P::PIECES>(r);
+      from[i] = (uint32_t)(r * sizeof(typename P::elem)) * (uint32_t)stride + 16 * piece;
+    }
+  }
+  __device__ __forceinline__ void operator()(const TreeParams& p, int page, int e, int key, bool v, unsigned char* tile, int g) const {
+    const int off = key & ((1 << p.shift) - 1), pg = min(max(page, 0), (int)p.num_pages - 1);
+    const int64_t* s = v ? p.vps : p.kps;
+    const __amdgpu_buffer_rsrc_t rows = buffer_at(reinterpret_cast<const unsigned char*>(v ? p.vp : p.kp) +
+                                                  (int64_t)sizeof(typename P::elem) * (pg * s[0] + e * s[1] + off * s[2]));
+#pragma unroll
+    for (int i = 0; i < N; ++i) copy16_to_lds(rows, from[i], 0, tile + (g * N + i) * 1024);
+  }
+};
+
 // The running softmax of one 32-row tile over 32 N more keys: scores -> weights in `s`, the sums rescaled where the maximum
 // moved (by more than 2^6, as in the prompt's kernel).
 template <int N, int CT>
@@ -229,7 +253,15 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
     for (int x = 0; x < 4; ++x)
       stage_new<P>(p, t.lo, e, key_group(16 * (x & 1), t.n - 1), x >> 1, to + (x >> 1) * STAGE / 2, x & 1, lane);
   };
+  const WholeGroup<P> whole_k(p.kps[2], lane), whole_v(p.vps[2], lane);
+  const int full = (t.c1 - t.c0) / 32;
   auto stage = [&](int at, unsigned char* to) {
+    if (at < full) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        (x >> 1 ? whole_v : whole_k)(p, x & 1 ? page1 : page0, e, t.c0 + 32 * at + 16 * (x & 1), x >> 1, to + (x >> 1) * STAGE / 2, x & 1);
+      return;
+    }
     if (at >= nt) return stage_drafts(to);
 #pragma unroll
     for (int x = 0; x < 4; ++x)
@@ -296,7 +328,6 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its slot may be written again
   };
-  const int full = (t.c1 - t.c0) / 32;
   int at = w, buf = 0;
   for (; at < full; at += W, buf ^= 1) step(std::true_type{}, at, mine + buf * STAGE, mine + (buf ^ 1) * STAGE);
 #pragma unroll 1
@@ -385,27 +416,15 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
   auto pages = [&](int at) {
     if (at < nt) page = page_of(p, b, key_group(t.c0 + KEYS * at + 16 * mine, t.c1 - 1).key);
   };
-  // where a lane's copies of sixteen keys that are all there come from, behind the first of them
-  constexpr int N = 16 * P::PIECES / 64, RPI = 64 / P::PIECES, OWN = KEYS == 64 ? 2 : 1;
-  uint32_t from[OWN][N];
-#pragma unroll
-  for (int x = 0; x < OWN; ++x)
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int r = i * RPI + lane / P::PIECES, piece = (lane % P::PIECES) ^ piece_swizzle<P::PIECES>(r);
-      from[x][i] = (uint32_t)(r * sizeof(E)) * (uint32_t)(OWN == 2 ? (x ? p.vps[2] : p.kps[2]) : (w >> 1 ? p.vps[2] : p.kps[2])) + 16 * piece;
-    }
+  const WholeGroup<P> whole_k(KEYS == 64 || w < 2 ? p.kps[2] : p.vps[2], lane), whole_v(p.vps[2], lane);
   auto stage_whole = [&](int at, unsigned char* to) {
-    const int off = (t.c0 + KEYS * at + 16 * mine) & ((1 << p.shift) - 1), pg = min(max(page, 0), (int)p.num_pages - 1);
-    auto part = [&](bool v, const uint32_t (&lane_off)[N]) {
-      const int64_t* st = v ? p.vps : p.kps;
-      const __amdgpu_buffer_rsrc_t rsrc =
-          buffer_at(reinterpret_cast<const unsigned char*>(v ? p.vp : p.kp) + sizeof(E) * (pg * st[0] + e * st[1] + off * st[2]));
-#pragma unroll
-      for (int i = 0; i < N; ++i) copy16_to_lds(rsrc, lane_off[i], 0, to + v * TILE + (mine * N + i) * 1024);
-    };
-    if constexpr (KEYS == 64) part(false, from[0]), part(true, from[OWN - 1]);
-    else part(w >> 1, from[0]);
+    const int key = t.c0 + KEYS * at + 16 * mine;
+    if constexpr (KEYS == 64) {
+      whole_k(p, page, e, key, false, to, mine);
+      whole_v(p, page, e, key, true, to + TILE, mine);
+    } else {
+      whole_k(p, page, e, key, w >> 1, to + (w >> 1) * TILE, mine);
+    }
   };
   const int full = (t.c1 - t.c0) / KEYS;
   auto stage = [&](int at, unsigned char* to) {
@@ -536,8 +555,8 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeParams p) {
 constexpr int MAX_CHUNK = 2048;
 // Keys of a chunk: 128 to 2048, the fewest with which the grid stays within 512 workgroups, or from 256 keys on 2048 (a
 // chunk's own cost, its queries and its partial sums, is that of a few dozen keys; short chunks even out unequal contexts).
-// With chunks of at most 1024 keys 16 trees of 40 drafts, contexts of 1500 to 16384, take 186 us where these take 177, one
-// token of 224 streams 396 where these take 378; with up to 4096 the 224 streams take 395.
+// With chunks of at most 1024 keys 16 trees of 40 drafts, contexts of 1500 to 16384, took 186 us where these took 177, one
+// token of 224 streams 396 where these took 378; with up to 4096 the 224 streams took 395.
 static int tree_chunk(const kdn_tree_attn_args* a) {
   const int64_t rows = a->max_new * (a->H / a->H_kv), blocks = rows <= 32 ? 1 : (rows + 127) / 128;
   int chunk = 128;

@@ -16,7 +16,7 @@ namespace kdn {
 // waves a SIMD overlap them in part.  One sequence of 16384 rows, 32 heads of 128 in bf16: 2.05 to 2.15 ms, 1.02 to 1.07
 // PFLOP/s, where a product of 16384-wide matrices reaches 1.35; the matrix cores are busy in 55 % of the cycles, at 1.6 GHz,
 // which the load holds the clock to (2.4 at most); no LDS bank conflicts.  Seven prompts of 33 to 2048 rows, 16 heads of 64:
-// 31 us, of which half is the longest one's walk.
+// 32 us.
 //   The walk over the keys is one chain, so that a batch with few rows takes the time of its longest row, however idle the
 // GPU: then SPLIT waves share 32 rows and take every SPLIT-th block of 32 keys of a tile each, and their sums meet at the end
 // (attn_split has the rule).

@@ -11,7 +11,7 @@
 // What bounds them: few rows, HBM (one token of 224 streams, contexts of 512 to 16384, 16 heads of 128 over 4: 2.07 GB in 373 us,
 // 5.5 TB/s; a large copy 4.9, a read 4.0); many, a wave's own chain of copies, products and softmax for each tile, two to a SIMD where
 // 160 rows are five waves on two workgroups, and the unequal chunks' tail (16 trees of 40 drafts, contexts of 1500 to 16384, 32 heads
-// over 8: 0.53 GB in 158 us, of which the join 14; matrix cores busy 17 %, CUs 78 %).
+// over 8: 0.53 GB in 158 us, of which the join 14; matrix cores busy 16 %, CUs 77 %).
 // One token of three streams, contexts of 700 to 2500, fp32: 14 us, a chunk's latency, and 4 for the join.
 #include <algorithm>
 #include <cmath>

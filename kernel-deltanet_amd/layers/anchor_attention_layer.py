@@ -36,15 +36,31 @@ class AnchorAttentionLayer(nn.Module):
         self.w_k = nn.Linear(d_model, self.num_kv_heads * self.d_head, bias=False)
         self.w_v = nn.Linear(d_model, self.num_kv_heads * self.d_head, bias=False)
         self.w_out = nn.Linear(num_heads * self.d_head, d_model, bias=False)
-        self._frequencies = dict(rotary_dim=self.d_head if rotary_dim is None else rotary_dim, base=base, scaling=scaling, factor=factor,
-                                 trained_length=trained_length)
-        self.magnitude = anchor.rotary_frequencies(**self._frequencies)[1]
-        self._inv_freq = None
+        frequencies = dict(rotary_dim=self.d_head if rotary_dim is None else rotary_dim, base=base, scaling=scaling, factor=factor,
+                           trained_length=trained_length)
+        with torch.inference_mode(False):  # a table that training can save, wherever the layer is made
+            self._host_freq, self.magnitude = anchor.rotary_frequencies(**frequencies, device="cpu")
+        self._place(self.w_q.weight.device)
+
+    def _place(self, device) -> None:
+        """The frequencies on `device`: float64 whatever the module's type is cast to (so no buffer), and there when this
+        returns, for any stream: a copy from pageable host memory is waited for."""
+        with torch.inference_mode(False):
+            self._inv_freq = self._host_freq.to(device)
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        if self._inv_freq.device != self.w_q.weight.device:
+            self._place(self.w_q.weight.device)
+        return self
 
     def inv_freq(self, device) -> torch.Tensor:
-        """The frequencies on `device`, in float64 whatever the module's type is cast to (so no buffer)."""
-        if self._inv_freq is None or self._inv_freq.device != device:
-            self._inv_freq = anchor.rotary_frequencies(**self._frequencies, device=device)[0]
+        """The frequencies on `device`: they move with the module.  Where its parameters came there by another way (assigned,
+        or a replica's), they are brought there now, which a graph's capture cannot do."""
+        if self._inv_freq.device != device:
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AnchorAttentionLayer: move the module to its device, or call it once, before a capture")
+            self._place(device)
         return self._inv_freq
 
     def _project(self, x: torch.Tensor, positions: torch.Tensor):

@@ -28,6 +28,8 @@ from .ops import _HERE, _tag, require_device
 
 _ref = ctypes.byref
 _BF16, _F32 = torch.bfloat16, torch.float32
+_FAR = (2**31 - 1) // 64     # bytes from a row to the next that the kernels' copies reach over
+_ODD_BF16, _ODD_F32 = ~(2**23 - 8), ~(2**22 - 4)  # bits that strides within reach of 16-byte rows do not have
 _raw_stream, _this_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 # The argument structs of include/kdn_anchor.h as packed bytes, in C's own alignment: a decode step's calls are host-bound,
@@ -58,12 +60,19 @@ def _heads(t: torch.Tensor, what: str, like: Optional[torch.Tensor] = None):
                          f"{tuple(t.shape)} on {t.device}")
     a, b, c = t.stride()
     p = t.data_ptr()
-    if c != 1 or p & 15 or (a | b) & (7 if dt is _BF16 else 3):
-        t = t.contiguous()  # a view that starts off 16 bytes may be contiguous already
-        t = t.clone() if t.data_ptr() & 15 else t
-        a, b, c = t.stride()
-        p = t.data_ptr()
+    if c != 1 or p & 15 or (a | b) & (_ODD_BF16 if dt is _BF16 else _ODD_F32):
+        n, h, d = t.shape
+        a, b = _steps(t)
+        if c != 1 or p & 15 or (a | b) & (7 if dt is _BF16 else 3) or a > _FAR // dt.itemsize:
+            # strides of an output of this shape: contiguous() leaves those of single tokens and heads as they were
+            t, a, b = t.clone(memory_format=torch.contiguous_format), h * d, d
+            p = t.data_ptr()
     return t, p, a, b
+
+
+def _steps(t: torch.Tensor):
+    """The strides of all dimensions but the last; of one that has a single entry, which may be any number, 0."""
+    return tuple(s if n > 1 else 0 for n, s in zip(t.shape[:-1], t.stride()))
 
 
 def _out(t: torch.Tensor, what: str, shape, like: torch.Tensor):
@@ -71,9 +80,10 @@ def _out(t: torch.Tensor, what: str, shape, like: torch.Tensor):
     require_device(t, what)
     if t.shape != shape or t.dtype is not like.dtype or t.device != like.device:
         raise ValueError(f"{what}: expects {tuple(shape)} {like.dtype} on {like.device}; got {tuple(t.shape)} {t.dtype} on {t.device}")
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s * t.element_size() % 16 for s in t.stride()[:2]):
+    a, b = _steps(t)
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or (a | b) * t.element_size() % 16:
         raise ValueError(f"{what}: needs contiguous heads whose rows start on 16 bytes")
-    return t, t.data_ptr(), t.stride(0), t.stride(1)
+    return t, t.data_ptr(), a, b
 
 
 def _new(like: torch.Tensor, shape):
@@ -319,7 +329,10 @@ def _pages(t: torch.Tensor, what: str, like: torch.Tensor):
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
     a, b, c, e = t.stride()
     p = t.data_ptr()
-    if e != 1 or p & 15 or (a | b | c) & (7 if t.dtype is _BF16 else 3):
+    odd = 7 if t.dtype is _BF16 else 3
+    if (a | b | c) & odd:
+        a, b, c = _steps(t)
+    if e != 1 or p & 15 or (a | b | c) & odd:
         raise ValueError(f"{what}: needs contiguous rows that start on 16 bytes (a cache is used where it is, never copied)")
     return t, p, a, b, c
 
@@ -462,7 +475,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: t
                          f"do not go together")
     dev = q.get_device()
     if page_table.get_device() != dev or page_table.dim() != 2 or page_table.dtype is not torch.int32 or \
-            (page_table.shape[1] and page_table.stride(1) != 1):
+            (page_table.shape[1] > 1 and page_table.stride(1) != 1):
         raise ValueError(f"tree_attention: page_table is (streams, width) int32 on {q.device}, got {tuple(page_table.shape)} "
                          f"{page_table.dtype} on {page_table.device}")
     B, width = page_table.shape

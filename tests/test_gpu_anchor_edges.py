@@ -3,6 +3,7 @@ rows that no sequence has, layouts with odd strides, autograd's other modes, ste
 import pytest
 import torch
 
+from kdn import anchor
 from layers import AnchorAttentionLayer
 
 DEV = "cuda:0"
@@ -58,3 +59,63 @@ def test_layer_trains_after_inference_mode():
     assert torch.equal(y.detach(), want.clone())
     y.sum().backward()
     assert all(torch.isfinite(p.grad).all() and p.grad.any() for p in layer.parameters())
+
+
+def odd_strides(t, single):
+    """t as a view whose strides are no multiples of 16 bytes in the dimensions in `single`, each of one entry."""
+    strides = list(t.contiguous().stride())
+    for i in single:
+        assert t.shape[i] == 1
+        strides[i] = strides[i] + 8 * i + 1
+    out = torch.as_strided(t.new_empty(4 * t.numel() + 64), t.shape, strides)
+    out.copy_(t)
+    assert out.stride() == tuple(strides)
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,KV", [(1, 2), (5, 1), (1, 1)])
+def test_strides_of_single_tokens_and_heads(n, KV, dtype):
+    """A dimension of one entry has any stride, in every operator: its results are those of contiguous tensors."""
+    d, P = 64, 16
+    g = torch.Generator(device=DEV).manual_seed(3)
+    q, k, v, dy = (torch.randn(n, h, d, generator=g, device=DEV).to(dtype) for h in (2 * KV, KV, KV, 2 * KV))
+    odd = lambda t: odd_strides(t, [i for i in (0, 1) if t.shape[i] == 1])  # noqa: E731
+    cu = torch.tensor([0, n], device=DEV)
+    f = anchor.rotary_frequencies(d, device=DEV)[0]
+    pos = torch.arange(n, device=DEV)
+    for a, b in zip(anchor.rotary(odd(q), odd(k), pos, f), anchor.rotary(q, k, pos, f)):
+        assert torch.equal(a, b)
+    want, got = [], []
+    for out, change in ((want, lambda t: t.clone()), (got, odd)):
+        leaves = [change(t).requires_grad_(True) for t in (q, k, v)]
+        y = anchor.attention(*leaves, cu)
+        out += [y.detach(), *torch.autograd.grad(y, leaves, change(dy))]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    held = odd(torch.zeros_like(q))
+    anchor.attention(q, k, v, cu, out=held)
+    assert torch.equal(held, want[0])
+    turned = odd(q)
+    anchor.rotary(turned, None, pos, f, in_place=True)
+    assert torch.equal(turned, anchor.rotary(q, None, pos, f)[0])
+    pages = [torch.zeros(1, KV, P, d, dtype=dtype, device=DEV) for _ in range(4)]
+    pages[2:] = [odd_strides(t, [i for i in (0, 1) if t.shape[i] == 1]) for t in pages[2:]]
+    anchor.page_append(k, v, pages[0], pages[1], pos)
+    anchor.page_append(odd(k), odd(v), pages[2], pages[3], pos)
+    assert torch.equal(pages[0], pages[2]) and torch.equal(pages[1], pages[3])
+    table, ctx = torch.zeros(1, 1, dtype=torch.int32, device=DEV), torch.tensor([n], dtype=torch.int32, device=DEV)
+    want = anchor.tree_attention(q, k, v, *pages[:2], table, ctx, cu)
+    wide = torch.zeros(1, 9, dtype=torch.int32, device=DEV).t()[3:4]  # one page number, strides (1, 9)
+    assert torch.equal(anchor.tree_attention(odd(q), odd(k), odd(v), *pages[2:], wide, ctx, cu, out=odd(torch.zeros_like(q))), want)
+
+
+@pytest.mark.gpu
+def test_tokens_further_apart_than_a_copy_reaches():
+    """Two tokens 2^25 elements apart (a copy of 64 such rows would pass 32-bit offsets): copied first, as other layouts are."""
+    far = torch.zeros(2**25 + 256, dtype=torch.float32, device=DEV)
+    q = torch.randn(2, 2, 64, device=DEV)
+    view = torch.as_strided(far, (2, 2, 64), (2**25, 64, 1))
+    view.copy_(q)
+    cu = torch.tensor([0, 2], device=DEV)
+    assert torch.equal(anchor.attention(view, view, view, cu), anchor.attention(q, q, q, cu))

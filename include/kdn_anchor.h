@@ -129,7 +129,9 @@ int64_t kdn_page_pool_free(const kdn_page_pool* pool);
  * along its parents the new tokens it hangs on: parents[cu_new[b] + t] is a number below t, or negative for one that hangs
  * on the context (parents NULL: each hangs on the one before it).  k and v hold the new tokens' own keys and values, which
  * need not be in the pages.  Softmax and heads as kdn_attn_fwd.  max_context bounds the context lengths (longer ones are
- * cut) and sizes the grid; nothing is read back to the host.  At 16 bytes: every row; workspace. */
+ * cut) and sizes the grid; nothing is read back to the host.  Rows of y that no such token has are zeros: those before
+ * cu_new[0], from cu_new[num_seqs] on (a step padded to a fixed size), and past max_new of a sequence.  At 16 bytes: every
+ * row; workspace. */
 typedef struct kdn_tree_attn_args {
   int64_t num_seqs, total_new, max_new, max_context;
   int64_t H, H_kv;

@@ -29,6 +29,7 @@ struct TreeParams {
   float *po, *pml;  // partial sums [sequence][key head][chunk][row][D] and maxima / sums [..][2]
   int64_t table_stride, num_pages, total, max_context;
   int H, KV, G, max_new, max_chunks, chunk, shift, nseq;
+  int zero_from;  // the workgroups from this number on have tree_zero's rows
   float scale;
 };
 
@@ -92,6 +93,32 @@ __device__ __forceinline__ TreeWork tree_work(const TreeParams& p, int u, int la
     t.c0 = t.ch * p.chunk;
     t.c1 = min(t.c0 + p.chunk, t.ctx);
     return t;
+  }
+}
+
+// Rows of y that no token within the bounds has, as zeros: those before the first sequence and behind the last (a step padded to
+// a fixed size), and those past max_new of a sequence.  The last ZERO_GROUPS workgroups of the grid: the first two kinds all of
+// them share, of the third, which no step should have, a wave writes what it finds.
+constexpr int ZERO_GROUPS = 16;
+template <class E, int D>
+__device__ __forceinline__ void tree_zero(const TreeParams& p, int group) {
+  constexpr int PIECES = D * (int)sizeof(E) / 16;
+  const int lane = threadIdx.x & 63, waves = ZERO_GROUPS * (blockDim.x / 64), wave = group * (blockDim.x / 64) + threadIdx.x / 64;
+  auto start = [&](int64_t b) { return min(max(p.cu[b], (int64_t)0), p.total); };
+  auto rows = [&](int64_t from, int64_t to, int64_t first, int64_t step) {
+    for (int64_t i = first; i < (to - from) * p.H * PIECES; i += step) {
+      const int64_t row = i / PIECES, t = from + row / p.H, h = row % p.H;
+      *reinterpret_cast<u32x4*>(reinterpret_cast<E*>(p.y) + t * p.ys[0] + h * p.ys[1] + i % PIECES * (16 / (int)sizeof(E))) = u32x4{0, 0, 0, 0};
+    }
+  };
+  rows(0, start(0), 64 * wave + lane, 64 * waves);
+  rows(start(p.nseq), p.total, 64 * wave + lane, 64 * waves);
+  for (int64_t b0 = 64 * wave; b0 < p.nseq; b0 += 64 * waves) {
+    const int64_t b = min(b0 + lane, (int64_t)p.nseq - 1), lo = start(b) + p.max_new, hi = start(b + 1);
+    for (uint64_t over = __ballot(b0 + lane < p.nseq && hi > lo); over; over &= over - 1) {
+      const int64_t at = b0 + __builtin_ctzll(over);
+      rows(start(at) + p.max_new, start(at + 1), lane, 64);
+    }
   }
 }
 
@@ -233,6 +260,7 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
   float(*wm)[32] = reinterpret_cast<float(*)[32]>(lds + TreeFew<P>::LDS), (*wl)[32] = wm + W;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if ((int)blockIdx.x >= p.zero_from) return tree_zero<E, D>(p, blockIdx.x - p.zero_from);
   const int e = blockIdx.x % p.KV;  // the key heads of a chunk next to one another: they go round the XCDs
   const TreeWork t = tree_work(p, blockIdx.x / p.KV, lane);
   if (t.b < 0) return;
@@ -397,6 +425,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
   __shared__ __attribute__((aligned(256))) unsigned char lds[2 * BUFS * TILE];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if ((int)blockIdx.x >= p.zero_from) return tree_zero<E, D>(p, blockIdx.x - p.zero_from);
   // The row blocks of one chunk on one XCD, one after another: its L2 has the keys from the second on.  Which comes first
   // changes every 32 workgroups, an XCD's CUs: a CU gets its turn's larger and smaller blocks (16 trees 198 -> 186 us).
   const int at8 = blockIdx.x / 8, unit = at8 / blocks * 8 + blockIdx.x % 8, rb = (at8 + at8 / blocks * blocks / 32) % blocks;
@@ -581,16 +610,18 @@ static int tree_check(const kdn_tree_attn_args* a) {
 }
 
 template <class P>
-static int launch_tree(const TreeParams& p, hipStream_t st) {
+static int launch_tree(TreeParams& p, hipStream_t st) {
   const int rows = p.max_new * p.G;
   const int64_t units = (int64_t)p.nseq * p.KV * p.max_chunks;
   if (rows <= 32) {
-    hipLaunchKernelGGL(tree_few_kernel<P>, dim3((unsigned)units), dim3(64 * TreeFew<P>::WAVES), 0, st, p);
+    p.zero_from = (int)units;
+    hipLaunchKernelGGL(tree_few_kernel<P>, dim3((unsigned)units + ZERO_GROUPS), dim3(64 * TreeFew<P>::WAVES), 0, st, p);
   } else {
     const int blocks = TreeMany<P>::blocks(rows);
-    hipLaunchKernelGGL(tree_many_kernel<P>, dim3((unsigned)((units + 7) / 8 * 8 * blocks)), dim3(256), 0, st, p, blocks, TreeMany<P>::per(rows));
+    p.zero_from = (int)((units + 7) / 8 * 8 * blocks);
+    hipLaunchKernelGGL(tree_many_kernel<P>, dim3((unsigned)p.zero_from + ZERO_GROUPS), dim3(256), 0, st, p, blocks, TreeMany<P>::per(rows));
   }
-  if (p.max_chunks > 1) {
+  if (p.max_chunks > 1 && p.nseq > 0) {
     const int64_t joins = (int64_t)p.nseq * p.KV * rows;
     hipLaunchKernelGGL((tree_join_kernel<typename P::elem, P::D>), dim3((unsigned)((joins + 3) / 4)), dim3(256), 0, st, p);
   }
@@ -617,9 +648,9 @@ extern "C" size_t kdn_tree_attn_workspace_bytes(const kdn_tree_attn_args* a) {
 extern "C" int kdn_tree_attn(const kdn_tree_attn_args* a, void* stream) {
   int rc = tree_check(a);
   if (rc != KDN_OK) return rc;
-  if (a->num_seqs == 0 || a->total_new == 0) return KDN_OK;
-  if (!a->cu_new || !a->context_lens || !a->q || !a->k || !a->v || !a->y ||
-      (a->max_context > 0 && (!a->page_table || !a->k_pages || !a->v_pages)))
+  if (a->total_new == 0) return KDN_OK;
+  if (!a->cu_new || !a->q || !a->k || !a->v || !a->y ||
+      (a->num_seqs > 0 && (!a->context_lens || (a->max_context > 0 && (!a->page_table || !a->k_pages || !a->v_pages)))))
     return KDN_ERR_INVALID_ARGUMENT;
   const int64_t per = 16 / (int64_t)dtype_size(a->dtype);
   bool fits = aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) && aligned(a->y, 16) && aligned(a->k_pages, 16) &&
@@ -629,7 +660,7 @@ extern "C" int kdn_tree_attn(const kdn_tree_attn_args* a, void* stream) {
     fits = fits && a->k_pages_stride[i] >= 0 && a->v_pages_stride[i] >= 0 && a->k_pages_stride[i] % per == 0 && a->v_pages_stride[i] % per == 0;
   if (!fits) return KDN_ERR_MISALIGNED;
   const int64_t chunks = tree_chunks(a), rows = a->max_new * (a->H / a->H_kv), blocks = rows <= 32 ? 1 : (rows + 127) / 128;  // at least as many as there will be
-  if (a->num_seqs * a->H_kv * chunks * blocks > INT32_MAX - 8 * blocks || a->num_seqs * a->H_kv * rows > INT32_MAX)
+  if (a->num_seqs * a->H_kv * chunks * blocks > INT32_MAX - 8 * blocks - ZERO_GROUPS || a->num_seqs * a->H_kv * rows > INT32_MAX)
     return KDN_ERR_UNSUPPORTED;
   // a copy's lanes have 32-bit offsets from its first row
   const int64_t size = (int64_t)dtype_size(a->dtype), far = INT32_MAX / (16 * size);

@@ -461,8 +461,9 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: t
     and along `parents` (tokens,) the new tokens before it: parents[i] is the number, within the stream's new tokens, of the
     one that token i hangs on, a lower one than its own, or -1 for the context (none given: a run, each on the one before).
     At most 64 new tokens a stream; max_new (64, or 1 without cu_seqlens) and max_context (what page_table holds) bound
-    them from the host, so that nothing is read back; the closer, the smaller the launch.  `workspace`: uint8, at least
-    `tree_workspace_bytes`, for a caller that allocates once."""
+    them from the host, so that nothing is read back; the closer, the smaller the launch.  Rows outside the offsets are
+    padding: zeros, as are those of a stream past max_new.  `workspace`: uint8, at least `tree_workspace_bytes`, for a caller
+    that allocates once."""
     what = "tree_attention"
     qs = _heads(q, "tree_attention q")
     ks, vs = _heads(k, "tree_attention k", q), _heads(v, "tree_attention v", q)

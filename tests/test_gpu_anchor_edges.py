@@ -119,3 +119,71 @@ def test_tokens_further_apart_than_a_copy_reaches():
     view.copy_(q)
     cu = torch.tensor([0, 2], device=DEV)
     assert torch.equal(anchor.attention(view, view, view, cu), anchor.attention(q, q, q, cu))
+
+
+def step_of(lens, new, pad, lead=0, H=8, KV=2, d=64, dtype=torch.bfloat16):
+    """A step's tensors with `lead` rows before the first stream's and `pad` behind the last's, the pages in order."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    n, P = lead + sum(new) + pad, 16
+    q, k, v = (torch.randn(n, h, d, generator=g, device=DEV).to(dtype) for h in (H, KV, KV))
+    per = max([1, *(-(-x // P) for x in lens)])
+    kp, vp = (torch.randn(max(1, len(lens)) * per, KV, P, d, generator=g, device=DEV).to(dtype) for _ in range(2))
+    table = torch.arange(len(lens) * per, dtype=torch.int32, device=DEV).view(len(lens), per)
+    cu = torch.tensor([lead, *new], device=DEV).cumsum(0)
+    return q, k, v, kp, vp, table, torch.tensor(lens, dtype=torch.int32, device=DEV), cu
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens,new,pad,lead", [([700, 20], [1, 1], 37, 0), ([700, 20], [1, 1], 0, 3), ([300, 0, 7], [20, 0, 33], 5, 2),
+                                               ([40] * 70, [1] * 70, 442, 0), ([50, 60], [0, 0], 9, 0)])
+def test_rows_that_no_stream_has_are_zeros(lens, new, pad, lead, d, dtype):
+    step = step_of(lens, new, pad, lead, d=d, dtype=dtype)
+    n, inside = step[0].shape[0], slice(lead, lead + sum(new))
+    want = anchor.tree_attention(*(t[inside] for t in step[:3]), *step[3:7], step[7] - lead)
+    for held in (torch.full_like(step[0], float("nan")), torch.full((n, 10, d), 7.0, dtype=dtype, device=DEV)[:, 1:9]):
+        y = anchor.tree_attention(*step, out=held)
+        assert torch.equal(y[inside], want)
+        assert not y[:lead].any() and not y[lead + sum(new):].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H", [4, 16])
+def test_tokens_past_max_new_are_zeros(H):
+    new = [5, 1, 3, 70, 0, 2]
+    step = step_of([30, 300, 0, 16, 3, 40], new, 4, H=H)
+    y = anchor.tree_attention(*step, max_new=3, out=torch.full_like(step[0], float("nan")))
+    own = torch.cat([torch.arange(n) < 3 for n in [*new]] + [torch.zeros(4, dtype=torch.bool)]).to(DEV)
+    assert not y[~own].any()
+    cut = [min(n, 3) for n in new]
+    want = anchor.tree_attention(*(t[own] for t in step[:3]), *step[3:7], torch.tensor([0, *cut], device=DEV).cumsum(0), max_new=3)
+    assert torch.equal(y[own], want)
+    y = anchor.tree_attention(*step, out=torch.full_like(step[0], float("nan")))  # 64 of the 70
+    assert torch.isfinite(y).all() and not y[9 + 64:9 + 70].any() and y[9 + 63].any()
+
+
+@pytest.mark.gpu
+def test_a_padded_step_without_streams_is_zeros():
+    q, k, v, kp, vp, table, ctx, cu = step_of([], [], 6)
+    y = anchor.tree_attention(q, k, v, kp, vp, table.view(0, 1), ctx, cu, out=torch.full_like(q, float("nan")))
+    assert not y.any()
+
+
+@pytest.mark.gpu
+def test_a_padded_step_in_a_graph():
+    """A step captured for eight streams' tokens, replayed with fewer of them."""
+    step = step_of([300, 20, 77, 1, 50, 60, 70, 5], [1] * 8, 0)
+    g = torch.cuda.CUDAGraph()
+    anchor.tree_attention(*step, max_new=1)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        y = anchor.tree_attention(*step, max_new=1)
+    for live in (8, 5, 2, 7):
+        step[7].copy_(torch.arange(9, device=DEV).clamp(max=live))
+        g.replay()
+        torch.cuda.synchronize()
+        want = anchor.tree_attention(*(t[:live] for t in step[:3]), *step[3:5], step[5][:live], step[6][:live], torch.arange(live + 1, device=DEV),
+                                     max_new=1, max_context=step[5].shape[1] * 16)
+        assert not y[live:].any()
+        assert float((y[:live].float() - want.float()).abs().max()) < 2.0 ** -6  # chunks of another length: their sums' order

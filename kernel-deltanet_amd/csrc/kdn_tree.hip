@@ -111,8 +111,8 @@ __device__ __forceinline__ void tree_zero(const TreeParams& p, int group) {
       *reinterpret_cast<u32x4*>(reinterpret_cast<E*>(p.y) + t * p.ys[0] + h * p.ys[1] + i % PIECES * (16 / (int)sizeof(E))) = u32x4{0, 0, 0, 0};
     }
   };
-  rows(0, start(0), 64 * wave + lane, 64 * waves);
-  rows(start(p.nseq), p.total, 64 * wave + lane, 64 * waves);
+  rows(0, p.nseq > 0 ? start(0) : p.total, 64 * wave + lane, 64 * waves);
+  if (p.nseq > 0) rows(start(p.nseq), p.total, 64 * wave + lane, 64 * waves);
   for (int64_t b0 = 64 * wave; b0 < p.nseq; b0 += 64 * waves) {
     const int64_t b = min(b0 + lane, (int64_t)p.nseq - 1), lo = start(b) + p.max_new, hi = start(b + 1);
     for (uint64_t over = __ballot(b0 + lane < p.nseq && hi > lo); over; over &= over - 1) {
@@ -648,9 +648,9 @@ extern "C" size_t kdn_tree_attn_workspace_bytes(const kdn_tree_attn_args* a) {
 extern "C" int kdn_tree_attn(const kdn_tree_attn_args* a, void* stream) {
   int rc = tree_check(a);
   if (rc != KDN_OK) return rc;
-  if (a->total_new == 0) return KDN_OK;
-  if (!a->cu_new || !a->q || !a->k || !a->v || !a->y ||
-      (a->num_seqs > 0 && (!a->context_lens || (a->max_context > 0 && (!a->page_table || !a->k_pages || !a->v_pages)))))
+  if (a->total_new == 0 || (a->num_seqs == 0 && !a->y)) return KDN_OK;
+  if (!a->y || (a->num_seqs > 0 && (!a->cu_new || !a->context_lens || !a->q || !a->k || !a->v ||
+                                    (a->max_context > 0 && (!a->page_table || !a->k_pages || !a->v_pages)))))
     return KDN_ERR_INVALID_ARGUMENT;
   const int64_t per = 16 / (int64_t)dtype_size(a->dtype);
   bool fits = aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) && aligned(a->y, 16) && aligned(a->k_pages, 16) &&

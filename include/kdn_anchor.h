@@ -23,7 +23,8 @@ int kdn_anchor_version(void);
 /* ---- Causal attention over packed sequences -------------------------------------------------------------------
  * y_i = sum_j p_ij v_j, p_i. = softmax over the visible j of scale q_i . k_j.  Sequence b is the query rows
  * cu_q[b] .. cu_q[b+1]-1 and the key rows cu_k[b] .. cu_k[b+1]-1; its query i sees the keys j <= i + (len_k - len_q)
- * (the last query sees the last key).  A row that sees no key gets zeros, its lse -infinity and its gradient zero.
+ * (the last query sees the last key).  A row that sees no key gets zeros, its lse -infinity and its gradient zero;
+ * so do rows that no sequence has (before the first offset, from the last on), and such keys' gradients are zero.
  * Query head h uses key head h / (H / H_kv).  Offsets are read on the device; the grid follows from total_q and num_seqs.
  * A row has an infinity or NaN of a key or value only if it sees that key. */
 typedef struct kdn_attn_args {
@@ -44,8 +45,8 @@ int kdn_attn_fwd(const kdn_attn_args* a, void* stream);
 
 /* Gradients of a loss through kdn_attn_fwd, given dy = dL/dy: `fwd` holds the forward's arguments with its y and lse
  * (both required) and y_low (if the forward wrote it: dy . y is formed from both; without it from the rounded y).  dq, dk,
- * dv in the inputs' dtype, each rounded once from fp32 sums, summed in a fixed order (the same bits every time); every row of
- * a sequence is written.  An infinity or NaN in a sequence's q, k, v or dy stays in that sequence's gradients, but may reach
+ * dv in the inputs' dtype, each rounded once from fp32 sums, summed in a fixed order (the same bits every time); every row is
+ * written.  An infinity or NaN in a sequence's q, k, v or dy stays in that sequence's gradients, but may reach
  * those of rows that do not see it.  workspace: kdn_attn_bwd_workspace_bytes, 16-byte aligned. */
 typedef struct kdn_attn_bwd_args {
   const kdn_attn_args* fwd;

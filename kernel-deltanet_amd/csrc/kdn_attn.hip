@@ -305,7 +305,7 @@ extern "C" int kdn_anchor_version(void) { return 1 << 16; }
 
 template <class P, int SPLIT>
 static int launch_fwd(const AttnParams& p, hipStream_t st) {
-  const int64_t slots = p.total_q / Fwd<P, SPLIT>::ROWS + p.nseq + 1, grid = slots * p.H;
+  const int64_t slots = tile_slots(p.total_q, Fwd<P, SPLIT>::ROWS, p.nseq), grid = slots * p.H;
   if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
   hipLaunchKernelGGL((attn_fwd_kernel<P, SPLIT>), dim3((unsigned)grid), dim3(256), 0, st, p, slots);
   return launch_status();

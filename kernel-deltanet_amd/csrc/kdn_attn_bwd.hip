@@ -372,8 +372,8 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1)
 
 template <class P, int SPLIT>
 static int launch_grads(const AttnParams& p, hipStream_t st) {
-  const int64_t slots_k = p.total_k > 0 ? p.total_k / Dkdv<P, SPLIT>::KEYS + p.nseq + 1 : 0;
-  const int64_t slots_q = p.total_q > 0 ? p.total_q / Dq<P, SPLIT>::ROWS + p.nseq + 1 : 0;
+  const int64_t slots_k = p.total_k > 0 ? tile_slots(p.total_k, Dkdv<P, SPLIT>::KEYS, p.nseq) : 0;
+  const int64_t slots_q = p.total_q > 0 ? tile_slots(p.total_q, Dq<P, SPLIT>::ROWS, p.nseq) : 0;
   const int64_t nk = slots_k * p.KV * p.subsets, part = (nk + 7) / 8 * 8;  // a workgroup's number mod 8 is its XCD
   const int64_t grid = part * (P::D == 64 ? 1 : 2) + slots_q * p.H;
   if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;

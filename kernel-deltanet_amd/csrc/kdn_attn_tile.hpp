@@ -337,9 +337,10 @@ __device__ __forceinline__ void join_sums(f32x16 (&o)[CT], float mine, unsigned 
 
 // Tile slots over a packed batch: sequence b has the slots [cu[b] / ROWS + b, cu[b + 1] / ROWS + b + 1), at least as many
 // as it has tiles of ROWS rows, so that a grid of total / ROWS + sequences slots covers every batch without its lengths
-// being known to the host.  The rows past the last sequence's end (a batch padded to a fixed size) are one sequence more,
-// number nseq, that sees nothing and that nothing sees.  The sequence of a slot is found 64 offsets at a time by the whole
-// wave.  Offsets are clamped to the tensor: a wrong one gives wrong rows, never an access outside.
+// being known to the host.  The rows outside the offsets are two sequences more, that see nothing and that nothing sees: those
+// before the first one, number -1, and those past the last one's end (a batch padded to a fixed size), number nseq.  They
+// count in the slots, `entry` being a sequence's number and one.  The sequence of a slot is found 64 offsets at a time by the
+// whole wave.  Offsets are clamped to the tensor: a wrong one gives wrong rows, never an access outside.
 struct SeqTile {
   int seq, row0;  // row0: first row of the tile in the sequence; negative: no tile
   int64_t lo;     // the sequence's first row
@@ -348,40 +349,44 @@ struct SeqTile {
 __device__ __forceinline__ int64_t seq_start(const int64_t* cu, int64_t total, int64_t b) {
   return min(max(cu[b], (int64_t)0), total);
 }
+__device__ __forceinline__ int64_t entry_start(const int64_t* cu, int64_t nseq, int64_t total, int64_t entry) {
+  const int64_t first = seq_start(cu, total, min(max(entry - 1, (int64_t)0), nseq));  // in every lane: no branch around a load
+  return entry == 0 ? 0 : entry > nseq + 1 ? total : first;
+}
+inline int64_t tile_slots(int64_t total, int64_t rows, int64_t nseq) { return total / rows + nseq + 2; }
 template <int ROWS>
 __device__ __forceinline__ SeqTile find_tile(const int64_t* cu, int64_t nseq, int64_t total, int64_t slot, int lane) {
-  int64_t lo = 0, n = nseq + 1;
+  int64_t lo = 0, n = nseq + 2;
   while (n > 1) {
     const int64_t step = (n + 63) / 64, at = lo + lane * step;
-    const bool before = lane * step < n && seq_start(cu, total, min(at, nseq)) / ROWS + at <= slot;
+    const bool before = lane * step < n && entry_start(cu, nseq, total, at) / ROWS + at <= slot;
     const int hits = __popcll(__ballot(before));
     const int64_t skip = (hits > 0 ? hits - 1 : 0) * step;
     lo += skip;
     n = min(step, n - skip);
   }
   SeqTile t;
-  t.seq = (int)lo;
-  t.lo = seq_start(cu, total, lo);
-  t.len = (int)((lo < nseq ? max(seq_start(cu, total, lo + 1), t.lo) : total) - t.lo);
+  t.seq = (int)lo - 1;
+  t.lo = entry_start(cu, nseq, total, lo);
+  t.len = (int)(max(entry_start(cu, nseq, total, lo + 1), t.lo) - t.lo);
   const int64_t tile = slot - (t.lo / ROWS + lo);
   t.row0 = tile < 0 || tile * ROWS >= t.len ? -1 : (int)(tile * ROWS);
   return t;
 }
 // The tile that is the id-th in the order of most work first, a tile's work being its place in its sequence (its rows see
 // that many tiles of keys; counted from the sequence's end for the keys, whose first ones the most rows see): what runs
-// longest starts first, whichever sequence it is of.  Up to 63 sequences; with more, slot `slots` - 1 - id of find_tile (each
-// sequence's own tiles most work first).  Lane b has sequence b's tiles nt; N(t), the tiles at place t or behind it, is
+// longest starts first, whichever sequence it is of.  Up to 62 sequences; with more, slot `slots` - 1 - id of find_tile (each
+// sequence's own tiles most work first).  Lane b has entry b's tiles nt; N(t), the tiles at place t or behind it, is
 // the sum of max(nt - t, 0), and the tile's place the last t with N(t) > id.
 template <int ROWS, bool FROM_END>
 __device__ __forceinline__ SeqTile find_heavy(const int64_t* cu, int64_t nseq, int64_t total, int64_t id, int64_t slots, int lane) {
-  if (nseq >= 64) {
+  if (nseq > 62) {
     SeqTile t = find_tile<ROWS>(cu, nseq, total, slots - 1 - id, lane);
     if (FROM_END && t.row0 >= 0) t.row0 = (t.len - 1) / ROWS * ROWS - t.row0;
     return t;
   }
-  const int n = (int)nseq + 1;
-  const int64_t lo = seq_start(cu, total, min((int64_t)lane, nseq));
-  const int64_t hi = lane < nseq ? max(seq_start(cu, total, lane + 1), lo) : total;
+  const int n = (int)nseq + 2;
+  const int64_t lo = entry_start(cu, nseq, total, lane), hi = max(entry_start(cu, nseq, total, lane + 1), lo);
   const int len = lane < n ? (int)(hi - lo) : 0, nt = (len + ROWS - 1) / ROWS;
   auto behind = [&](int t) {
     int sum = 0;
@@ -401,17 +406,19 @@ __device__ __forceinline__ SeqTile find_heavy(const int64_t* cu, int64_t nseq, i
   }
   const int rank = (int)id - behind(t + 1);
   const uint64_t there = __ballot(nt > t);
-  const int seq = __ffsll((unsigned long long)__ballot((there >> lane & 1) && __popcll(there & ((1ull << lane) - 1)) == rank)) - 1;
-  s.seq = __builtin_amdgcn_readfirstlane(seq);
-  s.len = __builtin_amdgcn_readlane(len, s.seq);
-  s.lo = (int64_t)__builtin_amdgcn_readlane((int)(lo >> 32), s.seq) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, s.seq);
-  s.row0 = (FROM_END ? __builtin_amdgcn_readlane(nt, s.seq) - 1 - t : t) * ROWS;
+  const int at = __ffsll((unsigned long long)__ballot((there >> lane & 1) && __popcll(there & ((1ull << lane) - 1)) == rank)) - 1;
+  const int entry = __builtin_amdgcn_readfirstlane(at);
+  s.seq = entry - 1;
+  s.len = __builtin_amdgcn_readlane(len, entry);
+  s.lo = (int64_t)__builtin_amdgcn_readlane((int)(lo >> 32), entry) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, entry);
+  s.row0 = (FROM_END ? __builtin_amdgcn_readlane(nt, entry) - 1 - t : t) * ROWS;
   return s;
 }
-// The other tensor's rows of a tile's sequence: none for the rows past the last one.
+// The other tensor's rows of a tile's sequence: none for the rows outside the offsets.
 __device__ __forceinline__ void other_rows(const int64_t* cu, int64_t nseq, int64_t total, int seq, int64_t& lo, int& len) {
-  lo = seq < nseq ? seq_start(cu, total, seq) : 0;
-  len = seq < nseq ? (int)(max(seq_start(cu, total, seq + 1), lo) - lo) : 0;
+  const bool there = seq >= 0 && seq < nseq;
+  lo = there ? seq_start(cu, total, seq) : 0;
+  len = there ? (int)(max(seq_start(cu, total, seq + 1), lo) - lo) : 0;
 }
 
 // Device-side arguments of the attention kernels (kdn_attn_args with the defaults filled in).

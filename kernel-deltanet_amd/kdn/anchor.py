@@ -294,7 +294,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Opt
               cu_seqlens_k: Optional[torch.Tensor] = None, scale: Optional[float] = None,
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal softmax attention of packed sequences: q (tokens, H, d), k and v (tokens, H_kv, d), sequence b the rows
-    cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (integers on the device; rows past the last offset are padding: zeros).  Or a
+    cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (integers on the device; rows outside the offsets are padding: zeros).  Or a
     uniform batch q (B, T, H, d), k and v (B, T, H_kv, d) without cu_seqlens.  H is a multiple of H_kv, query head h uses
     key head h / (H / H_kv).  With cu_seqlens_k the keys have lengths of their own, and a sequence's last query sees its
     last key: query i the keys j <= i + len_k - len_q (none: its row is zero).  scale: 1 / sqrt(d).

@@ -187,3 +187,33 @@ def test_a_padded_step_in_a_graph():
                                      max_new=1, max_context=step[5].shape[1] * 16)
         assert not y[live:].any()
         assert float((y[:live].float() - want.float()).abs().max()) < 2.0 ** -6  # chunks of another length: their sums' order
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lead,lead_k,lens,pad,pad_k,H,KV", [(5, 5, [70, 0, 33], 4, 4, 4, 2), (0, 200, [40, 130], 0, 3, 4, 1), (140, 0, [1, 129], 7, 0, 8, 8),
+                                                             (3, 9, [7] * 62, 5, 6, 4, 2), (3, 9, [7] * 63, 5, 6, 4, 2), (40, 150, [3] * 150, 33, 0, 4, 4),
+                                                             (600, 700, [2100], 300, 10, 32, 8), (9, 9, [], 0, 0, 4, 2), (260, 260, [4500], 0, 0, 32, 8)])
+def test_rows_outside_the_offsets(lead, lead_k, lens, pad, pad_k, H, KV, d, dtype):
+    """Rows before the first offset and behind the last: zeros, with lse -infinity and zero gradients, whatever is in memory;
+    the sequences are what they are without them."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    n = sum(lens)
+    q, k, v, dy = (torch.randn(x, h, d, generator=g, device=DEV).to(dtype) for x, h in
+                   ((lead + n + pad, H), (lead_k + n + pad_k, KV), (lead_k + n + pad_k, KV), (lead + n + pad, H)))
+    cu = torch.tensor([0, *lens], device=DEV).cumsum(0)
+    iq, ik = slice(lead, lead + n), slice(lead_k, lead_k + n)
+    nan = [torch.full((8 * max(q.numel(), 1024),), float("nan"), device=DEV)]
+    nan.clear()  # what the outputs and the workspace are likely made of
+    y, lse, low = anchor.attention_forward(q, k, v, cu + lead, cu + lead_k, out=torch.full_like(q, float("nan")), return_lse=True, return_low=True)
+    grads = anchor.attention_backward(q, k, v, y, lse, dy, cu + lead, cu + lead_k, low=low)
+    for t, i in ((y, iq), (grads[0], iq), (grads[1], ik), (grads[2], ik)):
+        assert not t[:i.start].any() and not t[i.stop:].any()
+    assert torch.isneginf(lse[:, :lead]).all() and torch.isneginf(lse[:, lead + n:]).all()
+    y2, lse2, low2 = anchor.attention_forward(q[iq], k[ik], v[ik], cu, return_lse=True, return_low=True)
+    want = [y2, *anchor.attention_backward(q[iq], k[ik], v[ik], y2, lse2, dy[iq], cu, low=low2)]
+    # another split of a row's keys or of a key's rows: fp32 sums in another order, then the rounding
+    for t, w in zip([y[iq], grads[0][iq], grads[1][ik], grads[2][ik]], want):
+        scale = float(w.float().norm()) + 1e-30
+        assert float((t.float() - w.float()).norm()) <= (2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -18) * scale

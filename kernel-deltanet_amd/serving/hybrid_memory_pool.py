@@ -114,6 +114,13 @@ class HybridMemoryPool:
         dev, P = self.anchor_slab.device, self._anchor.page_tokens
         context = [self._anchor.length(i) for i in ids]
         keep = depths is None
+        if not keep:
+            depths = torch.as_tensor(depths)
+            whole = not (depths.is_floating_point() or depths.is_complex() or depths.dtype is torch.bool)
+            if depths.is_cuda or depths.shape != (sum(new_tokens),) or (depths.numel() and not whole):
+                raise ValueError(f"anchor_plan: depths are {sum(new_tokens)} host integers, one a token; got {tuple(depths.shape)} {depths.dtype} "
+                                 f"on {depths.device}")
+            depths = depths.to(torch.int64)
         if keep:
             moves, done = [], []
             try:
@@ -139,7 +146,7 @@ class HybridMemoryPool:
                       torch.cat([self._anchor.rows(i, c, n) for i, c, n in zip(ids, context, new_tokens)] or [torch.empty(0, dtype=torch.int64)])]
         else:
             per = torch.repeat_interleave(torch.tensor(context, dtype=torch.int64), torch.tensor(list(new_tokens)))
-            parts += [per + torch.as_tensor(depths, dtype=torch.int64)]
+            parts += [per + depths]
         gather = keep and most > 64 and longest > 0  # a prompt's next piece reads its earlier keys whole
         if gather:
             parts += [torch.cat([self._anchor.rows(i, 0, c + n) for i, c, n in zip(ids, context, new_tokens)]),

@@ -1,7 +1,9 @@
 """The anchor layers' surface at its edges, with no GPU: the layer's frequencies, a plan's arguments, the operators' checks."""
+import pytest
 import torch
 
 from layers import AnchorAttentionLayer
+from serving import HybridMemoryPool
 
 
 def test_frequencies_are_made_with_the_layer():
@@ -28,3 +30,22 @@ def test_frequencies_follow_the_parameters():
     assert f.device.type == "cpu" and float(f[0]) == 1.0
     assert layer.inv_freq(torch.device("cpu")) is f
     assert "inv_freq" not in "".join(layer.state_dict())
+
+
+def pool_of(*lens, pages=8):
+    """A host pool (bookkeeping alone) whose streams have `lens` tokens."""
+    pool = HybridMemoryPool(4, 64, num_layers=1, num_heads=1, val_dim=16, lifted_dim=64, device="cpu", anchor_layers=1, anchor_heads=1,
+                            anchor_pages=pages)
+    streams = [pool.allocate_stream(n) for n in lens]
+    pool.anchor_plan(streams, list(lens))
+    return pool, streams
+
+
+@pytest.mark.parametrize("depths", [[0], [0, 1], [0, 1, 1, 2], [], [[0, 1, 2]], 0, [0.0, 1.0, 2.0], torch.tensor([0, 1]), torch.zeros(3, 1, dtype=torch.int64)])
+def test_a_plan_of_drafts_has_a_depth_for_each(depths):
+    pool, (s,) = pool_of(20)
+    with pytest.raises(ValueError):
+        pool.anchor_plan([s], [3], depths=depths)
+    for good in ([0, 1, 1], (0, 1, 1), torch.tensor([0, 1, 1]), torch.tensor([0, 1, 1], dtype=torch.int16)):
+        assert pool.anchor_plan([s], [3], depths=good).positions.tolist() == [20, 21, 21]
+    assert pool.anchor_tokens(s) == 20

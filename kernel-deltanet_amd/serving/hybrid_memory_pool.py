@@ -108,6 +108,8 @@ class HybridMemoryPool:
         filled are copied first).  With `depths` (host integers, one a token) the tokens are drafts, at positions context +
         depth, and no room is made: they may be refused.  If the pages do not suffice, RuntimeError, and no stream has
         changed."""
+        if len(new_tokens) != len(streams):
+            raise ValueError(f"anchor_plan: {len(streams)} streams and {len(new_tokens)} numbers of new tokens")
         ids = [self._anchor_stream[s] for s in streams]
         if len(set(ids)) != len(ids):
             raise ValueError("anchor_plan: a stream twice in one step")

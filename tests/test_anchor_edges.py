@@ -49,3 +49,12 @@ def test_a_plan_of_drafts_has_a_depth_for_each(depths):
     for good in ([0, 1, 1], (0, 1, 1), torch.tensor([0, 1, 1]), torch.tensor([0, 1, 1], dtype=torch.int16)):
         assert pool.anchor_plan([s], [3], depths=good).positions.tolist() == [20, 21, 21]
     assert pool.anchor_tokens(s) == 20
+
+
+@pytest.mark.parametrize("new", [[5], [5, 1, 1], []])
+@pytest.mark.parametrize("drafts", [False, True])
+def test_a_plan_has_a_number_of_tokens_for_each_stream(new, drafts):
+    pool, streams = pool_of(20, 3)
+    with pytest.raises(ValueError):
+        pool.anchor_plan(streams, new, depths=[0] * sum(new) if drafts else None)
+    assert [pool.anchor_tokens(s) for s in streams] == [20, 3]

@@ -15,6 +15,7 @@ gives what the layers' kernels take, the same for all layers; nothing waits for 
 """
 from __future__ import annotations
 
+import operator
 from typing import Optional, Sequence
 
 import torch
@@ -110,6 +111,9 @@ class HybridMemoryPool:
         changed."""
         if len(new_tokens) != len(streams):
             raise ValueError(f"anchor_plan: {len(streams)} streams and {len(new_tokens)} numbers of new tokens")
+        new_tokens = [operator.index(n) for n in new_tokens]
+        if min(new_tokens, default=0) < 0:
+            raise ValueError(f"anchor_plan: numbers of new tokens are not negative, got {new_tokens}")
         ids = [self._anchor_stream[s] for s in streams]
         if len(set(ids)) != len(ids):
             raise ValueError("anchor_plan: a stream twice in one step")
@@ -129,12 +133,12 @@ class HybridMemoryPool:
                 for i, n in zip(ids, new_tokens):
                     moves += self._anchor.extend(i, n)
                     done.append(i)
-            except RuntimeError:
+            except BaseException:
                 # the streams extended so far give their room back; copies that their shared pages got are made, so that
                 # what their tables name is there
-                self._copy_pages(moves)
                 for i, c in zip(done, context):
                     self._anchor.truncate(i, c)
+                self._copy_pages(moves)
                 raise
             self._copy_pages(moves)
         table = self._anchor.table(ids)

@@ -1,4 +1,5 @@
 """The anchor layers' surface at its edges, with no GPU: the layer's frequencies, a plan's arguments, the operators' checks."""
+import numpy as np
 import pytest
 import torch
 
@@ -58,3 +59,14 @@ def test_a_plan_has_a_number_of_tokens_for_each_stream(new, drafts):
     with pytest.raises(ValueError):
         pool.anchor_plan(streams, new, depths=[0] * sum(new) if drafts else None)
     assert [pool.anchor_tokens(s) for s in streams] == [20, 3]
+
+
+@pytest.mark.parametrize("bad,error", [(1.0, TypeError), ("1", TypeError), (None, TypeError), (-1, ValueError)])
+def test_a_refused_plan_changes_no_stream(bad, error):
+    pool, streams = pool_of(20, 3)
+    with pytest.raises(error):
+        pool.anchor_plan(streams, [5, bad])
+    assert [pool.anchor_tokens(s) for s in streams] == [20, 3] and pool.anchor_pages_used == 3
+    plan = pool.anchor_plan(streams, np.array([5, 1]))  # whole numbers of any kind
+    assert plan.positions.tolist() == [20, 21, 22, 23, 24, 3] and plan.max_new == 5
+    assert pool.anchor_plan(streams, torch.tensor([1, 2])).positions.tolist() == [25, 4, 5]

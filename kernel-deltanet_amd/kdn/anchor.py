@@ -385,8 +385,12 @@ class PagePool:
         N.check(N.lib().kdn_page_pool_create(self.num_pages, self.page_tokens, self.max_streams, _ref(self._h)), "kdn_page_pool_create")
 
     def __del__(self):
-        if getattr(self, "_h", None):
-            N.lib().kdn_page_pool_destroy(self._h)
+        h = getattr(self, "_h", None)
+        if h is not None and h.value:
+            try:
+                N.lib().kdn_page_pool_destroy(h)
+            except Exception:  # the interpreter ends, and its modules are gone
+                pass
             self._h = None
 
     @staticmethod

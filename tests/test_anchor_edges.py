@@ -1,8 +1,12 @@
 """The anchor layers' surface at its edges, with no GPU: the layer's frequencies, a plan's arguments, the operators' checks."""
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
 
+from kdn import anchor
 from layers import AnchorAttentionLayer
 from serving import HybridMemoryPool
 
@@ -70,3 +74,11 @@ def test_a_refused_plan_changes_no_stream(bad, error):
     plan = pool.anchor_plan(streams, np.array([5, 1]))  # whole numbers of any kind
     assert plan.positions.tolist() == [20, 21, 22, 23, 24, 3] and plan.max_new == 5
     assert pool.anchor_plan(streams, torch.tensor([1, 2])).positions.tolist() == [25, 4, 5]
+
+
+def test_a_pool_that_lives_to_the_end():
+    """Destroyed while the interpreter takes its modules apart: nothing is printed."""
+    path = anchor.__file__.rsplit("kdn", 1)[0]
+    code = f"import sys; sys.path.insert(0, {path!r}); from kdn import anchor; pool = anchor.PagePool(4, 16, 2); pool.open()"
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "PagePool" not in done.stderr, done.stderr

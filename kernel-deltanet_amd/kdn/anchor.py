@@ -24,7 +24,7 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 
 from . import _native as N
-from .ops import _HERE, _tag, require_device
+from .ops import _HERE, _tag, forward_only, require_device
 
 _ref = ctypes.byref
 _BF16, _F32 = torch.bfloat16, torch.float32
@@ -362,7 +362,9 @@ def page_copy(slab: torch.Tensor, pairs) -> None:
 def page_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, rows: torch.Tensor) -> None:
     """k and v (tokens, H_kv, d) into k_pages and v_pages (pages, H_kv, page_tokens, d): token i to place
     rows[i] % page_tokens of page rows[i] / page_tokens (`PagePool.rows`); one whose row is negative or past the pages is
-    skipped.  Rows are distinct."""
+    skipped.  Rows are distinct.  The pages have no gradient: k and v that need one are refused."""
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+        raise ValueError("page_append: the pages have no gradient; call it under torch.no_grad() or detach k and v")
     ks, vs = _heads(k, "page_append k"), _heads(v, "page_append v", k)
     kp, vp = _pages(k_pages, "page_append k_pages", k), _pages(v_pages, "page_append v_pages", k)
     n, KV, d = k.shape
@@ -467,7 +469,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: t
     At most 64 new tokens a stream; max_new (64, or 1 without cu_seqlens) and max_context (what page_table holds) bound
     them from the host, so that nothing is read back; the closer, the smaller the launch.  Rows outside the offsets are
     padding: zeros, as are those of a stream past max_new.  `workspace`: uint8, at least `tree_workspace_bytes`, for a caller
-    that allocates once."""
+    that allocates once.  Not differentiable: y raises on backward."""
     what = "tree_attention"
     qs = _heads(q, "tree_attention q")
     ks, vs = _heads(k, "tree_attention k", q), _heads(v, "tree_attention v", q)
@@ -504,7 +506,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: t
         N.check(N.lib().kdn_tree_attn(_TREE.pack(*sizes, cu.data_ptr(), lens.data_ptr(), page_table.data_ptr(), 0 if par is None else par.data_ptr(),
                                                  *qs[1:], *ks[1:], *vs[1:], *kp[1:], *vp[1:], *y[1:], workspace.data_ptr(), workspace.nbytes),
                                       _raw_stream(dev)), "kdn_tree_attn")
-    return y[0]
+    return forward_only(what, (y[0],), (q, k, v, k_pages, v_pages))[0]
 
 
 _NO_TENSORS = (0,) * 26  # the tensor fields of kdn_tree_attn_args, where only sizes are read

@@ -745,8 +745,8 @@ class ScanPlan:
 
 
 class _ForwardOnly(torch.autograd.Function):
-    """Identity on the scan outputs that ties them to the inputs' autograd graph; its backward raises,
-    so a training step fails loudly instead of computing gradients that skip the scan."""
+    """Identity on an operator's outputs that ties them to the inputs' autograd graph; its backward raises,
+    so a training step fails loudly instead of computing gradients that skip the operator."""
 
     @staticmethod
     def forward(ctx, what, n_out, *tensors):
@@ -755,8 +755,7 @@ class _ForwardOnly(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, *grads):
-        raise NotImplementedError(f"{ctx.what}: the backward pass of the scan is not implemented on MI355X "
-                                  "(forward/prefill only)")
+        raise NotImplementedError(f"{ctx.what}: has no backward pass on MI355X (forward/prefill only)")
 
 
 def forward_only(what: str, outputs, inputs):

@@ -217,3 +217,25 @@ def test_rows_outside_the_offsets(lead, lead_k, lens, pad, pad_k, H, KV, d, dtyp
     for t, w in zip([y[iq], grads[0][iq], grads[1][ik], grads[2][ik]], want):
         scale = float(w.float().norm()) + 1e-30
         assert float((t.float() - w.float()).norm()) <= (2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -18) * scale
+
+
+@pytest.mark.gpu
+def test_serving_operators_do_not_drop_gradients():
+    """As the ragged steps: the attention's output raises on backward; what goes into the pages is refused."""
+    q, k, v, kp, vp, table, ctx, cu = step_of([30, 0], [1, 2], 0)
+    want = anchor.tree_attention(q, k, v, kp, vp, table, ctx, cu)
+    for i in range(5):
+        args = [t.clone().requires_grad_(i == j) for j, t in enumerate((q, k, v, kp, vp))]
+        y = anchor.tree_attention(*args, table, ctx, cu)
+        assert torch.equal(y.detach(), want)
+        with pytest.raises(NotImplementedError, match="tree_attention"):
+            y.sum().backward()
+        with torch.no_grad():
+            assert not anchor.tree_attention(*args, table, ctx, cu).requires_grad
+    rows = torch.tensor([30, 32, 33], device=DEV)
+    for i in (0, 1):
+        args = [t.clone().requires_grad_(i == j) for j, t in enumerate((k, v))]
+        with pytest.raises(ValueError):
+            anchor.page_append(*args, kp, vp, rows)
+        with torch.no_grad():
+            anchor.page_append(*args, kp, vp, rows)

@@ -22,6 +22,7 @@ import struct
 from typing import List, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from .ops import _HERE, _tag, forward_only, require_device
@@ -185,7 +186,7 @@ class _Rotary(torch.autograd.Function):
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
         interleaved, magnitude, inverse = ctx.how
-        gq, gk = _rotate(dq, dk, positions, inv_freq, interleaved, magnitude, not inverse, False)
+        gq, gk = rotary(dq, dk, positions, inv_freq, interleaved, magnitude, not inverse)  # differentiable in dq and dk itself
         return gq, gk, None, None, None, None, None
 
 
@@ -285,6 +286,7 @@ class _Attention(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         q, k, v, y, lse, cu_q, cu_k, low = ctx.saved_tensors
         return (*attention_backward(q, k, v, y, lse, dy, cu_q, cu_k, ctx.scale, low), None, None, None)
@@ -299,7 +301,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Opt
     key head h / (H / H_kv).  With cu_seqlens_k the keys have lengths of their own, and a sequence's last query sees its
     last key: query i the keys j <= i + len_k - len_q (none: its row is zero).  scale: 1 / sqrt(d).
 
-    Differentiable in q, k and v; gradients come in their dtype, summed in fp32 in a fixed order.  `out`: where y goes
+    Differentiable in q, k and v, once; gradients come in their dtype, summed in fp32 in a fixed order.  `out`: where y goes
     (without autograd)."""
     if q.dim() == 4:
         if cu_seqlens is not None or cu_seqlens_k is not None or k.dim() != 4 or v.dim() != 4 or k.shape[:2] != q.shape[:2]:

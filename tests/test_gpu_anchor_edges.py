@@ -239,3 +239,26 @@ def test_serving_operators_do_not_drop_gradients():
             anchor.page_append(*args, kp, vp, rows)
         with torch.no_grad():
             anchor.page_append(*args, kp, vp, rows)
+
+
+@pytest.mark.gpu
+def test_second_derivatives():
+    """Of the attention they are refused; the rotation's are exact: with q' = R q, |dL/dq|^2 for L = |q'|^2 / 2 and a magnitude m
+    is m^4 |q|^2, whose derivative is 2 m^4 q."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q, k = (torch.randn(9, h, 64, generator=g, device=DEV).requires_grad_(True) for h in (4, 2))
+    f = anchor.rotary_frequencies(64, device=DEV)[0]
+    pos, cu = torch.arange(9, device=DEV), torch.tensor([0, 9], device=DEV)
+    for keys in (k, None):
+        a, b = anchor.rotary(q, keys, pos, f, magnitude=1.25)
+        loss = (a * a).sum() / 2 + (0 if keys is None else (b * b).sum() / 2)
+        leaves = [q] if keys is None else [q, k]
+        first = torch.autograd.grad(loss, leaves, create_graph=True)
+        second = torch.autograd.grad(sum((t * t).sum() for t in first), leaves)
+        for x, d in zip(leaves, second):
+            want = 2 * 1.25 ** 4 * x.detach()  # four turns, each within 8 units of 2^-24 of |a| + |b|
+            assert float((d - want).abs().max()) < 4 * 8 * 2.0 ** -24 * 2 * float(want.abs().max())
+    y = anchor.attention(q, k, k, cu)
+    dq, = torch.autograd.grad((y * y).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        (dq * dq).sum().backward()

@@ -22,6 +22,7 @@ import struct
 from typing import List, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -105,6 +106,16 @@ def _groups(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, what: str) -> Non
     if k.shape != v.shape or k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
         raise ValueError(f"{what}: k and v have one shape, and q a multiple of their heads; got q {tuple(q.shape)}, k {tuple(k.shape)}, "
                          f"v {tuple(v.shape)}")
+
+
+def _forward_mode(*tensors) -> bool:
+    """Whether one of them carries a forward-mode tangent, which a kernel's output would lose."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _tracked(*tensors) -> bool:
+    """Whether a call on them is recorded by autograd (its Function refuses forward mode by itself)."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or _forward_mode(*tensors)
 
 
 def _scale(scale: Optional[float], d: int, what: str) -> float:
@@ -196,7 +207,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     positions (tokens,) * inv_freq (float64, `rotary_frequencies`), in one launch: pairs (2j, 2j + 1) if interleaved, else
     (j, j + rotary_dim / 2); times `magnitude`; by the negative angle if inverse.  in_place writes q and k themselves.
     Differentiable (not in place)."""
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if _tracked(q, k):
         if in_place:
             raise ValueError("rotary: in_place has no gradient")
         return _Rotary.apply(q, k, positions, inv_freq, bool(interleaved), float(magnitude), bool(inverse))
@@ -313,7 +324,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Opt
         return y.view(q.shape)
     if cu_seqlens is None:
         raise ValueError("attention: packed (tokens, heads, d) tensors need cu_seqlens")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+    if _tracked(q, k, v):
         if out is not None:
             raise ValueError("attention: out has no gradient")
         return _Attention.apply(q, k, v, cu_seqlens, cu_seqlens_k, scale)
@@ -365,7 +376,7 @@ def page_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
     """k and v (tokens, H_kv, d) into k_pages and v_pages (pages, H_kv, page_tokens, d): token i to place
     rows[i] % page_tokens of page rows[i] / page_tokens (`PagePool.rows`); one whose row is negative or past the pages is
     skipped.  Rows are distinct.  The pages have no gradient: k and v that need one are refused."""
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+    if _tracked(k, v):
         raise ValueError("page_append: the pages have no gradient; call it under torch.no_grad() or detach k and v")
     ks, vs = _heads(k, "page_append k"), _heads(v, "page_append v", k)
     kp, vp = _pages(k_pages, "page_append k_pages", k), _pages(v_pages, "page_append v_pages", k)
@@ -473,6 +484,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: t
     padding: zeros, as are those of a stream past max_new.  `workspace`: uint8, at least `tree_workspace_bytes`, for a caller
     that allocates once.  Not differentiable: y raises on backward."""
     what = "tree_attention"
+    if _forward_mode(q, k, v, k_pages, v_pages):
+        raise NotImplementedError("tree_attention: has no forward-mode derivative")
     qs = _heads(q, "tree_attention q")
     ks, vs = _heads(k, "tree_attention k", q), _heads(v, "tree_attention v", q)
     _groups(q, k, v, what)

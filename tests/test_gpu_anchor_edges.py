@@ -2,6 +2,7 @@
 rows that no sequence has, layouts with odd strides, autograd's other modes, steps without tokens."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from kdn import anchor
 from layers import AnchorAttentionLayer
@@ -262,3 +263,25 @@ def test_second_derivatives():
     dq, = torch.autograd.grad((y * y).sum(), q, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         (dq * dq).sum().backward()
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    """A tangent is not lost: every operator that computes raises, with gradients enabled or not."""
+    q, k, v, kp, vp, table, ctx, cu = step_of([30, 0], [1, 2], 0, dtype=torch.float32)
+    f, pos = anchor.rotary_frequencies(64, device=DEV)[0], torch.arange(3, device=DEV)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for calls in ((lambda: anchor.rotary(dual(q), k, pos, f), lambda: anchor.rotary(q, dual(k), pos, f), lambda: anchor.rotary(dual(q), None, pos, f)),
+                      [lambda i=i: anchor.attention(*(dual(t) if i == j else t for j, t in enumerate((q, k, v))), cu) for i in range(3)],
+                      [lambda i=i: anchor.tree_attention(*(dual(t) if i == j else t for j, t in enumerate((q, k, v, kp, vp))), table, ctx, cu)
+                       for i in range(5)]):
+            for call in calls:
+                with pytest.raises(NotImplementedError):
+                    call()
+                with torch.no_grad(), pytest.raises(NotImplementedError):
+                    call()
+        with pytest.raises(ValueError):
+            anchor.page_append(dual(k), v, kp, vp, pos)
+        plain = anchor.attention(q, k, v, cu)  # nothing of it has a tangent
+    assert torch.equal(plain, anchor.attention(q, k, v, cu))

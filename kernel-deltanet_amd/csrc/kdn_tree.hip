@@ -599,7 +599,8 @@ static int64_t tree_chunks(const kdn_tree_attn_args* a) {
 
 static int tree_check(const kdn_tree_attn_args* a) {
   if (!a || a->num_seqs < 0 || a->total_new < 0 || a->H <= 0 || a->H_kv <= 0 || a->H > (1 << 20) || a->H % a->H_kv != 0 ||
-      !valid_dtype(a->dtype) || !(a->scale > 0.f) || !std::isfinite(a->scale) || a->max_context < 0 || a->max_new <= 0 ||
+      !valid_dtype(a->dtype) || !(a->scale > 0.f) || !std::isfinite(a->scale) || a->max_context < 0 ||
+      a->max_new < 0 || (a->max_new == 0 && a->total_new > 0) ||
       a->page_tokens <= 0 || a->num_pages < 0 || a->table_width < 0)
     return KDN_ERR_INVALID_ARGUMENT;
   if ((a->d != 64 && a->d != 128) || a->max_new > 64 || a->page_tokens < 16 || (a->page_tokens & (a->page_tokens - 1)) != 0 ||

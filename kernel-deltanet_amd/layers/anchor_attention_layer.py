@@ -75,7 +75,7 @@ class AnchorAttentionLayer(nn.Module):
         """Differentiable.  With cu_seqlens (device, the first 0) positions start anew in each sequence."""
         if cu_seqlens is None:
             B, T, _ = x.shape
-            flat, cu = x.reshape(B * T, -1), torch.arange(B + 1, device=x.device) * T
+            flat, cu = x.reshape(B * T, x.shape[-1]), torch.arange(B + 1, device=x.device) * T
             at = torch.arange(T, device=x.device).repeat(B)
         else:
             flat, cu = x, cu_seqlens.to(torch.int64)
@@ -83,7 +83,7 @@ class AnchorAttentionLayer(nn.Module):
             at = t - cu[(torch.bucketize(t, cu, right=True) - 1).clamp(min=0)]
         q, k, v = self._project(flat, at)
         y = anchor.attention(q, k, v, cu)
-        return self.w_out(y.reshape(flat.shape[0], -1)).view(*x.shape[:-1], -1)
+        return self.w_out(y.view(-1, self.num_heads * self.d_head)).view(x.shape)
 
     @torch.no_grad()
     def step(self, x: torch.Tensor, plan, k_pages: torch.Tensor, v_pages: torch.Tensor, parents: Optional[torch.Tensor] = None):
@@ -103,5 +103,5 @@ class AnchorAttentionLayer(nn.Module):
         else:  # a prompt's next piece: its stream's keys so far out of the pages
             page, off = plan.all_rows // k_pages.shape[2], plan.all_rows % k_pages.shape[2]
             y = anchor.attention(q, k_pages[page, :, off], v_pages[page, :, off], plan.cu_seqlens, plan.cu_all)
-        out = self.w_out(y.reshape(x.shape[0], -1))
+        out = self.w_out(y.view(-1, self.num_heads * self.d_head))
         return out if plan.keep else (out, k, v)

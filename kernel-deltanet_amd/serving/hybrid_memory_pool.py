@@ -151,7 +151,7 @@ class HybridMemoryPool:
             parts += [torch.cat([torch.arange(c, c + n) for c, n in zip(context, new_tokens)] or [torch.empty(0, dtype=torch.int64)]),
                       torch.cat([self._anchor.rows(i, c, n) for i, c, n in zip(ids, context, new_tokens)] or [torch.empty(0, dtype=torch.int64)])]
         else:
-            per = torch.repeat_interleave(torch.tensor(context, dtype=torch.int64), torch.tensor(list(new_tokens)))
+            per = torch.repeat_interleave(torch.tensor(context, dtype=torch.int64), torch.tensor(new_tokens, dtype=torch.int64))
             parts += [per + depths]
         gather = keep and most > 64 and longest > 0  # a prompt's next piece reads its earlier keys whole
         if gather:

@@ -1,4 +1,5 @@
 """The anchor layers' surface at its edges, with no GPU: the layer's frequencies, a plan's arguments, the operators' checks."""
+import ctypes
 import subprocess
 import sys
 
@@ -6,6 +7,7 @@ import numpy as np
 import pytest
 import torch
 
+from kdn import _native as N
 from kdn import anchor
 from layers import AnchorAttentionLayer
 from serving import HybridMemoryPool
@@ -82,3 +84,20 @@ def test_a_pool_that_lives_to_the_end():
     code = f"import sys; sys.path.insert(0, {path!r}); from kdn import anchor; pool = anchor.PagePool(4, 16, 2); pool.open()"
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "PagePool" not in done.stderr, done.stderr
+
+
+def test_plans_without_tokens():
+    pool, streams = pool_of(20, 3)
+    for plan in (pool.anchor_plan(streams, [0, 0]), pool.anchor_plan(streams, [0, 0], depths=[])):
+        assert plan.max_new == 0 and plan.positions.tolist() == [] and plan.cu_seqlens.tolist() == [0, 0, 0] and plan.context_lens.tolist() == [20, 3]
+    for plan in (pool.anchor_plan([], []), pool.anchor_plan([], [], depths=[])):
+        assert plan.max_new == 0 and plan.positions.tolist() == [] and plan.cu_seqlens.tolist() == [0] and plan.page_table.shape[0] == 0
+    assert pool.anchor_plan(streams, [0, 1]).positions.tolist() == [3]
+
+
+def test_a_call_without_new_tokens_needs_no_bound():
+    a = N.TreeAttnArgs()
+    a.num_seqs, a.H, a.H_kv, a.d, a.dtype, a.scale, a.page_tokens = 2, 8, 2, 128, 1, 0.1, 16
+    assert N.lib().kdn_tree_attn(ctypes.byref(a), None) == 0 and N.lib().kdn_tree_attn_workspace_bytes(ctypes.byref(a)) > 0
+    a.total_new = 1
+    assert N.lib().kdn_tree_attn(ctypes.byref(a), None) == -1 and N.lib().kdn_tree_attn_workspace_bytes(ctypes.byref(a)) == 0

@@ -6,6 +6,7 @@ from torch.autograd import forward_ad
 
 from kdn import anchor
 from layers import AnchorAttentionLayer
+from serving import HybridMemoryPool
 
 DEV = "cuda:0"
 
@@ -285,3 +286,30 @@ def test_forward_mode_is_refused():
             anchor.page_append(dual(k), v, kp, vp, pos)
         plain = anchor.attention(q, k, v, cu)  # nothing of it has a tangent
     assert torch.equal(plain, anchor.attention(q, k, v, cu))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_nothing_to_do(dtype):
+    """Steps of no tokens or no streams, and empty batches: outputs of their shape, and gradients of zero."""
+    layer = AnchorAttentionLayer(256, 4, 2).to(DEV, dtype)
+    pool = HybridMemoryPool(4, 64, num_layers=1, num_heads=1, val_dim=16, lifted_dim=64, device=DEV, anchor_layers=1, anchor_heads=2,
+                            anchor_pages=16, anchor_dtype=dtype)
+    some = [pool.allocate_stream(0) for _ in range(2)]
+    layer.step(torch.randn(21, 256, device=DEV).to(dtype), pool.anchor_plan(some, [20, 1]), *pool.anchor_pages(0))
+    x = torch.zeros(0, 256, dtype=dtype, device=DEV)
+    for streams in (some, []):
+        none = [0] * len(streams)
+        assert layer.step(x, pool.anchor_plan(streams, none), *pool.anchor_pages(0)).shape == (0, 256)
+        out, k, v = layer.step(x, pool.anchor_plan(streams, none, depths=[]), *pool.anchor_pages(0))
+        assert out.shape == (0, 256) and k.shape == v.shape == (0, 2, 64)
+    for shape, cu in (((0, 7, 256), None), ((3, 0, 256), None), ((0, 256), torch.tensor([0, 0, 0], device=DEV)), ((0, 256), torch.tensor([0], device=DEV))):
+        layer.zero_grad()
+        x = torch.zeros(shape, dtype=dtype, device=DEV, requires_grad=True)
+        y = layer(x, cu)
+        assert y.shape == shape
+        y.sum().backward()
+        assert x.grad.shape == shape and not any(p.grad.any() for p in layer.parameters())
+    q = torch.zeros(0, 4, 64, dtype=dtype, device=DEV)
+    assert anchor.tree_attention(q, q, q, *(torch.zeros(1, 4, 16, 64, dtype=dtype, device=DEV),) * 2, torch.zeros(0, 1, dtype=torch.int32, device=DEV),
+                                 torch.zeros(0, dtype=torch.int32, device=DEV)).shape == q.shape

@@ -54,11 +54,11 @@ extern "C" {
 typedef enum kdn_status {
   KDN_OK = 0,
   KDN_ERR_INVALID_ARGUMENT = -1,  /* null pointer, non-positive size, bad stride, bad dtype tag */
-  KDN_ERR_UNSUPPORTED = -2,       /* valid request outside what the kernels implement (d_k, D, d_v) */
+  KDN_ERR_UNSUPPORTED = -2,       /* valid request outside what the kernels implement (d_k, D, d_v; d, pages) */
   KDN_ERR_WORKSPACE_TOO_SMALL = -3,
   KDN_ERR_MISALIGNED = -4,        /* a pointer or row stride breaks the 16-byte vector-access rule */
   KDN_ERR_DEVICE = -5,            /* a HIP launch reported an error */
-  KDN_ERR_CAPACITY = -6           /* the state pool has no free slot */
+  KDN_ERR_CAPACITY = -6           /* a pool has no free slot, stream or page */
 } kdn_status;
 
 typedef enum kdn_dtype {

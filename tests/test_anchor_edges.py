@@ -101,3 +101,13 @@ def test_a_call_without_new_tokens_needs_no_bound():
     assert N.lib().kdn_tree_attn(ctypes.byref(a), None) == 0 and N.lib().kdn_tree_attn_workspace_bytes(ctypes.byref(a)) > 0
     a.total_new = 1
     assert N.lib().kdn_tree_attn(ctypes.byref(a), None) == -1 and N.lib().kdn_tree_attn_workspace_bytes(ctypes.byref(a)) == 0
+
+
+def test_errors_name_what_the_anchor_layers_support():
+    for status, words in ((-2, ("d 64 or 128", "64 new tokens", "pages", "d_k must be 64")), (-6, ("slot", "stream", "page"))):
+        text = N.lib().kdn_strerror(status).decode()
+        assert all(w in text for w in words), text
+    pool = anchor.PagePool(1, 16, 1)
+    s = pool.open()
+    with pytest.raises(RuntimeError, match="page"):
+        pool.extend(s, 17)

@@ -581,15 +581,23 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeParams p) {
   for (int i = 0; i < V; ++i) dst[i] = (E)(o[i] * g);
 }
 
+// A product of sizes that no caller's numbers take past 64 bits.
+static int64_t times(int64_t a, int64_t b) {
+  int64_t r;
+  return __builtin_mul_overflow(a, b, &r) ? INT64_MAX : r;
+}
+static int64_t tree_rows(const kdn_tree_attn_args* a) { return a->max_new * (a->H / a->H_kv); }  // to a sequence and key head
+static int64_t tree_blocks(const kdn_tree_attn_args* a) { return tree_rows(a) <= 32 ? 1 : (tree_rows(a) + 127) / 128; }
+
 constexpr int MAX_CHUNK = 2048;
 // Keys of a chunk: 128 to 2048, the fewest with which the grid stays within 512 workgroups, or from 256 keys on 2048 (a
 // chunk's own cost, its queries and its partial sums, is that of a few dozen keys; short chunks even out unequal contexts).
 // With chunks of at most 1024 keys 16 trees of 40 drafts, contexts of 1500 to 16384, took 186 us where these took 177, one
 // token of 224 streams 396 where these took 378; with up to 4096 the 224 streams took 395.
 static int tree_chunk(const kdn_tree_attn_args* a) {
-  const int64_t rows = a->max_new * (a->H / a->H_kv), blocks = rows <= 32 ? 1 : (rows + 127) / 128;
+  const int64_t each = times(a->num_seqs * a->H_kv, tree_blocks(a));
   int chunk = 128;
-  while (chunk < MAX_CHUNK && a->num_seqs * a->H_kv * blocks * ((a->max_context + chunk - 1) / chunk) > (chunk < 256 ? 512 : 2048)) chunk *= 2;
+  while (chunk < MAX_CHUNK && times(each, (a->max_context + chunk - 1) / chunk) > (chunk < 256 ? 512 : 2048)) chunk *= 2;
   return chunk;
 }
 static int64_t tree_chunks(const kdn_tree_attn_args* a) {
@@ -604,9 +612,15 @@ static int tree_check(const kdn_tree_attn_args* a) {
       a->page_tokens <= 0 || a->num_pages < 0 || a->table_width < 0)
     return KDN_ERR_INVALID_ARGUMENT;
   if ((a->d != 64 && a->d != 128) || a->max_new > 64 || a->page_tokens < 16 || (a->page_tokens & (a->page_tokens - 1)) != 0 ||
-      a->total_new > INT32_MAX || a->num_seqs > INT32_MAX || a->num_pages > INT32_MAX || a->max_context > (1 << 30))
+      a->page_tokens > (1 << 30) || a->total_new > INT32_MAX || a->num_seqs > INT32_MAX || a->num_pages > INT32_MAX ||
+      a->max_context > (1 << 30))
     return KDN_ERR_UNSUPPORTED;
-  if (a->max_context > 0 && (a->num_pages == 0 || a->max_context > a->table_width * a->page_tokens)) return KDN_ERR_INVALID_ARGUMENT;
+  if (a->max_context > 0 && (a->num_pages == 0 || (a->max_context + a->page_tokens - 1) / a->page_tokens > a->table_width))
+    return KDN_ERR_INVALID_ARGUMENT;
+  // a grid's workgroups, and the join's rows
+  const int64_t heads = a->num_seqs * a->H_kv, blocks = tree_blocks(a);
+  if (times(times(heads, tree_chunks(a)), blocks) > INT32_MAX - 8 * blocks - ZERO_GROUPS || times(heads, tree_rows(a)) > INT32_MAX)
+    return KDN_ERR_UNSUPPORTED;
   return KDN_OK;
 }
 
@@ -635,7 +649,7 @@ using namespace kdn;
 
 // Bytes of the partial sums of `units` chunks.
 static size_t tree_partial_bytes(const kdn_tree_attn_args* a, int64_t units) {
-  return (size_t)units * (size_t)(a->max_new * (a->H / a->H_kv)) * (size_t)(a->d + 2) * 4 + 16;
+  return (size_t)units * (size_t)tree_rows(a) * (size_t)(a->d + 2) * 4 + 16;
 }
 
 // Not the call's own number of chunks but a bound that grows with every size, so that a workspace for the largest call
@@ -660,9 +674,7 @@ extern "C" int kdn_tree_attn(const kdn_tree_attn_args* a, void* stream) {
   for (int i = 0; i < 3; ++i)
     fits = fits && a->k_pages_stride[i] >= 0 && a->v_pages_stride[i] >= 0 && a->k_pages_stride[i] % per == 0 && a->v_pages_stride[i] % per == 0;
   if (!fits) return KDN_ERR_MISALIGNED;
-  const int64_t chunks = tree_chunks(a), rows = a->max_new * (a->H / a->H_kv), blocks = rows <= 32 ? 1 : (rows + 127) / 128;  // at least as many as there will be
-  if (a->num_seqs * a->H_kv * chunks * blocks > INT32_MAX - 8 * blocks - ZERO_GROUPS || a->num_seqs * a->H_kv * rows > INT32_MAX)
-    return KDN_ERR_UNSUPPORTED;
+  const int64_t chunks = tree_chunks(a);
   // a copy's lanes have 32-bit offsets from its first row
   const int64_t size = (int64_t)dtype_size(a->dtype), far = INT32_MAX / (16 * size);
   if (a->k_stride[0] > far || a->v_stride[0] > far || a->k_pages_stride[2] > far || a->v_pages_stride[2] > far) return KDN_ERR_UNSUPPORTED;

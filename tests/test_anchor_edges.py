@@ -111,3 +111,26 @@ def test_errors_name_what_the_anchor_layers_support():
     s = pool.open()
     with pytest.raises(RuntimeError, match="page"):
         pool.extend(s, 17)
+
+
+def test_sizes_past_what_the_grid_takes():
+    """Refused from the numbers alone, however large: no product of them wraps into one that passes."""
+    def args(**kw):
+        a = N.TreeAttnArgs()
+        a.num_seqs, a.total_new, a.max_new, a.max_context, a.H, a.H_kv, a.d, a.dtype, a.scale = 2, 2, 1, 4096, 8, 2, 128, 1, 0.1
+        a.page_tokens, a.num_pages, a.table_width, a.table_stride = 16, 999, 256, 256
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return ctypes.byref(a)
+
+    size, call = N.lib().kdn_tree_attn_workspace_bytes, N.lib().kdn_tree_attn
+    big = 1 << 20
+    for bad in (dict(page_tokens=1 << 31, table_width=1), dict(page_tokens=1 << 32, table_width=1), dict(page_tokens=1 << 62, table_width=1),
+                dict(num_seqs=(1 << 31) - 1, H=big, H_kv=big, max_context=1 << 30, table_width=1 << 26),
+                dict(num_seqs=1 << 30, H=big, H_kv=big, max_context=1 << 25, table_width=1 << 21),
+                dict(num_seqs=1 << 30, H=big, H_kv=1, max_new=64), dict(num_seqs=1 << 20, H=big, H_kv=1, max_new=64)):
+        assert size(args(**bad)) == 0 and call(args(**bad), None) == -2, bad
+    for bad in (dict(table_width=255), dict(max_context=4097)):
+        assert size(args(**bad)) == 0 and call(args(**bad), None) == -1, bad
+    # a wide table of small pages, and one page of a whole context
+    assert size(args(table_width=1 << 60)) == size(args(page_tokens=1 << 30, table_width=1)) == size(args()) > 16

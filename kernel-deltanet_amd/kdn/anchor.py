@@ -350,6 +350,22 @@ def _pages(t: torch.Tensor, what: str, like: torch.Tensor):
     return t, p, a, b, c
 
 
+def _pairs(pairs) -> torch.Tensor:
+    """A page copy's list as the library reads it, (n, 2) int32 on the host."""
+    p = pairs if isinstance(pairs, torch.Tensor) else torch.as_tensor(pairs)
+    if p.is_cuda:
+        raise ValueError("page_copy: pairs are host numbers")
+    if p.dtype is torch.int32 and p.dim() == 2 and p.shape[1] == 2 and p.is_contiguous():
+        return p
+    if p.numel() and (p.is_floating_point() or p.dtype is torch.bool or p.dim() > 2 or (p.dim() == 2 and p.shape[1] != 2)):
+        raise ValueError(f"page_copy: pairs are (n, 2) whole numbers, got {tuple(p.shape)} {p.dtype}")
+    wide = p.reshape(-1, 2)
+    p = wide.to(torch.int32).contiguous()
+    if not torch.equal(p.to(wide.dtype), wide):
+        raise ValueError("page_copy: a page number is past 32 bits")
+    return p
+
+
 def page_copy(slab: torch.Tensor, pairs) -> None:
     """Page pairs[i][0] of slab (pages, ...; contiguous) to page pairs[i][1], for host pairs (a CPU int32 tensor (n, 2) or
     pairs of numbers) as `PagePool` gives them: no page is the target of two pairs, or a target and a source."""
@@ -357,11 +373,7 @@ def page_copy(slab: torch.Tensor, pairs) -> None:
         require_device(slab, "page_copy")
     if slab.dim() < 2 or not slab.is_contiguous():
         raise ValueError("page_copy: the slab must be contiguous, pages first")
-    p = pairs
-    if not isinstance(p, torch.Tensor) or p.dtype is not torch.int32 or p.dim() != 2 or p.shape[1] != 2 or not p.is_contiguous():
-        p = torch.as_tensor(pairs, dtype=torch.int32).reshape(-1, 2).contiguous()
-    if p.is_cuda:
-        raise ValueError("page_copy: pairs are host numbers")
+    p = _pairs(pairs)
     n = p.shape[0]
     if n == 0:
         return

@@ -134,3 +134,19 @@ def test_sizes_past_what_the_grid_takes():
         assert size(args(**bad)) == 0 and call(args(**bad), None) == -1, bad
     # a wide table of small pages, and one page of a whole context
     assert size(args(table_width=1 << 60)) == size(args(page_tokens=1 << 30, table_width=1)) == size(args()) > 16
+
+
+@pytest.mark.parametrize("bad", [torch.tensor([[0, 1 << 32]]), [(0, (1 << 32) + 1)], torch.tensor([[0, 2, 4], [1, 3, 5]]), [(0.0, 1.5)],
+                                 torch.tensor([[[0, 1]]]), torch.tensor([[True, False]])])
+def test_page_numbers_are_not_cut(bad):
+    """Numbers past 32 bits, fractions and lists of another shape name no pages: refused, not wrapped or cut into others."""
+    with pytest.raises(ValueError):
+        anchor._pairs(bad)
+
+
+@pytest.mark.parametrize("good", [[(0, 1), (2, 3)], torch.tensor([[0, 1], [2, 3]]), torch.tensor([[0, 2], [1, 3]], dtype=torch.int32).t(), np.array([[0, 1], [2, 3]]),
+                                  [0, 1, 2, 3]])
+def test_page_pairs_of_any_whole_numbers(good):
+    p = anchor._pairs(good)
+    assert p.dtype == torch.int32 and p.is_contiguous() and p.tolist() == [[0, 1], [2, 3]]
+    assert anchor._pairs([]).shape == (0, 2)

@@ -85,6 +85,7 @@ def _out(t: torch.Tensor, what: str, shape, like: torch.Tensor):
     a, b = _steps(t)
     if t.stride(-1) != 1 or t.data_ptr() % 16 or (a | b) * t.element_size() % 16:
         raise ValueError(f"{what}: needs contiguous heads whose rows start on 16 bytes")
+    torch.autograd.graph.increment_version(t)  # as torch's own writes: a backward that saved it refuses what it has become
     return t, t.data_ptr(), a, b
 
 

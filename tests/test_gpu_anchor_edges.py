@@ -313,3 +313,23 @@ def test_nothing_to_do(dtype):
     q = torch.zeros(0, 4, 64, dtype=dtype, device=DEV)
     assert anchor.tree_attention(q, q, q, *(torch.zeros(1, 4, 16, 64, dtype=dtype, device=DEV),) * 2, torch.zeros(0, 1, dtype=torch.int32, device=DEV),
                                  torch.zeros(0, dtype=torch.int32, device=DEV)).shape == q.shape
+
+
+@pytest.mark.gpu
+def test_writes_in_place_are_seen_by_autograd():
+    """A tensor that a backward saved and an operator then wrote: the backward refuses it, as after torch's own writes."""
+    q, k, v, kp, vp, table, ctx, cu = step_of([30, 0], [1, 2], 0, dtype=torch.float32)
+    f, pos = anchor.rotary_frequencies(64, device=DEV)[0], torch.arange(3, device=DEV)
+    w = torch.ones(64, device=DEV, requires_grad=True)
+    for write in (lambda t: anchor.rotary(t, None, pos, f, in_place=True), lambda t: anchor.rotary(k.clone().repeat(1, 4, 1), t, pos, f, in_place=True),
+                  lambda t: anchor.attention(q, k, v, cu, out=t), lambda t: anchor.tree_attention(q, k, v, kp, vp, table, ctx, cu, out=t)):
+        held = q.clone()
+        loss = (held * w).sum()
+        with torch.no_grad():
+            write(held)
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        held = q.clone()
+        anchor.rotary(held, None, pos, f, in_place=True)
+    assert torch.equal(held, anchor.rotary(q, None, pos, f)[0])

@@ -109,14 +109,18 @@ def _groups(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, what: str) -> Non
                          f"v {tuple(v.shape)}")
 
 
-def _forward_mode(*tensors) -> bool:
+def _dual(tensors) -> bool:
     """Whether one of them carries a forward-mode tangent, which a kernel's output would lose."""
-    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _tracked(*tensors) -> bool:
-    """Whether a call on them is recorded by autograd (its Function refuses forward mode by itself)."""
-    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or _forward_mode(*tensors)
+    """Whether autograd follows a call on them, in either mode (a Function without a forward mode refuses it by itself)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0 and _dual(tensors)
 
 
 def _scale(scale: Optional[float], d: int, what: str) -> float:
@@ -497,7 +501,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: t
     padding: zeros, as are those of a stream past max_new.  `workspace`: uint8, at least `tree_workspace_bytes`, for a caller
     that allocates once.  Not differentiable: y raises on backward."""
     what = "tree_attention"
-    if _forward_mode(q, k, v, k_pages, v_pages):
+    tracked = _tracked(q, k, v, k_pages, v_pages)
+    if tracked and forward_ad._current_level >= 0 and _dual((q, k, v, k_pages, v_pages)):
         raise NotImplementedError("tree_attention: has no forward-mode derivative")
     qs = _heads(q, "tree_attention q")
     ks, vs = _heads(k, "tree_attention k", q), _heads(v, "tree_attention v", q)
@@ -534,7 +539,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: t
         N.check(N.lib().kdn_tree_attn(_TREE.pack(*sizes, cu.data_ptr(), lens.data_ptr(), page_table.data_ptr(), 0 if par is None else par.data_ptr(),
                                                  *qs[1:], *ks[1:], *vs[1:], *kp[1:], *vp[1:], *y[1:], workspace.data_ptr(), workspace.nbytes),
                                       _raw_stream(dev)), "kdn_tree_attn")
-    return forward_only(what, (y[0],), (q, k, v, k_pages, v_pages))[0]
+    return forward_only(what, (y[0],), (q, k, v, k_pages, v_pages))[0] if tracked else y[0]
 
 
 _NO_TENSORS = (0,) * 26  # the tensor fields of kdn_tree_attn_args, where only sizes are read

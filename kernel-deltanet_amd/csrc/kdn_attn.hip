@@ -13,10 +13,10 @@
 namespace kdn {
 
 // What bounds it: a block of 32 rows and 32 keys at 128 features is 512 cycles of products and about 450 of softmax, and two
-// waves a SIMD overlap them in part.  One sequence of 16384 rows, 32 heads of 128 in bf16: 2.05 to 2.15 ms, 1.02 to 1.07
-// PFLOP/s, where a product of 16384-wide matrices reaches 1.35; the matrix cores are busy in 55 % of the cycles, at 1.6 GHz,
+// waves a SIMD overlap them in part.  One sequence of 16384 rows, 32 heads of 128 in bf16: 1.97 to 2.08 ms by card, 1.06 to
+// 1.12 PFLOP/s, where a product of 16384-wide matrices reaches 1.35; the matrix cores are busy in 55 % of the cycles, at 1.6 GHz,
 // which the load holds the clock to (2.4 at most); no LDS bank conflicts.  Seven prompts of 33 to 2048 rows, 16 heads of 64:
-// 32 us.
+// 32 us.  fp32, 4096 rows, 32 heads of 128: 1.2 to 1.3 ms, 105 to 114 TFLOP/s of 150; matrix cores busy 72 %.
 //   The walk over the keys is one chain, so that a batch with few rows takes the time of its longest row, however idle the
 // GPU: then SPLIT waves share 32 rows and take every SPLIT-th block of 32 keys of a tile each, and their sums meet at the end
 // (attn_split has the rule).
@@ -272,7 +272,9 @@ int attn_check_tensors(const kdn_attn_args* a) {
   return KDN_OK;
 }
 
-// Two workgroups run on each of the 256 CUs: fewer tiles of 128 rows than that leave CUs idle, twice that are two rounds.
+// Two workgroups on each of the 256 CUs: fewer tiles of 128 rows than that leave CUs idle, twice that are two rounds.  Two is
+// what bf16 has with one or two waves to a row; with four at 128 features, and in fp32, registers or LDS allow one (fp32 of 64
+// features with two waves, forward: two), and the rule has not been measured for them between 128 and 2048 tiles.
 // Measured, four / two / one wave to a row: three sequences of 101 to 1024 rows, 4 heads, fp32, gradients 53 / - / 158 us;
 // seven of 33 to 2048, 16 heads, bf16 56 / 33 / 39 us; one of 16384, 32 heads 5880 / 2560 / 2106 us.
 int attn_split(int64_t rows, int64_t heads) {

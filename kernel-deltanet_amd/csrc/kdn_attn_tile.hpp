@@ -21,7 +21,6 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LN2 = 0.6931471805599453f;
 
 __device__ __forceinline__ int rho(int half, int i) { return 8 * (i >> 2) + 4 * half + (i & 3); }
 

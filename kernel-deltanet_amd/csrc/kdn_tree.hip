@@ -11,8 +11,12 @@
 // What bounds them: few rows, HBM (one token of 224 streams, contexts of 512 to 16384, 16 heads of 128 over 4: 2.07 GB in 373 us,
 // 5.5 TB/s; a large copy 4.9, a read 4.0); many, a wave's own chain of copies, products and softmax for each tile, two to a SIMD where
 // 160 rows are five waves on two workgroups, and the unequal chunks' tail (16 trees of 40 drafts, contexts of 1500 to 16384, 32 heads
-// over 8: 0.53 GB in 158 us, of which the join 14; matrix cores busy 16 %, CUs 77 %).
-// One token of three streams, contexts of 700 to 2500, fp32: 14 us, a chunk's latency, and 4 for the join.
+// over 8: 0.53 GB in 158 us, of which the join 14; matrix cores busy 16 %, CUs 75 %).
+// One token of three streams, contexts of 700 to 2500, fp32: 14 us, and 5 for the join.  Of these the products take 3.4 (a wave has
+// two tiles in turn, 64 products of 64 cycles each, 4 of their 32 columns in use), the rest is the chain from the chunk's number
+// over its page's to the copies.  fp32 of larger sizes is bound by its products: one token of 64 streams, contexts of 512 to 16384,
+// 16 heads of 128 over 4: 655 us for 1.3 GB (one wave a workgroup, two of four SIMDs idle; with heads of 64 199 us for 0.65 GB); the
+// 16 trees 1315 us, matrix cores busy 30 %, one workgroup a CU.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

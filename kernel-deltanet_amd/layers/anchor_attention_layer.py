@@ -40,7 +40,8 @@ class AnchorAttentionLayer(nn.Module):
                            trained_length=trained_length)
         with torch.inference_mode(False):  # a table that training can save, wherever the layer is made
             self._host_freq, self.magnitude = anchor.rotary_frequencies(**frequencies, device="cpu")
-        self._place(self.w_q.weight.device)
+        self._inv_freq = self._host_freq
+        self._follow()
 
     def _place(self, device) -> None:
         """The frequencies on `device`: float64 whatever the module's type is cast to (so no buffer), and there when this
@@ -48,10 +49,14 @@ class AnchorAttentionLayer(nn.Module):
         with torch.inference_mode(False):
             self._inv_freq = self._host_freq.to(device)
 
+    def _follow(self) -> None:
+        device = next(self.parameters(), self._inv_freq).device  # (projections may be replaced by ones without parameters)
+        if self._inv_freq.device != device:
+            self._place(device)
+
     def _apply(self, fn, recurse=True):
         super()._apply(fn, recurse)
-        if self._inv_freq.device != self.w_q.weight.device:
-            self._place(self.w_q.weight.device)
+        self._follow()
         return self
 
     def inv_freq(self, device) -> torch.Tensor:

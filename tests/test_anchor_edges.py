@@ -37,6 +37,11 @@ def test_frequencies_follow_the_parameters():
     assert f.device.type == "cpu" and float(f[0]) == 1.0
     assert layer.inv_freq(torch.device("cpu")) is f
     assert "inv_freq" not in "".join(layer.state_dict())
+    for name in ("w_q", "w_k", "w_v", "w_out"):  # projections of another kind, without parameters of their own
+        setattr(layer, name, torch.nn.Identity())
+    assert layer.to("cpu")._inv_freq is f
+    layer.w_q = torch.nn.Linear(4, 4, device="meta")
+    assert layer.to(torch.float64)._inv_freq.device.type == "meta"
 
 
 def pool_of(*lens, pages=8):

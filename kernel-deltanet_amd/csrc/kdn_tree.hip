@@ -682,7 +682,7 @@ extern "C" int kdn_tree_attn(const kdn_tree_attn_args* a, void* stream) {
   // a copy's lanes have 32-bit offsets from its first row
   const int64_t size = (int64_t)dtype_size(a->dtype), far = INT32_MAX / (16 * size);
   if (a->k_stride[0] > far || a->v_stride[0] > far || a->k_pages_stride[2] > far || a->v_pages_stride[2] > far) return KDN_ERR_UNSUPPORTED;
-  if (chunks > 1 && (!a->workspace || a->workspace_bytes < tree_partial_bytes(a, a->num_seqs * a->H_kv * chunks))) return KDN_ERR_WORKSPACE_TOO_SMALL;
+  if (a->num_seqs > 0 && chunks > 1 && (!a->workspace || a->workspace_bytes < tree_partial_bytes(a, a->num_seqs * a->H_kv * chunks))) return KDN_ERR_WORKSPACE_TOO_SMALL;
   TreeParams p = {};
   p.q = a->q; p.k = a->k; p.v = a->v; p.kp = a->k_pages; p.vp = a->v_pages; p.y = a->y;
   for (int i = 0; i < 2; ++i) {

@@ -1,9 +1,12 @@
 """The anchor layers' surface at its edges on the GPU: first calls in a capture, on another stream and in inference mode,
 rows that no sequence has, layouts with odd strides, autograd's other modes, steps without tokens."""
+import ctypes
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+from kdn import _native as N
 from kdn import anchor
 from layers import AnchorAttentionLayer
 from serving import HybridMemoryPool
@@ -169,6 +172,17 @@ def test_tokens_past_max_new_are_zeros(H):
 def test_a_padded_step_without_streams_is_zeros():
     q, k, v, kp, vp, table, ctx, cu = step_of([], [], 6)
     y = anchor.tree_attention(q, k, v, kp, vp, table.view(0, 1), ctx, cu, out=torch.full_like(q, float("nan")))
+    assert not y.any()
+
+
+@pytest.mark.gpu
+def test_a_call_without_streams_needs_y_alone():
+    y = torch.full((6, 8, 64), float("nan"), dtype=torch.bfloat16, device=DEV)
+    a = N.TreeAttnArgs()
+    a.total_new, a.max_new, a.max_context, a.H, a.H_kv, a.d, a.dtype, a.scale = 6, 1, 4096, 8, 2, 64, N.KDN_DTYPE_BF16, 0.125
+    a.page_tokens, a.num_pages, a.table_width, a.table_stride, a.y = 16, 1, 256, 256, y.data_ptr()
+    a.y_stride[0], a.y_stride[1] = 512, 64
+    assert N.lib().kdn_tree_attn(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
     assert not y.any()
 
 

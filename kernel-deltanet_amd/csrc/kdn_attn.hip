@@ -28,7 +28,9 @@ struct Fwd {
   static constexpr int LDS = 2 * BUFS * TILE > JOIN ? 2 * BUFS * TILE : JOIN;
 };
 
-template <class P, int SPLIT>
+//   WIN: a row sees the last p.window keys and the first p.sinks.  The walk skips the tiles between (KeyWalk); tiles that the
+// window's edge or the sinks' end passes through select their scores as those on the diagonal do.
+template <class P, int SPLIT, bool WIN>
 __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) attn_fwd_kernel(AttnParams p, int64_t slots) {
   typedef typename P::elem E;
   typedef Fwd<P, SPLIT> S;
@@ -70,11 +72,13 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   const float c = p.scale * LOG2E;
 
   const int sees = min(lenk, t.row0 + S::ROWS + off);  // keys that any row of the workgroup sees
-  const int ntiles = sees > 0 ? (sees + KEYS - 1) / KEYS : 0;
+  const KeyWalk walk(t.row0 + off, sees, WIN ? p.window : (int)NO_WINDOW, WIN ? p.sinks : 0, KEYS);
+  const int ntiles = WIN ? walk.tiles : sees > 0 ? (sees + KEYS - 1) / KEYS : 0;
+  auto tile = [&](int j) { return WIN ? walk.at(j) : j; };
   const int wfirst = first_row + off, wlast = wfirst + 31;  // last key the wave's first / last row sees
   const Stager<P, KEYS, 4> stage_k(p.ks[0], w, lane), stage_v(p.vs[0], w, lane);
   auto stage = [&](int j, unsigned char* to) {
-    const int k0 = j * KEYS, last = min(lenk - 1 - k0, KEYS - 1);
+    const int k0 = tile(j) * KEYS, last = min(lenk - 1 - k0, KEYS - 1);
     stage_k(kb + k0 * p.ks[0], last, to);
     stage_v(vb + k0 * p.vs[0], last, to + TILE);
   };
@@ -82,8 +86,9 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   // (__restrict): it would wait for the copies before it reads V otherwise.
   auto step = [&](int j, const unsigned char* __restrict kt, unsigned char* __restrict next) {
     if (S::BUFS == 2 && j + 1 < ntiles) stage(j + 1, next);
-    const int r0 = 32 * S::BLOCKS * part, k0 = j * KEYS + r0;  // the wave's keys of the tile
+    const int r0 = 32 * S::BLOCKS * part, k0 = tile(j) * KEYS + r0;  // the wave's keys of the tile
     if (k0 > wlast) return;  // nothing of this tile is visible to the wave
+    if (WIN && window_hides(wfirst, k0, k0 + 32 * S::BLOCKS - 1, p.window, p.sinks)) return;
     const unsigned char* vt = kt + TILE;
     f32x16 s[S::BLOCKS];
 #pragma unroll
@@ -93,12 +98,16 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
 #pragma unroll
       for (int b = 0; b < S::BLOCKS; ++b) s[b] = P::mma(s[b], P::row_frag(kt, r0 + 32 * b + (lane & 31), ks, half), q[ks]);
     sched_products<P, KS * S::BLOCKS, P::ROW_READS>();
-    if (k0 + 32 * S::BLOCKS - 1 > wfirst) {
+    const bool cut = WIN && window_cuts(wlast, k0, k0 + 32 * S::BLOCKS - 1, p.window, p.sinks);
+    if (cut || k0 + 32 * S::BLOCKS - 1 > wfirst) {
       const int limit = row + off - k0;
 #pragma unroll
       for (int b = 0; b < S::BLOCKS; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][i] = 32 * b + rho(half, i) <= limit ? s[b][i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) {
+          const int x = 32 * b + rho(half, i);
+          s[b][i] = x <= limit && (!WIN || x > limit - p.window || x < p.sinks - k0) ? s[b][i] : -INFINITY;
+        }
     }
     float top = s[0][0];
 #pragma unroll
@@ -176,13 +185,14 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
         staged_barrier();
 #pragma unroll 1
         for (int b = 0; b < S::BLOCKS; ++b) {
-          const int r0 = 32 * (S::BLOCKS * part + b), limit = row + off - (j * KEYS + r0);  // keys of the block that the row sees
+          const int r0 = 32 * (S::BLOCKS * part + b), k0 = tile(j) * KEYS + r0, limit = row + off - k0;  // keys of the block that the row sees
           f32x16 x = zero16();
 #pragma unroll 1
           for (int ks = 0; ks < KS; ++ks) x = P::mma(x, P::row_frag(lds, r0 + (lane & 31), ks, half), P::load(src + 16 * ks + 8 * half));
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const bool sees = rho(half, i) <= limit;
+            const int key = rho(half, i);
+            const bool sees = key <= limit && (!WIN || key > limit - p.window || key < p.sinks - k0);
             x[i] = !sees ? 0.f : kind == 0 ? __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -mc)) : 1.f;
           }
 #pragma unroll
@@ -296,7 +306,15 @@ AttnParams attn_params(const kdn_attn_args* a) {
   p.nseq = a->num_seqs; p.total_q = a->total_q; p.total_k = a->total_k;
   p.H = (int)a->H; p.KV = (int)a->H_kv; p.G = (int)(a->H / a->H_kv);
   p.scale = a->scale;
+  p.window = (int)NO_WINDOW;
   return p;
+}
+
+// A window that reaches over all the keys, or that sinks fill up, is none.
+void attn_window(AttnParams& p, int64_t window, int64_t sinks) {
+  const bool none = window >= p.total_k || sinks >= p.total_k - window;
+  p.window = (int)(none ? NO_WINDOW : window);
+  p.sinks = (int)(none ? 0 : sinks);
 }
 
 }  // namespace kdn
@@ -304,31 +322,45 @@ AttnParams attn_params(const kdn_attn_args* a) {
 using namespace kdn;
 
 extern "C" int kdn_anchor_version(void) { return 1 << 16; }
+extern "C" int kdn_bounded_version(void) { return 1 << 16; }
 
-template <class P, int SPLIT>
+template <class P, int SPLIT, bool WIN>
 static int launch_fwd(const AttnParams& p, hipStream_t st) {
   const int64_t slots = tile_slots(p.total_q, Fwd<P, SPLIT>::ROWS, p.nseq), grid = slots * p.H;
   if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((attn_fwd_kernel<P, SPLIT>), dim3((unsigned)grid), dim3(256), 0, st, p, slots);
+  hipLaunchKernelGGL((attn_fwd_kernel<P, SPLIT, WIN>), dim3((unsigned)grid), dim3(256), 0, st, p, slots);
   return launch_status();
+}
+
+template <class P, bool WIN>
+static int launch_fwd(const AttnParams& p, hipStream_t st) {
+  switch (attn_split(p.total_q, p.H)) {
+    case 4: return launch_fwd<P, 4, WIN>(p, st);
+    case 2: return launch_fwd<P, 2, WIN>(p, st);
+    default: return launch_fwd<P, 1, WIN>(p, st);
+  }
 }
 
 template <class P>
 static int launch_fwd(const AttnParams& p, hipStream_t st) {
-  switch (attn_split(p.total_q, p.H)) {
-    case 4: return launch_fwd<P, 4>(p, st);
-    case 2: return launch_fwd<P, 2>(p, st);
-    default: return launch_fwd<P, 1>(p, st);
-  }
+  return p.window < NO_WINDOW ? launch_fwd<P, true>(p, st) : launch_fwd<P, false>(p, st);
 }
 
-extern "C" int kdn_attn_fwd(const kdn_attn_args* a, void* stream) {
+static int attn_fwd(const kdn_attn_args* a, int64_t window, int64_t sinks, void* stream) {
   int rc = attn_check(a);
   if (rc != KDN_OK) return rc;
   if (a->total_q == 0) return KDN_OK;
   if ((rc = attn_check_tensors(a)) != KDN_OK) return rc;
-  const AttnParams p = attn_params(a);
+  AttnParams p = attn_params(a);
+  attn_window(p, window, sinks);
   hipStream_t st = as_stream(stream);
   if (a->dtype == KDN_DTYPE_BF16) return a->d == 64 ? launch_fwd<AttnBF16<64>>(p, st) : launch_fwd<AttnBF16<128>>(p, st);
   return a->d == 64 ? launch_fwd<AttnF32<64>>(p, st) : launch_fwd<AttnF32<128>>(p, st);
+}
+
+extern "C" int kdn_attn_fwd(const kdn_attn_args* a, void* stream) { return attn_fwd(a, NO_WINDOW, 0, stream); }
+
+extern "C" int kdn_attn_window_fwd(const kdn_attn_args* a, int64_t window, int64_t sinks, void* stream) {
+  if (window < 1 || sinks < 0) return KDN_ERR_INVALID_ARGUMENT;
+  return attn_fwd(a, window, sinks, stream);
 }

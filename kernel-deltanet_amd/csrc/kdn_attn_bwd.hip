@@ -63,6 +63,22 @@ __device__ __forceinline__ const AttnParams& params_here() {
   return *(const AttnParams*)a;
 }
 
+// Under a window (WIN) the rows that see a tile of keys end `window` behind it, but for the first `sinks` keys, which all later
+// rows see: one workgroup that walked them all would run on when the others are done (a sequence of 65536 rows and a window of
+// 1024: fifty times as long).  So those rows are cut into segments of FAR_ROWS, a workgroup each, whose sums of the sinks' dk and
+// dv come to lie apart in fp32; attn_sinks_kernel adds them to the subsets' sums in a fixed order.
+constexpr int FAR_ROWS = 1024;
+// The query rows [from, to) of a sequence that see keys of the tile row0 .. row0 + keys - 1 for nearness, in whole tiles of `rows`.
+// Those from `to` on see of it the sinks alone.
+struct NearRows {
+  int from, to;
+  __device__ __forceinline__ NearRows(int row0, int off, int lenq, int window, int keys, int rows) {
+    from = max(row0 - off, 0) / rows * rows;
+    const int end = min(lenq, max(row0 + keys - 1 - off + window, 0));
+    to = from < end ? from + (end - from + rows - 1) / rows * rows : from;
+  }
+};
+
 // dk and dv of 128 / SPLIT keys: a wave owns 32 keys (a lane one), their K and V fragments and the transposed sums in
 // registers.  The query rows pass in tiles with their lse and delta; S = Q K^T and dP = dY V^T have the queries in
 // registers, so that P and dS are the B operands of dV^T += dY^T P and dK^T += Q^T dS.
@@ -76,8 +92,8 @@ struct Dkdv {
   static constexpr int LDS = BUFS * SLOT > JOIN ? BUFS * SLOT : JOIN;
 };
 
-template <class P, int SPLIT, bool DV, bool DK>
-__device__ __forceinline__ void dkdv(int id, int slots, unsigned char* lds) {
+template <class P, int SPLIT, bool DV, bool DK, bool WIN>
+__device__ __forceinline__ void dkdv(int id, int slots, int far, unsigned char* lds) {
   const AttnParams& p = params_here();
   typedef typename P::elem E;
   typedef Dkdv<P, SPLIT> S;
@@ -85,12 +101,24 @@ __device__ __forceinline__ void dkdv(int id, int slots, unsigned char* lds) {
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = w % SPLIT;
   const int e = id % p.KV, sub = id / p.KV % p.subsets, heads = p.G / p.subsets;
-  const SeqTile t = find_heavy<S::KEYS, true>(p.cu_k, p.nseq, p.total_k, id / p.KV / p.subsets, slots, lane);
-  if (t.row0 < 0) return;
-  const int lenk = t.len;
+  SeqTile t;  // the keys' tile
   int64_t qlo;
-  int lenq;
-  other_rows(p.cu_q, p.nseq, p.total_q, t.seq, qlo, lenq);
+  int lenq, far_slot = -1, segment = 0;
+  if (WIN && id < far) {
+    const int tiles = (p.sinks + S::KEYS - 1) / S::KEYS, u = id / p.KV / p.subsets;
+    far_slot = u / tiles;
+    const SeqTile rows = find_tile<FAR_ROWS>(p.cu_q, p.nseq, p.total_q, far_slot, lane);
+    if (rows.row0 < 0) return;
+    qlo = rows.lo, lenq = rows.len, segment = rows.row0;
+    t.row0 = u % tiles * S::KEYS;
+    other_rows(p.cu_k, p.nseq, p.total_k, rows.seq, t.lo, t.len);
+    if (t.row0 >= t.len) return;
+  } else {
+    t = find_heavy<S::KEYS, true>(p.cu_k, p.nseq, p.total_k, (WIN ? id - far : id) / p.KV / p.subsets, slots, lane);
+    if (t.row0 < 0) return;
+    other_rows(p.cu_q, p.nseq, p.total_q, t.seq, qlo, lenq);
+  }
+  const int lenk = t.len;
   const int off = lenk - lenq;
   const int first_key = t.row0 + 32 * (w / SPLIT), key = first_key + (lane & 31);
   const bool live = key < lenk;
@@ -114,11 +142,27 @@ __device__ __forceinline__ void dkdv(int id, int slots, unsigned char* lds) {
   const float c = p.scale * LOG2E;
 
   // the query tiles that see key row0: rows from row0 - off on, of each head of the subset
-  const int q0 = max(t.row0 - off, 0) / ROWS * ROWS;
-  const int per = q0 < lenq ? (lenq - q0 + ROWS - 1) / ROWS : 0;
+  int q0 = max(t.row0 - off, 0) / ROWS * ROWS, q1 = lenq;
+  if constexpr (WIN) {
+    const NearRows near(t.row0, off, lenq, p.window, S::KEYS, ROWS);
+    q1 = min(near.to, lenq);
+    if (far_slot >= 0) {
+      q0 = max(near.to, segment);
+      q1 = min(lenq, segment + FAR_ROWS);
+      if (q0 >= q1) return;
+    }
+  }
+  const int per = q0 < q1 ? (q1 - q0 + ROWS - 1) / ROWS : 0;
   const int ntiles = per * heads;
+  // the end of the rows that see the lane's key; from which first row on a block of 32 is past some of the wave's keys, and past all
+  const int last_row = !WIN || key < p.sinks ? lenq : min(lenq, key - off + p.window);
+  const int cut_from = WIN && first_key + 31 >= p.sinks ? first_key - 31 - off + p.window : INT32_MAX;
+  const int hidden_from = WIN && first_key >= p.sinks ? first_key + 31 - off + p.window : INT32_MAX;
   const Stager<P, ROWS, 4> stage_q(p.qs[0], w, lane), stage_y(p.dys[0], w, lane);
+  const AttnParams& first = p;
   auto stage = [&](int j, unsigned char* to) {
+    // at 128 features two waves a row and a window: read where they are used, or scalar registers are spilled to memory
+    const AttnParams& p = WIN && P::D == 128 && SPLIT == 2 ? params_here() : first;
     const int h = e * p.G + sub * heads + j / per, r0 = q0 + j % per * ROWS, last = min(lenq - 1 - r0, ROWS - 1);
     stage_q(reinterpret_cast<const E*>(p.q) + (qlo + r0) * p.qs[0] + (int64_t)h * p.qs[1], last, to);
     stage_y(reinterpret_cast<const E*>(p.dy) + (qlo + r0) * p.dys[0] + (int64_t)h * p.dys[1], last, to + TILE);
@@ -135,6 +179,7 @@ __device__ __forceinline__ void dkdv(int id, int slots, unsigned char* lds) {
     for (int u = 0; u < S::BLOCKS; ++u) {
       const int tr = 32 * (S::BLOCKS * part + u), i0 = q0 + j % per * ROWS + tr;  // the wave's rows of the tile: i0 .. i0 + 31
       if (i0 >= lenq || i0 + 31 + off < first_key) continue;                      // none of them sees a key of this wave
+      if (WIN && i0 >= hidden_from) continue;
       // bf16: the sums start at minus lse / scale and minus delta of their rows.  fp32 adds these last: a sum that starts at
       // 100 rounds each of its products at that size.
       constexpr bool START = sizeof(E) == 2;
@@ -164,8 +209,9 @@ __device__ __forceinline__ void dkdv(int id, int slots, unsigned char* lds) {
         sched_products<P, 2 * KS, P::ROW_READS>();
       }
       if constexpr (!START) add_stat();
-      const bool whole = i0 + off >= first_key + 31 && i0 + 32 <= lenq;
-      const int lo = max(key - off, 0) - i0, hi = lenq - i0;  // rows lo .. hi - 1 of the block see the key
+      const bool whole = i0 + off >= first_key + 31 && i0 + 32 <= lenq &&
+                         !(WIN && i0 >= cut_from);
+      const int lo = max(key - off, 0) - i0, hi = (WIN ? last_row : lenq) - i0;  // rows lo .. hi - 1 of the block see the key
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int r = rho(half, i);
@@ -202,12 +248,15 @@ __device__ __forceinline__ void dkdv(int id, int slots, unsigned char* lds) {
   }
   const AttnParams& out = params_here();
   const int64_t at = t.lo + key, part_at = (((int64_t)sub * out.total_k + at) * out.KV + e) * P::D;
+  const int64_t far_at = ((((int64_t)far_slot * out.subsets + sub) * out.sinks + key) * out.KV + e) * P::D;
   auto store_k = [&](int ct, const f32x16& x, float f) {
-    if (out.subsets > 1) store_row32(out.part_dk + part_at + 32 * ct, x, f, half, live);
+    if (WIN && far_slot >= 0) store_row32(out.far_dk + far_at + 32 * ct, x, f, half, live && key < out.sinks);
+    else if (out.subsets > 1 || (WIN && out.sinks > 0)) store_row32(out.part_dk + part_at + 32 * ct, x, f, half, live);
     else store_row32(reinterpret_cast<E*>(out.dk) + at * out.dks[0] + (int64_t)e * out.dks[1] + 32 * ct, x, f, half, live);
   };
   auto store_v = [&](int ct, const f32x16& x) {
-    if (out.subsets > 1) store_row32(out.part_dv + part_at + 32 * ct, x, 1.f, half, live);
+    if (WIN && far_slot >= 0) store_row32(out.far_dv + far_at + 32 * ct, x, 1.f, half, live && key < out.sinks);
+    else if (out.subsets > 1 || (WIN && out.sinks > 0)) store_row32(out.part_dv + part_at + 32 * ct, x, 1.f, half, live);
     else store_row32(reinterpret_cast<E*>(out.dv) + at * out.dvs[0] + (int64_t)e * out.dvs[1] + 32 * ct, x, 1.f, half, live);
   };
   if constexpr (SPLIT == 1) {
@@ -240,6 +289,41 @@ __global__ void __launch_bounds__(256) attn_subsets_kernel(AttnParams p) {
   store4(reinterpret_cast<E*>(p.dv) + at * p.dvs[0] + e * p.dvs[1] + d, y);
 }
 
+// The sinks' dk and dv: the subsets' sums of the near rows, then the segments of the far ones in order.  A thread has four
+// values of one sink of one sequence and key head; `keys` and `rows` are Dkdv's.
+template <class P>
+__global__ void __launch_bounds__(256) attn_sinks_kernel(AttnParams p, int keys, int rows) {
+  typedef typename P::elem E;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, each = (int64_t)p.sinks * p.KV * (P::D / 4);
+  const int64_t b = i / each;
+  if (b >= p.nseq) return;
+  const int64_t in = i % each, d = 4 * (in % (P::D / 4)), e = in / (P::D / 4) % p.KV;
+  const int key = (int)(in / (P::D / 4) / p.KV);
+  int64_t klo, qlo;
+  int lenk, lenq;
+  other_rows(p.cu_k, p.nseq, p.total_k, (int)b, klo, lenk);
+  other_rows(p.cu_q, p.nseq, p.total_q, (int)b, qlo, lenq);
+  if (key >= lenk) return;
+  f32x4 dk = zero4(), dv = zero4();
+  for (int s = 0; s < p.subsets; ++s) {
+    const int64_t at = (((int64_t)s * p.total_k + klo + key) * p.KV + e) * P::D + d;
+    dk += *reinterpret_cast<const f32x4*>(p.part_dk + at);
+    dv += *reinterpret_cast<const f32x4*>(p.part_dv + at);
+  }
+  const NearRows near(key / keys * keys, lenk - lenq, lenq, p.window, keys, rows);
+  for (int row = near.to; row < lenq; row = row / FAR_ROWS * FAR_ROWS + FAR_ROWS) {
+    const int64_t slot = qlo / FAR_ROWS + b + 1 + row / FAR_ROWS;
+    for (int s = 0; s < p.subsets; ++s) {
+      const int64_t at = (((slot * p.subsets + s) * p.sinks + key) * p.KV + e) * P::D + d;
+      dk += *reinterpret_cast<const f32x4*>(p.far_dk + at);
+      dv += *reinterpret_cast<const f32x4*>(p.far_dv + at);
+    }
+  }
+  const float x[4] = {dk[0], dk[1], dk[2], dk[3]}, y[4] = {dv[0], dv[1], dv[2], dv[3]};
+  store4(reinterpret_cast<E*>(p.dk) + (klo + key) * p.dks[0] + e * p.dks[1] + d, x);
+  store4(reinterpret_cast<E*>(p.dv) + (klo + key) * p.dvs[0] + e * p.dvs[1] + d, y);
+}
+
 // dq of 128 / SPLIT query rows of a head: the forward's walk over the keys with S^T = K Q^T and dP^T = V dY^T, and
 // dQ^T += K^T dS^T.
 template <class P, int SPLIT>
@@ -250,7 +334,7 @@ struct Dq {
   static constexpr int LDS = 2 * BUFS * TILE > JOIN ? 2 * BUFS * TILE : JOIN;
 };
 
-template <class P, int SPLIT>
+template <class P, int SPLIT, bool WIN>
 __device__ __forceinline__ void dq(int id, int slots, unsigned char* lds) {
   const AttnParams& p = params_here();
   typedef typename P::elem E;
@@ -294,11 +378,13 @@ __device__ __forceinline__ void dq(int id, int slots, unsigned char* lds) {
   for (int ct = 0; ct < CT; ++ct) sum[ct] = zero16();
 
   const int sees = min(lenk, t.row0 + S::ROWS + off);
-  const int ntiles = sees > 0 ? (sees + KEYS - 1) / KEYS : 0;
+  const KeyWalk walk(t.row0 + off, sees, WIN ? p.window : (int)NO_WINDOW, WIN ? p.sinks : 0, KEYS);
+  const int ntiles = WIN ? walk.tiles : sees > 0 ? (sees + KEYS - 1) / KEYS : 0;
+  auto tile = [&](int j) { return WIN ? walk.at(j) : j; };
   const int wfirst = first_row + off, wlast = wfirst + 31;
   const Stager<P, KEYS, 4> stage_k(p.ks[0], w, lane), stage_v(p.vs[0], w, lane);
   auto stage = [&](int j, unsigned char* to) {
-    const int k0 = j * KEYS, last = min(lenk - 1 - k0, KEYS - 1);
+    const int k0 = tile(j) * KEYS, last = min(lenk - 1 - k0, KEYS - 1);
     stage_k(kb + k0 * p.ks[0], last, to);
     stage_v(vb + k0 * p.vs[0], last, to + TILE);
   };
@@ -307,20 +393,21 @@ __device__ __forceinline__ void dq(int id, int slots, unsigned char* lds) {
     const unsigned char* vt = kt + TILE;
 #pragma unroll
     for (int u = 0; u < S::BLOCKS; ++u) {
-      const int r0 = 32 * (S::BLOCKS * part + u), j0 = j * KEYS + r0;  // the wave's keys of the tile
+      const int r0 = 32 * (S::BLOCKS * part + u), j0 = tile(j) * KEYS + r0;  // the wave's keys of the tile
       if (j0 > wlast || j0 >= lenk) continue;
+      if (WIN && window_hides(wfirst, j0, j0 + 31, p.window, p.sinks)) continue;
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) s = P::mma(s, P::row_frag(kt, r0 + (lane & 31), ks, half), q[ks]);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) dp = P::mma(dp, P::row_frag(vt, r0 + (lane & 31), ks, half), dy[ks]);
       sched_products<P, 2 * KS, P::ROW_READS>();
-      const bool whole = j0 + 31 <= wfirst;
+      const bool whole = j0 + 31 <= wfirst && !(WIN && window_cuts(wlast, j0, j0 + 31, p.window, p.sinks));
       const int limit = row + off - j0;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float d = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, ls)) * (dp[i] + de);
-        if (!whole) d = rho(half, i) <= limit ? d : 0.f;
+        if (!whole) d = rho(half, i) <= limit && (!WIN || rho(half, i) > limit - p.window || rho(half, i) < p.sinks - j0) ? d : 0.f;
         dp[i] = d;
       }
 #pragma unroll
@@ -354,39 +441,56 @@ __device__ __forceinline__ void dq(int id, int slots, unsigned char* lds) {
 // All of a backward's sums in one launch: dk's and dv's workgroups first (of 128 features dv's, then dk's), then dq's.  None
 // waits for another, and the last of one kind leave no CU idle.  Three sequences of 101 to 1024 rows, 4 heads, fp32: 53 us,
 // as two launches 51 and 38; 8192 rows, 32 heads, bf16: within 1 % of what the three launches took.
-template <class P, int SPLIT>
+template <class P, int SPLIT, bool WIN>
 __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1)
-    attn_grads_kernel(AttnParams p, int slots_k, int slots_q, int part, int nk) {
+    attn_grads_kernel(AttnParams p, int slots_k, int slots_q, int part, int nk, int far) {
   constexpr int LDS = Dkdv<P, SPLIT>::LDS > Dq<P, SPLIT>::LDS ? Dkdv<P, SPLIT>::LDS : Dq<P, SPLIT>::LDS;
   __shared__ __attribute__((aligned(256))) unsigned char lds[LDS];
   constexpr int PARTS = P::D == 64 ? 1 : 2;
   const int id = blockIdx.x;
-  if (id >= PARTS * part) return dq<P, SPLIT>(id - PARTS * part, slots_q, lds);
+  if (id >= PARTS * part) return dq<P, SPLIT, WIN>(id - PARTS * part, slots_q, lds);
   if constexpr (PARTS == 1) {
-    if (id < nk) dkdv<P, SPLIT, true, true>(id, slots_k, lds);
+    if (id < nk) dkdv<P, SPLIT, true, true, WIN>(id, slots_k, far, lds);
   } else if (id < part) {
-    if (id < nk) dkdv<P, SPLIT, true, false>(id, slots_k, lds);
+    if (id < nk) dkdv<P, SPLIT, true, false, WIN>(id, slots_k, far, lds);
   } else if (id - part < nk) {
-    dkdv<P, SPLIT, false, true>(id - part, slots_k, lds);
+    dkdv<P, SPLIT, false, true, WIN>(id - part, slots_k, far, lds);
   }
 }
 
-template <class P, int SPLIT>
+template <class P, int SPLIT, bool WIN>
 static int launch_grads(const AttnParams& p, hipStream_t st) {
   const int64_t slots_k = p.total_k > 0 ? tile_slots(p.total_k, Dkdv<P, SPLIT>::KEYS, p.nseq) : 0;
   const int64_t slots_q = p.total_q > 0 ? tile_slots(p.total_q, Dq<P, SPLIT>::ROWS, p.nseq) : 0;
-  const int64_t nk = slots_k * p.KV * p.subsets, part = (nk + 7) / 8 * 8;  // a workgroup's number mod 8 is its XCD
+  const int64_t far = WIN && p.sinks > 0 && p.total_q > 0 && p.total_k > 0
+                          ? tile_slots(p.total_q, FAR_ROWS, p.nseq) * ((p.sinks + Dkdv<P, SPLIT>::KEYS - 1) / Dkdv<P, SPLIT>::KEYS) * p.KV * p.subsets
+                          : 0;
+  const int64_t nk = slots_k * p.KV * p.subsets + far, part = (nk + 7) / 8 * 8;  // a workgroup's number mod 8 is its XCD
   const int64_t grid = part * (P::D == 64 ? 1 : 2) + slots_q * p.H;
   if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((attn_grads_kernel<P, SPLIT>), dim3((unsigned)grid), dim3(256), 0, st, p, (int)slots_k, (int)slots_q, (int)part, (int)nk);
+  hipLaunchKernelGGL((attn_grads_kernel<P, SPLIT, WIN>), dim3((unsigned)grid), dim3(256), 0, st, p, (int)slots_k, (int)slots_q, (int)part, (int)nk,
+                     (int)far);
   int rc = launch_status();
-  if (rc == KDN_OK && p.subsets > 1 && p.total_k > 0) {
+  const bool sinks = WIN && p.sinks > 0;
+  if (rc == KDN_OK && (p.subsets > 1 || sinks) && p.total_k > 0) {
     const int64_t blocks = (p.total_k * p.KV * (P::D / 4) + 255) / 256;
     if (blocks > INT32_MAX) return KDN_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(attn_subsets_kernel<P>, dim3((unsigned)blocks), dim3(256), 0, st, p);
+    if ((rc = launch_status()) != KDN_OK || !sinks || p.nseq == 0) return rc;
+    const int64_t far_blocks = (p.nseq * p.sinks * p.KV * (P::D / 4) + 255) / 256;
+    if (far_blocks > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(attn_sinks_kernel<P>, dim3((unsigned)far_blocks), dim3(256), 0, st, p, Dkdv<P, SPLIT>::KEYS, Dkdv<P, SPLIT>::ROWS);
     rc = launch_status();
   }
   return rc;
+}
+
+template <class P, bool WIN>
+static int launch_grads(const AttnParams& p, hipStream_t st) {
+  // one split for both walks, that of the one with fewer tiles (with as many keys as queries they agree: bwd_subsets; few rows
+  // over many keys split the keys' walk as well, which has not been measured)
+  const int split = std::max(attn_split(p.total_k, (int64_t)p.KV * p.subsets), attn_split(p.total_q, p.H));
+  return split == 4 ? launch_grads<P, 4, WIN>(p, st) : split == 2 ? launch_grads<P, 2, WIN>(p, st) : launch_grads<P, 1, WIN>(p, st);
 }
 
 template <class P>
@@ -398,10 +502,7 @@ static int launch_bwd(const AttnParams& p, float* stat, float* delta, hipStream_
     hipLaunchKernelGGL(attn_delta_kernel<P>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, p, stat, delta);
     if ((rc = launch_status()) != KDN_OK) return rc;
   }
-  // one split for both walks, that of the one with fewer tiles (with as many keys as queries they agree: bwd_subsets; few rows
-  // over many keys split the keys' walk as well, which has not been measured)
-  const int split = std::max(attn_split(p.total_k, (int64_t)p.KV * p.subsets), attn_split(p.total_q, p.H));
-  return split == 4 ? launch_grads<P, 4>(p, st) : split == 2 ? launch_grads<P, 2>(p, st) : launch_grads<P, 1>(p, st);
+  return p.window < NO_WINDOW ? launch_grads<P, true>(p, st) : launch_grads<P, false>(p, st);
 }
 
 // Subsets of the query heads that share a key head whose dk and dv are summed apart: as many as it takes to have eight
@@ -416,18 +517,27 @@ static int bwd_subsets(const kdn_attn_args* f) {
 }
 static size_t bwd_row_bytes(const kdn_attn_args* f) { return ((size_t)f->H * (size_t)f->total_q * 4 + 255) / 256 * 256 + 256; }
 static size_t bwd_part_bytes(const kdn_attn_args* f) { return (size_t)f->total_k * (size_t)f->H_kv * (size_t)f->d * 4; }
+// Of the far rows' segments, `sinks` after attn_window.
+static size_t bwd_far_bytes(const kdn_attn_args* f, int subsets, int64_t sinks) {
+  const size_t each = (size_t)subsets * (size_t)sinks * (size_t)f->H_kv * (size_t)f->d * 4;
+  size_t all;
+  return __builtin_mul_overflow((size_t)tile_slots(f->total_q, FAR_ROWS, f->num_seqs), each, &all) || all > ((size_t)1 << 48) ? (size_t)1 << 48 : all;
+}
 
 }  // namespace kdn
 
 using namespace kdn;
 
-extern "C" size_t kdn_attn_bwd_workspace_bytes(const kdn_attn_bwd_args* a) {
-  if (!a || attn_check(a->fwd) != KDN_OK) return 0;
+static size_t bwd_workspace_bytes(const kdn_attn_bwd_args* a, int64_t window, int64_t sinks) {
+  if (!a || attn_check(a->fwd) != KDN_OK || window < 1 || sinks < 0) return 0;
+  AttnParams p = attn_params(a->fwd);
+  attn_window(p, window, sinks);
   const int subsets = bwd_subsets(a->fwd);
-  return 2 * bwd_row_bytes(a->fwd) + (subsets > 1 ? 2 * subsets * bwd_part_bytes(a->fwd) : 0);
+  return 2 * bwd_row_bytes(a->fwd) + (subsets > 1 || p.sinks > 0 ? 2 * subsets * bwd_part_bytes(a->fwd) : 0) +
+         2 * bwd_far_bytes(a->fwd, subsets, p.sinks);
 }
 
-extern "C" int kdn_attn_bwd(const kdn_attn_bwd_args* a, void* stream) {
+static int attn_bwd(const kdn_attn_bwd_args* a, int64_t window, int64_t sinks, void* stream) {
   if (!a) return KDN_ERR_INVALID_ARGUMENT;
   const kdn_attn_args* f = a->fwd;
   int rc = attn_check(f);
@@ -444,7 +554,7 @@ extern "C" int kdn_attn_bwd(const kdn_attn_bwd_args* a, void* stream) {
       !attn_strides_ok(f->k_stride, f->dtype) || !attn_strides_ok(f->v_stride, f->dtype) || !aligned(f->k, 16) || !aligned(f->v, 16))
     return KDN_ERR_MISALIGNED;
   if (!stage_reach(a->dy_stride[0], f->dtype)) return KDN_ERR_UNSUPPORTED;
-  if (!a->workspace || a->workspace_bytes < kdn_attn_bwd_workspace_bytes(a)) return KDN_ERR_WORKSPACE_TOO_SMALL;
+  if (!a->workspace || a->workspace_bytes < bwd_workspace_bytes(a, window, sinks)) return KDN_ERR_WORKSPACE_TOO_SMALL;
   AttnParams p = attn_params(f);
   p.dy = a->dy; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
   float *stat = reinterpret_cast<float*>(a->workspace), *delta = stat + bwd_row_bytes(f) / 4;
@@ -453,6 +563,9 @@ extern "C" int kdn_attn_bwd(const kdn_attn_bwd_args* a, void* stream) {
   p.subsets = bwd_subsets(f);
   p.part_dk = reinterpret_cast<float*>((unsigned char*)a->workspace + 2 * bwd_row_bytes(f));
   p.part_dv = p.part_dk + (size_t)p.subsets * bwd_part_bytes(f) / 4;
+  attn_window(p, window, sinks);
+  p.far_dk = p.part_dv + (size_t)p.subsets * bwd_part_bytes(f) / 4;
+  p.far_dv = p.far_dk + bwd_far_bytes(f, p.subsets, p.sinks) / 4;
   for (int i = 0; i < 2; ++i) {
     p.dys[i] = a->dy_stride[i]; p.dqs[i] = a->dq_stride[i]; p.dks[i] = a->dk_stride[i]; p.dvs[i] = a->dv_stride[i];
   }
@@ -460,4 +573,15 @@ extern "C" int kdn_attn_bwd(const kdn_attn_bwd_args* a, void* stream) {
   if (f->dtype == KDN_DTYPE_BF16)
     return f->d == 64 ? launch_bwd<AttnBF16<64>>(p, stat, delta, st) : launch_bwd<AttnBF16<128>>(p, stat, delta, st);
   return f->d == 64 ? launch_bwd<AttnF32<64>>(p, stat, delta, st) : launch_bwd<AttnF32<128>>(p, stat, delta, st);
+}
+
+extern "C" size_t kdn_attn_bwd_workspace_bytes(const kdn_attn_bwd_args* a) { return bwd_workspace_bytes(a, NO_WINDOW, 0); }
+extern "C" int kdn_attn_bwd(const kdn_attn_bwd_args* a, void* stream) { return attn_bwd(a, NO_WINDOW, 0, stream); }
+
+extern "C" size_t kdn_attn_window_bwd_workspace_bytes(const kdn_attn_bwd_args* a, int64_t window, int64_t sinks) {
+  return bwd_workspace_bytes(a, window, sinks);
+}
+extern "C" int kdn_attn_window_bwd(const kdn_attn_bwd_args* a, int64_t window, int64_t sinks, void* stream) {
+  if (window < 1 || sinks < 0) return KDN_ERR_INVALID_ARGUMENT;
+  return attn_bwd(a, window, sinks, stream);
 }

@@ -12,7 +12,7 @@
 #pragma once
 #include "kdn_frag.hpp"
 #include "kdn_internal.hpp"
-#include "../../include/kdn_anchor.h"
+#include "../../include/kdn_bounded.h"
 
 namespace kdn {
 
@@ -420,6 +420,23 @@ __device__ __forceinline__ void other_rows(const int64_t* cu, int64_t nseq, int6
   len = there ? (int)(max(seq_start(cu, total, seq + 1), lo) - lo) : 0;
 }
 
+// The key tiles that a block of rows walks over, under a window: those of the first `sinks` keys, then from the first one that
+// the window of the block's first row (at position `first`) reaches into, up to key `sees`.  KEYS keys a tile.
+struct KeyWalk {
+  int tiles, sink_tiles, skip;
+  __device__ __forceinline__ KeyWalk(int first, int sees, int window, int sinks, int keys) {
+    const int all = sees > 0 ? (sees + keys - 1) / keys : 0, near = min(max(first - window + 1, 0) / keys, all);
+    sink_tiles = min((min(sinks, max(sees, 0)) + keys - 1) / keys, near);
+    tiles = sink_tiles + all - near;
+    skip = near - sink_tiles;
+  }
+  __device__ __forceinline__ int at(int t) const { return t < sink_tiles ? t : t + skip; }
+};
+// Whether some row at the positions first .. last does not see some of the keys k0 .. k1 for the window's sake (they may also be
+// too late for it), and whether none of those rows sees any.
+__device__ __forceinline__ bool window_cuts(int last, int k0, int k1, int window, int sinks) { return k0 <= last - window && k1 >= sinks; }
+__device__ __forceinline__ bool window_hides(int first, int k0, int k1, int window, int sinks) { return k1 <= first - window && k0 >= sinks; }
+
 // Device-side arguments of the attention kernels (kdn_attn_args with the defaults filled in).
 struct AttnParams {
   const void *q, *k, *v, *y, *dy;
@@ -434,12 +451,17 @@ struct AttnParams {
   float *part_dk, *part_dv;  // [subset][total_k][KV][D] sums of dk and dv over a subset of a key head's query heads (subsets > 1)
   int H, KV, G, subsets;
   float scale;
+  // under a window: the keys that a row sees besides the first `sinks` end at its own position and are `window` at most
+  int window, sinks;
+  float *far_dk, *far_dv;  // [slot][subset][sink][KV][D]: what the rows of a segment behind the window give to the sinks' dk and dv
 };
 
 int attn_check(const kdn_attn_args* a);          // sizes
 int attn_check_tensors(const kdn_attn_args* a);  // pointers, strides, alignment
 bool attn_strides_ok(const int64_t s[2], int dtype);
 AttnParams attn_params(const kdn_attn_args* a);
+void attn_window(AttnParams& p, int64_t window, int64_t sinks);
 int attn_split(int64_t rows, int64_t heads);     // waves that share 32 rows
+constexpr int64_t NO_WINDOW = 1 << 30;           // more keys than a tensor has
 
 }  // namespace kdn

@@ -277,7 +277,7 @@ class TreeAttnArgs(ctypes.Structure):
 
 
 def _declare_anchor(L: ctypes.CDLL) -> None:
-    """Argument and result types of include/kdn_anchor.h."""
+    """Argument and result types of include/kdn_anchor.h and include/kdn_bounded.h."""
     vp, i64, ci, sz, ptr = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.POINTER
     for name, args, res in (
             # the argument structs go over as their packed bytes (kdn/anchor.py) or as a mirror's address
@@ -302,7 +302,12 @@ def _declare_anchor(L: ctypes.CDLL) -> None:
             ("kdn_page_pool_used", [vp], i64),
             ("kdn_page_pool_free", [vp], i64),
             ("kdn_tree_attn_workspace_bytes", [vp], sz),
-            ("kdn_tree_attn", [vp, vp], ci)):
+            ("kdn_tree_attn", [vp, vp], ci),
+            # include/kdn_bounded.h
+            ("kdn_bounded_version", [], ci),
+            ("kdn_attn_window_fwd", [vp, i64, i64, vp], ci),
+            ("kdn_attn_window_bwd_workspace_bytes", [vp, i64, i64], sz),
+            ("kdn_attn_window_bwd", [vp, i64, i64, vp], ci)):
         fn = getattr(L, name)
         fn.argtypes, fn.restype = args, res
 

@@ -2,7 +2,7 @@
 its recurrent ones, and the pages their keys and values live in.
 
     rotary            positions of q and k, with gradients
-    attention         causal attention over packed prompts with grouped heads, with gradients
+    attention         causal attention over packed prompts with grouped heads, whole or in a window, with gradients
     PagePool          which pages a stream's tokens lie on: fork, extend, truncate, compact, free (host)
     page_copy         whole pages (forks about to write, compaction)
     page_append       new tokens' keys and values into their pages
@@ -18,6 +18,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import operator
 import struct
 from typing import List, Optional, Sequence, Tuple
 
@@ -128,6 +129,14 @@ def _scale(scale: Optional[float], d: int, what: str) -> float:
     if not (s > 0.0 and math.isfinite(s)):
         raise ValueError(f"{what}: scale must be positive, got {scale}")
     return s
+
+
+def _window(window: Optional[int], sinks: int, what: str) -> Tuple[int, int]:
+    """(window, sinks) as the library takes them; (0, 0) without a window."""
+    n, s = 0 if window is None else operator.index(window), operator.index(sinks)
+    if s < 0 or (window is not None and n < 1):
+        raise ValueError(f"{what}: a window is 1 or more and sinks are 0 or more; got {window}, {sinks}")
+    return (min(n, 2**62), min(s, 2**62)) if n else (0, 0)
 
 
 # ------------------------------------------------------------------------------------------------- rotary positions
@@ -244,10 +253,11 @@ def _pack_attn(qs, ks, vs, cu_q, cu_k, scale, y, lse, low) -> bytes:
 
 
 def attention_forward(q, k, v, cu_seqlens, cu_seqlens_k=None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
-                      return_lse: bool = False, return_low: bool = False):
+                      return_lse: bool = False, return_low: bool = False, window: Optional[int] = None, sinks: int = 0):
     """`attention` without autograd: y; or with return_lse (y, lse (H, tokens) float32); or with return_low too (y, lse, low),
     low what rounding took from y (None in float32), which makes the gradients' dy . y exact."""
     qs, ks, vs, cu_q, cu_k = _attn_inputs(q, k, v, cu_seqlens, cu_seqlens_k)
+    near, first = _window(window, sinks, "attention")
     n, H, d = q.shape
     y = _new(q, (n, H, d)) if out is None else _out(out, "attention out", q.shape, q)
     lse = q.new_empty((H, n), dtype=_F32) if return_lse or return_low else None
@@ -255,21 +265,26 @@ def attention_forward(q, k, v, cu_seqlens, cu_seqlens_k=None, scale: Optional[fl
     args = _pack_attn(qs, ks, vs, cu_q, cu_k, _scale(scale, d, "attention"), y, lse, low)
     dev = q.get_device()
     with _device(dev):
-        N.check(N.lib().kdn_attn_fwd(args, _raw_stream(dev)), "kdn_attn_fwd")
+        if near:
+            N.check(N.lib().kdn_attn_window_fwd(args, near, first, _raw_stream(dev)), "kdn_attn_window_fwd")
+        else:
+            N.check(N.lib().kdn_attn_fwd(args, _raw_stream(dev)), "kdn_attn_fwd")
     return (y[0], lse, None if low is None else low[0]) if return_low else (y[0], lse) if return_lse else y[0]
 
 
 @functools.lru_cache(maxsize=64)
-def _bwd_bytes(nseq: int, nq: int, nk: int, H: int, KV: int, d: int, dtype: int) -> int:
-    """kdn_attn_bwd_workspace_bytes, which reads sizes only."""
+def _bwd_bytes(nseq: int, nq: int, nk: int, H: int, KV: int, d: int, dtype: int, window: int, sinks: int) -> int:
+    """kdn_attn_bwd_workspace_bytes (or a window's), which reads sizes only."""
     fwd = ctypes.c_char_p(_ATTN.pack(nseq, nq, nk, H, KV, d, dtype, 1.0, 1, 1, *(0,) * 16))
-    return N.lib().kdn_attn_bwd_workspace_bytes(_ATTN_BWD.pack(ctypes.cast(fwd, ctypes.c_void_p).value, *(0,) * 14))
+    args = _ATTN_BWD.pack(ctypes.cast(fwd, ctypes.c_void_p).value, *(0,) * 14)
+    return N.lib().kdn_attn_window_bwd_workspace_bytes(args, window, sinks) if window else N.lib().kdn_attn_bwd_workspace_bytes(args)
 
 
 def attention_backward(q, k, v, y, lse, dy, cu_seqlens, cu_seqlens_k=None, scale: Optional[float] = None,
-                       low: Optional[torch.Tensor] = None):
+                       low: Optional[torch.Tensor] = None, window: Optional[int] = None, sinks: int = 0):
     """(dq, dk, dv) of `attention_forward`'s y, lse and low (optional) for dL/dy, in the inputs' dtype, the same bits every
     time."""
+    near, first = _window(window, sinks, "attention backward")
     qs, ks, vs, cu_q, cu_k = _attn_inputs(q, k, v, cu_seqlens, cu_seqlens_k)
     ys, dys = _heads(y, "attention y", q), _heads(dy, "attention dy", q)
     if y.shape != q.shape or dy.shape != q.shape or tuple(lse.shape) != (q.shape[1], q.shape[0]) or lse.dtype is not _F32 or \
@@ -286,18 +301,23 @@ def attention_backward(q, k, v, y, lse, dy, cu_seqlens, cu_seqlens_k=None, scale
     at = ctypes.cast(fwd, ctypes.c_void_p).value
     dev = q.get_device()
     with _device(dev):
-        nbytes = _bwd_bytes(cu_q.shape[0] - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], _tag(q.dtype, "attention"))
+        nbytes = _bwd_bytes(cu_q.shape[0] - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2], _tag(q.dtype, "attention"),
+                            near, first)
         ws = q.new_empty(nbytes, dtype=torch.uint8)
-        N.check(N.lib().kdn_attn_bwd(_ATTN_BWD.pack(at, *dys[1:], *dq[1:], *dk[1:], *dv[1:], ws.data_ptr(), nbytes), _raw_stream(dev)),
-                "kdn_attn_bwd")
+        args = _ATTN_BWD.pack(at, *dys[1:], *dq[1:], *dk[1:], *dv[1:], ws.data_ptr(), nbytes)
+        if near:
+            N.check(N.lib().kdn_attn_window_bwd(args, near, first, _raw_stream(dev)), "kdn_attn_window_bwd")
+        else:
+            N.check(N.lib().kdn_attn_bwd(args, _raw_stream(dev)), "kdn_attn_bwd")
     return dq[0], dk[0], dv[0]
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, cu_q, cu_k, scale):
-        y, lse, low = attention_forward(q, k, v, cu_q, cu_k, scale, return_lse=True, return_low=True)
+    def forward(ctx, q, k, v, cu_q, cu_k, scale, window, sinks):
+        y, lse, low = attention_forward(q, k, v, cu_q, cu_k, scale, return_lse=True, return_low=True, window=window, sinks=sinks)
         ctx.save_for_backward(q, k, v, y, lse, cu_q, cu_k, low)
+        ctx.how = (window, sinks)
         ctx.scale = scale
         return y
 
@@ -305,17 +325,18 @@ class _Attention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         q, k, v, y, lse, cu_q, cu_k, low = ctx.saved_tensors
-        return (*attention_backward(q, k, v, y, lse, dy, cu_q, cu_k, ctx.scale, low), None, None, None)
+        return (*attention_backward(q, k, v, y, lse, dy, cu_q, cu_k, ctx.scale, low, *ctx.how), None, None, None, None, None)
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
               cu_seqlens_k: Optional[torch.Tensor] = None, scale: Optional[float] = None,
-              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+              out: Optional[torch.Tensor] = None, window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
     """Causal softmax attention of packed sequences: q (tokens, H, d), k and v (tokens, H_kv, d), sequence b the rows
     cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (integers on the device; rows outside the offsets are padding: zeros).  Or a
     uniform batch q (B, T, H, d), k and v (B, T, H_kv, d) without cu_seqlens.  H is a multiple of H_kv, query head h uses
     key head h / (H / H_kv).  With cu_seqlens_k the keys have lengths of their own, and a sequence's last query sees its
-    last key: query i the keys j <= i + len_k - len_q (none: its row is zero).  scale: 1 / sqrt(d).
+    last key: query i the keys j <= p = i + len_k - len_q (none: its row is zero).  scale: 1 / sqrt(d).
+    With `window` a query sees of these only the last `window`, j > p - window, and the first `sinks`, j < sinks.
 
     Differentiable in q, k and v, once; gradients come in their dtype, summed in fp32 in a fixed order.  `out`: where y goes
     (without autograd)."""
@@ -325,15 +346,15 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Opt
         B, T = q.shape[:2]
         cu = torch.arange(0, (B + 1) * T, T, device=q.device) if T > 0 else torch.zeros(B + 1, dtype=torch.int64, device=q.device)
         flat = [t.reshape(B * T, *t.shape[2:]) for t in (q, k, v)]
-        y = attention(*flat, cu, scale=scale, out=None if out is None else out.view(B * T, *out.shape[2:]))
+        y = attention(*flat, cu, scale=scale, out=None if out is None else out.view(B * T, *out.shape[2:]), window=window, sinks=sinks)
         return y.view(q.shape)
     if cu_seqlens is None:
         raise ValueError("attention: packed (tokens, heads, d) tensors need cu_seqlens")
     if _tracked(q, k, v):
         if out is not None:
             raise ValueError("attention: out has no gradient")
-        return _Attention.apply(q, k, v, cu_seqlens, cu_seqlens_k, scale)
-    return attention_forward(q, k, v, cu_seqlens, cu_seqlens_k, scale, out)
+        return _Attention.apply(q, k, v, cu_seqlens, cu_seqlens_k, scale, window, sinks)
+    return attention_forward(q, k, v, cu_seqlens, cu_seqlens_k, scale, out, window=window, sinks=sinks)
 
 
 # ------------------------------------------------------------------------------------------------- pages

@@ -23,9 +23,9 @@ def softmax(z: torch.Tensor, seen: torch.Tensor):
     return torch.where(s > 0, e / s, torch.zeros_like(e)), (torch.log(s) + top).squeeze(-1)
 
 
-def attention(q, k, v, cu_q, cu_k=None, scale=None, dy=None):
+def attention(q, k, v, cu_q, cu_k=None, scale=None, dy=None, visible=_visible):
     """{"y", "lse" (H, tokens)} and, with dy, {"dq", "dk", "dv"}; under "bounds" for each the sums that rounding errors scale
-    with ({name: (of rounded weights, of rounded dy . y)})."""
+    with ({name: (of rounded weights, of rounded dy . y)}).  `visible`: which keys queries see, of their numbers."""
     q, k, v = (t.detach().cpu().double() for t in (q, k, v))
     cu_q = [int(x) for x in cu_q]
     cu_k = cu_q if cu_k is None else [int(x) for x in cu_k]
@@ -39,7 +39,7 @@ def attention(q, k, v, cu_q, cu_k=None, scale=None, dy=None):
         b.update(dq=torch.zeros_like(q), dk=torch.zeros_like(k), dv=torch.zeros_like(v))
     most = 0.0
     for i0, i1, j0, j1 in zip(cu_q, cu_q[1:], cu_k, cu_k[1:]):
-        seen = _visible(i1 - i0, j1 - j0)
+        seen = visible(i1 - i0, j1 - j0)
         for h in range(H):
             e = h // G
             qq, kk, vv = q[i0:i1, h], k[j0:j1, e], v[j0:j1, e]

@@ -35,21 +35,41 @@ struct TreeParams {
   int H, KV, G, max_new, max_chunks, chunk, shift, nseq;
   int zero_from;  // the workgroups from this number on have tree_zero's rows
   float scale;
+  // under a window: a stream's context is taken as its sinks' tiles and its window's, one behind the other, in steps of `unit` keys
+  int window, sinks, unit;
+  // with weights: the scores (in bits, of base 2) [sequence][key head][row][room], and what they are added to
+  float *scores, *weights;
+  const int32_t* slots;
+  int64_t weights_stride[2], room, places, num_slots;
 };
 
 // What a workgroup works on: chunk `ch` of sequence b.
 struct TreeWork {
   int64_t lo;          // first new token
   int n, c0, c1;       // new tokens; the chunk's keys
-  int chunks, ctx;     // chunks of the sequence; its context
+  int chunks, ctx;     // chunks of the sequence; its context, under a window what is left of it
   int b, ch;           // b negative: nothing
 };
 
+// A context of `all` keys under a window: of its keys the first `first` stay, then those from first + skip on, in whole units;
+// token 0 sees the keys below p.sinks and those from all - window + 1 on, later ones no others.
+struct TreeBound {
+  int all, first, skip;
+  __device__ __forceinline__ TreeBound(const TreeParams& p, int ctx) : all(ctx) {
+    const int near = max(ctx - p.window + 1, 0) / p.unit * p.unit;
+    first = min((min(p.sinks, ctx) + p.unit - 1) / p.unit * p.unit, near);
+    skip = near - first;
+  }
+  __device__ __forceinline__ int key(int at) const { return at < first ? at : at + skip; }
+};
+
+template <bool WIN>
 __device__ __forceinline__ TreeWork tree_seq(const TreeParams& p, int b) {
   TreeWork t;
   t.lo = min(max(p.cu[b], (int64_t)0), p.total);
   t.n = (int)min(min(max(p.cu[b + 1], t.lo), p.total) - t.lo, (int64_t)p.max_new);
   t.ctx = (int)min((int64_t)max(p.lens[b], 0), p.max_context);
+  if constexpr (WIN) t.ctx -= TreeBound(p, t.ctx).skip;
   t.chunks = t.n > 0 ? max(1, (t.ctx + p.chunk - 1) / p.chunk) : 0;
   return t;
 }
@@ -62,6 +82,7 @@ __device__ __forceinline__ int lane_value(int v, int at) { return __builtin_amdg
 // sequence and place, the workgroups without a chunk came between the others, each holding a CU for its start: 16 trees
 // over 6000 tokens took 244 us, the CUs two thirds busy.)  Every lane counts the chunks of its share of the sequences, 64
 // shares make a prefix sum, and the share that has chunk u is looked through in the same way.
+template <bool WIN>
 __device__ __forceinline__ TreeWork tree_work(const TreeParams& p, int u, int lane) {
   TreeWork mine = {};
   int first = 0, n = p.nseq;  // the sequences still in question
@@ -69,7 +90,7 @@ __device__ __forceinline__ TreeWork tree_work(const TreeParams& p, int u, int la
     const int share = (n + 63) / 64, begin = first + min(lane * share, n), end = first + min(lane * share + share, n);
     int count = 0;
     for (int b = begin; b < end; ++b) {
-      mine = tree_seq(p, b);
+      mine = tree_seq<WIN>(p, b);
       count += mine.chunks;
     }
     int upto = count;
@@ -142,6 +163,27 @@ __device__ __forceinline__ uint64_t ancestors(const TreeParams& p, const TreeWor
     up = up < 0 ? -1 : next;
   }
   return sees;
+}
+
+// Of those the ones within the window: u stays if it is less than `window` steps up, or at a place below `sinks`; all lanes' depths.
+__device__ __forceinline__ uint64_t near_ancestors(const TreeParams& p, int n, int ctx, uint64_t sees, int depth) {
+  if (p.window < n)
+    for (int u = 0; u < n; ++u) {
+      const int above = __builtin_amdgcn_readlane(depth, u);
+      if (depth - above >= p.window && ctx + above >= p.sinks) sees &= ~(1ull << u);
+    }
+  return sees;
+}
+// The lowest n bits (none or all where n is out of their number).
+template <class B>
+__device__ __forceinline__ B low_bits(int n) {
+  constexpr int BITS = 8 * (int)sizeof(B);
+  return n <= 0 ? (B)0 : n >= BITS ? ~(B)0 : ((B)1 << n) - 1;
+}
+// The keys from `key` on that a token at position `at` sees of a context of `all`.
+template <class B>
+__device__ __forceinline__ B near_keys(const TreeParams& p, int key, int at, int all) {
+  return low_bits<B>(all - key) & (~low_bits<B>(at - p.window + 1 - key) | low_bits<B>(p.sinks - key));
 }
 
 // Sixteen keys (or values) into rows 16 g .. of an LDS tile: row r from base + min(r, last) * row_bytes, the base the same
@@ -256,7 +298,9 @@ struct TreeFew {
   static_assert(WAVES * 32 * PITCH * 4 <= LDS, "the waves' sums meet in the stages' place");
 };
 
-template <class P>
+// WIN: under a window, whose edge and sinks make the chunk's first tiles ones that are seen in part.  SCORES: the scores go to
+// the workspace too, in bits, for tree_weights.
+template <class P, bool WIN, bool SCORES>
 __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreeParams p) {
   typedef typename P::elem E;
   constexpr int D = P::D, KS = D / 16, CT = D / 32, W = TreeFew<P>::WAVES, STAGE = TreeFew<P>::STAGE;
@@ -266,9 +310,11 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if ((int)blockIdx.x >= p.zero_from) return tree_zero<E, D>(p, blockIdx.x - p.zero_from);
   const int e = blockIdx.x % p.KV;  // the key heads of a chunk next to one another: they go round the XCDs
-  const TreeWork t = tree_work(p, blockIdx.x / p.KV, lane);
+  const TreeWork t = tree_work<WIN>(p, blockIdx.x / p.KV, lane);
   if (t.b < 0) return;
   const int b = t.b, ch = t.ch, be = b * p.KV + e;
+  const TreeBound bound(p, WIN ? __builtin_amdgcn_readfirstlane((int)min((int64_t)max(p.lens[b], 0), p.max_context)) : 0);
+  auto key_at = [&](int at) { return WIN ? bound.key(at) : at; };
   const int rows = t.n * p.G, row = min(lane & 31, rows - 1), tok = row / p.G, h = e * p.G + row % p.G;
   const bool drafts = ch == t.chunks - 1;  // the last chunk has the new tokens too
   const int nt = t.c1 > t.c0 ? (t.c1 - t.c0 + 31) / 32 : 0, total = nt + (drafts ? 1 : 0);
@@ -277,34 +323,43 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
   int page0 = 0, page1 = 0;
   auto pages = [&](int at) {
     if (at >= nt) return;
-    page0 = page_of(p, b, key_group(t.c0 + 32 * at, t.c1 - 1).key);
-    page1 = page_of(p, b, key_group(t.c0 + 32 * at + 16, t.c1 - 1).key);
+    const int key = key_at(t.c0 + 32 * at), last = key_at(t.c1 - 1);
+    page0 = page_of(p, b, key_group(key, last).key);
+    page1 = page_of(p, b, key_group(key + 16, last).key);
   };
-  auto stage_drafts = [&](unsigned char* to) {
+  auto stage_drafts = [&](unsigned char* to) __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < 4; ++x)
       stage_new<P>(p, t.lo, e, key_group(16 * (x & 1), t.n - 1), x >> 1, to + (x >> 1) * STAGE / 2, x & 1, lane);
   };
   const WholeGroup<P> whole_k(p.kps[2], lane), whole_v(p.vps[2], lane);
   const int full = (t.c1 - t.c0) / 32;
-  auto stage = [&](int at, unsigned char* to) {
+  auto stage = [&](int at, unsigned char* to) __attribute__((always_inline)) {
     if (at < full) {
 #pragma unroll
       for (int x = 0; x < 4; ++x)
-        (x >> 1 ? whole_v : whole_k)(p, x & 1 ? page1 : page0, e, t.c0 + 32 * at + 16 * (x & 1), x >> 1, to + (x >> 1) * STAGE / 2, x & 1);
+        (x >> 1 ? whole_v : whole_k)(p, x & 1 ? page1 : page0, e, key_at(t.c0 + 32 * at) + 16 * (x & 1), x >> 1, to + (x >> 1) * STAGE / 2, x & 1);
       return;
     }
     if (at >= nt) return stage_drafts(to);
 #pragma unroll
     for (int x = 0; x < 4; ++x)
-      stage_paged<P>(p, x & 1 ? page1 : page0, e, key_group(t.c0 + 32 * at + 16 * (x & 1), t.c1 - 1), x >> 1, to + (x >> 1) * STAGE / 2, x & 1, lane);
+      stage_paged<P>(p, x & 1 ? page1 : page0, e, key_group(key_at(t.c0 + 32 * at) + 16 * (x & 1), key_at(t.c1 - 1)), x >> 1, to + (x >> 1) * STAGE / 2, x & 1, lane);
   };
   pages(w);
   if (w < total) stage(w, mine);
   pages(w + W);
   uint64_t sees = 0;
-  if (drafts) {
-    const uint64_t all = ancestors(p, t, lane);
+  int here = 0, head = 0;  // the token's position; tiles at the chunk's start that are seen in part
+  if (WIN || drafts) {
+    uint64_t all = ancestors(p, t, lane);
+    if constexpr (WIN) {
+      const int depth = __popcll(all) - 1;
+      all = near_ancestors(p, t.n, bound.all, all, depth);
+      here = bound.all + __shfl(depth, tok);
+      const int cut = bound.all + t.n - p.window;  // below it some token does not see a key that is no sink
+      if (cut > 0) head = min(max(((cut + 31) / 32 * 32 - bound.skip - t.c0) / 32, 0), full);
+    }
     sees = (uint64_t)__shfl((uint32_t)(all >> 32), tok) << 32 | __shfl((uint32_t)all, tok);
   }
   typename P::frag q[KS];
@@ -318,11 +373,12 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
   for (int ct = 0; ct < CT; ++ct) o[ct] = zero16();
   float m = -INFINITY, l = 0.f;
   const float c = p.scale * LOG2E;
+  float* scores = SCORES ? p.scores + ((int64_t)be * p.max_new * p.G + row) * p.room + t.c0 : nullptr;
   // one tile, read from `kt` while the next one's copies go to `next` (as in the prompt's kernel);
   // `whole`: of the context, all 32 keys of it there
   auto step = [&](auto whole, int at, const unsigned char* __restrict kt, unsigned char* __restrict next) {
     if (at + W < total) {
-      if constexpr (whole.value) {
+      if constexpr (WIN || whole.value) {
         stage(at + W, next);
         pages(at + 2 * W);
       } else {
@@ -342,9 +398,17 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
     sched_products<P, KS, P::ROW_READS>();
     uint32_t bits = ~0u;  // the keys of the tile that the row sees
     if constexpr (!whole.value) {
-      bits = at >= nt ? (uint32_t)sees : (uint32_t)((1ull << (t.c1 - t.c0 - 32 * at)) - 1);
+      bits = at >= nt ? (uint32_t)sees : WIN ? near_keys<uint32_t>(p, key_at(t.c0 + 32 * at), here, bound.all) : (uint32_t)((1ull << (t.c1 - t.c0 - 32 * at)) - 1);
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[0][i] = bits >> rho(half, i) & 1 ? s[0][i] : -INFINITY;
+    }
+    if constexpr (SCORES) {
+      if ((lane & 31) < rows)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+          const f32x4 x = {s[0][4 * a] * c, s[0][4 * a + 1] * c, s[0][4 * a + 2] * c, s[0][4 * a + 3] * c};
+          *reinterpret_cast<f32x4*>(scores + 32 * at + 8 * a + 4 * half) = x;
+        }
     }
     softmax_step<1>(s, m, l, o, c);
     if constexpr (whole.value) {
@@ -361,9 +425,17 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its slot may be written again
   };
   int at = w, buf = 0;
-  for (; at < full; at += W, buf ^= 1) step(std::true_type{}, at, mine + buf * STAGE, mine + (buf ^ 1) * STAGE);
+  if constexpr (WIN) {
 #pragma unroll 1
-  for (; at < total; at += W, buf ^= 1) step(std::false_type{}, at, mine + buf * STAGE, mine + (buf ^ 1) * STAGE);
+    for (; at < total; at += W, buf ^= 1) {
+      if (at >= head && at < full) step(std::true_type{}, at, mine + buf * STAGE, mine + (buf ^ 1) * STAGE);
+      else step(std::false_type{}, at, mine + buf * STAGE, mine + (buf ^ 1) * STAGE);
+    }
+  } else {
+    for (; at < full; at += W, buf ^= 1) step(std::true_type{}, at, mine + buf * STAGE, mine + (buf ^ 1) * STAGE);
+#pragma unroll 1
+    for (; at < total; at += W, buf ^= 1) step(std::false_type{}, at, mine + buf * STAGE, mine + (buf ^ 1) * STAGE);
+  }
   // the waves' sums, each scaled to the common maximum, added in the waves' order
   l = half_sum(l);
   if (half == 0) wm[w][lane] = m, wl[w][lane] = l;
@@ -407,6 +479,10 @@ __global__ void __launch_bounds__(64 * TreeFew<P>::WAVES) tree_few_kernel(TreePa
       *reinterpret_cast<f32x4*>(p.po + at * D + d) = x;
       if (d == 0) p.pml[2 * at] = wm[0][r] * c, p.pml[2 * at + 1] = wl[0][r];
     }
+    if (SCORES && d == 0 && t.chunks == 1) {
+      const int64_t at = (int64_t)be * p.max_chunks * p.max_new * p.G + r;
+      p.pml[2 * at] = wm[0][r] * c, p.pml[2 * at + 1] = wl[0][r];
+    }
   }
 }
 
@@ -421,7 +497,7 @@ struct TreeMany {
   static int per(int rows) { return ((rows + 31) / 32 + blocks(rows) - 1) / blocks(rows); }
 };
 
-template <class P>
+template <class P, bool WIN>
 __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tree_many_kernel(TreeParams p, int blocks, int per) {
   typedef typename P::elem E;
   constexpr int D = P::D, KS = D / 16, CT = D / 32, KEYS = TreeMany<P>::KEYS, TILE = TreeMany<P>::TILE;
@@ -434,9 +510,11 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
   // changes every 32 workgroups, an XCD's CUs: a CU gets its turn's larger and smaller blocks (16 trees 198 -> 186 us).
   const int at8 = blockIdx.x / 8, unit = at8 / blocks * 8 + blockIdx.x % 8, rb = (at8 + at8 / blocks * blocks / 32) % blocks;
   const int e = unit % p.KV;
-  const TreeWork t = tree_work(p, unit / p.KV, lane);
+  const TreeWork t = tree_work<WIN>(p, unit / p.KV, lane);
   if (t.b < 0) return;
   const int b = t.b, ch = t.ch, be = b * p.KV + e;
+  const TreeBound bound(p, WIN ? __builtin_amdgcn_readfirstlane((int)min((int64_t)max(p.lens[b], 0), p.max_context)) : 0);
+  auto key_at = [&](int at) { return WIN ? bound.key(at) : at; };
   const int rows = t.n * p.G, first = 32 * (per * rb + w);
   if (32 * per * rb >= rows) return;
   const bool busy = w < per && first < rows, live = busy && first + (lane & 31) < rows;
@@ -447,11 +525,11 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
   const int mine = KEYS == 64 ? w : w & 1;
   int page = 0;
   auto pages = [&](int at) {
-    if (at < nt) page = page_of(p, b, key_group(t.c0 + KEYS * at + 16 * mine, t.c1 - 1).key);
+    if (at < nt) page = page_of(p, b, key_group(key_at(t.c0 + KEYS * at) + 16 * mine, key_at(t.c1 - 1)).key);
   };
   const WholeGroup<P> whole_k(KEYS == 64 || w < 2 ? p.kps[2] : p.vps[2], lane), whole_v(p.vps[2], lane);
   auto stage_whole = [&](int at, unsigned char* to) {
-    const int key = t.c0 + KEYS * at + 16 * mine;
+    const int key = key_at(t.c0 + KEYS * at) + 16 * mine;
     if constexpr (KEYS == 64) {
       whole_k(p, page, e, key, false, to, mine);
       whole_v(p, page, e, key, true, to + TILE, mine);
@@ -460,9 +538,9 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
     }
   };
   const int full = (t.c1 - t.c0) / KEYS;
-  auto stage = [&](int at, unsigned char* to) {
+  auto stage = [&](int at, unsigned char* to) __attribute__((always_inline)) {
     if (at < full) return stage_whole(at, to);
-    const Group g = at < nt ? key_group(t.c0 + KEYS * at + 16 * mine, t.c1 - 1) : key_group(KEYS * (at - nt) + 16 * mine, t.n - 1);
+    const Group g = at < nt ? key_group(key_at(t.c0 + KEYS * at) + 16 * mine, key_at(t.c1 - 1)) : key_group(KEYS * (at - nt) + 16 * mine, t.n - 1);
     auto part = [&](bool v) {
       if (at < nt) stage_paged<P>(p, page, e, g, v, to + v * TILE, mine, lane);
       else stage_new<P>(p, t.lo, e, g, v, to + v * TILE, mine, lane);
@@ -477,8 +555,16 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
   }
   pages(BUFS - 1);
   uint64_t sees = 0;
-  if (drafts) {
-    const uint64_t all = ancestors(p, t, lane);
+  int here = 0, head = 0;  // as in the kernel of few rows
+  if (WIN || drafts) {
+    uint64_t all = ancestors(p, t, lane);
+    if constexpr (WIN) {
+      const int depth = __popcll(all) - 1;
+      all = near_ancestors(p, t.n, bound.all, all, depth);
+      here = bound.all + __shfl(depth, tok);
+      const int cut = bound.all + t.n - p.window;
+      if (cut > 0) head = min(max(((cut + KEYS - 1) / KEYS * KEYS - bound.skip - t.c0) / KEYS, 0), full);
+    }
     sees = (uint64_t)__shfl((uint32_t)(all >> 32), tok) << 32 | __shfl((uint32_t)all, tok);
   }
   typename P::frag q[KS];
@@ -509,7 +595,7 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
     sched_products<P, KEYS / 32 * KS, P::ROW_READS>();
     uint64_t bits = ~0ull;  // the keys of the tile that the row sees
     if constexpr (!whole.value) {
-      bits = at >= nt ? sees >> (KEYS * (at - nt)) : (1ull << (t.c1 - t.c0 - KEYS * at)) - 1;
+      bits = at >= nt ? sees >> (KEYS * (at - nt)) : WIN ? near_keys<uint64_t>(p, key_at(t.c0 + KEYS * at), here, bound.all) : (1ull << (t.c1 - t.c0 - KEYS * at)) - 1;
 #pragma unroll
       for (int u = 0; u < KEYS / 32; ++u)
 #pragma unroll
@@ -536,6 +622,10 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
     step(whole, at, lds + now * 2 * TILE, lds + then * 2 * TILE);
     now = now == BUFS - 1 ? 0 : now + 1;
   };
+  if constexpr (WIN) {
+#pragma unroll 1
+    for (; at < head; ++at) turn(std::false_type{});
+  }
   for (; at < full; ++at) turn(std::true_type{});
 #pragma unroll 1
   for (; at < total; ++at) turn(std::false_type{});
@@ -554,15 +644,15 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
 }
 
 // The chunks of one row joined in their order: a wave a row, D / 64 values a lane.
-template <class E, int D>
-__global__ void __launch_bounds__(256) tree_join_kernel(TreeParams p) {
+template <class E, int D, bool WIN>
+__device__ __forceinline__ void tree_join(const TreeParams& p) {
   const int lane = threadIdx.x & 63;
   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int most = p.max_new * p.G, r = (int)(id % most);
   const int64_t be = id / most;
   if (be >= (int64_t)p.nseq * p.KV) return;
   const int b = (int)(be / p.KV), e = (int)(be % p.KV);
-  const TreeWork t = tree_seq(p, b);
+  const TreeWork t = tree_seq<WIN>(p, b);
   if (r >= t.n * p.G || t.chunks == 1) return;
   const int64_t first = be * p.max_chunks * most + r;
   float top = -INFINITY;
@@ -585,6 +675,63 @@ __global__ void __launch_bounds__(256) tree_join_kernel(TreeParams p) {
   for (int i = 0; i < V; ++i) dst[i] = (E)(o[i] * g);
 }
 
+template <class E, int D, bool WIN>
+__global__ void __launch_bounds__(256) tree_join_kernel(TreeParams p) {
+  tree_join<E, D, WIN>(p);
+}
+
+// What each key of a sequence got from the rows of a key head, added to its weight (a new token's own place: set): a workgroup
+// has 1024 keys, a thread four, the rows in order.
+constexpr int WEIGHT_KEYS = 1024, WEIGHT_ROWS = 32;
+template <bool WIN>
+__device__ __forceinline__ void tree_weights(const TreeParams& p, int id) {
+  __shared__ float norm[WEIGHT_ROWS];
+  const int blocks = (int)((p.room + WEIGHT_KEYS - 1) / WEIGHT_KEYS), part = id % blocks, be = id / blocks, b = be / p.KV, e = be % p.KV;
+  const TreeWork t = tree_seq<WIN>(p, b);
+  const int slot = p.slots ? p.slots[b] : b, most = p.max_new * p.G, rows = t.n * p.G, end = (t.ctx + 31) / 32 * 32;  // the new tokens' scores start there
+  if (rows == 0 || slot < 0 || slot >= p.num_slots || part * WEIGHT_KEYS >= end + t.n) return;
+  if ((int)threadIdx.x < rows) {
+    const int64_t first = (int64_t)be * p.max_chunks * most + threadIdx.x;
+    float top = -INFINITY, sum = 0.f;
+    for (int x = 0; x < t.chunks; ++x) top = fmaxf(top, p.pml[2 * (first + (int64_t)x * most)]);
+    for (int x = 0; x < t.chunks; ++x) {
+      const int64_t at = first + (int64_t)x * most;
+      const float m = p.pml[2 * at];
+      sum += m == -INFINITY ? 0.f : p.pml[2 * at + 1] * __builtin_amdgcn_exp2f(m - top);
+    }
+    norm[threadIdx.x] = top + __builtin_amdgcn_logf(sum);  // (a row sees itself: the sum is positive)
+  }
+  __syncthreads();
+  const int v = part * WEIGHT_KEYS + 4 * threadIdx.x;
+  if (v >= end + t.n) return;
+  f32x4 sum = zero4();
+  for (int r = 0; r < rows; ++r) {
+    const f32x4 s = *reinterpret_cast<const f32x4*>(p.scores + ((int64_t)be * most + r) * p.room + v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(s[i] - norm[r]);
+  }
+  const TreeBound bound(p, (int)min((int64_t)max(p.lens[b], 0), p.max_context));
+  float* w = p.weights + slot * p.weights_stride[0] + e * p.weights_stride[1];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = v + i;
+    if (at >= end) {
+      const int64_t place = (int64_t)bound.all + at - end;
+      if (at - end < t.n && place < p.places) w[place] = sum[i];
+    } else if (at < t.ctx) {
+      const int place = WIN ? bound.key(at) : at;
+      if (place < p.places) w[place] += sum[i];
+    }
+  }
+}
+
+// The chunks' join, if there are chunks, and the weights, which need no joined sums.
+template <class E, int D, bool WIN>
+__global__ void __launch_bounds__(256) tree_finish_kernel(TreeParams p, int joins) {
+  if ((int)blockIdx.x < joins) tree_join<E, D, WIN>(p);
+  else tree_weights<WIN>(p, blockIdx.x - joins);
+}
+
 // A product of sizes that no caller's numbers take past 64 bits.
 static int64_t times(int64_t a, int64_t b) {
   int64_t r;
@@ -593,20 +740,37 @@ static int64_t times(int64_t a, int64_t b) {
 static int64_t tree_rows(const kdn_tree_attn_args* a) { return a->max_new * (a->H / a->H_kv); }  // to a sequence and key head
 static int64_t tree_blocks(const kdn_tree_attn_args* a) { return tree_rows(a) <= 32 ? 1 : (tree_rows(a) + 127) / 128; }
 
+// What a call's window and weights come to: one that leaves every key to see is none; the longest context that is walked over, which
+// the grid and the workspace go by; the keys that a tile holds; the scores that a row has room for.
+struct TreePlan {
+  bool window, weights;
+  int64_t longest, room;
+  int unit;
+  TreePlan(const kdn_tree_attn_args* a, const kdn_tree_bound_args* b) {
+    unit = tree_rows(a) > 32 && a->d * (int)dtype_size(a->dtype) <= 128 ? 64 : 32;
+    const int64_t all = a->max_context + a->max_new;
+    window = b && b->window > 0 && b->window < all && b->sinks < all;
+    weights = b && b->weights;
+    // the sinks' tiles, and window - 1 keys that need not start a tile
+    longest = window ? std::min(a->max_context, (std::min(b->sinks, a->max_context) + unit - 1) / unit * unit + b->window + unit) : a->max_context;
+    room = weights ? (longest + 31) / 32 * 32 + 32 : 0;
+  }
+};
+
 constexpr int MAX_CHUNK = 2048;
 // Keys of a chunk: 128 to 2048, the fewest with which the grid stays within 512 workgroups, or from 256 keys on 2048 (a
 // chunk's own cost, its queries and its partial sums, is that of a few dozen keys; short chunks even out unequal contexts).
 // With chunks of at most 1024 keys 16 trees of 40 drafts, contexts of 1500 to 16384, took 186 us where these took 177, one
 // token of 224 streams 396 where these took 378; with up to 4096 the 224 streams took 395.
-static int tree_chunk(const kdn_tree_attn_args* a) {
+static int tree_chunk(const kdn_tree_attn_args* a, int64_t longest) {
   const int64_t each = times(a->num_seqs * a->H_kv, tree_blocks(a));
   int chunk = 128;
-  while (chunk < MAX_CHUNK && times(each, (a->max_context + chunk - 1) / chunk) > (chunk < 256 ? 512 : 2048)) chunk *= 2;
+  while (chunk < MAX_CHUNK && times(each, (longest + chunk - 1) / chunk) > (chunk < 256 ? 512 : 2048)) chunk *= 2;
   return chunk;
 }
-static int64_t tree_chunks(const kdn_tree_attn_args* a) {
-  const int chunk = tree_chunk(a);
-  return a->max_context > 0 ? (a->max_context + chunk - 1) / chunk : 1;
+static int64_t tree_chunks(const kdn_tree_attn_args* a, int64_t longest) {
+  const int chunk = tree_chunk(a, longest);
+  return longest > 0 ? (longest + chunk - 1) / chunk : 1;
 }
 
 static int tree_check(const kdn_tree_attn_args* a) {
@@ -623,28 +787,37 @@ static int tree_check(const kdn_tree_attn_args* a) {
     return KDN_ERR_INVALID_ARGUMENT;
   // a grid's workgroups, and the join's rows
   const int64_t heads = a->num_seqs * a->H_kv, blocks = tree_blocks(a);
-  if (times(times(heads, tree_chunks(a)), blocks) > INT32_MAX - 8 * blocks - ZERO_GROUPS || times(heads, tree_rows(a)) > INT32_MAX)
+  if (times(times(heads, tree_chunks(a, a->max_context)), blocks) > INT32_MAX - 8 * blocks - ZERO_GROUPS || times(heads, tree_rows(a)) > INT32_MAX)
     return KDN_ERR_UNSUPPORTED;
   return KDN_OK;
 }
 
-template <class P>
+template <class P, bool WIN>
 static int launch_tree(TreeParams& p, hipStream_t st) {
   const int rows = p.max_new * p.G;
   const int64_t units = (int64_t)p.nseq * p.KV * p.max_chunks;
   if (rows <= 32) {
     p.zero_from = (int)units;
-    hipLaunchKernelGGL(tree_few_kernel<P>, dim3((unsigned)units + ZERO_GROUPS), dim3(64 * TreeFew<P>::WAVES), 0, st, p);
+    if (p.weights) hipLaunchKernelGGL((tree_few_kernel<P, WIN, true>), dim3((unsigned)units + ZERO_GROUPS), dim3(64 * TreeFew<P>::WAVES), 0, st, p);
+    else hipLaunchKernelGGL((tree_few_kernel<P, WIN, false>), dim3((unsigned)units + ZERO_GROUPS), dim3(64 * TreeFew<P>::WAVES), 0, st, p);
   } else {
     const int blocks = TreeMany<P>::blocks(rows);
     p.zero_from = (int)((units + 7) / 8 * 8 * blocks);
-    hipLaunchKernelGGL(tree_many_kernel<P>, dim3((unsigned)p.zero_from + ZERO_GROUPS), dim3(256), 0, st, p, blocks, TreeMany<P>::per(rows));
+    hipLaunchKernelGGL((tree_many_kernel<P, WIN>), dim3((unsigned)p.zero_from + ZERO_GROUPS), dim3(256), 0, st, p, blocks, TreeMany<P>::per(rows));
   }
-  if (p.max_chunks > 1 && p.nseq > 0) {
-    const int64_t joins = (int64_t)p.nseq * p.KV * rows;
-    hipLaunchKernelGGL((tree_join_kernel<typename P::elem, P::D>), dim3((unsigned)((joins + 3) / 4)), dim3(256), 0, st, p);
+  const int64_t joins = p.max_chunks > 1 ? ((int64_t)p.nseq * p.KV * rows + 3) / 4 : 0;
+  if (p.weights && p.nseq > 0) {
+    const int64_t parts = (p.room + WEIGHT_KEYS - 1) / WEIGHT_KEYS * p.nseq * p.KV;
+    hipLaunchKernelGGL((tree_finish_kernel<typename P::elem, P::D, WIN>), dim3((unsigned)(joins + parts)), dim3(256), 0, st, p, (int)joins);
+  } else if (joins > 0) {
+    hipLaunchKernelGGL((tree_join_kernel<typename P::elem, P::D, WIN>), dim3((unsigned)joins), dim3(256), 0, st, p);
   }
   return launch_status();
+}
+
+template <class P>
+static int launch_tree(TreeParams& p, bool window, hipStream_t st) {
+  return window ? launch_tree<P, true>(p, st) : launch_tree<P, false>(p, st);
 }
 
 }  // namespace kdn
@@ -658,14 +831,41 @@ static size_t tree_partial_bytes(const kdn_tree_attn_args* a, int64_t units) {
 
 // Not the call's own number of chunks but a bound that grows with every size, so that a workspace for the largest call
 // holds for the others: the rule for a chunk's length gives a smaller call shorter chunks, and at times more of them.
-extern "C" size_t kdn_tree_attn_workspace_bytes(const kdn_tree_attn_args* a) {
-  if (tree_check(a) != KDN_OK) return 0;
-  const int64_t heads = a->num_seqs * a->H_kv, fine = heads * ((a->max_context + 127) / 128), coarse = heads * ((a->max_context + MAX_CHUNK - 1) / MAX_CHUNK);
-  return a->max_context <= 128 ? 16 : tree_partial_bytes(a, std::min(fine, std::max<int64_t>(2048, coarse)));
+static size_t tree_bytes(const kdn_tree_attn_args* a, int64_t longest) {
+  const int64_t heads = a->num_seqs * a->H_kv, fine = heads * ((longest + 127) / 128), coarse = heads * ((longest + MAX_CHUNK - 1) / MAX_CHUNK);
+  return longest <= 128 ? 16 : tree_partial_bytes(a, std::min(fine, std::max<int64_t>(2048, coarse)));
+}
+// The scores of a call with weights, and each row's maxima and sums where one chunk has no partial sums.
+static size_t tree_score_bytes(const kdn_tree_attn_args* a, const TreePlan& plan) {
+  if (!plan.weights) return 0;
+  return ((size_t)a->num_seqs * (size_t)a->H_kv * (size_t)tree_rows(a) * ((size_t)plan.room + (size_t)a->d + 2)) * 4 + 32;
 }
 
-extern "C" int kdn_tree_attn(const kdn_tree_attn_args* a, void* stream) {
+static int bound_check(const kdn_tree_attn_args* a, const kdn_tree_bound_args* b) {
+  if (!b || b->window < 0 || b->sinks < 0 || (b->weights && (b->places < 0 || b->num_slots < 0))) return KDN_ERR_INVALID_ARGUMENT;
+  if (!b->weights) return KDN_OK;
+  if (a->parents) return KDN_ERR_INVALID_ARGUMENT;
+  const TreePlan plan(a, b);
+  const int64_t heads = a->num_seqs * a->H_kv, parts = times(heads, (plan.room + WEIGHT_KEYS - 1) / WEIGHT_KEYS);
+  if (tree_rows(a) > WEIGHT_ROWS || b->num_slots > INT32_MAX || times(heads, tree_rows(a)) > (1 << 30) || parts > (1 << 30)) return KDN_ERR_UNSUPPORTED;
+  if (!b->slots && b->num_slots < a->num_seqs) return KDN_ERR_INVALID_ARGUMENT;
+  return aligned(b->weights, 4) && aligned(b->slots, 4) ? KDN_OK : KDN_ERR_MISALIGNED;
+}
+
+extern "C" size_t kdn_tree_attn_workspace_bytes(const kdn_tree_attn_args* a) {
+  if (tree_check(a) != KDN_OK) return 0;
+  return tree_bytes(a, a->max_context);
+}
+
+extern "C" size_t kdn_tree_attn_bounded_workspace_bytes(const kdn_tree_attn_args* a, const kdn_tree_bound_args* b) {
+  if (tree_check(a) != KDN_OK || bound_check(a, b) != KDN_OK) return 0;
+  const TreePlan plan(a, b);
+  return tree_bytes(a, plan.longest) + tree_score_bytes(a, plan);
+}
+
+static int tree_attn(const kdn_tree_attn_args* a, const kdn_tree_bound_args* b, void* stream) {
   int rc = tree_check(a);
+  if (rc == KDN_OK && b) rc = bound_check(a, b);
   if (rc != KDN_OK) return rc;
   if (a->total_new == 0 || (a->num_seqs == 0 && !a->y)) return KDN_OK;
   if (!a->y || (a->num_seqs > 0 && (!a->cu_new || !a->context_lens || !a->q || !a->k || !a->v ||
@@ -678,11 +878,13 @@ extern "C" int kdn_tree_attn(const kdn_tree_attn_args* a, void* stream) {
   for (int i = 0; i < 3; ++i)
     fits = fits && a->k_pages_stride[i] >= 0 && a->v_pages_stride[i] >= 0 && a->k_pages_stride[i] % per == 0 && a->v_pages_stride[i] % per == 0;
   if (!fits) return KDN_ERR_MISALIGNED;
-  const int64_t chunks = tree_chunks(a);
+  const TreePlan plan(a, b);
+  const int64_t chunks = tree_chunks(a, plan.longest);
   // a copy's lanes have 32-bit offsets from its first row
   const int64_t size = (int64_t)dtype_size(a->dtype), far = INT32_MAX / (16 * size);
   if (a->k_stride[0] > far || a->v_stride[0] > far || a->k_pages_stride[2] > far || a->v_pages_stride[2] > far) return KDN_ERR_UNSUPPORTED;
-  if (a->num_seqs > 0 && chunks > 1 && (!a->workspace || a->workspace_bytes < tree_partial_bytes(a, a->num_seqs * a->H_kv * chunks))) return KDN_ERR_WORKSPACE_TOO_SMALL;
+  const size_t partial = chunks > 1 ? tree_partial_bytes(a, a->num_seqs * a->H_kv * chunks) : 0;
+  if (a->num_seqs > 0 && (chunks > 1 || plan.weights) && (!a->workspace || a->workspace_bytes < partial + tree_score_bytes(a, plan))) return KDN_ERR_WORKSPACE_TOO_SMALL;
   TreeParams p = {};
   p.q = a->q; p.k = a->k; p.v = a->v; p.kp = a->k_pages; p.vp = a->v_pages; p.y = a->y;
   for (int i = 0; i < 2; ++i) {
@@ -694,12 +896,28 @@ extern "C" int kdn_tree_attn(const kdn_tree_attn_args* a, void* stream) {
   p.cu = a->cu_new; p.lens = a->context_lens; p.table = a->page_table; p.parents = a->parents;
   p.table_stride = a->table_stride; p.num_pages = a->num_pages; p.total = a->total_new; p.max_context = a->max_context;
   p.H = (int)a->H; p.KV = (int)a->H_kv; p.G = (int)(a->H / a->H_kv);
-  p.max_new = (int)a->max_new; p.max_chunks = (int)chunks; p.chunk = tree_chunk(a); p.nseq = (int)a->num_seqs;
+  p.max_new = (int)a->max_new; p.max_chunks = (int)chunks; p.chunk = tree_chunk(a, plan.longest); p.nseq = (int)a->num_seqs;
   p.shift = __builtin_ctz((unsigned)a->page_tokens);
   p.scale = a->scale;
   p.po = reinterpret_cast<float*>(a->workspace);
   p.pml = p.po + (size_t)a->num_seqs * a->H * chunks * a->max_new * a->d;
+  p.window = plan.window ? (int)b->window : (int)NO_WINDOW;
+  p.sinks = plan.window ? (int)b->sinks : 0;
+  p.unit = plan.unit;
+  if (plan.weights && a->num_seqs > 0) {
+    p.scores = p.pml + (size_t)a->num_seqs * a->H * chunks * a->max_new * 2;
+    p.scores += (16 - (uintptr_t)p.scores % 16) % 16 / 4;
+    p.room = plan.room;
+    p.weights = b->weights; p.places = b->places; p.slots = b->slots; p.num_slots = b->num_slots;
+    p.weights_stride[0] = b->weights_stride[0]; p.weights_stride[1] = b->weights_stride[1];
+  }
   hipStream_t st = as_stream(stream);
-  if (a->dtype == KDN_DTYPE_BF16) return a->d == 64 ? launch_tree<AttnBF16<64>>(p, st) : launch_tree<AttnBF16<128>>(p, st);
-  return a->d == 64 ? launch_tree<AttnF32<64>>(p, st) : launch_tree<AttnF32<128>>(p, st);
+  if (a->dtype == KDN_DTYPE_BF16) return a->d == 64 ? launch_tree<AttnBF16<64>>(p, plan.window, st) : launch_tree<AttnBF16<128>>(p, plan.window, st);
+  return a->d == 64 ? launch_tree<AttnF32<64>>(p, plan.window, st) : launch_tree<AttnF32<128>>(p, plan.window, st);
+}
+
+extern "C" int kdn_tree_attn(const kdn_tree_attn_args* a, void* stream) { return tree_attn(a, nullptr, stream); }
+
+extern "C" int kdn_tree_attn_bounded(const kdn_tree_attn_args* a, const kdn_tree_bound_args* b, void* stream) {
+  return b ? tree_attn(a, b, stream) : KDN_ERR_INVALID_ARGUMENT;
 }

@@ -86,6 +86,16 @@ ANCHOR_EXPORTED = (
     "kdn_tree_attn",
 )
 
+# Exported symbols of include/kdn_bounded.h (checked by tests/test_bounded_host.py).
+BOUNDED_EXPORTED = (
+    "kdn_bounded_version",
+    "kdn_attn_window_fwd",
+    "kdn_attn_window_bwd_workspace_bytes",
+    "kdn_attn_window_bwd",
+    "kdn_tree_attn_bounded_workspace_bytes",
+    "kdn_tree_attn_bounded",
+)
+
 KDN_ERR_CAPACITY = -6
 KDN_ERR_WORKSPACE_TOO_SMALL = -3
 NOALLOC_SCRATCH_BYTES = 256 << 20   # KDN_NOALLOC_SCRATCH_BYTES of include/kdn.h
@@ -276,6 +286,17 @@ class TreeAttnArgs(ctypes.Structure):
     ]
 
 
+class TreeBoundArgs(ctypes.Structure):
+    """Mirror of struct kdn_tree_bound_args (include/kdn_bounded.h)."""
+
+    _fields_ = [
+        ("window", _i64), ("sinks", _i64),
+        ("weights", ctypes.c_void_p), ("weights_stride", _i64x2),
+        ("places", _i64), ("num_slots", _i64),
+        ("slots", ctypes.c_void_p),
+    ]
+
+
 def _declare_anchor(L: ctypes.CDLL) -> None:
     """Argument and result types of include/kdn_anchor.h and include/kdn_bounded.h."""
     vp, i64, ci, sz, ptr = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.POINTER
@@ -307,7 +328,9 @@ def _declare_anchor(L: ctypes.CDLL) -> None:
             ("kdn_bounded_version", [], ci),
             ("kdn_attn_window_fwd", [vp, i64, i64, vp], ci),
             ("kdn_attn_window_bwd_workspace_bytes", [vp, i64, i64], sz),
-            ("kdn_attn_window_bwd", [vp, i64, i64, vp], ci)):
+            ("kdn_attn_window_bwd", [vp, i64, i64, vp], ci),
+            ("kdn_tree_attn_bounded_workspace_bytes", [vp, vp], sz),
+            ("kdn_tree_attn_bounded", [vp, vp, vp], ci)):
         fn = getattr(L, name)
         fn.argtypes, fn.restype = args, res
 

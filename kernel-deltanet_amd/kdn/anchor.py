@@ -6,7 +6,8 @@ its recurrent ones, and the pages their keys and values live in.
     PagePool          which pages a stream's tokens lie on: fork, extend, truncate, compact, free (host)
     page_copy         whole pages (forks about to write, compaction)
     page_append       new tokens' keys and values into their pages
-    tree_attention    one new token a stream, a run of them, or a tree of drafts, over the pages
+    tree_attention    one new token a stream, a run of them, or a tree of drafts, over the pages, whole or in a window; and what
+                      weight each key got
 
 torch supplies device memory and the current HIP stream; every computation is a HIP kernel in libkdn.so.  The tensors are
 gfx950 device tensors, (tokens, heads, d) with d = 64 or 128 in bfloat16 or float32, in any strides with contiguous heads
@@ -43,6 +44,7 @@ _ATTN_BWD = struct.Struct("@P" + 4 * "Pqq" + "PN")
 _ROTARY = struct.Struct("@qqqiiiiifPP" + 4 * "Pqq")
 _APPEND = struct.Struct("@qqiiqqP" + 2 * "Pqq" + 2 * "Pqqq")
 _TREE = struct.Struct("@qqqqqqiifqqqqPPPP" + 3 * "Pqq" + 2 * "Pqqq" + "Pqq" + "PN")
+_BOUND = struct.Struct("@qqPqqqqP")  # include/kdn_bounded.h
 
 
 def _device(index: int):
@@ -505,11 +507,29 @@ class PagePool:
 # ------------------------------------------------------------------------------------------------- attention over pages
 
 
+def _key_weights(weights: torch.Tensor, slots: Optional[torch.Tensor], streams: int, heads: Tuple[int, ...], like: torch.Tensor, what: str):
+    """(slots, their address or 0) of weights that a call writes where they are, (slots, *heads, places) float32 on like's device."""
+    require_device(weights, f"{what} weights")
+    if weights.dim() != 2 + len(heads) or tuple(weights.shape[1:-1]) != heads or weights.dtype is not _F32 or weights.device != like.device or \
+            (weights.shape[-1] > 1 and weights.stride(-1) != 1):
+        raise ValueError(f"{what}: weights are (slots, {', '.join(map(str, heads))}, places) float32 on {like.device}, places next to one another; "
+                         f"got {tuple(weights.shape)} {weights.dtype} on {weights.device}")
+    if weights.requires_grad:
+        raise ValueError(f"{what}: weights have no gradient")
+    if slots is None:
+        if weights.shape[0] != streams:
+            raise ValueError(f"{what}: weights of {weights.shape[0]} slots for {streams} streams need slots")
+        return None, 0
+    slots = _ints(slots, f"{what} slots", torch.int32, like.get_device(), streams)
+    return slots, slots.data_ptr()
+
+
 def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                    page_table: torch.Tensor, context_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
                    parents: Optional[torch.Tensor] = None, scale: Optional[float] = None, max_context: Optional[int] = None,
-                   max_new: Optional[int] = None, out: Optional[torch.Tensor] = None,
-                   workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   max_new: Optional[int] = None, out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+                   window: Optional[int] = None, sinks: int = 0, weights: Optional[torch.Tensor] = None,
+                   slots: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of new tokens over their streams' pages and over themselves.
 
     q (tokens, H, d), k and v (tokens, H_kv, d): the new tokens, stream b's the rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1
@@ -520,7 +540,15 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: t
     At most 64 new tokens a stream; max_new (64, or 1 without cu_seqlens) and max_context (what page_table holds) bound
     them from the host, so that nothing is read back; the closer, the smaller the launch.  Rows outside the offsets are
     padding: zeros, as are those of a stream past max_new.  `workspace`: uint8, at least `tree_workspace_bytes`, for a caller
-    that allocates once.  Not differentiable: y raises on backward."""
+    that allocates once.  Not differentiable: y raises on backward.
+
+    With `window` a new token, at position context + its depth (how many new tokens it sees besides itself), sees only the last
+    `window` positions, its own among them, and the first `sinks`.
+
+    `weights` (slots, H_kv, places) float32: to the weight of each key of a stream's context is added the sum of its softmax weights
+    over the stream's new tokens and the query heads of its head, and those of the new tokens' own places, behind the
+    context, are set to theirs.  `slots` (streams,): which row is a stream's (none given: its number), no two the same; of those out of
+    range nothing is written.  Runs of tokens alone (no parents), at most 32 rows of new tokens and query heads to a key head."""
     what = "tree_attention"
     tracked = _tracked(q, k, v, k_pages, v_pages)
     if tracked and forward_ad._current_level >= 0 and _dual((q, k, v, k_pages, v_pages)):
@@ -550,24 +578,44 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: t
     par = None if parents is None else _ints(parents, "tree_attention parents", torch.int32, dev, n)
     room = width * P
     ctx = room if max_context is None else min(int(max_context), room)
+    near, first = _window(window, sinks, what)
+    bound = None
+    if weights is not None:
+        if par is not None:
+            raise ValueError("tree_attention: weights are of runs of tokens, not of trees (a refused draft would count)")
+        slots, slots_at = _key_weights(weights, slots, B, (KV,), q, what)
+        bound = _BOUND.pack(near, first, weights.data_ptr(), weights.stride(0), weights.stride(1), weights.shape[2], weights.shape[0], slots_at)
+        torch.autograd.graph.increment_version(weights)
+    elif near:
+        bound = _BOUND.pack(near, first, 0, 0, 0, 0, 0, 0)
     y = _new(q, (n, H, d)) if out is None else _out(out, "tree_attention out", q.shape, q)
     sizes = (B, n, most, ctx, H, KV, d, _tag(q.dtype, what), _scale(scale, d, what), P, pages, width, page_table.stride(0))
     with _device(dev):
         if workspace is None:
-            workspace = q.new_empty(N.lib().kdn_tree_attn_workspace_bytes(_TREE.pack(*sizes, *_NO_TENSORS)), dtype=torch.uint8)
+            workspace = q.new_empty(_tree_bytes(_TREE.pack(*sizes, *_NO_TENSORS), bound), dtype=torch.uint8)
         elif workspace.get_device() != dev or not workspace.is_contiguous():
             raise ValueError(f"tree_attention: the workspace is contiguous on {q.device}")
-        N.check(N.lib().kdn_tree_attn(_TREE.pack(*sizes, cu.data_ptr(), lens.data_ptr(), page_table.data_ptr(), 0 if par is None else par.data_ptr(),
-                                                 *qs[1:], *ks[1:], *vs[1:], *kp[1:], *vp[1:], *y[1:], workspace.data_ptr(), workspace.nbytes),
-                                      _raw_stream(dev)), "kdn_tree_attn")
+        args = _TREE.pack(*sizes, cu.data_ptr(), lens.data_ptr(), page_table.data_ptr(), 0 if par is None else par.data_ptr(), *qs[1:], *ks[1:],
+                          *vs[1:], *kp[1:], *vp[1:], *y[1:], workspace.data_ptr(), workspace.nbytes)
+        if bound is None:
+            N.check(N.lib().kdn_tree_attn(args, _raw_stream(dev)), "kdn_tree_attn")
+        else:
+            N.check(N.lib().kdn_tree_attn_bounded(args, bound, _raw_stream(dev)), "kdn_tree_attn_bounded")
     return forward_only(what, (y[0],), (q, k, v, k_pages, v_pages))[0] if tracked else y[0]
 
 
 _NO_TENSORS = (0,) * 26  # the tensor fields of kdn_tree_attn_args, where only sizes are read
 
 
+def _tree_bytes(args: bytes, bound: Optional[bytes]) -> int:
+    return N.lib().kdn_tree_attn_workspace_bytes(args) if bound is None else N.lib().kdn_tree_attn_bounded_workspace_bytes(args, bound)
+
+
 def tree_workspace_bytes(streams: int, H: int, H_kv: int, d: int, dtype: torch.dtype, page_tokens: int, max_context: int,
-                         max_new: int = 1) -> int:
-    """Bytes of `tree_attention`'s workspace for up to these sizes (0: not supported)."""
-    return int(N.lib().kdn_tree_attn_workspace_bytes(_TREE.pack(streams, streams, max_new, max_context, H, H_kv, d, _tag(dtype, "tree_attention"),
-                                                                1.0, page_tokens, 1, -(-max_context // page_tokens), 0, *_NO_TENSORS)))
+                         max_new: int = 1, window: Optional[int] = None, sinks: int = 0, weights: bool = False) -> int:
+    """Bytes of `tree_attention`'s workspace for up to these sizes (0: not supported), with this window, with or without weights."""
+    near, first = _window(window, sinks, "tree_attention")
+    # (an address that only says that there are weights; each stream has a slot)
+    bound = _BOUND.pack(near, first, 4 if weights else 0, 0, 0, 0, streams, 0) if near or weights else None
+    return int(_tree_bytes(_TREE.pack(streams, streams, max_new, max_context, H, H_kv, d, _tag(dtype, "tree_attention"), 1.0, page_tokens, 1,
+                                      -(-max_context // page_tokens), 0, *_NO_TENSORS), bound))

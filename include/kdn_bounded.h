@@ -45,6 +45,61 @@ size_t kdn_tree_attn_bounded_workspace_bytes(const kdn_tree_attn_args* a, const 
                                                                          and whether there are weights */
 int kdn_tree_attn_bounded(const kdn_tree_attn_args* a, const kdn_tree_bound_args* b, void* stream);
 
+/* ---- What each key of a prompt got -------------------------------------------------------------------------------
+ * weights[slot of b][e][j] = the sum, over the query rows of sequence b that see its key j and the query heads of key head e, of
+ * exp(scale q.k - lse): with kdn_attn_fwd's lse, the column sums of its softmax.  Rows and offsets as there (the rows may be the
+ * last ones of a sequence alone), window as above, 0: none.  With `add` the keys before a sequence's first row (j < len_k - len_q),
+ * whose earlier rows' weights are there already, are added to; all others are set.  Places past `places`, and slots out of range,
+ * are skipped; slots are distinct.  Summed in a fixed order. */
+typedef struct kdn_attn_weights_args {
+  int64_t num_seqs, total_q, total_k;
+  int64_t H, H_kv;
+  int d, dtype, add;
+  float scale;
+  int64_t window, sinks;
+  const int64_t* cu_q;          /* device [num_seqs + 1] */
+  const int64_t* cu_k;          /* device [num_seqs + 1]; NULL: cu_q */
+  const void* q; int64_t q_stride[2];   /* [token][head] */
+  const void* k; int64_t k_stride[2];
+  const float* lse;             /* [H][total_q] */
+  float* weights; int64_t weights_stride[2];  /* [slot][head], places next to one another */
+  int64_t places, num_slots;
+  const int32_t* slots;         /* device [num_seqs]: a sequence's slot; NULL: its number */
+  void* workspace; size_t workspace_bytes;
+} kdn_attn_weights_args;
+size_t kdn_attn_weights_workspace_bytes(const kdn_attn_weights_args* a);   /* 0: invalid; reads sizes only, and whether there are slots */
+int kdn_attn_weights(const kdn_attn_weights_args* a, void* stream);
+
+/* ---- Eviction ----------------------------------------------------------------------------------------------------
+ * Cuts each stream's cache from L = lens[b] places to N = min(L, keep[b]), of each layer and key head on its own.  Place j of a
+ * stream holds the token at position positions[slot][layer][head][j] if j < settled[b], else j + evicted[b] (what a stream's
+ * tokens so far are more than its places).  Of the places stay: those of positions below `sinks`, then those of the last `recent` of
+ * the L + evicted[b] positions, then those of largest weight (a weight that is no positive number counts as 0); of equals the
+ * lowest.  The kept places from N on move, in order, to the given-up ones before it, in order: key, value, weight and position;
+ * afterwards positions[0 .. N) are all there (settled is N, evicted L - N more).  What lies from N on is left as it is.
+ * The pages of places below N are the stream's own: no other stream has them.  Slots out of range are skipped; slots and pages are
+ * distinct.  Needs max_len >= every lens[b] (longer ones are cut), `places` and the page table's room for it. */
+typedef struct kdn_evict_args {
+  int64_t num_seqs, layers, H_kv;
+  int d, dtype;
+  int64_t page_tokens, num_pages, table_width, table_stride;
+  int64_t max_len, sinks, recent;
+  const int32_t* page_table;    /* device [num_seqs][table_width], rows table_stride apart */
+  const int32_t* lens;          /* device [num_seqs] */
+  const int32_t* keep;          /* device [num_seqs] */
+  const int32_t* settled;       /* device [num_seqs], or NULL: 0 */
+  const int32_t* evicted;       /* device [num_seqs], or NULL: 0 */
+  const int32_t* slots;         /* device [num_seqs]: a stream's slot; NULL: its number */
+  void* k_pages; int64_t k_pages_stride[4];      /* [page][layer][head][token] */
+  void* v_pages; int64_t v_pages_stride[4];
+  float* weights; int64_t weights_stride[3];     /* [slot][layer][head], places next to one another */
+  int32_t* positions; int64_t positions_stride[3];
+  int64_t places, num_slots;
+  void* workspace; size_t workspace_bytes;       /* 16-byte aligned */
+} kdn_evict_args;
+size_t kdn_evict_workspace_bytes(const kdn_evict_args* a);   /* 0: invalid; reads sizes only, and whether there are slots */
+int kdn_evict(const kdn_evict_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,224 @@
+// The attention weight that each key of a packed batch got: w_ej = sum over the rows i that see key j and the query heads h that share
+// key head e of exp(scale q_ih.k_je - lse_hi), the column sums of the softmax, for a cache that keeps the keys of largest weight.
+//
+// As dk's and dv's walk without their products (kdn_attn_bwd.hip): a wave owns 32 keys, or two times 32, with their K fragments in
+// registers, and the query rows of the heads pass through LDS in tiles of 64; S = Q K^T has a key a lane and its rows in the lane's
+// registers, so that a column's sum is register arithmetic and one exchange between the halves of the wave.
+#include <algorithm>
+#include <cmath>
+#include "kdn_attn_tile.hpp"
+
+namespace kdn {
+
+struct WeightsParams {
+  AttnParams a;        // q, k, their strides, lse, offsets, heads, scale, window
+  float* weights;      // [slot][key head], places next to one another
+  int64_t weights_stride[2], places, num_slots;
+  const int32_t* slots;
+  float* part;         // [part][key head][total_k], or NULL: the sums go to their places at once
+  int parts, add;
+};
+
+template <class P>
+struct WeightsTile {
+  static constexpr int BLOCKS = P::ROW <= 256 ? 2 : 1;  // of 32 keys to a wave: as many as leave the registers of two waves a SIMD
+  static constexpr int KEYS = 128 * BLOCKS, ROWS = 64, TILE = ROWS * P::ROW, SLOT = TILE + ROWS * 4;
+};
+
+// A key's sum to its place: those before the sequence's first row are added to if the call says so, others are set.
+__device__ __forceinline__ void put_weight(const WeightsParams& p, int seq, int e, int key, int off, float sum) {
+  if (seq < 0 || seq >= p.a.nseq || key >= p.places) return;
+  const int64_t slot = p.slots ? p.slots[seq] : seq;
+  if (slot < 0 || slot >= p.num_slots) return;
+  float* w = p.weights + slot * p.weights_stride[0] + e * p.weights_stride[1] + key;
+  *w = p.add && key < off ? *w + sum : sum;
+}
+
+// `parts` workgroups share the tiles of query rows of a tile of keys evenly, each the next stretch of them.
+template <class P, bool WIN>
+__global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) attn_weights_kernel(WeightsParams wp, int64_t slots) {
+  typedef typename P::elem E;
+  typedef WeightsTile<P> S;
+  constexpr int KS = P::D / 16, BLOCKS = S::BLOCKS, ROWS = S::ROWS;
+  __shared__ __attribute__((aligned(256))) unsigned char lds[2 * S::SLOT];
+  const AttnParams& p = wp.a;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int e = blockIdx.x % p.KV, part = blockIdx.x / p.KV % wp.parts;
+  const SeqTile t = find_heavy<S::KEYS, true>(p.cu_k, p.nseq, p.total_k, blockIdx.x / p.KV / wp.parts, slots, lane);
+  if (t.row0 < 0) return;
+  const int lenk = t.len;
+  int64_t qlo;
+  int lenq;
+  other_rows(p.cu_q, p.nseq, p.total_q, t.seq, qlo, lenq);
+  const int off = lenk - lenq;
+  const int first_key = t.row0 + 32 * BLOCKS * w, key = first_key + (lane & 31);
+  typename P::frag k[BLOCKS][KS];
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) {
+    const E* src = reinterpret_cast<const E*>(p.k) + (t.lo + min(key + 32 * b, lenk - 1)) * p.ks[0] + (int64_t)e * p.ks[1];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) k[b][ks] = P::load(src + 16 * ks + 8 * half);
+  }
+  float sum[BLOCKS];
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) sum[b] = 0.f;
+  const float c = p.scale * LOG2E;
+
+  // the rows that see a key of the tile; past the window only the sinks are seen
+  const int q0 = max(t.row0 - off, 0) / ROWS * ROWS;
+  const int q1 = WIN && t.row0 >= p.sinks ? min(lenq, max(t.row0 + S::KEYS - 1 - off + p.window, 0)) : lenq;
+  const int per = q0 < q1 ? (q1 - q0 + ROWS - 1) / ROWS : 0;
+  const int64_t all = (int64_t)per * p.G;
+  const int j0 = (int)(all * part / wp.parts), j1 = (int)(all * (part + 1) / wp.parts);
+  const Stager<P, ROWS, 4> stage_q(p.qs[0], w, lane);
+  auto stage = [&](int j, unsigned char* to) {
+    const int h = e * p.G + j / per, r0 = q0 + j % per * ROWS, last = min(lenq - 1 - r0, ROWS - 1);
+    stage_q(reinterpret_cast<const E*>(p.q) + (qlo + r0) * p.qs[0] + (int64_t)h * p.qs[1], last, to);
+    if (w == 0) copy4_to_lds(buffer_at(p.lse + (int64_t)h * p.total_q + qlo + r0), 4 * min(lane, last), to + S::TILE);
+  };
+  auto step = [&](int j, const unsigned char* __restrict qt, unsigned char* __restrict next) {
+    if (j + 1 < j1) stage(j + 1, next);
+    const float* lse = reinterpret_cast<const float*>(qt + S::TILE);
+#pragma unroll
+    for (int u = 0; u < ROWS / 32; ++u) {
+      const int i0 = q0 + j % per * ROWS + 32 * u;  // the rows i0 .. i0 + 31
+      if (i0 >= lenq || i0 + 31 + off < first_key) continue;
+      if (WIN && window_hides(i0 + off, first_key, first_key + 32 * BLOCKS - 1, p.window, p.sinks)) continue;
+      f32x16 s[BLOCKS];
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) s[b] = zero16();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const typename P::frag a = P::row_frag(qt, 32 * u + (lane & 31), ks, half);
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) s[b] = P::mma(s[b], a, k[b][ks]);
+      }
+      float l[16];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(lse + 32 * u + 8 * a + 4 * half);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) l[4 * a + y] = x[y] * -LOG2E;
+      }
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        const int fk = first_key + 32 * b, kk = key + 32 * b;
+        const bool whole = i0 + off >= fk + 31 && i0 + 32 <= lenq && !(WIN && window_cuts(i0 + 31 + off, fk, fk + 31, p.window, p.sinks));
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum[b] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, l[i]));
+        } else {
+          const int lo = max(kk - off, 0) - i0, hi = (WIN && kk >= p.sinks ? min(lenq, kk - off + p.window) : lenq) - i0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int r = rho(half, i);
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, l[i]));
+            sum[b] += r >= lo && r < hi ? x : 0.f;
+          }
+        }
+      }
+    }
+  };
+  if (j0 < j1) stage(j0, lds);
+  for (int j = j0; j < j1; ++j) {
+    staged_barrier();
+    step(j, lds + ((j - j0) & 1) * S::SLOT, lds + ((j - j0 + 1) & 1) * S::SLOT);
+  }
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) {
+    const int kk = key + 32 * b;
+    const float x = half_sum(sum[b]);
+    if (half != 0 || kk >= lenk) continue;
+    if (wp.part) wp.part[((int64_t)part * p.KV + e) * p.total_k + t.lo + kk] = x;
+    else put_weight(wp, t.seq, e, kk, off, x);
+  }
+}
+
+// The parts' sums in order, a thread a key.
+__global__ void __launch_bounds__(256) attn_weights_join_kernel(WeightsParams wp) {
+  const AttnParams& p = wp.a;
+  const int e = blockIdx.x % p.KV;
+  const SeqTile t = find_tile<256>(p.cu_k, p.nseq, p.total_k, blockIdx.x / p.KV, threadIdx.x & 63);
+  if (t.row0 < 0) return;
+  const int key = t.row0 + (int)threadIdx.x;
+  if (key >= t.len) return;
+  int64_t qlo;
+  int lenq;
+  other_rows(p.cu_q, p.nseq, p.total_q, t.seq, qlo, lenq);
+  float sum = 0.f;
+  for (int i = 0; i < wp.parts; ++i) sum += wp.part[((int64_t)i * p.KV + e) * p.total_k + t.lo + key];
+  put_weight(wp, t.seq, e, key, t.len - lenq, sum);
+}
+
+static int weights_check(const kdn_attn_weights_args* a) {
+  if (!a || a->num_seqs < 0 || a->total_q < 0 || a->total_k < 0 || a->H <= 0 || a->H_kv <= 0 || a->H > (1 << 20) || a->H % a->H_kv != 0 ||
+      !valid_dtype(a->dtype) || !(a->scale > 0.f) || !std::isfinite(a->scale) || a->window < 0 || a->sinks < 0 || a->places < 0 || a->num_slots < 0)
+    return KDN_ERR_INVALID_ARGUMENT;
+  if ((a->d != 64 && a->d != 128) || a->total_q > (1 << 30) || a->total_k > (1 << 30) || a->num_seqs > (1 << 30) || a->num_slots > INT32_MAX)
+    return KDN_ERR_UNSUPPORTED;
+  if ((!a->cu_k && a->total_k != a->total_q) || (!a->slots && a->num_slots < a->num_seqs)) return KDN_ERR_INVALID_ARGUMENT;
+  return KDN_OK;
+}
+
+static int weights_keys(const kdn_attn_weights_args* a) { return a->d * (int)dtype_size(a->dtype) <= 256 ? 256 : 128; }
+
+// Workgroups that share a tile of keys: enough that there are 2048 (the first keys have twice the average's work), but none
+// without a tile of an average sequence's rows.
+static int weights_parts(const kdn_attn_weights_args* a) {
+  const int64_t tiles = tile_slots(a->total_k, weights_keys(a), a->num_seqs) * a->H_kv;
+  const int64_t rows = (a->total_q / std::max<int64_t>(a->num_seqs, 1) / 64 + 1) * (a->H / a->H_kv);
+  return (int)std::max<int64_t>(1, std::min<int64_t>({(2048 + tiles - 1) / tiles, rows, 16}));
+}
+
+template <class P>
+static int launch_weights(const WeightsParams& p, hipStream_t st) {
+  const int64_t slots = tile_slots(p.a.total_k, WeightsTile<P>::KEYS, p.a.nseq), grid = slots * p.a.KV * p.parts;
+  const int64_t joins = p.parts > 1 ? tile_slots(p.a.total_k, 256, p.a.nseq) * p.a.KV : 0;
+  if (grid > INT32_MAX || joins > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  if (p.a.window < NO_WINDOW) hipLaunchKernelGGL((attn_weights_kernel<P, true>), dim3((unsigned)grid), dim3(256), 0, st, p, slots);
+  else hipLaunchKernelGGL((attn_weights_kernel<P, false>), dim3((unsigned)grid), dim3(256), 0, st, p, slots);
+  if (joins > 0) hipLaunchKernelGGL(attn_weights_join_kernel, dim3((unsigned)joins), dim3(256), 0, st, p);
+  return launch_status();
+}
+
+}  // namespace kdn
+
+using namespace kdn;
+
+extern "C" size_t kdn_attn_weights_workspace_bytes(const kdn_attn_weights_args* a) {
+  if (weights_check(a) != KDN_OK) return 0;
+  const size_t parts = (size_t)weights_parts(a);
+  return parts > 1 ? parts * (size_t)a->H_kv * (size_t)a->total_k * 4 : 4;
+}
+
+extern "C" int kdn_attn_weights(const kdn_attn_weights_args* a, void* stream) {
+  int rc = weights_check(a);
+  if (rc != KDN_OK) return rc;
+  if (a->total_k == 0 || a->num_seqs == 0) return KDN_OK;
+  if (!a->cu_q || !a->k || (a->total_q > 0 && (!a->q || !a->lse)) || (a->num_slots > 0 && a->places > 0 && !a->weights)) return KDN_ERR_INVALID_ARGUMENT;
+  if (!aligned(a->q, 16) || !aligned(a->k, 16) || !aligned(a->lse, 4) || !aligned(a->weights, 4) || !aligned(a->slots, 4) ||
+      !aligned(a->workspace, 4) || !attn_strides_ok(a->q_stride, a->dtype) || !attn_strides_ok(a->k_stride, a->dtype))
+    return KDN_ERR_MISALIGNED;
+  if (!stage_reach(a->q_stride[0], a->dtype)) return KDN_ERR_UNSUPPORTED;
+  WeightsParams p = {};
+  p.parts = weights_parts(a);
+  if (p.parts > 1 && (!a->workspace || a->workspace_bytes < kdn_attn_weights_workspace_bytes(a))) return KDN_ERR_WORKSPACE_TOO_SMALL;
+  p.a.q = a->q; p.a.k = a->k;
+  for (int i = 0; i < 2; ++i) {
+    p.a.qs[i] = a->q_stride[i]; p.a.ks[i] = a->k_stride[i]; p.weights_stride[i] = a->weights_stride[i];
+  }
+  p.a.lse = const_cast<float*>(a->lse);
+  p.a.cu_q = a->cu_q;
+  p.a.cu_k = a->cu_k ? a->cu_k : a->cu_q;
+  p.a.nseq = a->num_seqs; p.a.total_q = a->total_q; p.a.total_k = a->total_k;
+  p.a.H = (int)a->H; p.a.KV = (int)a->H_kv; p.a.G = (int)(a->H / a->H_kv);
+  p.a.scale = a->scale;
+  attn_window(p.a, a->window > 0 ? a->window : NO_WINDOW, a->sinks);
+  p.weights = a->weights; p.places = a->places; p.num_slots = a->num_slots; p.slots = a->slots;
+  p.part = p.parts > 1 ? reinterpret_cast<float*>(a->workspace) : nullptr;
+  p.add = a->add != 0;
+  hipStream_t st = as_stream(stream);
+  if (a->dtype == KDN_DTYPE_BF16) return a->d == 64 ? launch_weights<AttnBF16<64>>(p, st) : launch_weights<AttnBF16<128>>(p, st);
+  return a->d == 64 ? launch_weights<AttnF32<64>>(p, st) : launch_weights<AttnF32<128>>(p, st);
+}

@@ -94,6 +94,10 @@ BOUNDED_EXPORTED = (
     "kdn_attn_window_bwd",
     "kdn_tree_attn_bounded_workspace_bytes",
     "kdn_tree_attn_bounded",
+    "kdn_attn_weights_workspace_bytes",
+    "kdn_attn_weights",
+    "kdn_evict_workspace_bytes",
+    "kdn_evict",
 )
 
 KDN_ERR_CAPACITY = -6
@@ -297,6 +301,43 @@ class TreeBoundArgs(ctypes.Structure):
     ]
 
 
+class AttnWeightsArgs(ctypes.Structure):
+    """Mirror of struct kdn_attn_weights_args (include/kdn_bounded.h)."""
+
+    _fields_ = [
+        ("num_seqs", _i64), ("total_q", _i64), ("total_k", _i64), ("H", _i64), ("H_kv", _i64),
+        ("d", ctypes.c_int), ("dtype", ctypes.c_int), ("add", ctypes.c_int), ("scale", ctypes.c_float),
+        ("window", _i64), ("sinks", _i64),
+        ("cu_q", ctypes.c_void_p), ("cu_k", ctypes.c_void_p),
+        ("q", ctypes.c_void_p), ("q_stride", _i64x2),
+        ("k", ctypes.c_void_p), ("k_stride", _i64x2),
+        ("lse", ctypes.c_void_p),
+        ("weights", ctypes.c_void_p), ("weights_stride", _i64x2),
+        ("places", _i64), ("num_slots", _i64),
+        ("slots", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class EvictArgs(ctypes.Structure):
+    """Mirror of struct kdn_evict_args (include/kdn_bounded.h)."""
+
+    _fields_ = [
+        ("num_seqs", _i64), ("layers", _i64), ("H_kv", _i64),
+        ("d", ctypes.c_int), ("dtype", ctypes.c_int),
+        ("page_tokens", _i64), ("num_pages", _i64), ("table_width", _i64), ("table_stride", _i64),
+        ("max_len", _i64), ("sinks", _i64), ("recent", _i64),
+        ("page_table", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("keep", ctypes.c_void_p),
+        ("settled", ctypes.c_void_p), ("evicted", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+        ("k_pages", ctypes.c_void_p), ("k_pages_stride", _i64x4),
+        ("v_pages", ctypes.c_void_p), ("v_pages_stride", _i64x4),
+        ("weights", ctypes.c_void_p), ("weights_stride", _i64x3),
+        ("positions", ctypes.c_void_p), ("positions_stride", _i64x3),
+        ("places", _i64), ("num_slots", _i64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 def _declare_anchor(L: ctypes.CDLL) -> None:
     """Argument and result types of include/kdn_anchor.h and include/kdn_bounded.h."""
     vp, i64, ci, sz, ptr = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t, ctypes.POINTER
@@ -330,7 +371,11 @@ def _declare_anchor(L: ctypes.CDLL) -> None:
             ("kdn_attn_window_bwd_workspace_bytes", [vp, i64, i64], sz),
             ("kdn_attn_window_bwd", [vp, i64, i64, vp], ci),
             ("kdn_tree_attn_bounded_workspace_bytes", [vp, vp], sz),
-            ("kdn_tree_attn_bounded", [vp, vp, vp], ci)):
+            ("kdn_tree_attn_bounded", [vp, vp, vp], ci),
+            ("kdn_attn_weights_workspace_bytes", [vp], sz),
+            ("kdn_attn_weights", [vp, vp], ci),
+            ("kdn_evict_workspace_bytes", [vp], sz),
+            ("kdn_evict", [vp, vp], ci)):
         fn = getattr(L, name)
         fn.argtypes, fn.restype = args, res
 

@@ -16,7 +16,7 @@ PKG_ROOT = os.path.dirname(_HERE)
 CSRC = os.path.join(PKG_ROOT, "csrc")
 SOURCES = ["kdn_api.hip", "kdn_lift.hip", "kdn_prep.hip", "kdn_scan.hip", "kdn_chain.hip", "kdn_serve.hip", "kdn_pool.hip",
            "kdn_bwd.hip", "kdn_general.hip", "kdn_noalloc.hip", "kdn_frep.hip", "kdn_attn.hip", "kdn_attn_bwd.hip",
-           "kdn_rotary.hip", "kdn_pages.hip", "kdn_tree.hip"]
+           "kdn_rotary.hip", "kdn_pages.hip", "kdn_tree.hip", "kdn_weights.hip", "kdn_evict.hip"]
 OUT = os.path.join(_HERE, "libkdn.so")
 OBJDIR = os.path.join(_HERE, "_build")
 ARCH = "gfx950"

@@ -100,6 +100,15 @@ typedef struct kdn_evict_args {
 size_t kdn_evict_workspace_bytes(const kdn_evict_args* a);   /* 0: invalid; reads sizes only, and whether there are slots */
 int kdn_evict(const kdn_evict_args* a, void* stream);
 
+/* ---- The pages' bookkeeping for it (host only, as kdn_page_pool_*) -------------------------------------------------- */
+/* The pages of the stream's first `tokens` tokens become its own: each that another stream has is replaced, and pairs[0 .. 2 n) are
+ * the copies to make before anything is written; n is returned (KDN_ERR_CAPACITY, and nothing changed, if it is over room or the
+ * free pages). */
+int64_t kdn_page_pool_own(kdn_page_pool* pool, int stream, int64_t tokens, int32_t* pairs, int64_t room);
+/* Takes the full pages first .. first + pages - 1 out of the stream: those behind them move up, and the stream is pages *
+ * page_tokens shorter (what no window reaches any more). */
+int kdn_page_pool_drop(kdn_page_pool* pool, int stream, int64_t first, int64_t pages);
+
 #ifdef __cplusplus
 }
 #endif

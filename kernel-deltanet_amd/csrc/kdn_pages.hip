@@ -7,7 +7,7 @@
 #include <vector>
 #include "kdn_io.hpp"
 #include "kdn_internal.hpp"
-#include "../../include/kdn_anchor.h"
+#include "../../include/kdn_bounded.h"
 
 namespace kdn {
 
@@ -315,6 +315,37 @@ extern "C" int64_t kdn_page_pool_compact(kdn_page_pool* pool, int32_t* pairs, in
     for (int64_t page = pool->num_pages; page-- > used;) pool->free_pages.push_back((int32_t)page);
     return moves;
   });
+}
+
+extern "C" int64_t kdn_page_pool_own(kdn_page_pool* pool, int stream, int64_t tokens, int32_t* pairs, int64_t room) {
+  kdn_page_pool::Stream* s = pool ? pool->at(stream) : nullptr;
+  if (!s || tokens < 0 || tokens > s->tokens || room < 0 || (room > 0 && !pairs)) return KDN_ERR_INVALID_ARGUMENT;
+  const size_t n = (size_t)((tokens + pool->page_tokens - 1) / pool->page_tokens);
+  int64_t shared = 0;
+  for (size_t i = 0; i < n; ++i) shared += pool->shares[(size_t)s->pages[i]] > 1;
+  if (shared > room || shared > (int64_t)pool->free_pages.size()) return KDN_ERR_CAPACITY;
+  int64_t at = 0;
+  for (size_t i = 0; i < n; ++i) {
+    const int32_t from = s->pages[i];
+    if (pool->shares[(size_t)from] == 1) continue;
+    const int32_t to = pool->free_pages.back();
+    pool->free_pages.pop_back();
+    pairs[2 * at] = from, pairs[2 * at + 1] = to;
+    ++at;
+    --pool->shares[(size_t)from];  // over one before
+    pool->shares[(size_t)to] = 1;
+    s->pages[i] = to;
+  }
+  return at;
+}
+
+extern "C" int kdn_page_pool_drop(kdn_page_pool* pool, int stream, int64_t first, int64_t pages) {
+  kdn_page_pool::Stream* s = pool ? pool->at(stream) : nullptr;
+  if (!s || first < 0 || pages < 0 || first > s->tokens / pool->page_tokens - pages) return KDN_ERR_INVALID_ARGUMENT;
+  for (int64_t i = first + pages; i-- > first;) pool->drop(s->pages[(size_t)i]);
+  s->pages.erase(s->pages.begin() + first, s->pages.begin() + first + pages);
+  s->tokens -= pages * pool->page_tokens;
+  return KDN_OK;
 }
 
 extern "C" int64_t kdn_page_pool_free(const kdn_page_pool* pool) { return pool ? (int64_t)pool->free_pages.size() : 0; }

@@ -98,6 +98,8 @@ BOUNDED_EXPORTED = (
     "kdn_attn_weights",
     "kdn_evict_workspace_bytes",
     "kdn_evict",
+    "kdn_page_pool_own",
+    "kdn_page_pool_drop",
 )
 
 KDN_ERR_CAPACITY = -6
@@ -375,7 +377,9 @@ def _declare_anchor(L: ctypes.CDLL) -> None:
             ("kdn_attn_weights_workspace_bytes", [vp], sz),
             ("kdn_attn_weights", [vp, vp], ci),
             ("kdn_evict_workspace_bytes", [vp], sz),
-            ("kdn_evict", [vp, vp], ci)):
+            ("kdn_evict", [vp, vp], ci),
+            ("kdn_page_pool_own", [vp, ci, i64, vp, i64], i64),
+            ("kdn_page_pool_drop", [vp, ci, i64, i64], ci)):
         fn = getattr(L, name)
         fn.argtypes, fn.restype = args, res
 

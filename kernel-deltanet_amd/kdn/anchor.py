@@ -3,7 +3,7 @@ its recurrent ones, and the pages their keys and values live in.
 
     rotary            positions of q and k, with gradients
     attention         causal attention over packed prompts with grouped heads, whole or in a window, with gradients
-    PagePool          which pages a stream's tokens lie on: fork, extend, truncate, compact, free (host)
+    PagePool          which pages a stream's tokens lie on: fork, extend, truncate, own, drop, compact, free (host)
     page_copy         whole pages (forks about to write, compaction)
     page_append       new tokens' keys and values into their pages
     tree_attention    one new token a stream, a run of them, or a tree of drafts, over the pages, whole or in a window; and what
@@ -494,6 +494,16 @@ class PagePool:
         """Moves the pages in use to the lowest numbers: the copies to make, (n, 2) int32, before anything else."""
         pairs = torch.empty(self.num_pages, 2, dtype=torch.int32)
         return pairs[:self._num(N.lib().kdn_page_pool_compact(self._h, pairs.data_ptr(), self.num_pages), "kdn_page_pool_compact")]
+
+    def own(self, stream: int, tokens: int) -> torch.Tensor:
+        """The pages of the stream's first `tokens` tokens become its own (`evict` writes them): the copies to make, (n, 2) int32,
+        before anything is written."""
+        pairs = torch.empty(-(-max(tokens, 0) // self.page_tokens), 2, dtype=torch.int32)
+        return pairs[:self._num(N.lib().kdn_page_pool_own(self._h, stream, tokens, pairs.data_ptr(), pairs.shape[0]), "kdn_page_pool_own")]
+
+    def drop(self, stream: int, first: int, pages: int) -> None:
+        """Takes full pages out of the stream, from its page `first` on; the ones behind move up."""
+        self._num(N.lib().kdn_page_pool_drop(self._h, stream, first, pages), "kdn_page_pool_drop")
 
     @property
     def used(self) -> int:

@@ -7,6 +7,10 @@ of kdn.anchor.
     .step(x, plan, k_pages, v_pages)   serving: new tokens of streams whose keys and values live in pages
                                        (HybridMemoryPool.anchor_plan); one token a stream, a run of them, or a tree of drafts
 
+A layer with a `window` sees the last `window` positions and the first `sinks` alone (HybridMemoryPool.anchor_slide frees the pages
+between).  A step that is given the pool's weights (HybridMemoryPool.anchor_weights) adds to them what each key gets, by which
+HybridMemoryPool.anchor_evict chooses what stays.
+
 The reference keeps pages for such layers (serving/hybrid_memory_pool.{h,cpp}) and leaves the layers to its host framework.
 """
 from __future__ import annotations
@@ -16,7 +20,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 
-from kdn import anchor
+from kdn import anchor, bounded
 
 _RUN = 64  # new tokens that tree_attention takes of a stream
 
@@ -24,8 +28,10 @@ _RUN = 64  # new tokens that tree_attention takes of a stream
 class AnchorAttentionLayer(nn.Module):
     def __init__(self, d_model: int, num_heads: int, num_kv_heads: Optional[int] = None, d_head: Optional[int] = None,
                  rotary_dim: Optional[int] = None, interleaved: bool = False, base: float = 10000.0, scaling: str = "none",
-                 factor: float = 1.0, trained_length: int = 4096):
+                 factor: float = 1.0, trained_length: int = 4096, window: Optional[int] = None, sinks: int = 0):
         super().__init__()
+        anchor._window(window, sinks, "AnchorAttentionLayer")
+        self.window, self.sinks = window, sinks
         self.num_heads, self.num_kv_heads = num_heads, num_heads if num_kv_heads is None else num_kv_heads
         self.d_head = d_model // num_heads if d_head is None else d_head
         if self.d_head not in (64, 128) or num_heads % self.num_kv_heads:
@@ -87,26 +93,39 @@ class AnchorAttentionLayer(nn.Module):
             t = torch.arange(x.shape[0], device=x.device)
             at = t - cu[(torch.bucketize(t, cu, right=True) - 1).clamp(min=0)]
         q, k, v = self._project(flat, at)
-        y = anchor.attention(q, k, v, cu)
+        y = anchor.attention(q, k, v, cu, window=self.window, sinks=self.sinks)
         return self.w_out(y.view(-1, self.num_heads * self.d_head)).view(x.shape)
 
     @torch.no_grad()
-    def step(self, x: torch.Tensor, plan, k_pages: torch.Tensor, v_pages: torch.Tensor, parents: Optional[torch.Tensor] = None):
+    def step(self, x: torch.Tensor, plan, k_pages: torch.Tensor, v_pages: torch.Tensor, parents: Optional[torch.Tensor] = None,
+             weights: Optional[torch.Tensor] = None):
         """x (tokens, d_model), the new tokens of plan's streams, against this layer's pages.  Returns the layer's output; for
         a plan of drafts (`keep` false) (output, k, v), of which the caller puts the accepted ones into the pages
-        (anchor.page_append at the rows of a plan made for them)."""
+        (anchor.page_append at the rows of a plan made for them).  `weights`: this layer's, to be added to (drafts add nothing)."""
+        if self.window is not None and not plan.in_order:
+            raise ValueError("AnchorAttentionLayer: a window has no meaning over places that an eviction has filled out of order")
+        weights = weights if plan.keep else None
+        if weights is not None and plan.slots is None:
+            raise ValueError("AnchorAttentionLayer: the plan's pool keeps no weights")
         q, k, v = self._project(x, plan.positions)
         if plan.keep:
             anchor.page_append(k, v, k_pages, v_pages, plan.rows)
-        if plan.max_new <= _RUN:
+        how = dict(window=self.window, sinks=self.sinks)
+        if plan.max_new <= (_RUN if weights is None else plan.run):
             y = anchor.tree_attention(q, k, v, k_pages, v_pages, plan.page_table, plan.context_lens, plan.cu_seqlens, parents,
-                                      max_context=plan.max_context, max_new=plan.max_new)
+                                      max_context=plan.max_context, max_new=plan.max_new, weights=weights,
+                                      slots=None if weights is None else plan.slots, **how)
         elif parents is not None or not plan.keep:
             raise ValueError(f"AnchorAttentionLayer: at most {_RUN} drafts a stream, got {plan.max_new}")
-        elif plan.max_context == 0:
-            y = anchor.attention(q, k, v, plan.cu_seqlens)
-        else:  # a prompt's next piece: its stream's keys so far out of the pages
-            page, off = plan.all_rows // k_pages.shape[2], plan.all_rows % k_pages.shape[2]
-            y = anchor.attention(q, k_pages[page, :, off], v_pages[page, :, off], plan.cu_seqlens, plan.cu_all)
+        else:
+            cu_all = None
+            if plan.max_context > 0:  # a prompt's next piece: its stream's keys so far out of the pages
+                page, off = plan.all_rows // k_pages.shape[2], plan.all_rows % k_pages.shape[2]
+                k, v, cu_all = k_pages[page, :, off], v_pages[page, :, off], plan.cu_all
+            if weights is None:
+                y = anchor.attention(q, k, v, plan.cu_seqlens, cu_all, **how)
+            else:
+                y, lse = anchor.attention_forward(q, k, v, plan.cu_seqlens, cu_all, return_lse=True, **how)
+                bounded.attention_weights(q, k, lse, weights, plan.cu_seqlens, cu_all, add=True, slots=plan.slots, **how)
         out = self.w_out(y.view(-1, self.num_heads * self.d_head))
         return out if plan.keep else (out, k, v)

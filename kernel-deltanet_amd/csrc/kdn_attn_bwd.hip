@@ -66,7 +66,7 @@ __device__ __forceinline__ const AttnParams& params_here() {
 // Under a window (WIN) the rows that see a tile of keys end `window` behind it, but for the first `sinks` keys, which all later
 // rows see: one workgroup that walked them all would run on when the others are done (a sequence of 65536 rows and a window of
 // 1024: fifty times as long).  So those rows are cut into segments of FAR_ROWS, a workgroup each, whose sums of the sinks' dk and
-// dv come to lie apart in fp32; attn_sinks_kernel adds them to the subsets' sums in a fixed order.
+// dv come to lie apart in fp32, as the near rows' do a second time; attn_sinks_kernel adds them in a fixed order.
 constexpr int FAR_ROWS = 1024;
 // The query rows [from, to) of a sequence that see keys of the tile row0 .. row0 + keys - 1 for nearness, in whole tiles of `rows`.
 // Those from `to` on see of it the sinks alone.
@@ -248,15 +248,18 @@ __device__ __forceinline__ void dkdv(int id, int slots, int far, unsigned char* 
   }
   const AttnParams& out = params_here();
   const int64_t at = t.lo + key, part_at = (((int64_t)sub * out.total_k + at) * out.KV + e) * P::D;
-  const int64_t far_at = ((((int64_t)far_slot * out.subsets + sub) * out.sinks + key) * out.KV + e) * P::D;
+  const int64_t far_at = ((((int64_t)(far_slot >= 0 ? far_slot : out.far_slots + t.seq) * out.subsets + sub) * out.sinks + key) * out.KV + e) * P::D;
+  const bool sinks = t.row0 < out.sinks && (far_slot >= 0 || (t.seq >= 0 && t.seq < out.nseq));  // (keys outside the offsets have none)
   auto store_k = [&](int ct, const f32x16& x, float f) {
-    if (WIN && far_slot >= 0) store_row32(out.far_dk + far_at + 32 * ct, x, f, half, live && key < out.sinks);
-    else if (out.subsets > 1 || (WIN && out.sinks > 0)) store_row32(out.part_dk + part_at + 32 * ct, x, f, half, live);
+    if (WIN && sinks) store_row32(out.far_dk + far_at + 32 * ct, x, f, half, live && key < out.sinks);
+    if (WIN && far_slot >= 0) return;
+    if (out.subsets > 1) store_row32(out.part_dk + part_at + 32 * ct, x, f, half, live);
     else store_row32(reinterpret_cast<E*>(out.dk) + at * out.dks[0] + (int64_t)e * out.dks[1] + 32 * ct, x, f, half, live);
   };
   auto store_v = [&](int ct, const f32x16& x) {
-    if (WIN && far_slot >= 0) store_row32(out.far_dv + far_at + 32 * ct, x, 1.f, half, live && key < out.sinks);
-    else if (out.subsets > 1 || (WIN && out.sinks > 0)) store_row32(out.part_dv + part_at + 32 * ct, x, 1.f, half, live);
+    if (WIN && sinks) store_row32(out.far_dv + far_at + 32 * ct, x, 1.f, half, live && key < out.sinks);
+    if (WIN && far_slot >= 0) return;
+    if (out.subsets > 1) store_row32(out.part_dv + part_at + 32 * ct, x, 1.f, half, live);
     else store_row32(reinterpret_cast<E*>(out.dv) + at * out.dvs[0] + (int64_t)e * out.dvs[1] + 32 * ct, x, 1.f, half, live);
   };
   if constexpr (SPLIT == 1) {
@@ -289,8 +292,8 @@ __global__ void __launch_bounds__(256) attn_subsets_kernel(AttnParams p) {
   store4(reinterpret_cast<E*>(p.dv) + at * p.dvs[0] + e * p.dvs[1] + d, y);
 }
 
-// The sinks' dk and dv: the subsets' sums of the near rows, then the segments of the far ones in order.  A thread has four
-// values of one sink of one sequence and key head; `keys` and `rows` are Dkdv's.
+// The sinks' dk and dv: the sums of the near rows, then of the far ones' segments in order, of each the subsets in turn.  A thread
+// has four values of one sink of one sequence and key head; `keys` and `rows` are Dkdv's.
 template <class P>
 __global__ void __launch_bounds__(256) attn_sinks_kernel(AttnParams p, int keys, int rows) {
   typedef typename P::elem E;
@@ -305,20 +308,18 @@ __global__ void __launch_bounds__(256) attn_sinks_kernel(AttnParams p, int keys,
   other_rows(p.cu_q, p.nseq, p.total_q, (int)b, qlo, lenq);
   if (key >= lenk) return;
   f32x4 dk = zero4(), dv = zero4();
-  for (int s = 0; s < p.subsets; ++s) {
-    const int64_t at = (((int64_t)s * p.total_k + klo + key) * p.KV + e) * P::D + d;
-    dk += *reinterpret_cast<const f32x4*>(p.part_dk + at);
-    dv += *reinterpret_cast<const f32x4*>(p.part_dv + at);
-  }
-  const NearRows near(key / keys * keys, lenk - lenq, lenq, p.window, keys, rows);
-  for (int row = near.to; row < lenq; row = row / FAR_ROWS * FAR_ROWS + FAR_ROWS) {
-    const int64_t slot = qlo / FAR_ROWS + b + 1 + row / FAR_ROWS;
+  auto add = [&](int64_t slot) {
     for (int s = 0; s < p.subsets; ++s) {
       const int64_t at = (((slot * p.subsets + s) * p.sinks + key) * p.KV + e) * P::D + d;
       dk += *reinterpret_cast<const f32x4*>(p.far_dk + at);
       dv += *reinterpret_cast<const f32x4*>(p.far_dv + at);
     }
-  }
+  };
+  add(p.far_slots + b);
+  const NearRows near(key / keys * keys, lenk - lenq, lenq, p.window, keys, rows);
+  const int64_t first = qlo / FAR_ROWS + b + 1, end = near.to < lenq ? (lenq + FAR_ROWS - 1) / FAR_ROWS : 0;
+#pragma unroll 4
+  for (int64_t i = near.to / FAR_ROWS; i < end; ++i) add(first + i);
   const float x[4] = {dk[0], dk[1], dk[2], dk[3]}, y[4] = {dv[0], dv[1], dv[2], dv[3]};
   store4(reinterpret_cast<E*>(p.dk) + (klo + key) * p.dks[0] + e * p.dks[1] + d, x);
   store4(reinterpret_cast<E*>(p.dv) + (klo + key) * p.dvs[0] + e * p.dvs[1] + d, y);
@@ -471,12 +472,13 @@ static int launch_grads(const AttnParams& p, hipStream_t st) {
   hipLaunchKernelGGL((attn_grads_kernel<P, SPLIT, WIN>), dim3((unsigned)grid), dim3(256), 0, st, p, (int)slots_k, (int)slots_q, (int)part, (int)nk,
                      (int)far);
   int rc = launch_status();
-  const bool sinks = WIN && p.sinks > 0;
-  if (rc == KDN_OK && (p.subsets > 1 || sinks) && p.total_k > 0) {
+  if (rc == KDN_OK && p.subsets > 1 && p.total_k > 0) {
     const int64_t blocks = (p.total_k * p.KV * (P::D / 4) + 255) / 256;
     if (blocks > INT32_MAX) return KDN_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(attn_subsets_kernel<P>, dim3((unsigned)blocks), dim3(256), 0, st, p);
-    if ((rc = launch_status()) != KDN_OK || !sinks || p.nseq == 0) return rc;
+    rc = launch_status();
+  }
+  if (rc == KDN_OK && far > 0 && p.nseq > 0) {
     const int64_t far_blocks = (p.nseq * p.sinks * p.KV * (P::D / 4) + 255) / 256;
     if (far_blocks > INT32_MAX) return KDN_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(attn_sinks_kernel<P>, dim3((unsigned)far_blocks), dim3(256), 0, st, p, Dkdv<P, SPLIT>::KEYS, Dkdv<P, SPLIT>::ROWS);
@@ -508,20 +510,21 @@ static int launch_bwd(const AttnParams& p, float* stat, float* delta, hipStream_
 // Subsets of the query heads that share a key head whose dk and dv are summed apart: as many as it takes to have eight
 // workgroups of 128 keys for each CU (two run there at a time, and the first keys have twice the average's work).  8192 rows,
 // 32 heads over 8: four subsets 2900 us a training step, two 2935.
-static int bwd_subsets(const kdn_attn_args* f) {
+// Under a window all tiles have about the same work: four workgroups of each CU's are enough.
+static int bwd_subsets(const kdn_attn_args* f, bool window) {
   const int G = (int)(f->H / f->H_kv);
   const int64_t tiles = f->total_k / 128 * f->H_kv;
   int n = 1;
-  while (n < G && (tiles * n < 2048 || G % n != 0)) ++n;
+  while (n < G && (tiles * n < (window ? 1024 : 2048) || G % n != 0)) ++n;
   return n;
 }
 static size_t bwd_row_bytes(const kdn_attn_args* f) { return ((size_t)f->H * (size_t)f->total_q * 4 + 255) / 256 * 256 + 256; }
 static size_t bwd_part_bytes(const kdn_attn_args* f) { return (size_t)f->total_k * (size_t)f->H_kv * (size_t)f->d * 4; }
-// Of the far rows' segments, `sinks` after attn_window.
+// Of the far rows' segments and the near rows of each sequence, `sinks` after attn_window.
 static size_t bwd_far_bytes(const kdn_attn_args* f, int subsets, int64_t sinks) {
   const size_t each = (size_t)subsets * (size_t)sinks * (size_t)f->H_kv * (size_t)f->d * 4;
   size_t all;
-  return __builtin_mul_overflow((size_t)tile_slots(f->total_q, FAR_ROWS, f->num_seqs), each, &all) || all > ((size_t)1 << 48) ? (size_t)1 << 48 : all;
+  return __builtin_mul_overflow((size_t)(tile_slots(f->total_q, FAR_ROWS, f->num_seqs) + f->num_seqs), each, &all) || all > ((size_t)1 << 48) ? (size_t)1 << 48 : all;
 }
 
 }  // namespace kdn
@@ -532,8 +535,8 @@ static size_t bwd_workspace_bytes(const kdn_attn_bwd_args* a, int64_t window, in
   if (!a || attn_check(a->fwd) != KDN_OK || window < 1 || sinks < 0) return 0;
   AttnParams p = attn_params(a->fwd);
   attn_window(p, window, sinks);
-  const int subsets = bwd_subsets(a->fwd);
-  return 2 * bwd_row_bytes(a->fwd) + (subsets > 1 || p.sinks > 0 ? 2 * subsets * bwd_part_bytes(a->fwd) : 0) +
+  const int subsets = bwd_subsets(a->fwd, p.window < NO_WINDOW);
+  return 2 * bwd_row_bytes(a->fwd) + (subsets > 1 ? 2 * subsets * bwd_part_bytes(a->fwd) : 0) +
          2 * bwd_far_bytes(a->fwd, subsets, p.sinks);
 }
 
@@ -560,11 +563,12 @@ static int attn_bwd(const kdn_attn_bwd_args* a, int64_t window, int64_t sinks, v
   float *stat = reinterpret_cast<float*>(a->workspace), *delta = stat + bwd_row_bytes(f) / 4;
   p.stat = stat;
   p.delta = delta;
-  p.subsets = bwd_subsets(f);
+  attn_window(p, window, sinks);
+  p.subsets = bwd_subsets(f, p.window < NO_WINDOW);
   p.part_dk = reinterpret_cast<float*>((unsigned char*)a->workspace + 2 * bwd_row_bytes(f));
   p.part_dv = p.part_dk + (size_t)p.subsets * bwd_part_bytes(f) / 4;
-  attn_window(p, window, sinks);
-  p.far_dk = p.part_dv + (size_t)p.subsets * bwd_part_bytes(f) / 4;
+  p.far_slots = tile_slots(p.total_q, FAR_ROWS, p.nseq);
+  p.far_dk = p.subsets > 1 ? p.part_dv + (size_t)p.subsets * bwd_part_bytes(f) / 4 : p.part_dk;
   p.far_dv = p.far_dk + bwd_far_bytes(f, p.subsets, p.sinks) / 4;
   for (int i = 0; i < 2; ++i) {
     p.dys[i] = a->dy_stride[i]; p.dqs[i] = a->dq_stride[i]; p.dks[i] = a->dk_stride[i]; p.dvs[i] = a->dv_stride[i];

@@ -453,7 +453,10 @@ struct AttnParams {
   float scale;
   // under a window: the keys that a row sees besides the first `sinks` end at its own position and are `window` at most
   int window, sinks;
-  float *far_dk, *far_dv;  // [slot][subset][sink][KV][D]: what the rows of a segment behind the window give to the sinks' dk and dv
+  // [slot][subset][sink][KV][D]: what the sinks' dk and dv get from a segment of the rows behind the window, and, from slot
+  // far_slots on, from a sequence's rows before those
+  float *far_dk, *far_dv;
+  int64_t far_slots;
 };
 
 int attn_check(const kdn_attn_args* a);          // sizes

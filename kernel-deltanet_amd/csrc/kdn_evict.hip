@@ -69,15 +69,28 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_select_kernel(EvictParams
     return;
   }
   const int64_t latest = len + s.evicted - p.recent;  // positions from here on stay if they can
-  auto form = [&](int j) -> uint32_t {
-    const int64_t at = position(j);
-    const float x = weights[j];
+  auto rank_of = [&](int64_t at, float x) -> uint32_t {
     return at < p.sinks ? RANK_SINK : at >= latest ? RANK_RECENT : x > 0.f ? __builtin_bit_cast(uint32_t, x) : 0u;
   };
   const int cached = min(len, EVICT_CACHED);
-  for (int j = tid; j < cached; j += EVICT_THREADS) ranks[j] = form(j);
+  constexpr int AHEAD = 8;  // loads on their way at a time: one by one a head's 16384 places take 25 us
+  for (int j0 = tid; j0 < cached; j0 += AHEAD * EVICT_THREADS) {
+    float x[AHEAD];
+    int32_t at[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int j = min(j0 + i * EVICT_THREADS, cached - 1);
+      x[i] = weights[j];
+      at[i] = j < s.settled ? positions[j] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int j = j0 + i * EVICT_THREADS;
+      if (j < cached) ranks[j] = rank_of(j < s.settled ? at[i] : j + s.evicted, x[i]);
+    }
+  }
   __syncthreads();
-  auto rank = [&](int j) -> uint32_t { return j < EVICT_CACHED ? ranks[j] : form(j); };
+  auto rank = [&](int j) -> uint32_t { return j < EVICT_CACHED ? ranks[j] : rank_of(position(j), weights[j]); };
 
   // the rank of the kept-th place, and how many of its equals stay
   uint32_t last = 0;
@@ -168,10 +181,23 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_select_kernel(EvictParams
   }
   __syncthreads();
   const int moves = found[0];
-  for (int i = tid; i < moves; i += EVICT_THREADS) {
-    const int from = fillers[i], to = holes[i];
-    weights[to] = weights[from];
-    positions[to] = (int32_t)position(from);
+  for (int i0 = tid; i0 < moves; i0 += 4 * EVICT_THREADS) {
+    int from[4], to[4];
+    float x[4];
+    int32_t at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int m = min(i0 + i * EVICT_THREADS, moves - 1);
+      from[i] = fillers[m], to[i] = holes[m];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = weights[from[i]];
+      at[i] = (int32_t)position(from[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i0 + i * EVICT_THREADS < moves) weights[to[i]] = x[i], positions[to[i]] = at[i];
   }
 }
 

@@ -690,16 +690,23 @@ __device__ __forceinline__ void tree_weights(const TreeParams& p, int id) {
   const TreeWork t = tree_seq<WIN>(p, b);
   const int slot = p.slots ? p.slots[b] : b, most = p.max_new * p.G, rows = t.n * p.G, end = (t.ctx + 31) / 32 * 32;  // the new tokens' scores start there
   if (rows == 0 || slot < 0 || slot >= p.num_slots || part * WEIGHT_KEYS >= end + t.n) return;
-  if ((int)threadIdx.x < rows) {
-    const int64_t first = (int64_t)be * p.max_chunks * most + threadIdx.x;
+  const int lane = threadIdx.x & 63;
+  for (int r = threadIdx.x >> 6; r < rows; r += 4) {  // a wave a row, its chunks over the lanes
+    const int64_t first = (int64_t)be * p.max_chunks * most + r;
     float top = -INFINITY, sum = 0.f;
-    for (int x = 0; x < t.chunks; ++x) top = fmaxf(top, p.pml[2 * (first + (int64_t)x * most)]);
-    for (int x = 0; x < t.chunks; ++x) {
+    for (int x = lane; x < t.chunks; x += 64) {
       const int64_t at = first + (int64_t)x * most;
-      const float m = p.pml[2 * at];
-      sum += m == -INFINITY ? 0.f : p.pml[2 * at + 1] * __builtin_amdgcn_exp2f(m - top);
+      const float m = p.pml[2 * at], l = p.pml[2 * at + 1], next = fmaxf(top, m);
+      sum = next == -INFINITY ? 0.f : sum * __builtin_amdgcn_exp2f(top - next) + l * __builtin_amdgcn_exp2f(m - next);
+      top = next;
     }
-    norm[threadIdx.x] = top + __builtin_amdgcn_logf(sum);  // (a row sees itself: the sum is positive)
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) {
+      const float m = __shfl_xor(top, s), l = __shfl_xor(sum, s), next = fmaxf(top, m);
+      sum = next == -INFINITY ? 0.f : sum * __builtin_amdgcn_exp2f(top - next) + l * __builtin_amdgcn_exp2f(m - next);
+      top = next;
+    }
+    if (lane == 0) norm[r] = top + __builtin_amdgcn_logf(sum);  // (a row sees itself: the sum is positive)
   }
   __syncthreads();
   const int v = part * WEIGHT_KEYS + 4 * threadIdx.x;
@@ -768,9 +775,11 @@ static int tree_chunk(const kdn_tree_attn_args* a, int64_t longest) {
   while (chunk < MAX_CHUNK && times(each, (longest + chunk - 1) / chunk) > (chunk < 256 ? 512 : 2048)) chunk *= 2;
   return chunk;
 }
-static int64_t tree_chunks(const kdn_tree_attn_args* a, int64_t longest) {
-  const int chunk = tree_chunk(a, longest);
-  return longest > 0 ? (longest + chunk - 1) / chunk : 1;
+static int64_t tree_chunks(int64_t longest, int64_t chunk) { return longest > 0 ? (longest + chunk - 1) / chunk : 1; }
+// Under a window most contexts come to the longest one: as many chunks as share it evenly, none of a few keys left over.
+static int tree_chunk(const kdn_tree_attn_args* a, const TreePlan& plan) {
+  const int64_t chunk = tree_chunk(a, plan.longest), n = (plan.longest + chunk / 4) / chunk;
+  return !plan.window || n == 0 ? (int)chunk : (int)(((plan.longest + n - 1) / n + 63) / 64 * 64);
 }
 
 static int tree_check(const kdn_tree_attn_args* a) {
@@ -787,7 +796,7 @@ static int tree_check(const kdn_tree_attn_args* a) {
     return KDN_ERR_INVALID_ARGUMENT;
   // a grid's workgroups, and the join's rows
   const int64_t heads = a->num_seqs * a->H_kv, blocks = tree_blocks(a);
-  if (times(times(heads, tree_chunks(a, a->max_context)), blocks) > INT32_MAX - 8 * blocks - ZERO_GROUPS || times(heads, tree_rows(a)) > INT32_MAX)
+  if (times(times(heads, tree_chunks(a->max_context, tree_chunk(a, a->max_context))), blocks) > INT32_MAX - 8 * blocks - ZERO_GROUPS || times(heads, tree_rows(a)) > INT32_MAX)
     return KDN_ERR_UNSUPPORTED;
   return KDN_OK;
 }
@@ -879,7 +888,8 @@ static int tree_attn(const kdn_tree_attn_args* a, const kdn_tree_bound_args* b, 
     fits = fits && a->k_pages_stride[i] >= 0 && a->v_pages_stride[i] >= 0 && a->k_pages_stride[i] % per == 0 && a->v_pages_stride[i] % per == 0;
   if (!fits) return KDN_ERR_MISALIGNED;
   const TreePlan plan(a, b);
-  const int64_t chunks = tree_chunks(a, plan.longest);
+  const int chunk = tree_chunk(a, plan);
+  const int64_t chunks = tree_chunks(plan.longest, chunk);
   // a copy's lanes have 32-bit offsets from its first row
   const int64_t size = (int64_t)dtype_size(a->dtype), far = INT32_MAX / (16 * size);
   if (a->k_stride[0] > far || a->v_stride[0] > far || a->k_pages_stride[2] > far || a->v_pages_stride[2] > far) return KDN_ERR_UNSUPPORTED;
@@ -896,7 +906,7 @@ static int tree_attn(const kdn_tree_attn_args* a, const kdn_tree_bound_args* b, 
   p.cu = a->cu_new; p.lens = a->context_lens; p.table = a->page_table; p.parents = a->parents;
   p.table_stride = a->table_stride; p.num_pages = a->num_pages; p.total = a->total_new; p.max_context = a->max_context;
   p.H = (int)a->H; p.KV = (int)a->H_kv; p.G = (int)(a->H / a->H_kv);
-  p.max_new = (int)a->max_new; p.max_chunks = (int)chunks; p.chunk = tree_chunk(a, plan.longest); p.nseq = (int)a->num_seqs;
+  p.max_new = (int)a->max_new; p.max_chunks = (int)chunks; p.chunk = chunk; p.nseq = (int)a->num_seqs;
   p.shift = __builtin_ctz((unsigned)a->page_tokens);
   p.scale = a->scale;
   p.po = reinterpret_cast<float*>(a->workspace);

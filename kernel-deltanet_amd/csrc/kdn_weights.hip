@@ -105,18 +105,20 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
       for (int b = 0; b < BLOCKS; ++b) {
         const int fk = first_key + 32 * b, kk = key + 32 * b;
         const bool whole = i0 + off >= fk + 31 && i0 + 32 <= lenq && !(WIN && window_cuts(i0 + 31 + off, fk, fk + 31, p.window, p.sinks));
+        float part = 0.f;  // of a block, then of the walk: a long column's terms are added to few large sums
         if (whole) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sum[b] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, l[i]));
+          for (int i = 0; i < 16; ++i) part += __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, l[i]));
         } else {
           const int lo = max(kk - off, 0) - i0, hi = (WIN && kk >= p.sinks ? min(lenq, kk - off + p.window) : lenq) - i0;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int r = rho(half, i);
             const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, l[i]));
-            sum[b] += r >= lo && r < hi ? x : 0.f;
+            part += r >= lo && r < hi ? x : 0.f;
           }
         }
+        sum[b] += part;
       }
     }
   };

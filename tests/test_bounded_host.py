@@ -74,7 +74,7 @@ def test_window_arguments():
     size = lambda w, s: L.kdn_attn_window_bwd_workspace_bytes(ctypes.byref(b), w, s)  # noqa: E731
     none = L.kdn_attn_bwd_workspace_bytes(ctypes.byref(b))
     assert size(8, 0) == size(4, 4) == size(2 ** 62, 2 ** 62) == size(4, 0) == none  # no window, or none with sinks
-    assert size(4, 3) == none + 2 * (8 // 1024 + 3) * 2 * 3 * 2 * 64 * 4             # slots, subsets, sinks, heads
+    assert size(4, 3) == none + 2 * (8 // 1024 + 3 + 1) * 2 * 3 * 2 * 64 * 4         # slots and sequences, subsets, sinks, heads
     b.workspace, b.workspace_bytes, a.lse = 1 << 12, size(4, 3) - 1, 1 << 12
     b.dy = b.dq = b.dk = b.dv = 1 << 12
     assert L.kdn_attn_window_bwd(ctypes.byref(b), 4, 3, None) == -3

@@ -519,8 +519,9 @@ class PagePool:
 
 def _key_weights(weights: torch.Tensor, slots: Optional[torch.Tensor], streams: int, heads: Tuple[int, ...], like: torch.Tensor, what: str):
     """(slots, their address or 0) of weights that a call writes where they are, (slots, *heads, places) float32 on like's device."""
-    require_device(weights, f"{what} weights")
-    if weights.dim() != 2 + len(heads) or tuple(weights.shape[1:-1]) != heads or weights.dtype is not _F32 or weights.device != like.device or \
+    if not weights.is_cuda:
+        require_device(weights, f"{what} weights")
+    if weights.dim() != 2 + len(heads) or weights.shape[1:-1] != heads or weights.dtype is not _F32 or weights.get_device() != like.get_device() or \
             (weights.shape[-1] > 1 and weights.stride(-1) != 1):
         raise ValueError(f"{what}: weights are (slots, {', '.join(map(str, heads))}, places) float32 on {like.device}, places next to one another; "
                          f"got {tuple(weights.shape)} {weights.dtype} on {weights.device}")
@@ -594,7 +595,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: t
         if par is not None:
             raise ValueError("tree_attention: weights are of runs of tokens, not of trees (a refused draft would count)")
         slots, slots_at = _key_weights(weights, slots, B, (KV,), q, what)
-        bound = _BOUND.pack(near, first, weights.data_ptr(), weights.stride(0), weights.stride(1), weights.shape[2], weights.shape[0], slots_at)
+        s0, s1, _ = weights.stride()
+        bound = _BOUND.pack(near, first, weights.data_ptr(), s0, s1, weights.shape[2], weights.shape[0], slots_at)
         torch.autograd.graph.increment_version(weights)
     elif near:
         bound = _BOUND.pack(near, first, 0, 0, 0, 0, 0, 0)

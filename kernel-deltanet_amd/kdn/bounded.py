@@ -12,6 +12,7 @@ the device.  The reference never bounds its anchor pages (serving/hybrid_memory_
 """
 from __future__ import annotations
 
+import functools
 import operator
 import struct
 from typing import Optional
@@ -25,6 +26,12 @@ from .ops import _tag, require_device
 # The argument structs of include/kdn_bounded.h as packed bytes (tests/test_bounded_host.py holds them against the mirrors).
 _WEIGHTS = struct.Struct("@qqqqqiiifqqPP" + 2 * "Pqq" + "P" + "Pqq" + "qqPPN")
 _EVICT = struct.Struct("@qqqiiqqqqqqq" + 6 * "P" + 2 * "Pqqqq" + 2 * "Pqqq" + "qqPN")
+
+
+@functools.lru_cache(maxsize=64)
+def _weights_bytes(nseq: int, nq: int, nk: int, H: int, KV: int, d: int, dtype: int) -> int:
+    """kdn_attn_weights_workspace_bytes, which reads sizes only (each sequence has a slot)."""
+    return N.lib().kdn_attn_weights_workspace_bytes(_WEIGHTS.pack(nseq, nq, nk, H, KV, d, dtype, 0, 1.0, 0, 0, 4, 4, *(0,) * 10, 0, nseq, 0, 0, 0))
 
 
 def attention_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weights: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -60,33 +67,44 @@ def attention_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weigh
     B = cu_q.shape[0] - 1
     slots, slots_at = _key_weights(weights, slots, B, (KV,), q, what)
     lse = lse.contiguous()
-
-    def args(ws, nbytes):
-        return _WEIGHTS.pack(B, n, k.shape[0], H, KV, d, _tag(q.dtype, what), bool(add), _scale(scale, d, what), near, first, cu_q.data_ptr(),
-                             0 if cu_k is None else cu_k.data_ptr(), *qs[1:], *ks[1:], lse.data_ptr(), weights.data_ptr(), weights.stride(0),
-                             weights.stride(1), weights.shape[2], weights.shape[0], slots_at, ws, nbytes)
-
+    tag, s0, s1, _ = _tag(q.dtype, what), *weights.stride()
     torch.autograd.graph.increment_version(weights)
     with _device(dev):
-        nbytes = N.lib().kdn_attn_weights_workspace_bytes(args(0, 0))
+        nbytes = _weights_bytes(B, n, k.shape[0], H, KV, d, tag)
         ws = q.new_empty(nbytes, dtype=torch.uint8)
-        N.check(N.lib().kdn_attn_weights(args(ws.data_ptr(), nbytes), _raw_stream(dev)), "kdn_attn_weights")
+        N.check(N.lib().kdn_attn_weights(_WEIGHTS.pack(B, n, k.shape[0], H, KV, d, tag, bool(add), _scale(scale, d, what), near, first, cu_q.data_ptr(),
+                                                       0 if cu_k is None else cu_k.data_ptr(), *qs[1:], *ks[1:], lse.data_ptr(), weights.data_ptr(),
+                                                       s0, s1, weights.shape[2], weights.shape[0], slots_at, ws.data_ptr(), nbytes),
+                                         _raw_stream(dev)), "kdn_attn_weights")
     return weights
 
 
 def _layers(t: torch.Tensor, what: str):
-    """A cache's pages (pages, layers, heads, page_tokens, d), or of one layer without that dimension: (t with it, its address, the
-    page, layer, head and token strides); used where it is, never copied."""
-    require_device(t, what)
-    if t.dim() == 4:
-        t = t.unsqueeze(1)
-    if t.dim() != 5 or t.shape[4] not in (64, 128) or t.dtype not in (_BF16, _F32):
+    """A cache's pages (pages, layers, heads, page_tokens, d), or of one layer without that dimension: (its address, the page, layer,
+    head and token strides); used where it is, never copied."""
+    if not t.is_cuda:
+        require_device(t, what)
+    dim, dt = t.dim(), t.dtype
+    if dim not in (4, 5) or t.shape[-1] not in (64, 128) or (dt is not _BF16 and dt is not _F32):
         raise ValueError(f"{what}: expects (pages, layers, heads, page_tokens, d), or without layers, of bfloat16 or float32 and d = 64 or 128; "
-                         f"got {tuple(t.shape)} {t.dtype}")
-    steps = _steps(t)
-    if t.stride(4) != 1 or t.data_ptr() % 16 or any(s * t.element_size() % 16 for s in steps):
+                         f"got {tuple(t.shape)} {dt}")
+    a, *rest, last = t.stride()
+    steps = (a, 0, *rest) if dim == 4 else (a, *rest)
+    p, odd = t.data_ptr(), 7 if dt is _BF16 else 3
+    if (steps[0] | steps[1] | steps[2] | steps[3]) & odd:
+        steps = _steps(t)
+        steps = (steps[0], 0, *steps[1:]) if dim == 4 else steps
+    if last != 1 or p & 15 or (steps[0] | steps[1] | steps[2] | steps[3]) & odd:
         raise ValueError(f"{what}: needs contiguous rows that start on 16 bytes (a cache is used where it is, never copied)")
-    return t, t.data_ptr(), *steps
+    return p, *steps
+
+
+@functools.lru_cache(maxsize=64)
+def _evict_bytes(*sizes) -> int:
+    """kdn_evict_workspace_bytes, which reads sizes and whether there are slots only."""
+    streams, layers, heads, d, dtype, page_tokens, pages, width, max_len, slots, places, rows = sizes
+    return N.lib().kdn_evict_workspace_bytes(_EVICT.pack(streams, layers, heads, d, dtype, page_tokens, pages, width, 0, max_len, 0, 0, *(0,) * 5,
+                                                         4 if slots else 0, *(0,) * 18, places, rows, 0, 0))
 
 
 def evict(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, keep: torch.Tensor,
@@ -106,24 +124,24 @@ def evict(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor
     went.  What lies behind stays as it is.  The pages of places below the new length have to be the stream's own
     (`PagePool.own`), slots and pages distinct.  `slots` as in `attention_weights`; `max_len` (what page_table holds and there are places
     for) bounds lens from the host, longer ones are cut to it: nothing is read back."""
-    what = "evict"
     if _tracked(k_pages, v_pages, weights):
         raise ValueError("evict: the pages have no gradient; call it under torch.no_grad()")
-    plain = k_pages.dim() == 4
     kp, vp = _layers(k_pages, "evict k_pages"), _layers(v_pages, "evict v_pages")
-    pages, layers, KV, P, d = kp[0].shape
-    if v_pages.shape != k_pages.shape or v_pages.dtype is not k_pages.dtype or v_pages.device != k_pages.device:
-        raise ValueError(f"evict: pages {tuple(k_pages.shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype} differ")
-    dev = k_pages.get_device()
+    shape, dev, dt = k_pages.shape, k_pages.get_device(), k_pages.dtype
+    plain = len(shape) == 4
+    pages, P, d = shape[0], shape[-2], shape[-1]
+    heads = shape[1:2] if plain else shape[1:3]
+    if v_pages.shape != shape or v_pages.dtype is not dt or v_pages.get_device() != dev:
+        raise ValueError(f"evict: pages {tuple(shape)} {dt} and {tuple(v_pages.shape)} {v_pages.dtype} differ")
     if page_table.get_device() != dev or page_table.dim() != 2 or page_table.dtype is not torch.int32 or \
             (page_table.shape[1] > 1 and page_table.stride(1) != 1):
         raise ValueError(f"evict: page_table is (streams, width) int32 on {k_pages.device}, got {tuple(page_table.shape)} {page_table.dtype} "
                          f"on {page_table.device}")
     B, width = page_table.shape
-    heads = (KV,) if plain else (layers, KV)
-    slots, slots_at = _key_weights(weights, slots, B, heads, k_pages, what)
-    if positions.shape != weights.shape or positions.dtype is not torch.int32 or positions.device != weights.device or \
-            (positions.shape[-1] > 1 and positions.stride(-1) != 1):
+    slots, slots_at = _key_weights(weights, slots, B, heads, k_pages, "evict")
+    rows, places = weights.shape[0], weights.shape[-1]
+    if positions.shape != weights.shape or positions.dtype is not torch.int32 or positions.get_device() != dev or \
+            (places > 1 and positions.stride(-1) != 1):
         raise ValueError(f"evict: positions are {tuple(weights.shape)} int32 on {weights.device}, places next to one another; got "
                          f"{tuple(positions.shape)} {positions.dtype} on {positions.device}")
     lens, keep = _ints(lens, "evict lens", torch.int32, dev, B), _ints(keep, "evict keep", torch.int32, dev, B)
@@ -132,24 +150,20 @@ def evict(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor
     sinks, recent = operator.index(sinks), operator.index(recent)
     if sinks < 0 or recent < 0:
         raise ValueError(f"evict: sinks and recent are 0 or more, got {sinks}, {recent}")
-    room = min(width * P, weights.shape[-1])
-    most = room if max_len is None else min(operator.index(max_len), room)
-    if most < 0:
-        raise ValueError(f"evict: max_len is 0 or more, got {max_len}")
-
-    def strides(t):
-        s = _steps(t)
-        return (s[0], 0, s[1]) if plain else s
-
-    def args(ws, nbytes):
-        return _EVICT.pack(B, layers, KV, d, _tag(k_pages.dtype, what), P, pages, width, page_table.stride(0), most, min(sinks, 2**62),
-                           min(recent, 2**62), page_table.data_ptr(), lens.data_ptr(), keep.data_ptr(), 0 if settled is None else settled.data_ptr(),
-                           0 if evicted is None else evicted.data_ptr(), slots_at, *kp[1:], *vp[1:], weights.data_ptr(), *strides(weights),
-                           positions.data_ptr(), *strides(positions), weights.shape[-1], weights.shape[0], ws, nbytes)
-
-    for t in (k_pages, v_pages, weights, positions):
-        torch.autograd.graph.increment_version(t)
+    most = min(width * P, places)
+    if max_len is not None:
+        most = min(operator.index(max_len), most)
+        if most < 0:
+            raise ValueError(f"evict: max_len is 0 or more, got {max_len}")
+    w0, *w1 = weights.stride()
+    p0, *p1 = positions.stride()
+    layers, KV = (1, *heads) if plain else heads
+    torch.autograd.graph.increment_version((k_pages, v_pages, weights, positions))
     with _device(dev):
-        nbytes = N.lib().kdn_evict_workspace_bytes(args(0, 0))
+        nbytes = _evict_bytes(B, layers, KV, d, _tag(dt, "evict"), P, pages, width, most, slots_at != 0, places, rows)
         ws = weights.new_empty(nbytes, dtype=torch.uint8)
-        N.check(N.lib().kdn_evict(args(ws.data_ptr(), nbytes), _raw_stream(dev)), "kdn_evict")
+        N.check(N.lib().kdn_evict(_EVICT.pack(B, layers, KV, d, _tag(dt, "evict"), P, pages, width, page_table.stride(0), most, min(sinks, 2**62),
+                                              min(recent, 2**62), page_table.data_ptr(), lens.data_ptr(), keep.data_ptr(),
+                                              0 if settled is None else settled.data_ptr(), 0 if evicted is None else evicted.data_ptr(), slots_at,
+                                              *kp, *vp, weights.data_ptr(), w0, *((0,) if plain else ()), *w1[:-1], positions.data_ptr(), p0,
+                                              *((0,) if plain else ()), *p1[:-1], places, rows, ws.data_ptr(), nbytes), _raw_stream(dev)), "kdn_evict")

@@ -25,6 +25,62 @@ struct WeightsTile {
   static constexpr int KEYS = 128 * BLOCKS, ROWS = 64, TILE = ROWS * P::ROW, SLOT = TILE + ROWS * 4;
 };
 
+// exp(scale q.k - lse) of 32 rows from i0 on and a wave's keys, added to the keys' sums: `rows` the tile in LDS, r0 the first row in it,
+// `bits` their -lse in bits.
+struct WeightsMask {
+  int off, lenq, window, sinks;
+};
+template <class P, int BLOCKS, bool WIN>
+__device__ __forceinline__ void add_weights(float (&sum)[BLOCKS], const typename P::frag (&k)[BLOCKS][P::D / 16], const unsigned char* rows, int r0,
+                                            const float* bits, int i0, int first_key, int lane, float c, const WeightsMask& m) {
+  constexpr int KS = P::D / 16, AHEAD = KS < P::AHEAD ? KS : P::AHEAD;
+  const int half = lane >> 5;
+  float l[16];
+#pragma unroll
+  for (int a = 0; a < 4; ++a) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(bits + 8 * a + 4 * half);
+#pragma unroll
+    for (int y = 0; y < 4; ++y) l[4 * a + y] = x[y];
+  }
+  f32x16 s[BLOCKS];
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) s[b] = zero16();
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const typename P::frag a = P::row_frag(rows, r0 + (lane & 31), ks, half);
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) s[b] = P::mma(s[b], a, k[b][ks]);
+  }
+  // as sched_products, an operand for BLOCKS products; the rows' bits first
+  __builtin_amdgcn_sched_group_barrier(0x100, 4 + AHEAD * P::ROW_READS, 0);
+#pragma unroll
+  for (int i = 0; i < KS - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, P::MFMAS * BLOCKS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, P::ROW_READS, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, AHEAD * P::MFMAS * BLOCKS, 0);
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) {
+    const int fk = first_key + 32 * b, kk = fk + (lane & 31);
+    const bool whole = i0 + m.off >= fk + 31 && i0 + 32 <= m.lenq && !(WIN && window_cuts(i0 + 31 + m.off, fk, fk + 31, m.window, m.sinks));
+    float part = 0.f;  // of a block, then of the walk: a long column's terms are added to few large sums
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) part += __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, l[i]));
+    } else {
+      int lo = max(kk - m.off, 0) - i0, hi = (WIN && kk >= m.sinks ? min(m.lenq, kk - m.off + m.window) : m.lenq) - i0;
+      asm volatile("" : "+v"(lo), "+v"(hi));  // the comparisons stay here: formed for every block they were an eighth of the vector instructions
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = rho(half, i);
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, l[i]));
+        part += r >= lo && r < hi ? x : 0.f;
+      }
+    }
+    sum[b] += part;
+  }
+}
+
 // A key's sum to its place: those before the sequence's first row are added to if the call says so, others are set.
 __device__ __forceinline__ void put_weight(const WeightsParams& p, int seq, int e, int key, int off, float sum) {
   if (seq < 0 || seq >= p.a.nseq || key >= p.places) return;
@@ -72,60 +128,29 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   const int64_t all = (int64_t)per * p.G;
   const int j0 = (int)(all * part / wp.parts), j1 = (int)(all * (part + 1) / wp.parts);
   const Stager<P, ROWS, 4> stage_q(p.qs[0], w, lane);
+  float lse = 0.f;  // the first wave's: of the tile that is on its way
   auto stage = [&](int j, unsigned char* to) {
     const int h = e * p.G + j / per, r0 = q0 + j % per * ROWS, last = min(lenq - 1 - r0, ROWS - 1);
     stage_q(reinterpret_cast<const E*>(p.q) + (qlo + r0) * p.qs[0] + (int64_t)h * p.qs[1], last, to);
-    if (w == 0) copy4_to_lds(buffer_at(p.lse + (int64_t)h * p.total_q + qlo + r0), 4 * min(lane, last), to + S::TILE);
+    if (w == 0) lse = p.lse[(int64_t)h * p.total_q + qlo + r0 + min(lane, last)];
   };
-  auto step = [&](int j, const unsigned char* __restrict qt, unsigned char* __restrict next) {
+  auto step = [&](int j, int r0, const unsigned char* __restrict qt, unsigned char* __restrict next) {
     if (j + 1 < j1) stage(j + 1, next);
-    const float* lse = reinterpret_cast<const float*>(qt + S::TILE);
 #pragma unroll
     for (int u = 0; u < ROWS / 32; ++u) {
-      const int i0 = q0 + j % per * ROWS + 32 * u;  // the rows i0 .. i0 + 31
+      const int i0 = r0 + 32 * u;  // the rows i0 .. i0 + 31
       if (i0 >= lenq || i0 + 31 + off < first_key) continue;
       if (WIN && window_hides(i0 + off, first_key, first_key + 32 * BLOCKS - 1, p.window, p.sinks)) continue;
-      f32x16 s[BLOCKS];
-#pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) s[b] = zero16();
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const typename P::frag a = P::row_frag(qt, 32 * u + (lane & 31), ks, half);
-#pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) s[b] = P::mma(s[b], a, k[b][ks]);
-      }
-      float l[16];
-#pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(lse + 32 * u + 8 * a + 4 * half);
-#pragma unroll
-        for (int y = 0; y < 4; ++y) l[4 * a + y] = x[y] * -LOG2E;
-      }
-#pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) {
-        const int fk = first_key + 32 * b, kk = key + 32 * b;
-        const bool whole = i0 + off >= fk + 31 && i0 + 32 <= lenq && !(WIN && window_cuts(i0 + 31 + off, fk, fk + 31, p.window, p.sinks));
-        float part = 0.f;  // of a block, then of the walk: a long column's terms are added to few large sums
-        if (whole) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) part += __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, l[i]));
-        } else {
-          const int lo = max(kk - off, 0) - i0, hi = (WIN && kk >= p.sinks ? min(lenq, kk - off + p.window) : lenq) - i0;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int r = rho(half, i);
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], c, l[i]));
-            part += r >= lo && r < hi ? x : 0.f;
-          }
-        }
-        sum[b] += part;
-      }
+      add_weights<P, BLOCKS, WIN>(sum, k, qt, 32 * u, reinterpret_cast<const float*>(qt + S::TILE) + 32 * u, i0, first_key, lane, c,
+                                  {off, lenq, p.window, p.sinks});
     }
   };
   if (j0 < j1) stage(j0, lds);
-  for (int j = j0; j < j1; ++j) {
+  int row = per > 0 ? j0 % per * ROWS : 0;
+  for (int j = j0; j < j1; ++j, row = row + ROWS < per * ROWS ? row + ROWS : 0) {
+    if (w == 0) reinterpret_cast<float*>(lds + ((j - j0) & 1) * S::SLOT + S::TILE)[lane] = lse * -LOG2E;  // (read last two tiles ago)
     staged_barrier();
-    step(j, lds + ((j - j0) & 1) * S::SLOT, lds + ((j - j0 + 1) & 1) * S::SLOT);
+    step(j, q0 + row, lds + ((j - j0) & 1) * S::SLOT, lds + ((j - j0 + 1) & 1) * S::SLOT);
   }
 #pragma unroll
   for (int b = 0; b < BLOCKS; ++b) {
@@ -134,6 +159,116 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
     if (half != 0 || kk >= lenk) continue;
     if (wp.part) wp.part[((int64_t)part * p.KV + e) * p.total_k + t.lo + kk] = x;
     else put_weight(wp, t.seq, e, kk, off, x);
+  }
+}
+
+// Few rows over many keys (the last rows of prompts): a sequence's rows of all heads of a key head stay in LDS while the workgroup
+// goes along the keys, `per` tiles of them one after another, each wave's next K fragments on their way as it works on the present
+// ones.  What is read is K, once.  More rows than LDS holds come in batches, for each tile of keys anew.
+template <class P>
+struct WeightsFew {
+  static constexpr int BLOCKS = WeightsTile<P>::BLOCKS, KEYS = 128 * BLOCKS, ROWS = 64, TILE = ROWS * P::ROW;
+  static constexpr int TILES = 65536 / TILE, LDS = TILES * (TILE + ROWS * 4);  // two workgroups a CU
+};
+
+template <class P, bool WIN>
+__global__ void __launch_bounds__(256, 2) attn_weights_few_kernel(WeightsParams wp, int64_t slots, int64_t per) {
+  typedef typename P::elem E;
+  typedef WeightsFew<P> S;
+  constexpr int KS = P::D / 16, BLOCKS = S::BLOCKS, KEYS = S::KEYS, ROWS = S::ROWS, TILES = S::TILES;
+  __shared__ __attribute__((aligned(256))) unsigned char lds[S::LDS];
+  const AttnParams& p = wp.a;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int e = blockIdx.x % p.KV;
+  int64_t slot = blockIdx.x / p.KV * per - 1;
+  const int64_t end = min(slot + 1 + per, slots);
+  SeqTile now;
+  now.row0 = -1;
+  now.len = 0;
+  // the tile after `t`, one with keys, or with a negative first row the end
+  auto after = [&](SeqTile t) {
+    while (++slot < end) {
+      if (t.row0 >= 0 && t.row0 + KEYS < t.len) {
+        t.row0 += KEYS;
+        return t;
+      }
+      t = find_tile<KEYS>(p.cu_k, p.nseq, p.total_k, slot, lane);
+      if (t.row0 >= 0) return t;
+    }
+    t.row0 = -1;
+    return t;
+  };
+  typename P::frag k[BLOCKS][KS], next[BLOCKS][KS];
+  auto load = [&](const SeqTile& t, typename P::frag (&to)[BLOCKS][KS]) {
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      const int64_t key = t.lo + min(t.row0 + 32 * (BLOCKS * w + b) + (lane & 31), t.len - 1);
+      const E* src = reinterpret_cast<const E*>(p.k) + key * p.ks[0] + (int64_t)e * p.ks[1];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) to[b][ks] = P::load(src + 16 * ks + 8 * half);
+    }
+    asm volatile("" ::: "memory");  // they are issued here, not where they are used
+  };
+  const float c = p.scale * LOG2E;
+  const Stager<P, ROWS, 4> stage_q(p.qs[0], w, lane);
+  now = after(now);
+  if (now.row0 < 0) return;
+  load(now, k);
+  int staged = -2;  // the sequence whose rows are in LDS, all of them
+  int64_t qlo = 0;
+  int lenq = 0;
+  while (now.row0 >= 0) {
+    const SeqTile then = after(now);
+    other_rows(p.cu_q, p.nseq, p.total_q, now.seq, qlo, lenq);
+    const int off = now.len - lenq, first_key = now.row0 + 32 * BLOCKS * w;
+    const int each = (lenq + ROWS - 1) / ROWS;
+    const int64_t tiles = (int64_t)each * p.G;
+    float sum[BLOCKS];
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) sum[b] = 0.f;
+    bool loaded = false;
+    for (int64_t j0 = 0; j0 < tiles; j0 += TILES) {
+      const int n = (int)min((int64_t)TILES, tiles - j0);
+      int r0 = (int)(j0 % each) * ROWS;  // the batch's first tile's first row
+      if (staged != now.seq || tiles > TILES) {
+        __syncthreads();  // the rows before are read
+        int h = e * p.G + (int)(j0 / each), r = r0;
+        for (int j = 0; j < n; ++j) {
+          const int last = min(lenq - 1 - r, ROWS - 1);
+          stage_q(reinterpret_cast<const E*>(p.q) + (qlo + r) * p.qs[0] + (int64_t)h * p.qs[1], last, lds + j * S::TILE);
+          if (w == j % 4) reinterpret_cast<float*>(lds + TILES * S::TILE)[j * ROWS + lane] = p.lse[(int64_t)h * p.total_q + qlo + r + min(lane, last)] * -LOG2E;
+          r += ROWS;
+          if (r >= lenq) r = 0, ++h;
+        }
+        staged_barrier();
+        staged = now.seq;
+      }
+      if (!loaded && then.row0 >= 0) load(then, next);
+      loaded = true;
+      for (int j = 0; j < n; ++j) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int i0 = r0 + 32 * u;
+          if (i0 >= lenq || i0 + 31 + off < first_key) continue;
+          if (WIN && window_hides(i0 + off, first_key, first_key + 32 * BLOCKS - 1, p.window, p.sinks)) continue;
+          add_weights<P, BLOCKS, WIN>(sum, k, lds + j * S::TILE, 32 * u, reinterpret_cast<const float*>(lds + TILES * S::TILE) + j * ROWS + 32 * u, i0,
+                                      first_key, lane, c, {off, lenq, p.window, p.sinks});
+        }
+        r0 += ROWS;
+        if (r0 >= lenq) r0 = 0;
+      }
+    }
+    if (!loaded && then.row0 >= 0) load(then, next);  // (a sequence without rows)
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      const int key = first_key + 32 * b + (lane & 31);
+      const float x = half_sum(sum[b]);
+      if (half == 0 && key < now.len) put_weight(wp, now.seq, e, key, off, x);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) k[b][ks] = next[b][ks];
+    }
+    now = then;
   }
 }
 
@@ -165,16 +300,35 @@ static int weights_check(const kdn_attn_weights_args* a) {
 
 static int weights_keys(const kdn_attn_weights_args* a) { return a->d * (int)dtype_size(a->dtype) <= 256 ? 256 : 128; }
 
+// Whether an average sequence's rows come to two batches at most of the kernel of few rows.
+static bool weights_few(const kdn_attn_weights_args* a) {
+  const int64_t tiles = (a->total_q / std::max<int64_t>(a->num_seqs, 1) + 63) / 64 * (a->H / a->H_kv);
+  return tiles <= 2 * 65536 / (64 * a->d * (int64_t)dtype_size(a->dtype));
+}
+
 // Workgroups that share a tile of keys: enough that there are 2048 (the first keys have twice the average's work), but none
 // without a tile of an average sequence's rows.
 static int weights_parts(const kdn_attn_weights_args* a) {
+  if (weights_few(a)) return 1;
   const int64_t tiles = tile_slots(a->total_k, weights_keys(a), a->num_seqs) * a->H_kv;
   const int64_t rows = (a->total_q / std::max<int64_t>(a->num_seqs, 1) / 64 + 1) * (a->H / a->H_kv);
   return (int)std::max<int64_t>(1, std::min<int64_t>({(2048 + tiles - 1) / tiles, rows, 16}));
 }
 
 template <class P>
-static int launch_weights(const WeightsParams& p, hipStream_t st) {
+static int launch_weights_few(const WeightsParams& p, hipStream_t st) {
+  // as many workgroups as there is room for at a time, each as many tiles
+  const int64_t slots = tile_slots(p.a.total_k, WeightsFew<P>::KEYS, p.a.nseq), groups = std::max<int64_t>(1, 512 / p.a.KV);
+  const int64_t per = (slots + groups - 1) / groups, grid = (slots + per - 1) / per * p.a.KV;
+  if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  if (p.a.window < NO_WINDOW) hipLaunchKernelGGL((attn_weights_few_kernel<P, true>), dim3((unsigned)grid), dim3(256), 0, st, p, slots, per);
+  else hipLaunchKernelGGL((attn_weights_few_kernel<P, false>), dim3((unsigned)grid), dim3(256), 0, st, p, slots, per);
+  return launch_status();
+}
+
+template <class P>
+static int launch_weights(const WeightsParams& p, bool few, hipStream_t st) {
+  if (few) return launch_weights_few<P>(p, st);
   const int64_t slots = tile_slots(p.a.total_k, WeightsTile<P>::KEYS, p.a.nseq), grid = slots * p.a.KV * p.parts;
   const int64_t joins = p.parts > 1 ? tile_slots(p.a.total_k, 256, p.a.nseq) * p.a.KV : 0;
   if (grid > INT32_MAX || joins > INT32_MAX) return KDN_ERR_UNSUPPORTED;
@@ -221,6 +375,7 @@ extern "C" int kdn_attn_weights(const kdn_attn_weights_args* a, void* stream) {
   p.part = p.parts > 1 ? reinterpret_cast<float*>(a->workspace) : nullptr;
   p.add = a->add != 0;
   hipStream_t st = as_stream(stream);
-  if (a->dtype == KDN_DTYPE_BF16) return a->d == 64 ? launch_weights<AttnBF16<64>>(p, st) : launch_weights<AttnBF16<128>>(p, st);
-  return a->d == 64 ? launch_weights<AttnF32<64>>(p, st) : launch_weights<AttnF32<128>>(p, st);
+  const bool few = weights_few(a);
+  if (a->dtype == KDN_DTYPE_BF16) return a->d == 64 ? launch_weights<AttnBF16<64>>(p, few, st) : launch_weights<AttnBF16<128>>(p, few, st);
+  return a->d == 64 ? launch_weights<AttnF32<64>>(p, few, st) : launch_weights<AttnF32<128>>(p, few, st);
 }

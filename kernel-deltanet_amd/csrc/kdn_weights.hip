@@ -22,8 +22,9 @@ struct WeightsParams {
 template <class P>
 struct WeightsTile {
   static constexpr int BLOCKS = P::ROW <= 256 ? 2 : 1;  // of 32 keys to a wave: as many as leave the registers of two waves a SIMD
-  static constexpr int KEYS = 128 * BLOCKS, ROWS = 64, TILE = ROWS * P::ROW, SLOT = TILE + ROWS * 4;
+  static constexpr int KEYS = 128 * BLOCKS, ROWS = P::ROW <= 128 ? 128 : 64, TILE = ROWS * P::ROW, SLOT = TILE + ROWS * 4;
 };
+
 
 // exp(scale q.k - lse) of 32 rows from i0 on and a wave's keys, added to the keys' sums: `rows` the tile in LDS, r0 the first row in it,
 // `bits` their -lse in bits.
@@ -90,7 +91,8 @@ __device__ __forceinline__ void put_weight(const WeightsParams& p, int seq, int 
   *w = p.add && key < off ? *w + sum : sum;
 }
 
-// `parts` workgroups share the tiles of query rows of a tile of keys evenly, each the next stretch of them.
+// `parts` workgroups share the tiles of query rows of a tile of keys evenly, each the next stretch of them.  (Fewer for the later
+// keys, which fewer rows see: three prompts of 1000 to 8192 rows 131 us and more, for 127.)
 template <class P, bool WIN>
 __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) attn_weights_kernel(WeightsParams wp, int64_t slots) {
   typedef typename P::elem E;
@@ -121,21 +123,26 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   for (int b = 0; b < BLOCKS; ++b) sum[b] = 0.f;
   const float c = p.scale * LOG2E;
 
-  // the rows that see a key of the tile; past the window only the sinks are seen
+  // the rows that see a key of the tile, in whole tiles; past the window only the sinks are seen
   const int q0 = max(t.row0 - off, 0) / ROWS * ROWS;
   const int q1 = WIN && t.row0 >= p.sinks ? min(lenq, max(t.row0 + S::KEYS - 1 - off + p.window, 0)) : lenq;
   const int per = q0 < q1 ? (q1 - q0 + ROWS - 1) / ROWS : 0;
-  const int64_t all = (int64_t)per * p.G;
-  const int j0 = (int)(all * part / wp.parts), j1 = (int)(all * (part + 1) / wp.parts);
+  const int64_t all = (int64_t)per * p.G, j0 = all * part / wp.parts;
+  const int tiles = (int)(all * (part + 1) / wp.parts - j0);
   const Stager<P, ROWS, 4> stage_q(p.qs[0], w, lane);
-  float lse = 0.f;  // the first wave's: of the tile that is on its way
-  auto stage = [&](int j, unsigned char* to) {
-    const int h = e * p.G + j / per, r0 = q0 + j % per * ROWS, last = min(lenq - 1 - r0, ROWS - 1);
-    stage_q(reinterpret_cast<const E*>(p.q) + (qlo + r0) * p.qs[0] + (int64_t)h * p.qs[1], last, to);
-    if (w == 0) lse = p.lse[(int64_t)h * p.total_q + qlo + r0 + min(lane, last)];
+  float lse = 0.f;  // of the tile that is on its way, 64 rows a wave
+  int head = e * p.G, row = q0;  // of that tile
+  if (per > 0) head += (int)(j0 / per), row += (int)(j0 % per) * ROWS;
+  auto stage = [&](unsigned char* to) {
+    const int last = min(lenq - 1 - row, ROWS - 1);
+    stage_q(reinterpret_cast<const E*>(p.q) + (qlo + row) * p.qs[0] + (int64_t)head * p.qs[1], last, to);
+    if (64 * w < ROWS) lse = p.lse[(int64_t)head * p.total_q + qlo + row + min(64 * w + lane, last)];
   };
-  auto step = [&](int j, int r0, const unsigned char* __restrict qt, unsigned char* __restrict next) {
-    if (j + 1 < j1) stage(j + 1, next);
+  auto step = [&](int j, const unsigned char* __restrict qt, unsigned char* __restrict next) {
+    const int r0 = row;
+    row += ROWS;
+    if (row >= q0 + per * ROWS) row = q0, ++head;
+    if (j + 1 < tiles) stage(next);
 #pragma unroll
     for (int u = 0; u < ROWS / 32; ++u) {
       const int i0 = r0 + 32 * u;  // the rows i0 .. i0 + 31
@@ -145,12 +152,12 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
                                   {off, lenq, p.window, p.sinks});
     }
   };
-  if (j0 < j1) stage(j0, lds);
-  int row = per > 0 ? j0 % per * ROWS : 0;
-  for (int j = j0; j < j1; ++j, row = row + ROWS < per * ROWS ? row + ROWS : 0) {
-    if (w == 0) reinterpret_cast<float*>(lds + ((j - j0) & 1) * S::SLOT + S::TILE)[lane] = lse * -LOG2E;  // (read last two tiles ago)
+  if (tiles > 0) stage(lds);
+  for (int j = 0; j < tiles; ++j) {
+    unsigned char* slot = lds + (j & 1) * S::SLOT;
+    if (64 * w < ROWS) reinterpret_cast<float*>(slot + S::TILE)[64 * w + lane] = lse * -LOG2E;  // (read last two tiles ago)
     staged_barrier();
-    step(j, q0 + row, lds + ((j - j0) & 1) * S::SLOT, lds + ((j - j0 + 1) & 1) * S::SLOT);
+    step(j, slot, lds + (~j & 1) * S::SLOT);
   }
 #pragma unroll
   for (int b = 0; b < BLOCKS; ++b) {

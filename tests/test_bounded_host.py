@@ -131,7 +131,9 @@ def test_weights_arguments():
         assert size(args(**kw)) == 0 and call(args(**kw), None) == status
     for kw, status in ((dict(q=None), -1), (dict(lse=None), -1), (dict(weights=None), -1), (dict(k=8), -4), (dict(q_stride=N._i64x2(257, 64)), -4)):
         assert size(args(**kw)) > 0 and call(args(**kw), None) == status
-    assert size(args()) == 4 * 2 * 2 * 8 and call(args(), None) == -3  # two heads' tiles of rows apart, no workspace
+    assert size(args()) == 4  # few rows: no partial sums
+    long = dict(total_q=4096, total_k=4096)
+    assert size(args(**long)) == 16 * 2 * 4096 * 4 and call(args(**long), None) == -3  # sixteen workgroups to a tile, no workspace
     assert call(args(num_seqs=0, num_slots=0), None) == 0 and call(args(total_k=0, total_q=0), None) == 0
 
 

@@ -493,12 +493,12 @@ struct TreeMany {
   static constexpr int KEYS = P::ROW <= 128 ? 64 : 32, TILE = KEYS * P::ROW;
   // tiles in LDS, all but the one in use on their way; two workgroups a CU, or of fp32, whose registers allow one, one
   static constexpr int BUFS = 4, COPIES = KEYS / 32 * 16 * P::PIECES / 64;  // copies of a wave and tile
-  static int blocks(int rows) { return (rows + 127) / 128; }
-  static int per(int rows) { return ((rows + 31) / 32 + blocks(rows) - 1) / blocks(rows); }
+  __device__ __host__ static constexpr int blocks(int rows) { return (rows + 127) / 128; }
+  __device__ __host__ static constexpr int per(int rows) { return ((rows + 31) / 32 + blocks(rows) - 1) / blocks(rows); }
 };
 
 template <class P, bool WIN>
-__global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tree_many_kernel(TreeParams p, int blocks, int per) {
+__global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tree_many_kernel(TreeParams p, int blocks) {
   typedef typename P::elem E;
   constexpr int D = P::D, KS = D / 16, CT = D / 32, KEYS = TreeMany<P>::KEYS, TILE = TreeMany<P>::TILE;
   constexpr int BUFS = TreeMany<P>::BUFS, COPIES = TreeMany<P>::COPIES;
@@ -515,7 +515,8 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
   const int b = t.b, ch = t.ch, be = b * p.KV + e;
   const TreeBound bound(p, WIN ? __builtin_amdgcn_readfirstlane((int)min((int64_t)max(p.lens[b], 0), p.max_context)) : 0);
   auto key_at = [&](int at) { return WIN ? bound.key(at) : at; };
-  const int rows = t.n * p.G, first = 32 * (per * rb + w);
+  // as many workgroups as the sequence's own rows need: one of four waves for 128
+  const int rows = t.n * p.G, per = TreeMany<P>::per(rows), first = 32 * (per * rb + w);
   if (32 * per * rb >= rows) return;
   const bool busy = w < per && first < rows, live = busy && first + (lane & 31) < rows;
   const int row = min(first + (lane & 31), rows - 1), tok = row / p.G, h = e * p.G + row % p.G;
@@ -812,7 +813,7 @@ static int launch_tree(TreeParams& p, hipStream_t st) {
   } else {
     const int blocks = TreeMany<P>::blocks(rows);
     p.zero_from = (int)((units + 7) / 8 * 8 * blocks);
-    hipLaunchKernelGGL((tree_many_kernel<P, WIN>), dim3((unsigned)p.zero_from + ZERO_GROUPS), dim3(256), 0, st, p, blocks, TreeMany<P>::per(rows));
+    hipLaunchKernelGGL((tree_many_kernel<P, WIN>), dim3((unsigned)p.zero_from + ZERO_GROUPS), dim3(256), 0, st, p, blocks);
   }
   const int64_t joins = p.max_chunks > 1 ? ((int64_t)p.nseq * p.KV * rows + 3) / 4 : 0;
   if (p.weights && p.nseq > 0) {

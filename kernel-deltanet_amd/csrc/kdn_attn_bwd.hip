@@ -65,8 +65,10 @@ __device__ __forceinline__ const AttnParams& params_here() {
 
 // Under a window (WIN) the rows that see a tile of keys end `window` behind it, but for the first `sinks` keys, which all later
 // rows see: one workgroup that walked them all would run on when the others are done (a sequence of 65536 rows and a window of
-// 1024: fifty times as long).  So those rows are cut into segments of FAR_ROWS, a workgroup each, whose sums of the sinks' dk and
-// dv come to lie apart in fp32, as the near rows' do a second time; attn_sinks_kernel adds them in a fixed order.
+// 1024: fifty times as long).  So those rows are cut into segments of FAR_ROWS, a workgroup each and 32 sinks, whose waves share the
+// rows (one wave with all of them: the gradients of 16384 rows in a window
+// of 1024, 32 heads of 128, 1448 us, so 1429).  Their sums of the sinks' dk
+// and dv come to lie apart in fp32, as the near rows' do a second time; attn_sinks_kernel adds them in a fixed order.
 constexpr int FAR_ROWS = 1024;
 // The query rows [from, to) of a sequence that see keys of the tile row0 .. row0 + keys - 1 for nearness, in whole tiles of `rows`.
 // Those from `to` on see of it the sinks alone.
@@ -88,7 +90,7 @@ template <class P, int SPLIT>
 struct Dkdv {
   static constexpr int KEYS = 128 / SPLIT, ROWS = SPLIT == 4 ? 128 : 64, BLOCKS = ROWS / 32 / SPLIT;
   static constexpr int TILE = ROWS * P::ROW, SLOT = 2 * TILE + 2 * ROWS * 4, BUFS = 2 * SLOT <= 160 * 1024 ? 2 : 1;
-  static constexpr int JOIN = SPLIT > 1 ? 4 * (P::D / 32) * 4096 : 0;
+  static constexpr int JOIN = 4 * (P::D / 32) * 4096;
   static constexpr int LDS = BUFS * SLOT > JOIN ? BUFS * SLOT : JOIN;
 };
 
@@ -105,12 +107,12 @@ __device__ __forceinline__ void dkdv(int id, int slots, int far, unsigned char* 
   int64_t qlo;
   int lenq, far_slot = -1, segment = 0;
   if (WIN && id < far) {
-    const int tiles = (p.sinks + S::KEYS - 1) / S::KEYS, u = id / p.KV / p.subsets;
+    const int tiles = (p.sinks + 31) / 32, u = id / p.KV / p.subsets;
     far_slot = u / tiles;
     const SeqTile rows = find_tile<FAR_ROWS>(p.cu_q, p.nseq, p.total_q, far_slot, lane);
     if (rows.row0 < 0) return;
     qlo = rows.lo, lenq = rows.len, segment = rows.row0;
-    t.row0 = u % tiles * S::KEYS;
+    t.row0 = u % tiles * 32;
     other_rows(p.cu_k, p.nseq, p.total_k, rows.seq, t.lo, t.len);
     if (t.row0 >= t.len) return;
   } else {
@@ -120,7 +122,8 @@ __device__ __forceinline__ void dkdv(int id, int slots, int far, unsigned char* 
   }
   const int lenk = t.len;
   const int off = lenk - lenq;
-  const int first_key = t.row0 + 32 * (w / SPLIT), key = first_key + (lane & 31);
+  const bool is_far = WIN && far_slot >= 0;
+  const int first_key = t.row0 + (is_far ? 0 : 32 * (w / SPLIT)), key = first_key + (lane & 31);
   const bool live = key < lenk;
   typename P::frag k[KS], v[DK ? KS : 1];
   {
@@ -144,9 +147,9 @@ __device__ __forceinline__ void dkdv(int id, int slots, int far, unsigned char* 
   // the query tiles that see key row0: rows from row0 - off on, of each head of the subset
   int q0 = max(t.row0 - off, 0) / ROWS * ROWS, q1 = lenq;
   if constexpr (WIN) {
-    const NearRows near(t.row0, off, lenq, p.window, S::KEYS, ROWS);
+    const NearRows near(t.row0 / S::KEYS * S::KEYS, off, lenq, p.window, S::KEYS, ROWS);
     q1 = min(near.to, lenq);
-    if (far_slot >= 0) {
+    if (is_far) {
       q0 = max(near.to, segment);
       q1 = min(lenq, segment + FAR_ROWS);
       if (q0 >= q1) return;
@@ -179,7 +182,7 @@ __device__ __forceinline__ void dkdv(int id, int slots, int far, unsigned char* 
     for (int u = 0; u < S::BLOCKS; ++u) {
       const int tr = 32 * (S::BLOCKS * part + u), i0 = q0 + j % per * ROWS + tr;  // the wave's rows of the tile: i0 .. i0 + 31
       if (i0 >= lenq || i0 + 31 + off < first_key) continue;                      // none of them sees a key of this wave
-      if (WIN && i0 >= hidden_from) continue;
+      if (WIN && (i0 >= hidden_from || (is_far && ((j * (ROWS / 32) + tr / 32) & 3) != w))) continue;
       // bf16: the sums start at minus lse / scale and minus delta of their rows.  fp32 adds these last: a sum that starts at
       // 100 rounds each of its products at that size.
       constexpr bool START = sizeof(E) == 2;
@@ -249,20 +252,24 @@ __device__ __forceinline__ void dkdv(int id, int slots, int far, unsigned char* 
   const AttnParams& out = params_here();
   const int64_t at = t.lo + key, part_at = (((int64_t)sub * out.total_k + at) * out.KV + e) * P::D;
   const int64_t far_at = ((((int64_t)(far_slot >= 0 ? far_slot : out.far_slots + t.seq) * out.subsets + sub) * out.sinks + key) * out.KV + e) * P::D;
-  const bool sinks = t.row0 < out.sinks && (far_slot >= 0 || (t.seq >= 0 && t.seq < out.nseq));  // (keys outside the offsets have none)
+  const bool sinks = t.row0 < out.sinks && (is_far || (t.seq >= 0 && t.seq < out.nseq));  // (keys outside the offsets have none)
   auto store_k = [&](int ct, const f32x16& x, float f) {
     if (WIN && sinks) store_row32(out.far_dk + far_at + 32 * ct, x, f, half, live && key < out.sinks);
-    if (WIN && far_slot >= 0) return;
+    if (is_far) return;
     if (out.subsets > 1) store_row32(out.part_dk + part_at + 32 * ct, x, f, half, live);
     else store_row32(reinterpret_cast<E*>(out.dk) + at * out.dks[0] + (int64_t)e * out.dks[1] + 32 * ct, x, f, half, live);
   };
   auto store_v = [&](int ct, const f32x16& x) {
     if (WIN && sinks) store_row32(out.far_dv + far_at + 32 * ct, x, 1.f, half, live && key < out.sinks);
-    if (WIN && far_slot >= 0) return;
+    if (is_far) return;
     if (out.subsets > 1) store_row32(out.part_dv + part_at + 32 * ct, x, 1.f, half, live);
     else store_row32(reinterpret_cast<E*>(out.dv) + at * out.dvs[0] + (int64_t)e * out.dvs[1] + 32 * ct, x, 1.f, half, live);
   };
-  if constexpr (SPLIT == 1) {
+  if (WIN && SPLIT < 4 && is_far) {
+    staged_barrier();
+    if constexpr (DK) join_sums<4>(dk, out.scale, lds, w, lane, [&](int ct, const f32x16& x) { store_k(ct, x, 1.f); });
+    if constexpr (DV) join_sums<4>(dv, 1.f, lds, w, lane, store_v);
+  } else if constexpr (SPLIT == 1) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       if constexpr (DK) store_k(ct, dk[ct], out.scale);
@@ -464,7 +471,7 @@ static int launch_grads(const AttnParams& p, hipStream_t st) {
   const int64_t slots_k = p.total_k > 0 ? tile_slots(p.total_k, Dkdv<P, SPLIT>::KEYS, p.nseq) : 0;
   const int64_t slots_q = p.total_q > 0 ? tile_slots(p.total_q, Dq<P, SPLIT>::ROWS, p.nseq) : 0;
   const int64_t far = WIN && p.sinks > 0 && p.total_q > 0 && p.total_k > 0
-                          ? tile_slots(p.total_q, FAR_ROWS, p.nseq) * ((p.sinks + Dkdv<P, SPLIT>::KEYS - 1) / Dkdv<P, SPLIT>::KEYS) * p.KV * p.subsets
+                          ? tile_slots(p.total_q, FAR_ROWS, p.nseq) * ((p.sinks + 31) / 32) * p.KV * p.subsets
                           : 0;
   const int64_t nk = slots_k * p.KV * p.subsets + far, part = (nk + 7) / 8 * 8;  // a workgroup's number mod 8 is its XCD
   const int64_t grid = part * (P::D == 64 ? 1 : 2) + slots_q * p.H;

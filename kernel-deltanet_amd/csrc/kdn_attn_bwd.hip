@@ -70,6 +70,7 @@ __device__ __forceinline__ const AttnParams& params_here() {
 // of 1024, 32 heads of 128, 1448 us, so 1429).  Their sums of the sinks' dk
 // and dv come to lie apart in fp32, as the near rows' do a second time; attn_sinks_kernel adds them in a fixed order.
 constexpr int FAR_ROWS = 1024;
+constexpr int FAR_SINKS = 256;  // with more, their tiles are many themselves, and walked by one workgroup each: no segments
 // The query rows [from, to) of a sequence that see keys of the tile row0 .. row0 + keys - 1 for nearness, in whole tiles of `rows`.
 // Those from `to` on see of it the sinks alone.
 struct NearRows {
@@ -148,7 +149,7 @@ __device__ __forceinline__ void dkdv(int id, int slots, int far, unsigned char* 
   int q0 = max(t.row0 - off, 0) / ROWS * ROWS, q1 = lenq;
   if constexpr (WIN) {
     const NearRows near(t.row0 / S::KEYS * S::KEYS, off, lenq, p.window, S::KEYS, ROWS);
-    q1 = min(near.to, lenq);
+    if (p.far_slots > 0 || t.row0 >= p.sinks) q1 = min(near.to, lenq);
     if (is_far) {
       q0 = max(near.to, segment);
       q1 = min(lenq, segment + FAR_ROWS);
@@ -252,7 +253,7 @@ __device__ __forceinline__ void dkdv(int id, int slots, int far, unsigned char* 
   const AttnParams& out = params_here();
   const int64_t at = t.lo + key, part_at = (((int64_t)sub * out.total_k + at) * out.KV + e) * P::D;
   const int64_t far_at = ((((int64_t)(far_slot >= 0 ? far_slot : out.far_slots + t.seq) * out.subsets + sub) * out.sinks + key) * out.KV + e) * P::D;
-  const bool sinks = t.row0 < out.sinks && (is_far || (t.seq >= 0 && t.seq < out.nseq));  // (keys outside the offsets have none)
+  const bool sinks = out.far_slots > 0 && t.row0 < out.sinks && (is_far || (t.seq >= 0 && t.seq < out.nseq));  // (keys outside the offsets have none)
   auto store_k = [&](int ct, const f32x16& x, float f) {
     if (WIN && sinks) store_row32(out.far_dk + far_at + 32 * ct, x, f, half, live && key < out.sinks);
     if (is_far) return;
@@ -470,12 +471,11 @@ template <class P, int SPLIT, bool WIN>
 static int launch_grads(const AttnParams& p, hipStream_t st) {
   const int64_t slots_k = p.total_k > 0 ? tile_slots(p.total_k, Dkdv<P, SPLIT>::KEYS, p.nseq) : 0;
   const int64_t slots_q = p.total_q > 0 ? tile_slots(p.total_q, Dq<P, SPLIT>::ROWS, p.nseq) : 0;
-  const int64_t far = WIN && p.sinks > 0 && p.total_q > 0 && p.total_k > 0
-                          ? tile_slots(p.total_q, FAR_ROWS, p.nseq) * ((p.sinks + 31) / 32) * p.KV * p.subsets
-                          : 0;
+  const int64_t far = WIN && p.total_q > 0 ? p.far_slots * ((p.sinks + 31) / 32) * p.KV * p.subsets : 0;
+  const int64_t far_blocks = far > 0 ? (p.nseq * p.sinks * p.KV * (P::D / 4) + 255) / 256 : 0;
   const int64_t nk = slots_k * p.KV * p.subsets + far, part = (nk + 7) / 8 * 8;  // a workgroup's number mod 8 is its XCD
   const int64_t grid = part * (P::D == 64 ? 1 : 2) + slots_q * p.H;
-  if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  if (grid > INT32_MAX || far_blocks > INT32_MAX) return KDN_ERR_UNSUPPORTED;
   hipLaunchKernelGGL((attn_grads_kernel<P, SPLIT, WIN>), dim3((unsigned)grid), dim3(256), 0, st, p, (int)slots_k, (int)slots_q, (int)part, (int)nk,
                      (int)far);
   int rc = launch_status();
@@ -485,9 +485,7 @@ static int launch_grads(const AttnParams& p, hipStream_t st) {
     hipLaunchKernelGGL(attn_subsets_kernel<P>, dim3((unsigned)blocks), dim3(256), 0, st, p);
     rc = launch_status();
   }
-  if (rc == KDN_OK && far > 0 && p.nseq > 0) {
-    const int64_t far_blocks = (p.nseq * p.sinks * p.KV * (P::D / 4) + 255) / 256;
-    if (far_blocks > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  if (rc == KDN_OK && far_blocks > 0) {
     hipLaunchKernelGGL(attn_sinks_kernel<P>, dim3((unsigned)far_blocks), dim3(256), 0, st, p, Dkdv<P, SPLIT>::KEYS, Dkdv<P, SPLIT>::ROWS);
     rc = launch_status();
   }
@@ -527,11 +525,17 @@ static int bwd_subsets(const kdn_attn_args* f, bool window) {
 }
 static size_t bwd_row_bytes(const kdn_attn_args* f) { return ((size_t)f->H * (size_t)f->total_q * 4 + 255) / 256 * 256 + 256; }
 static size_t bwd_part_bytes(const kdn_attn_args* f) { return (size_t)f->total_k * (size_t)f->H_kv * (size_t)f->d * 4; }
-// Of the far rows' segments and the near rows of each sequence, `sinks` after attn_window.
+// Slots of the far rows' segments, `sinks` after attn_window.
+static int64_t bwd_far_slots(const kdn_attn_args* f, int64_t sinks) {
+  return sinks > 0 && sinks <= FAR_SINKS ? tile_slots(f->total_q, FAR_ROWS, f->num_seqs) : 0;
+}
+// Of those and the near rows of each sequence.
 static size_t bwd_far_bytes(const kdn_attn_args* f, int subsets, int64_t sinks) {
+  const int64_t slots = bwd_far_slots(f, sinks);
+  if (slots == 0) return 0;
   const size_t each = (size_t)subsets * (size_t)sinks * (size_t)f->H_kv * (size_t)f->d * 4;
   size_t all;
-  return __builtin_mul_overflow((size_t)(tile_slots(f->total_q, FAR_ROWS, f->num_seqs) + f->num_seqs), each, &all) || all > ((size_t)1 << 48) ? (size_t)1 << 48 : all;
+  return __builtin_mul_overflow((size_t)(slots + f->num_seqs), each, &all) || all > ((size_t)1 << 48) ? (size_t)1 << 48 : all;
 }
 
 }  // namespace kdn
@@ -574,7 +578,7 @@ static int attn_bwd(const kdn_attn_bwd_args* a, int64_t window, int64_t sinks, v
   p.subsets = bwd_subsets(f, p.window < NO_WINDOW);
   p.part_dk = reinterpret_cast<float*>((unsigned char*)a->workspace + 2 * bwd_row_bytes(f));
   p.part_dv = p.part_dk + (size_t)p.subsets * bwd_part_bytes(f) / 4;
-  p.far_slots = tile_slots(p.total_q, FAR_ROWS, p.nseq);
+  p.far_slots = bwd_far_slots(f, p.sinks);
   p.far_dk = p.subsets > 1 ? p.part_dv + (size_t)p.subsets * bwd_part_bytes(f) / 4 : p.part_dk;
   p.far_dv = p.far_dk + bwd_far_bytes(f, p.subsets, p.sinks) / 4;
   for (int i = 0; i < 2; ++i) {

@@ -527,6 +527,8 @@ def _key_weights(weights: torch.Tensor, slots: Optional[torch.Tensor], streams: 
                          f"got {tuple(weights.shape)} {weights.dtype} on {weights.device}")
     if weights.requires_grad:
         raise ValueError(f"{what}: weights have no gradient")
+    if 0 in weights.stride() and any(s == 0 and n > 1 for s, n in zip(weights.stride(), weights.shape)):
+        raise ValueError(f"{what}: weights are written where they are, and these lie on one another (an expanded tensor)")
     if slots is None:
         if weights.shape[0] != streams:
             raise ValueError(f"{what}: weights of {weights.shape[0]} slots for {streams} streams need slots")

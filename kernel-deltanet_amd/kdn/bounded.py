@@ -141,8 +141,8 @@ def evict(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor
     slots, slots_at = _key_weights(weights, slots, B, heads, k_pages, "evict")
     rows, places = weights.shape[0], weights.shape[-1]
     if positions.shape != weights.shape or positions.dtype is not torch.int32 or positions.get_device() != dev or \
-            (places > 1 and positions.stride(-1) != 1):
-        raise ValueError(f"evict: positions are {tuple(weights.shape)} int32 on {weights.device}, places next to one another; got "
+            (places > 1 and positions.stride(-1) != 1) or any(s == 0 and n > 1 for s, n in zip(positions.stride(), positions.shape)):
+        raise ValueError(f"evict: positions are {tuple(weights.shape)} int32 on {weights.device}, places next to one another and none twice; got "
                          f"{tuple(positions.shape)} {positions.dtype} on {positions.device}")
     lens, keep = _ints(lens, "evict lens", torch.int32, dev, B), _ints(keep, "evict keep", torch.int32, dev, B)
     settled = None if settled is None else _ints(settled, "evict settled", torch.int32, dev, B)

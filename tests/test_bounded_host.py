@@ -75,6 +75,10 @@ def test_window_arguments():
     none = L.kdn_attn_bwd_workspace_bytes(ctypes.byref(b))
     assert size(8, 0) == size(4, 4) == size(2 ** 62, 2 ** 62) == size(4, 0) == none  # no window, or none with sinks
     assert size(4, 3) == none + 2 * (8 // 1024 + 3 + 1) * 2 * 3 * 2 * 64 * 4         # slots and sequences, subsets, sinks, heads
+    long = _attn(total_q=4096, total_k=4096)
+    g = N.AttnBwdArgs()
+    g.fwd = ctypes.addressof(long)
+    assert L.kdn_attn_window_bwd_workspace_bytes(ctypes.byref(g), 64, 257) == L.kdn_attn_bwd_workspace_bytes(ctypes.byref(g))  # no segments
     b.workspace, b.workspace_bytes, a.lse = 1 << 12, size(4, 3) - 1, 1 << 12
     b.dy = b.dq = b.dk = b.dv = 1 << 12
     assert L.kdn_attn_window_bwd(ctypes.byref(b), 4, 3, None) == -3

@@ -71,7 +71,7 @@ def test_own_key_lengths_and_empty_rows(lens_q, lens_k, window, sinks, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64)])
-@pytest.mark.parametrize("sinks", [0, 4, 150])
+@pytest.mark.parametrize("sinks", [0, 4, 150, 256, 257, 400])
 def test_rows_far_behind_the_sinks(sinks, dtype, d):
     """More than one segment of far rows to a sequence, their first inside a segment."""
     check([2500, 1100, 40], window=100, sinks=sinks, d=d, dtype=dtype)

@@ -195,7 +195,7 @@ def test_refusals():
     w = torch.zeros(1, 2, 64, device=DEV)
     for bad in (dict(window=0), dict(window=4, sinks=-1), dict(weights=w, parents=parents), dict(weights=w.double()), dict(weights=w[:, :1]),
                 dict(weights=w.cpu()), dict(weights=w.expand(2, 2, 64)), dict(weights=w.transpose(1, 2).contiguous().transpose(1, 2)),
-                dict(weights=w.clone().requires_grad_(True)), dict(weights=w, slots=torch.zeros(2, dtype=torch.int32, device=DEV))):
+                dict(weights=w.clone().requires_grad_(True)), dict(weights=w[:, :1].expand(1, 2, 64), max_new=2), dict(weights=w, slots=torch.zeros(2, dtype=torch.int32, device=DEV))):
         with pytest.raises((ValueError, RuntimeError)):
             anchor.tree_attention(*dev, **bad)
     with pytest.raises(RuntimeError):  # 64 new tokens of 4 heads are more than 32 rows

@@ -222,12 +222,13 @@ __global__ void __launch_bounds__(256, 2) attn_weights_few_kernel(WeightsParams 
   now = after(now);
   if (now.row0 < 0) return;
   load(now, k);
-  int staged = -2;  // the sequence whose rows are in LDS, all of them
+  int staged = -2, known = -2;  // the sequences whose rows are in LDS, all of them, and whose offsets are here
   int64_t qlo = 0;
   int lenq = 0;
   while (now.row0 >= 0) {
     const SeqTile then = after(now);
-    other_rows(p.cu_q, p.nseq, p.total_q, now.seq, qlo, lenq);
+    if (known != now.seq) other_rows(p.cu_q, p.nseq, p.total_q, now.seq, qlo, lenq);
+    known = now.seq;
     const int off = now.len - lenq, first_key = now.row0 + 32 * BLOCKS * w;
     const int each = (lenq + ROWS - 1) / ROWS;
     const int64_t tiles = (int64_t)each * p.G;

@@ -716,7 +716,7 @@ __device__ __forceinline__ void tree_weights(const TreeParams& p, int id) {
   for (int r = 0; r < rows; ++r) {
     const f32x4 s = *reinterpret_cast<const f32x4*>(p.scores + ((int64_t)be * most + r) * p.room + v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(s[i] - norm[r]);
+    for (int i = 0; i < 4; ++i) sum[i] += s[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[i] - norm[r]);  // (not NaN where a row's other scores are)
   }
   const TreeBound bound(p, (int)min((int64_t)max(p.lens[b], 0), p.max_context));
   float* w = p.weights + slot * p.weights_stride[0] + e * p.weights_stride[1];

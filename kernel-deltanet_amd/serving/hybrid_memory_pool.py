@@ -61,7 +61,8 @@ class HybridMemoryPool:
             self._anchor = anchor.PagePool(pages, page_tokens, max_streams)
             self.anchor_slab = torch.empty(pages, anchor_layers, 2, anchor_heads, page_tokens, anchor_dim, dtype=anchor_dtype, device=device)
             self._anchor_stream = {}
-            self._gone, self._settled = {}, {}  # of a stream: tokens that have no place any more; places whose positions are held
+            # of a stream: tokens that have no place any more; places whose positions are held; the fewest places to which it can go back
+            self._gone, self._settled, self._least = {}, {}, {}
             self._weights = None
             if anchor_queries is not None:
                 if anchor_queries < 1 or anchor_queries % anchor_heads:
@@ -86,7 +87,7 @@ class HybridMemoryPool:
             self.prompt_len[slot] = prompt_len
             if self._anchor is not None:
                 self._anchor_stream[slot] = self._anchor.open()
-                self._gone[slot] = self._settled[slot] = 0
+                self._gone[slot] = self._settled[slot] = self._least[slot] = 0
                 if self._weights is not None:
                     self._weights[slot] = 0  # as those of all places behind a stream's last, until a step adds to them
         return slot
@@ -100,7 +101,8 @@ class HybridMemoryPool:
             self.prompt_len[child] = self.prompt_len.get(parent_stream_id, 0)
             if self._anchor is not None:
                 self._anchor_stream[child] = self._anchor.fork(self._anchor_stream[parent_stream_id])
-                self._gone[child], self._settled[child] = self._gone[parent_stream_id], self._settled[parent_stream_id]
+                for t in (self._gone, self._settled, self._least):
+                    t[child] = t[parent_stream_id]
                 if self._weights is not None:
                     for t in (self._weights, self._positions):
                         t[child] = t[parent_stream_id]
@@ -114,7 +116,7 @@ class HybridMemoryPool:
         self.prompt_len.pop(stream_id, None)
         if self._anchor is not None:
             self._anchor.close(self._anchor_stream.pop(stream_id))
-            del self._gone[stream_id], self._settled[stream_id]
+            del self._gone[stream_id], self._settled[stream_id], self._least[stream_id]
 
     # ---- the anchor layers' pages
 
@@ -206,9 +208,14 @@ class HybridMemoryPool:
                           in_order=not any(self._settled[s] for s in streams))
 
     def anchor_truncate(self, stream_id: int, tokens: int) -> None:
-        """The stream's first `tokens` places stay; pages behind them are free."""
+        """The stream's first `tokens` places stay; pages behind them are free.  Not back into places that an eviction filled out
+        of order, nor to where a window reaches pages that have been freed; with 0 the stream begins anew."""
+        if 0 < tokens < self._least[stream_id]:
+            raise ValueError(f"anchor_truncate: stream {stream_id} goes back to {self._least[stream_id]} places at the least (an eviction filled those "
+                             "before, or a window's pages are freed), or to none")
         self._anchor.truncate(self._anchor_stream[stream_id], tokens)
-        self._settled[stream_id] = min(self._settled[stream_id], tokens)
+        if tokens == 0:
+            self._gone[stream_id] = self._settled[stream_id] = self._least[stream_id] = 0
         if self._weights is not None:
             self._weights[stream_id, :, :, tokens:] = 0
 
@@ -225,6 +232,7 @@ class HybridMemoryPool:
             if end > first:
                 self._anchor.drop(i, first, end - first)
                 self._gone[s] += (end - first) * P
+                self._least[s] = max(self._least[s], first * P + window - 1)
                 freed += end - first
         return freed
 
@@ -264,7 +272,7 @@ class HybridMemoryPool:
         for s, i, L in zip(long, ids, lens):
             self._anchor.truncate(i, keep)
             self._gone[s] += L - keep
-            self._settled[s] = keep
+            self._settled[s] = self._least[s] = keep
 
     def anchor_compact(self) -> int:
         """Moves the pages in use to the front of the slab; the number of pages moved.  Plans made before are void."""

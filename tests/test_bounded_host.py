@@ -209,6 +209,10 @@ def test_a_slid_stream_keeps_its_positions():
     assert pool.anchor_slide([s], 50, 20) == 0 and pool.anchor_slide([s], 500) == 0
     f = pool.fork_stream(s)
     assert pool.anchor_plan([f], [1]).positions.tolist() == [202]
+    with pytest.raises(ValueError):  # the window of a token at place 80 begins at 31, where freed pages were
+        pool.anchor_truncate(f, 80)
+    pool.anchor_truncate(f, 81)
+    assert pool.anchor_plan([f], [1]).positions.tolist() == [193]
     with pytest.raises(ValueError):
         pool.anchor_slide([s], 0)
     with pytest.raises(ValueError):
@@ -230,8 +234,14 @@ def test_a_cut_stream_keeps_its_positions():
     plan = pool.anchor_plan([f, s], [1, 3])
     assert plan.positions.tolist() == [100, 100, 101, 102] and not plan.in_order and plan.slots.tolist() == [f, s]
     assert pool.anchor_plan([s], [9]).all_rows.numel() == 112  # more than run: the keys before it whole
-    pool.anchor_truncate(f, 0)
-    assert pool.anchor_plan([f], [1]).in_order
+    for back in (39, 1):  # into the places that are in no order
+        with pytest.raises(ValueError):
+            pool.anchor_truncate(f, back)
+    pool.anchor_truncate(f, 40)
+    assert pool.anchor_plan([f], [1]).positions.tolist() == [100]
+    pool.anchor_truncate(f, 0)  # begins anew
+    plan = pool.anchor_plan([f], [1])
+    assert plan.in_order and plan.positions.tolist() == [0]
     for bad in (dict(streams=[s], keep=-1), dict(streams=[s], keep=4, sinks=-1), dict(streams=[s, s], keep=4)):
         with pytest.raises(ValueError):
             pool.anchor_evict(**bad)

@@ -66,9 +66,11 @@ __device__ __forceinline__ const AttnParams& params_here() {
 // Under a window (WIN) the rows that see a tile of keys end `window` behind it, but for the first `sinks` keys, which all later
 // rows see: one workgroup that walked them all would run on when the others are done (a sequence of 65536 rows and a window of
 // 1024: fifty times as long).  So those rows are cut into segments of FAR_ROWS, a workgroup each and 32 sinks, whose waves share the
-// rows (one wave with all of them: the gradients of 16384 rows in a window
-// of 1024, 32 heads of 128, 1448 us, so 1429).  Their sums of the sinks' dk
-// and dv come to lie apart in fp32, as the near rows' do a second time; attn_sinks_kernel adds them in a fixed order.
+// rows (one wave with all of them: the gradients of 16384 rows in a window of 1024, four sinks, 32 heads of 128 over 8, bf16, 1448 us, so
+// 1429).  Their sums of the sinks' dk and dv come to lie apart in fp32, as the near rows' do a second time; attn_sinks_kernel adds them
+// in a fixed order.
+//   Of those 1429 us dv takes a quarter, dk and dq a third each, the far rows a twentieth; matrix cores busy 39 %, at 2.0 GHz.  With the
+// products that the formulas need, 0.47 PFLOP/s: eight are formed for five, and a tile of 128 keys walks 1152 rows for 1024.
 constexpr int FAR_ROWS = 1024;
 constexpr int FAR_SINKS = 256;  // with more, their tiles are many themselves, and walked by one workgroup each: no segments
 // The query rows [from, to) of a sequence that see keys of the tile row0 .. row0 + keys - 1 for nearness, in whole tiles of `rows`.
@@ -316,18 +318,26 @@ __global__ void __launch_bounds__(256) attn_sinks_kernel(AttnParams p, int keys,
   other_rows(p.cu_q, p.nseq, p.total_q, (int)b, qlo, lenq);
   if (key >= lenk) return;
   f32x4 dk = zero4(), dv = zero4();
-  auto add = [&](int64_t slot) {
-    for (int s = 0; s < p.subsets; ++s) {
-      const int64_t at = (((slot * p.subsets + s) * p.sinks + key) * p.KV + e) * P::D + d;
-      dk += *reinterpret_cast<const f32x4*>(p.far_dk + at);
-      dv += *reinterpret_cast<const f32x4*>(p.far_dv + at);
+  const int64_t step = (int64_t)p.sinks * p.KV * P::D, at = ((int64_t)key * p.KV + e) * P::D + d;
+  auto add = [&](int64_t slot, int64_t slots) {  // of consecutive slots
+    const float *k = p.far_dk + slot * p.subsets * step + at, *v = p.far_dv + slot * p.subsets * step + at;
+    const int64_t n = slots * p.subsets;
+    for (int64_t i0 = 0; i0 < n; i0 += 8) {  // eight on their way at a time
+      f32x4 x[8], y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = *reinterpret_cast<const f32x4*>(k + min(i0 + i, n - 1) * step);
+        y[i] = *reinterpret_cast<const f32x4*>(v + min(i0 + i, n - 1) * step);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i0 + i < n) dk += x[i], dv += y[i];
     }
   };
-  add(p.far_slots + b);
+  add(p.far_slots + b, 1);
   const NearRows near(key / keys * keys, lenk - lenq, lenq, p.window, keys, rows);
   const int64_t first = qlo / FAR_ROWS + b + 1, end = near.to < lenq ? (lenq + FAR_ROWS - 1) / FAR_ROWS : 0;
-#pragma unroll 4
-  for (int64_t i = near.to / FAR_ROWS; i < end; ++i) add(first + i);
+  add(first + near.to / FAR_ROWS, end - near.to / FAR_ROWS);
   const float x[4] = {dk[0], dk[1], dk[2], dk[3]}, y[4] = {dv[0], dv[1], dv[2], dv[3]};
   store4(reinterpret_cast<E*>(p.dk) + (klo + key) * p.dks[0] + e * p.dks[1] + d, x);
   store4(reinterpret_cast<E*>(p.dv) + (klo + key) * p.dvs[0] + e * p.dvs[1] + d, y);
@@ -515,7 +525,8 @@ static int launch_bwd(const AttnParams& p, float* stat, float* delta, hipStream_
 // Subsets of the query heads that share a key head whose dk and dv are summed apart: as many as it takes to have eight
 // workgroups of 128 keys for each CU (two run there at a time, and the first keys have twice the average's work).  8192 rows,
 // 32 heads over 8: four subsets 2900 us a training step, two 2935.
-// Under a window all tiles have about the same work: four workgroups of each CU's are enough.
+// Under a window all tiles have about the same work, and four workgroups for each CU are enough: 16384 rows in a window of 1024, one
+// subset 1951 us a step, two (and their sums' launch) 2062.
 static int bwd_subsets(const kdn_attn_args* f, bool window) {
   const int G = (int)(f->H / f->H_kv);
   const int64_t tiles = f->total_k / 128 * f->H_kv;

@@ -5,7 +5,9 @@
 //     negative is that of their bits), and above all weights the sinks and the latest tokens.  The rank of the last place that stays is
 //     found by its digits from the top, 11, 11 and 10 bits: a histogram in LDS of the places that agree with the digits so
 //     far, and the bin that the wanted count falls into.  Then every wave goes over its stretch of the places three times: equals
-//     of that rank (the lowest of them stay), holes and fillers counted, holes and fillers listed.
+//     of that rank (the lowest of them stay), holes and fillers counted, holes and fillers listed.  32 streams, two layers, eight heads,
+//     4096 to 16384 places, half kept: 48 us for 22 MB of weights read and as much of lists written: a chain of passes over LDS, with a
+//     barrier after each.  144 heads of 1025 places, of which one goes: 12.6.  (The weights one load at a time: 82 for 48.)
 //   move: the i-th filler's key, value go to the i-th hole.  The two lists are disjoint (fillers lie behind the new length), so that
 //     the moves need no order, and no row moves that has not to.
 #include <algorithm>

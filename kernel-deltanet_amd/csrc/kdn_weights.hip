@@ -2,8 +2,13 @@
 // key head e of exp(scale q_ih.k_je - lse_hi), the column sums of the softmax, for a cache that keeps the keys of largest weight.
 //
 // As dk's and dv's walk without their products (kdn_attn_bwd.hip): a wave owns 32 keys, or two times 32, with their K fragments in
-// registers, and the query rows of the heads pass through LDS in tiles of 64; S = Q K^T has a key a lane and its rows in the lane's
+// registers, and the query rows of the heads pass through LDS in tiles of 64 or 128; S = Q K^T has a key a lane and its rows in the lane's
 // registers, so that a column's sum is register arithmetic and one exchange between the halves of the wave.
+//   What bounds it: the exponential of each pair and the multiplication and the addition around it, at 64 features more than the
+// products.  Three prompts of 1000 to 8192 rows, 16 heads of 64 over 4, bf16: 116 us, of which the join 5, 0.73 PFLOP/s; 14.6 vector
+// instructions for each of the matrix cores' (12 are the arithmetic's), which are busy 30 %.  From four keys a row, 32 to a wave, it was
+// 150; with the comparisons of the cut tiles out of the loop 133; with 128 rows a tile 123.  The products of one block beside the
+// exponentials of the one before, in one wave, took 147 for 128 (230 registers).
 #include <algorithm>
 #include <cmath>
 #include "kdn_attn_tile.hpp"
@@ -24,7 +29,6 @@ struct WeightsTile {
   static constexpr int BLOCKS = P::ROW <= 256 ? 2 : 1;  // of 32 keys to a wave: as many as leave the registers of two waves a SIMD
   static constexpr int KEYS = 128 * BLOCKS, ROWS = P::ROW <= 128 ? 128 : 64, TILE = ROWS * P::ROW, SLOT = TILE + ROWS * 4;
 };
-
 
 // exp(scale q.k - lse) of 32 rows from i0 on and a wave's keys, added to the keys' sums: `rows` the tile in LDS, r0 the first row in it,
 // `bits` their -lse in bits.
@@ -171,7 +175,10 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
 
 // Few rows over many keys (the last rows of prompts): a sequence's rows of all heads of a key head stay in LDS while the workgroup
 // goes along the keys, `per` tiles of them one after another, each wave's next K fragments on their way as it works on the present
-// ones.  What is read is K, once.  More rows than LDS holds come in batches, for each tile of keys anew.
+// ones.  What is read is K, once.  More rows than LDS holds come in batches, for each tile of keys anew.  The last 64 rows of five prompts
+// of up to 32768 keys, 32 heads of 128 over 8, bf16: 72 us, 0.19 GB at 2.6 TB/s, 0.33 PFLOP/s: the products and exponentials of a tile come
+// after its keys rather than beside the next one's (matrix cores busy 26 %, CUs 73 %).  By the kernel above, whose workgroups stage the
+// rows anew for every 256 keys: 88.
 template <class P>
 struct WeightsFew {
   static constexpr int BLOCKS = WeightsTile<P>::BLOCKS, KEYS = 128 * BLOCKS, ROWS = 64, TILE = ROWS * P::ROW;
@@ -308,7 +315,8 @@ static int weights_check(const kdn_attn_weights_args* a) {
 
 static int weights_keys(const kdn_attn_weights_args* a) { return a->d * (int)dtype_size(a->dtype) <= 256 ? 256 : 128; }
 
-// Whether an average sequence's rows come to two batches at most of the kernel of few rows.
+// Whether an average sequence's rows come to two batches at most of the kernel of few rows (with 64 rows, four heads to a key head, one:
+// 72 us, the other kernel 88).
 static bool weights_few(const kdn_attn_weights_args* a) {
   const int64_t tiles = (a->total_q / std::max<int64_t>(a->num_seqs, 1) + 63) / 64 * (a->H / a->H_kv);
   return tiles <= 2 * 65536 / (64 * a->d * (int64_t)dtype_size(a->dtype));
@@ -325,7 +333,7 @@ static int weights_parts(const kdn_attn_weights_args* a) {
 
 template <class P>
 static int launch_weights_few(const WeightsParams& p, hipStream_t st) {
-  // as many workgroups as there is room for at a time, each as many tiles
+  // as many workgroups as there is room for at a time, each as many tiles (twice or four times as many: 84 and 83 us for 81)
   const int64_t slots = tile_slots(p.a.total_k, WeightsFew<P>::KEYS, p.a.nseq), groups = std::max<int64_t>(1, 512 / p.a.KV);
   const int64_t per = (slots + groups - 1) / groups, grid = (slots + per - 1) / per * p.a.KV;
   if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;

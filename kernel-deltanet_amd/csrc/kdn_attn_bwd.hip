@@ -506,8 +506,13 @@ template <class P, bool WIN>
 static int launch_grads(const AttnParams& p, hipStream_t st) {
   // one split for both walks, that of the one with fewer tiles (with as many keys as queries they agree: bwd_subsets; few rows
   // over many keys split the keys' walk as well, which has not been measured)
-  const int split = std::max(attn_split(p.total_k, (int64_t)p.KV * p.subsets), attn_split(p.total_q, p.H));
-  return split == 4 ? launch_grads<P, 4, WIN>(p, st) : split == 2 ? launch_grads<P, 2, WIN>(p, st) : launch_grads<P, 1, WIN>(p, st);
+  auto rule = [](int64_t rows, int64_t heads) {
+    return WIN ? window_split(rows, heads, WINDOW_FOUR<P>, sizeof(typename P::elem)) : attn_split(rows, heads);
+  };
+  const int split = std::max(rule(p.total_k, (int64_t)p.KV * p.subsets), rule(p.total_q, p.H));
+  if constexpr (!WIN || WINDOW_FOUR<P>)
+    if (split == 4) return launch_grads<P, 4, WIN>(p, st);
+  return split == 2 ? launch_grads<P, 2, WIN>(p, st) : launch_grads<P, 1, WIN>(p, st);
 }
 
 template <class P>

@@ -185,8 +185,8 @@ struct WeightsFew {
   static constexpr int TILES = 65536 / TILE, LDS = TILES * (TILE + ROWS * 4);  // two workgroups a CU
 };
 
-template <class P, bool WIN>
-__global__ void __launch_bounds__(256, 2) attn_weights_few_kernel(WeightsParams wp, int64_t slots, int64_t per) {
+template <class P, bool WIN>  // (fp32's keys of 128 features, two tiles of them, take the registers of two waves)
+__global__ void __launch_bounds__(256, P::ROW <= 256 ? 2 : 1) attn_weights_few_kernel(WeightsParams wp, int64_t slots, int64_t per) {
   typedef typename P::elem E;
   typedef WeightsFew<P> S;
   constexpr int KS = P::D / 16, BLOCKS = S::BLOCKS, KEYS = S::KEYS, ROWS = S::ROWS, TILES = S::TILES;

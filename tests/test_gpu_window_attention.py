@@ -85,6 +85,14 @@ def test_waves_with_rows_of_their_own(heads, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,d,dtype", [(10, 64, torch.bfloat16), (10, 64, torch.float32), (20, 64, torch.bfloat16), (10, 128, torch.bfloat16),
+                                           (20, 128, torch.bfloat16), (10, 128, torch.float32), (36, 128, torch.float32)])
+def test_batches_between(heads, d, dtype):
+    """Two waves to 32 rows, or one, at sizes between the smallest and those above, with rows far behind the sinks."""
+    check([1350, 600], window=70, sinks=5, H=heads, KV=heads // 2, d=d, dtype=dtype)
+
+
+@pytest.mark.gpu
 def test_many_short_sequences():
     check([(7 * i) % 23 for i in range(150)], window=6, sinks=2, H=2, KV=1)
 

@@ -21,7 +21,8 @@ struct WeightsParams {
   int64_t weights_stride[2], places, num_slots;
   const int32_t* slots;
   float* part;         // [part][key head][total_k], or NULL: the sums go to their places at once
-  int parts, add;
+  float* far_part;     // [far][sequence][key head][sink]: of the rows behind a window, which see the sinks alone
+  int parts, far, far_tiles, add;  // shares of a tile's rows; of the far ones', and tiles of the keys that have some
 };
 
 template <class P>
@@ -97,6 +98,9 @@ __device__ __forceinline__ void put_weight(const WeightsParams& p, int seq, int 
 
 // `parts` workgroups share the tiles of query rows of a tile of keys evenly, each the next stretch of them.  (Fewer for the later
 // keys, which fewer rows see: three prompts of 1000 to 8192 rows 131 us and more, for 127.)
+//   WIN: the rows that see a tile of keys end `window` behind it, but for the sinks'.  Where prompts are long the rows behind are shared
+// by `far` workgroups more for each tile with sinks: one that walked them all would run on when the others are done (one prompt of 8000
+// rows in a window of 300, 32 heads of 128 over 8, as many shares for all tiles: 109 us with 16, 178 with eight).
 template <class P, bool WIN>
 __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) attn_weights_kernel(WeightsParams wp, int64_t slots) {
   typedef typename P::elem E;
@@ -106,33 +110,48 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
   const AttnParams& p = wp.a;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int e = blockIdx.x % p.KV, part = blockIdx.x / p.KV % wp.parts;
-  const SeqTile t = find_heavy<S::KEYS, true>(p.cu_k, p.nseq, p.total_k, blockIdx.x / p.KV / wp.parts, slots, lane);
-  if (t.row0 < 0) return;
+  const int e = blockIdx.x % p.KV;
+  const int64_t u = blockIdx.x / p.KV, nfar = WIN ? p.nseq * wp.far_tiles * wp.far : 0;
+  const bool is_far = WIN && u < nfar;
+  const int parts = is_far ? wp.far : wp.parts, part = (int)((is_far ? u : u - nfar) % parts);
+  SeqTile t;
+  if (is_far) {
+    t.seq = (int)(u / parts / wp.far_tiles);
+    t.row0 = (int)(u / parts % wp.far_tiles) * S::KEYS;
+    other_rows(p.cu_k, p.nseq, p.total_k, t.seq, t.lo, t.len);
+    if (t.row0 >= t.len) return;
+  } else {
+    t = find_heavy<S::KEYS, true>(p.cu_k, p.nseq, p.total_k, (u - nfar) / parts, slots, lane);
+    if (t.row0 < 0) return;
+  }
   const int lenk = t.len;
   int64_t qlo;
   int lenq;
   other_rows(p.cu_q, p.nseq, p.total_q, t.seq, qlo, lenq);
   const int off = lenk - lenq;
   const int first_key = t.row0 + 32 * BLOCKS * w, key = first_key + (lane & 31);
+  // the rows that see a key of the tile, in whole tiles; past the window only the sinks are seen
+  int q0 = max(t.row0 - off, 0) / ROWS * ROWS, q1 = lenq;
+  if (WIN && (wp.far > 0 || t.row0 >= p.sinks)) {
+    const int end = min(lenq, max(t.row0 + S::KEYS - 1 - off + p.window, 0));
+    const int to = q0 < end ? q0 + (end - q0 + ROWS - 1) / ROWS * ROWS : q0;  // whole tiles: the far rows begin behind them
+    if (is_far) q0 = to;
+    else q1 = min(to, lenq);
+  }
+  const int per = q0 < q1 ? (q1 - q0 + ROWS - 1) / ROWS : 0;
+  const int64_t all = (int64_t)per * p.G, j0 = all * part / parts;
+  const int tiles = (int)(all * (part + 1) / parts - j0);
   typename P::frag k[BLOCKS][KS];
+  float sum[BLOCKS];
 #pragma unroll
   for (int b = 0; b < BLOCKS; ++b) {
+    sum[b] = 0.f;
+    if (tiles == 0) continue;  // (behind a window most keys have no rows here)
     const E* src = reinterpret_cast<const E*>(p.k) + (t.lo + min(key + 32 * b, lenk - 1)) * p.ks[0] + (int64_t)e * p.ks[1];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) k[b][ks] = P::load(src + 16 * ks + 8 * half);
   }
-  float sum[BLOCKS];
-#pragma unroll
-  for (int b = 0; b < BLOCKS; ++b) sum[b] = 0.f;
   const float c = p.scale * LOG2E;
-
-  // the rows that see a key of the tile, in whole tiles; past the window only the sinks are seen
-  const int q0 = max(t.row0 - off, 0) / ROWS * ROWS;
-  const int q1 = WIN && t.row0 >= p.sinks ? min(lenq, max(t.row0 + S::KEYS - 1 - off + p.window, 0)) : lenq;
-  const int per = q0 < q1 ? (q1 - q0 + ROWS - 1) / ROWS : 0;
-  const int64_t all = (int64_t)per * p.G, j0 = all * part / wp.parts;
-  const int tiles = (int)(all * (part + 1) / wp.parts - j0);
   const Stager<P, ROWS, 4> stage_q(p.qs[0], w, lane);
   float lse = 0.f;  // of the tile that is on its way, 64 rows a wave
   int head = e * p.G, row = q0;  // of that tile
@@ -168,7 +187,9 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
     const int kk = key + 32 * b;
     const float x = half_sum(sum[b]);
     if (half != 0 || kk >= lenk) continue;
-    if (wp.part) wp.part[((int64_t)part * p.KV + e) * p.total_k + t.lo + kk] = x;
+    if (is_far) {
+      if (kk < p.sinks) wp.far_part[(((int64_t)part * p.nseq + t.seq) * p.KV + e) * p.sinks + kk] = x;
+    } else if (wp.part) wp.part[((int64_t)part * p.KV + e) * p.total_k + t.lo + kk] = x;
     else put_weight(wp, t.seq, e, kk, off, x);
   }
 }
@@ -185,8 +206,8 @@ struct WeightsFew {
   static constexpr int TILES = 65536 / TILE, LDS = TILES * (TILE + ROWS * 4);  // two workgroups a CU
 };
 
-template <class P, bool WIN>  // (fp32's keys of 128 features, two tiles of them, take the registers of two waves)
-__global__ void __launch_bounds__(256, P::ROW <= 256 ? 2 : 1) attn_weights_few_kernel(WeightsParams wp, int64_t slots, int64_t per) {
+template <class P>
+__global__ void __launch_bounds__(256, 2) attn_weights_few_kernel(WeightsParams wp, int64_t slots, int64_t per) {
   typedef typename P::elem E;
   typedef WeightsFew<P> S;
   constexpr int KS = P::D / 16, BLOCKS = S::BLOCKS, KEYS = S::KEYS, ROWS = S::ROWS, TILES = S::TILES;
@@ -266,9 +287,8 @@ __global__ void __launch_bounds__(256, P::ROW <= 256 ? 2 : 1) attn_weights_few_k
         for (int u = 0; u < 2; ++u) {
           const int i0 = r0 + 32 * u;
           if (i0 >= lenq || i0 + 31 + off < first_key) continue;
-          if (WIN && window_hides(i0 + off, first_key, first_key + 32 * BLOCKS - 1, p.window, p.sinks)) continue;
-          add_weights<P, BLOCKS, WIN>(sum, k, lds + j * S::TILE, 32 * u, reinterpret_cast<const float*>(lds + TILES * S::TILE) + j * ROWS + 32 * u, i0,
-                                      first_key, lane, c, {off, lenq, p.window, p.sinks});
+          add_weights<P, BLOCKS, false>(sum, k, lds + j * S::TILE, 32 * u, reinterpret_cast<const float*>(lds + TILES * S::TILE) + j * ROWS + 32 * u, i0,
+                                      first_key, lane, c, {off, lenq, 0, 0});
         }
         r0 += ROWS;
         if (r0 >= lenq) r0 = 0;
@@ -300,6 +320,17 @@ __global__ void __launch_bounds__(256) attn_weights_join_kernel(WeightsParams wp
   other_rows(p.cu_q, p.nseq, p.total_q, t.seq, qlo, lenq);
   float sum = 0.f;
   for (int i = 0; i < wp.parts; ++i) sum += wp.part[((int64_t)i * p.KV + e) * p.total_k + t.lo + key];
+  if (wp.far > 0 && key < p.sinks && t.seq >= 0 && t.seq < p.nseq) {
+    const float* from = wp.far_part + ((int64_t)t.seq * p.KV + e) * p.sinks + key;
+    const int64_t step = p.nseq * p.KV * p.sinks;
+    for (int i0 = 0; i0 < wp.far; i0 += 8) {  // eight on their way at a time
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = from[min(i0 + i, wp.far - 1) * step];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += i0 + i < wp.far ? x[i] : 0.f;
+    }
+  }
   put_weight(wp, t.seq, e, key, t.len - lenq, sum);
 }
 
@@ -313,23 +344,42 @@ static int weights_check(const kdn_attn_weights_args* a) {
   return KDN_OK;
 }
 
-static int weights_keys(const kdn_attn_weights_args* a) { return a->d * (int)dtype_size(a->dtype) <= 256 ? 256 : 128; }
-
-// Whether an average sequence's rows come to two batches at most of the kernel of few rows (with 64 rows, four heads to a key head, one:
-// 72 us, the other kernel 88).
-static bool weights_few(const kdn_attn_weights_args* a) {
-  const int64_t tiles = (a->total_q / std::max<int64_t>(a->num_seqs, 1) + 63) / 64 * (a->H / a->H_kv);
-  return tiles <= 2 * 65536 / (64 * a->d * (int64_t)dtype_size(a->dtype));
-}
-
-// Workgroups that share a tile of keys: enough that there are 2048 (the first keys have twice the average's work), but none
-// without a tile of an average sequence's rows.
-static int weights_parts(const kdn_attn_weights_args* a) {
-  if (weights_few(a)) return 1;
-  const int64_t tiles = tile_slots(a->total_k, weights_keys(a), a->num_seqs) * a->H_kv;
-  const int64_t rows = (a->total_q / std::max<int64_t>(a->num_seqs, 1) / 64 + 1) * (a->H / a->H_kv);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({(2048 + tiles - 1) / tiles, rows, 16}));
-}
+// How a call is shared out: by the kernel of few rows or by the other one, there by how many workgroups to a tile of keys, and by how
+// many more to a tile with sinks.
+struct WeightsPlan {
+  bool few;
+  int parts, far, far_tiles;
+  int window, sinks;
+  explicit WeightsPlan(const kdn_attn_weights_args* a) : parts(1), far(0), far_tiles(0) {
+    AttnParams p = {};
+    p.total_k = a->total_k;
+    attn_window(p, a->window > 0 ? a->window : NO_WINDOW, a->sinks);
+    window = p.window, sinks = p.sinks;
+    const bool win = window < NO_WINDOW, bf16 = a->dtype == KDN_DTYPE_BF16;
+    const int row = a->d * (int)dtype_size(a->dtype), keys = row <= 256 ? 256 : 128, rows = row <= 128 ? 128 : 64;
+    const int64_t tiles = tile_slots(a->total_k, keys, a->num_seqs) * a->H_kv, G = a->H / a->H_kv;
+    const int64_t each = a->total_q / std::max<int64_t>(a->num_seqs, 1);  // an average sequence's rows
+    // Few rows: as long as reading K, not the products, is most of it, and there is a tile for every CU.  bf16, us by that kernel and the
+    // other: 128 features, four heads to a key head, four prompts of 16000, their last 1, 64, 256, 512 rows 44 (54), 51 (62), 157 (163),
+    // 299 (293); 64 features 21 (23), 25 (27), 65 (60).  One prompt of 8000, 64 rows: 15 (15).  One of 500, 64 features, 256 rows: 28 (13).
+    // Never fp32 (four prompts of 16000, 64 rows 49 and 54, the other 48 and 52), and no window, which leaves most keys fewer rows.
+    few = bf16 && !win && tiles >= 256 && (each + 63) / 64 * G <= (a->d == 64 ? 4 : 16);
+    if (few) return;
+    // Parts: a part costs a workgroup's start, and all of them a launch, so that there are as many as fill the CUs once, twice if each
+    // has two tiles of rows left, eight times if eight (and an eighth more);
+    // in bf16 a tile of a few rows is too little.  One prompt of 8000, 16 heads of 64 over 4, with 1, 4 and 16 parts: 1 row 11, 12,
+    // 25; 256 rows 28, 18, 30; all rows 538, 159, 103.  Nine of 3000, 32 heads of 128 over 8: 256 rows 90, 105, 206; all rows 431, 417, 551.
+    const int64_t walk = ((win ? std::min<int64_t>(each, window + keys) : each) + rows - 1) / rows * G;
+    const int64_t st = (sinks + keys - 1) / keys;
+    const int64_t busy = win ? std::min(tiles, (((each + window) / keys + 2 + st) * a->num_seqs) * a->H_kv) : tiles;  // tiles that have rows
+    for (int n = 2; n <= 16 && each >= (bf16 ? 32 : 1); ++n)
+      if ((busy * n <= 288 && walk >= (tiles * n <= 2304 ? n : 4 * n)) || (busy * n <= 576 && walk >= 2 * n) || (busy * n <= 2048 && walk >= 8 * n)) parts = n;
+    if (win && sinks > 0 && each > (int64_t)window + 2 * keys && st <= 512 && a->num_seqs <= 512 && a->H_kv <= 512 && st * a->num_seqs * a->H_kv <= 512) {
+      far_tiles = (int)st;
+      far = (int)std::max<int64_t>(1, std::min<int64_t>({1024 / (st * a->num_seqs * a->H_kv), each / rows * G / 2, 64}));
+    }
+  }
+};
 
 template <class P>
 static int launch_weights_few(const WeightsParams& p, hipStream_t st) {
@@ -337,16 +387,17 @@ static int launch_weights_few(const WeightsParams& p, hipStream_t st) {
   const int64_t slots = tile_slots(p.a.total_k, WeightsFew<P>::KEYS, p.a.nseq), groups = std::max<int64_t>(1, 512 / p.a.KV);
   const int64_t per = (slots + groups - 1) / groups, grid = (slots + per - 1) / per * p.a.KV;
   if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
-  if (p.a.window < NO_WINDOW) hipLaunchKernelGGL((attn_weights_few_kernel<P, true>), dim3((unsigned)grid), dim3(256), 0, st, p, slots, per);
-  else hipLaunchKernelGGL((attn_weights_few_kernel<P, false>), dim3((unsigned)grid), dim3(256), 0, st, p, slots, per);
+  hipLaunchKernelGGL(attn_weights_few_kernel<P>, dim3((unsigned)grid), dim3(256), 0, st, p, slots, per);
   return launch_status();
 }
 
 template <class P>
 static int launch_weights(const WeightsParams& p, bool few, hipStream_t st) {
-  if (few) return launch_weights_few<P>(p, st);
-  const int64_t slots = tile_slots(p.a.total_k, WeightsTile<P>::KEYS, p.a.nseq), grid = slots * p.a.KV * p.parts;
-  const int64_t joins = p.parts > 1 ? tile_slots(p.a.total_k, 256, p.a.nseq) * p.a.KV : 0;
+  if constexpr (sizeof(typename P::elem) == 2)
+    if (few) return launch_weights_few<P>(p, st);
+  const int64_t slots = tile_slots(p.a.total_k, WeightsTile<P>::KEYS, p.a.nseq);
+  const int64_t grid = (slots * p.parts + (p.far > 0 ? p.a.nseq * p.far_tiles * p.far : 0)) * p.a.KV;
+  const int64_t joins = p.part ? tile_slots(p.a.total_k, 256, p.a.nseq) * p.a.KV : 0;
   if (grid > INT32_MAX || joins > INT32_MAX) return KDN_ERR_UNSUPPORTED;
   if (p.a.window < NO_WINDOW) hipLaunchKernelGGL((attn_weights_kernel<P, true>), dim3((unsigned)grid), dim3(256), 0, st, p, slots);
   else hipLaunchKernelGGL((attn_weights_kernel<P, false>), dim3((unsigned)grid), dim3(256), 0, st, p, slots);
@@ -360,8 +411,9 @@ using namespace kdn;
 
 extern "C" size_t kdn_attn_weights_workspace_bytes(const kdn_attn_weights_args* a) {
   if (weights_check(a) != KDN_OK) return 0;
-  const size_t parts = (size_t)weights_parts(a);
-  return parts > 1 ? parts * (size_t)a->H_kv * (size_t)a->total_k * 4 : 4;
+  const WeightsPlan plan(a);
+  if (plan.parts == 1 && plan.far == 0) return 4;
+  return ((size_t)plan.parts * (size_t)a->total_k + (size_t)plan.far * (size_t)a->num_seqs * (size_t)plan.sinks) * (size_t)a->H_kv * 4;
 }
 
 extern "C" int kdn_attn_weights(const kdn_attn_weights_args* a, void* stream) {
@@ -374,8 +426,10 @@ extern "C" int kdn_attn_weights(const kdn_attn_weights_args* a, void* stream) {
     return KDN_ERR_MISALIGNED;
   if (!stage_reach(a->q_stride[0], a->dtype)) return KDN_ERR_UNSUPPORTED;
   WeightsParams p = {};
-  p.parts = weights_parts(a);
-  if (p.parts > 1 && (!a->workspace || a->workspace_bytes < kdn_attn_weights_workspace_bytes(a))) return KDN_ERR_WORKSPACE_TOO_SMALL;
+  const WeightsPlan plan(a);
+  p.parts = plan.parts, p.far = plan.far, p.far_tiles = plan.far_tiles;
+  const bool join = plan.parts > 1 || plan.far > 0;
+  if (join && (!a->workspace || a->workspace_bytes < kdn_attn_weights_workspace_bytes(a))) return KDN_ERR_WORKSPACE_TOO_SMALL;
   p.a.q = a->q; p.a.k = a->k;
   for (int i = 0; i < 2; ++i) {
     p.a.qs[i] = a->q_stride[i]; p.a.ks[i] = a->k_stride[i]; p.weights_stride[i] = a->weights_stride[i];
@@ -386,12 +440,13 @@ extern "C" int kdn_attn_weights(const kdn_attn_weights_args* a, void* stream) {
   p.a.nseq = a->num_seqs; p.a.total_q = a->total_q; p.a.total_k = a->total_k;
   p.a.H = (int)a->H; p.a.KV = (int)a->H_kv; p.a.G = (int)(a->H / a->H_kv);
   p.a.scale = a->scale;
-  attn_window(p.a, a->window > 0 ? a->window : NO_WINDOW, a->sinks);
+  p.a.window = plan.window, p.a.sinks = plan.sinks;
   p.weights = a->weights; p.places = a->places; p.num_slots = a->num_slots; p.slots = a->slots;
-  p.part = p.parts > 1 ? reinterpret_cast<float*>(a->workspace) : nullptr;
+  p.part = join ? reinterpret_cast<float*>(a->workspace) : nullptr;
+  p.far_part = plan.far > 0 ? p.part + (size_t)plan.parts * (size_t)a->H_kv * (size_t)a->total_k : nullptr;
   p.add = a->add != 0;
   hipStream_t st = as_stream(stream);
-  const bool few = weights_few(a);
+  const bool few = plan.few;
   if (a->dtype == KDN_DTYPE_BF16) return a->d == 64 ? launch_weights<AttnBF16<64>>(p, few, st) : launch_weights<AttnBF16<128>>(p, few, st);
   return a->d == 64 ? launch_weights<AttnF32<64>>(p, few, st) : launch_weights<AttnF32<128>>(p, few, st);
 }

@@ -29,9 +29,9 @@ _EVICT = struct.Struct("@qqqiiqqqqqqq" + 6 * "P" + 2 * "Pqqqq" + 2 * "Pqqq" + "q
 
 
 @functools.lru_cache(maxsize=64)
-def _weights_bytes(nseq: int, nq: int, nk: int, H: int, KV: int, d: int, dtype: int) -> int:
+def _weights_bytes(nseq: int, nq: int, nk: int, H: int, KV: int, d: int, dtype: int, window: int, sinks: int) -> int:
     """kdn_attn_weights_workspace_bytes, which reads sizes only (each sequence has a slot)."""
-    return N.lib().kdn_attn_weights_workspace_bytes(_WEIGHTS.pack(nseq, nq, nk, H, KV, d, dtype, 0, 1.0, 0, 0, 4, 4, *(0,) * 10, 0, nseq, 0, 0, 0))
+    return N.lib().kdn_attn_weights_workspace_bytes(_WEIGHTS.pack(nseq, nq, nk, H, KV, d, dtype, 0, 1.0, window, sinks, 4, 4, *(0,) * 10, 0, nseq, 0, 0, 0))
 
 
 def attention_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weights: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -70,7 +70,7 @@ def attention_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weigh
     tag, s0, s1, _ = _tag(q.dtype, what), *weights.stride()
     torch.autograd.graph.increment_version(weights)
     with _device(dev):
-        nbytes = _weights_bytes(B, n, k.shape[0], H, KV, d, tag)
+        nbytes = _weights_bytes(B, n, k.shape[0], H, KV, d, tag, near, first)
         ws = q.new_empty(nbytes, dtype=torch.uint8)
         N.check(N.lib().kdn_attn_weights(_WEIGHTS.pack(B, n, k.shape[0], H, KV, d, tag, bool(add), _scale(scale, d, what), near, first, cu_q.data_ptr(),
                                                        0 if cu_k is None else cu_k.data_ptr(), *qs[1:], *ks[1:], lse.data_ptr(), weights.data_ptr(),

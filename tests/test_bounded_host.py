@@ -137,7 +137,12 @@ def test_weights_arguments():
         assert size(args(**kw)) > 0 and call(args(**kw), None) == status
     assert size(args()) == 4  # few rows: no partial sums
     long = dict(total_q=4096, total_k=4096)
-    assert size(args(**long)) == 16 * 2 * 4096 * 4 and call(args(**long), None) == -3  # sixteen workgroups to a tile, no workspace
+    assert 4 < size(args(**long)) <= 16 * 2 * 4096 * 4 and call(args(**long), None) == -3  # workgroups that share a tile, and no workspace
+    sinks = size(args(window=64, sinks=9, **long)) - size(args(window=64, **long))  # partial sums of the rows far behind the sinks
+    assert sinks > 0 and sinks % (2 * 9 * 4) == 0 and size(args(window=64, sinks=4032, **long)) == size(args(**long))
+    for kw in (dict(window=64, sinks=9, num_seqs=1 << 30, num_slots=1 << 30, H=1 << 20, H_kv=1 << 20), dict(window=1, sinks=1 << 29, total_k=1 << 30, total_q=1 << 30),
+               dict(window=2 ** 62, sinks=2 ** 62)):
+        assert size(args(**kw)) > 0
     assert call(args(num_seqs=0, num_slots=0), None) == 0 and call(args(total_k=0, total_q=0), None) == 0
 
 

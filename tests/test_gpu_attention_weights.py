@@ -78,6 +78,23 @@ def test_many_sequences():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("add", [False, True])
+@pytest.mark.parametrize("rows,H,KV,d", [(9, 8, 4, 64), (120, 8, 4, 64), (1, 4, 4, 128), (400, 16, 4, 128)])
+def test_few_rows_over_many_keys(rows, H, KV, d, add):
+    """Rows that stay in LDS while the keys pass: sequences of many and of no rows and keys, more rows than LDS holds among them."""
+    lens_k = [(37 * i) % 400 for i in range(66)] + [3000]
+    check([min(rows * (i % 3) // 2, n + 5) if i != 40 else rows for i, n in enumerate(lens_k)], lens_k, H=H, KV=KV, d=d, add=add)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64), (torch.float32, 128)])
+@pytest.mark.parametrize("lens_q,lens_k,window,sinks", [([2600], [2600], 100, 5), ([2100, 20, 1900], [2100, 20, 1900], 33, 300), ([1500], [1700], 1, 1),
+                                                       ([1500], [1300], 70, 257), ([0, 3000, 0], [50, 2999, 0], 64, 64)])
+def test_rows_far_behind_the_sinks(lens_q, lens_k, window, sinks, dtype, d):
+    check(lens_q, lens_k, d=d, dtype=dtype, window=window, sinks=sinks, add=sinks == 1)
+
+
+@pytest.mark.gpu
 def test_one_workgroup_to_a_tile_of_keys():
     """So many keys that no two workgroups share a tile's rows."""
     check([40, 30], [9000, 8000], H=32, KV=32, d=64)

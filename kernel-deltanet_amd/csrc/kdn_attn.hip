@@ -297,15 +297,14 @@ int attn_split(int64_t rows, int64_t heads) {
 }
 
 // Under a window a row's walk is short, and what waves that share rows pay for it, the copies of tiles that serve fewer rows, weighs more:
-// four while their workgroups are no more than the CUs, two while the tiles themselves are not (fp32, one workgroup a CU: twice the CUs).
-// us with one, two and four waves a row, forward (gradients): bf16, 64 features, 64 tiles, 512 keys 20 (36), 13.5 (29), 11.2 (27); 256 tiles
-// 21 (57), 17 (55), 26 (69); 464 tiles, 64 keys 16 (56), 17.5 (61), 34 (88).  128 features, where four leave one workgroup a CU: 60
-// tiles, 512 keys 24 (46), 17 (40), 17.5 (56); 232 tiles 26 (83), 23 (87), 59 (186); 512 tiles, 256 keys 27 (104), 32 (120), 97 (296).
-// fp32, 64 features, 512 keys: 64 tiles 61 (112), 35 (66), 26 (70); 256 tiles 64 (226), 55 (216), 96 (260); 464 tiles 124 (363), 99 (367), 168 (455).
-int window_split(int64_t rows, int64_t heads, bool four, size_t elem) {
+// four while their workgroups are no more than the CUs, two while the tiles themselves are not.  us with one, two and four waves a row,
+// forward (gradients): bf16, 64 features, 64 tiles, 512 keys 20 (36), 13.5 (29), 11.2 (27); 256 tiles 21 (57), 17 (55), 26 (69); 464 tiles,
+// 64 keys 16 (56), 17.5 (61), 34 (88).  128 features, where four leave one workgroup a CU: 60 tiles, 512 keys 24 (46), 17 (40), 17.5 (56);
+// 232 tiles 26 (83), 23 (87), 59 (186); 512 tiles, 256 keys 27 (104), 32 (120), 97 (296).  fp32, 64 features, 512 keys: 64 tiles 61 (112),
+// 35 (66), 26 (70); 256 tiles 64 (226), 55 (216), 96 (260).
+int window_split(int64_t rows, int64_t heads, bool four) {
   const int64_t tiles = rows / 128 * heads;
-  if (tiles <= 64 && four) return 4;
-  return tiles <= (elem == 4 ? 512 : 256) ? 2 : 1;
+  return tiles <= 64 && four ? 4 : tiles <= 256 ? 2 : 1;
 }
 
 AttnParams attn_params(const kdn_attn_args* a) {
@@ -350,10 +349,13 @@ static int launch_fwd(const AttnParams& p, hipStream_t st) {
 
 template <class P, bool WIN>
 static int launch_fwd(const AttnParams& p, hipStream_t st) {
-  const int split = WIN ? window_split(p.total_q, p.H, WINDOW_FOUR<P>, sizeof(typename P::elem)) : attn_split(p.total_q, p.H);
+  const int split = WIN ? window_split(p.total_q, p.H, WINDOW_FOUR<P>) : attn_split(p.total_q, p.H);
   if constexpr (!WIN || WINDOW_FOUR<P>)
     if (split == 4) return launch_fwd<P, 4, WIN>(p, st);
-  return split == 2 ? launch_fwd<P, 2, WIN>(p, st) : launch_fwd<P, 1, WIN>(p, st);
+  // fp32 with 64 features always shares them: so two workgroups' registers fit on a CU (2240 tiles, 256 keys 328 us, so 258)
+  if constexpr (!WIN || P::D == 128 || sizeof(typename P::elem) == 2)
+    if (split == 1) return launch_fwd<P, 1, WIN>(p, st);
+  return launch_fwd<P, 2, WIN>(p, st);
 }
 
 template <class P>

@@ -507,7 +507,7 @@ static int launch_grads(const AttnParams& p, hipStream_t st) {
   // one split for both walks, that of the one with fewer tiles (with as many keys as queries they agree: bwd_subsets; few rows
   // over many keys split the keys' walk as well, which has not been measured)
   auto rule = [](int64_t rows, int64_t heads) {
-    return WIN ? window_split(rows, heads, WINDOW_FOUR<P>, sizeof(typename P::elem)) : attn_split(rows, heads);
+    return WIN ? window_split(rows, heads, WINDOW_FOUR<P>) : attn_split(rows, heads);
   };
   const int split = std::max(rule(p.total_k, (int64_t)p.KV * p.subsets), rule(p.total_q, p.H));
   if constexpr (!WIN || WINDOW_FOUR<P>)

@@ -465,7 +465,7 @@ bool attn_strides_ok(const int64_t s[2], int dtype);
 AttnParams attn_params(const kdn_attn_args* a);
 void attn_window(AttnParams& p, int64_t window, int64_t sinks);
 int attn_split(int64_t rows, int64_t heads);     // waves that share 32 rows
-int window_split(int64_t rows, int64_t heads, bool four, size_t elem);  // the same under a window
+int window_split(int64_t rows, int64_t heads, bool four);  // the same under a window
 template <class P> constexpr bool WINDOW_FOUR = P::D == 64 || sizeof(typename P::elem) == 4;  // whether four ever share them there
 constexpr int64_t NO_WINDOW = 1 << 30;           // more keys than a tensor has
 

@@ -14,7 +14,7 @@
 // over 8: 0.53 GB in 158 us, of which the join 14; matrix cores busy 16 %, CUs 75 %).
 //   Under a window (WIN) a context is what its sinks' and its window's tiles hold, one behind the other, and contexts come to the same
 // length: chunks that share it evenly, 224 streams of up to 32768 keys in a window of 2048 158 us for 0.79 GB (5.0 TB/s), with chunks of
-// 2048 and a rest 176.  The 16 trees in a window of 4096: 99 us, 0.24 GB, bound as without one.
+// 2048 and a rest 176.  The 16 trees in a window of 4096: 84 us, 0.24 GB, bound as without one.
 //   Weights (SCORES): a row's sum is known when its walk is over, so the walk leaves its scores, 4 bytes a row and key, and tree_weights
 // adds up their exponentials.  64 streams of 512 to 16384 keys, 32 heads of 128 over 8: 286 + 20 us, without weights 247 + 6; of the walk's
 // 39 more as many remain with a quarter of the scores written, or in other layouts, or nontemporal.  A second pass over the keys
@@ -784,10 +784,26 @@ static int tree_chunk(const kdn_tree_attn_args* a, int64_t longest) {
   return chunk;
 }
 static int64_t tree_chunks(int64_t longest, int64_t chunk) { return longest > 0 ? (longest + chunk - 1) / chunk : 1; }
-// Under a window most contexts come to the longest one: as many chunks as share it evenly, none of a few keys left over.
+// Under a window most contexts come to the longest one: even chunks, in bf16 as many as fill the GPU once, two workgroups a CU, by the
+// rows that there are rather than the most that a stream may have; where there are more workgroups than that anyway, of 2600 keys, which
+// evens out shorter contexts.  us with as many as the rule above says, and so: 32 heads of 128 over 8, a window of 4000, one token of 16
+// streams 44, 38, eight of 16 54, 40, eight of 64 158, 144, up to 64 of four 55, 47, of 16 112, 107 (but up to 33 of 16 74, 78); a window of
+// 1000, eight of 64 67, 54, up to 64 of 16 69, 50.  Short chunks of many rows do not pay for their partial sums.  fp32, whose products
+// take the time, is the slower for it (64 streams, eight heads of 64 over two, a window of 4000, up to 33 tokens 174, 223).
 static int tree_chunk(const kdn_tree_attn_args* a, const TreePlan& plan) {
-  const int64_t chunk = tree_chunk(a, plan.longest), n = (plan.longest + chunk / 4) / chunk;
-  return !plan.window || n == 0 ? (int)chunk : (int)(((plan.longest + n - 1) / n + 63) / 64 * 64);
+  if (!plan.window || plan.longest == 0) return tree_chunk(a, plan.longest);
+  if (a->dtype != KDN_DTYPE_BF16) {
+    const int64_t chunk = tree_chunk(a, plan.longest), n = std::max<int64_t>(1, (plan.longest + chunk / 4) / chunk);
+    return (int)(((plan.longest + n - 1) / n + 63) / 64 * 64);
+  }
+  const int64_t heads = a->num_seqs * a->H_kv, blocks = tree_blocks(a), rows = times(a->total_new, a->H / a->H_kv);  // rows of all streams to a key head
+  const int64_t units = std::max<int64_t>(1, blocks == 1 ? heads : std::min(std::max(times(rows / 64 + a->num_seqs, a->H_kv) / 2, heads), times(heads, blocks)));
+  const int64_t most = units >= 768 ? (plan.longest + 1300) / 2600 : (512 + units / 2) / units;
+  const int64_t fit = tree_rows(a) <= 32 ? (plan.longest + 32) / 128
+                      : units >= 200    ? plan.longest / 800
+                                        : std::max(plan.longest / 256, std::min(256 / units, plan.longest / 128));
+  const int64_t n = std::max<int64_t>(1, std::min(most, fit)), chunk = ((plan.longest + n - 1) / n + 63) / 64 * 64;
+  return n >= 16 && chunk < 256 ? 128 : (int)chunk;
 }
 
 static int tree_check(const kdn_tree_attn_args* a) {

@@ -30,8 +30,8 @@ struct Fwd {
 
 //   WIN: a row sees the last p.window keys and the first p.sinks.  The walk skips the tiles between (KeyWalk); tiles that the
 // window's edge or the sinks' end passes through select their scores as those on the diagonal do.  One sequence of 32768 rows, 32 heads of
-// 128, bf16, a window of 4096 and four sinks: 2.08 ms, 0.99 PFLOP/s of the pairs that are seen, 1.05 of the tiles' (matrix cores busy
-// 49 %, at 1.7 GHz).  The shorter the window, the more its edges weigh: 16384 rows, 1024 keys 420 us, 0.62 PFLOP/s seen; a workgroup's 45 us
+// 128, bf16, a window of 4096 and four sinks: 2.0 to 2.2 ms by card, 0.94 to 1.03 PFLOP/s of the pairs that are seen (matrix cores busy
+// 49 %, at 1.7 to 1.8 GHz).  The shorter the window, the more its edges weigh: 16384 rows, 1024 keys 420 us, 0.62 PFLOP/s seen; a workgroup's 45 us
 // are 18.4 tiles of 1.94 for the 16 that it sees, 5.3 before the second one, 4.3 for the end.  Seven prompts of 33 to 2048 rows, 16 heads
 // of 64, 256 keys: 23 us, one workgroup's walk of six tiles and what starts and ends it.
 template <class P, int SPLIT, bool WIN>

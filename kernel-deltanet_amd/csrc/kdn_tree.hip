@@ -14,7 +14,7 @@
 // over 8: 0.53 GB in 158 us, of which the join 14; matrix cores busy 16 %, CUs 75 %).
 //   Under a window (WIN) a context is what its sinks' and its window's tiles hold, one behind the other, and contexts come to the same
 // length: chunks that share it evenly, 224 streams of up to 32768 keys in a window of 2048 158 us for 0.79 GB (5.0 TB/s), with chunks of
-// 2048 and a rest 176.  The 16 trees in a window of 4096: 84 us, 0.24 GB, bound as without one.
+// 2048 and a rest 176.  The 16 trees in a window of 4096: 81 us, 0.24 GB, bound as without one.
 //   Weights (SCORES): a row's sum is known when its walk is over, so the walk leaves its scores, 4 bytes a row and key, and tree_weights
 // adds up their exponentials.  64 streams of 512 to 16384 keys, 32 heads of 128 over 8: 286 + 20 us, without weights 247 + 6; of the walk's
 // 39 more as many remain with a quarter of the scores written, or in other layouts, or nontemporal.  A second pass over the keys

@@ -663,19 +663,41 @@ __device__ __forceinline__ void tree_join(const TreeParams& p) {
   const TreeWork t = tree_seq<WIN>(p, b);
   if (r >= t.n * p.G || t.chunks == 1) return;
   const int64_t first = be * p.max_chunks * most + r;
-  float top = -INFINITY;
-  for (int x = lane; x < t.chunks; x += 64) top = fmaxf(top, p.pml[2 * (first + (int64_t)x * most)]);
+  constexpr int V = D / 64, AHEAD = 4;  // chunks whose sums are on their way at a time
+  auto load = [&](int x0, float (&v)[AHEAD][V]) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[j][i] = p.po[(first + (int64_t)min(x0 + j, t.chunks - 1) * most) * D + V * lane + i];
+  };
+  float v[AHEAD][V], top = -INFINITY, ms = -INFINITY, ls = 0.f;  // the maxima and sums of 64 chunks, one a lane
+  load(0, v);
+  auto stats = [&](int x) {
+    const bool there = x + lane < t.chunks;
+    const float* at = p.pml + 2 * (first + (int64_t)min(x + lane, t.chunks - 1) * most);
+    ms = there ? at[0] : -INFINITY;
+    ls = at[1];
+  };
+  for (int x = (t.chunks - 1) / 64 * 64; x >= 0; x -= 64) {
+    stats(x);
+    top = fmaxf(top, ms);
+  }
 #pragma unroll
   for (int s = 1; s < 64; s *= 2) top = fmaxf(top, __shfl_xor(top, s));
-  constexpr int V = D / 64;
   float sum = 0.f, o[V] = {};
-#pragma unroll 4
-  for (int x = 0; x < t.chunks; ++x) {
-    const int64_t at = first + (int64_t)x * most;
-    const float m = p.pml[2 * at], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-    sum += p.pml[2 * at + 1] * f;
+  for (int x0 = 0; x0 < t.chunks; x0 += AHEAD) {
+    if (x0 > 0) load(x0, v);
+    if (x0 > 0 && x0 % 64 == 0) stats(x0);
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = __builtin_fmaf(p.po[at * D + V * lane + i], f, o[i]);
+    for (int j = 0; j < AHEAD; ++j) {
+      if (x0 + j >= t.chunks) break;
+      const float m = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ms), (x0 + j) % 64));
+      const float l = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ls), (x0 + j) % 64));
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+      sum += l * f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = __builtin_fmaf(v[j][i], f, o[i]);
+    }
   }
   const float g = sum == 0.f ? 0.f : 1.f / sum;
   E* dst = reinterpret_cast<E*>(p.y) + (t.lo + r / p.G) * p.ys[0] + (int64_t)(e * p.G + r % p.G) * p.ys[1] + V * lane;

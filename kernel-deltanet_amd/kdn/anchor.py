@@ -341,7 +341,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Opt
     With `window` a query sees of these only the last `window`, j > p - window, and the first `sinks`, j < sinks.
 
     Differentiable in q, k and v, once; gradients come in their dtype, summed in fp32 in a fixed order.  `out`: where y goes
-    (without autograd)."""
+    (without autograd).  A step that is captured into a graph needs leaves of which no eager graph is left (torch runs a leaf's
+    part of the backward on the stream that it was first used on)."""
     if q.dim() == 4:
         if cu_seqlens is not None or cu_seqlens_k is not None or k.dim() != 4 or v.dim() != 4 or k.shape[:2] != q.shape[:2]:
             raise ValueError("attention: (B, T, heads, d) tensors take no cu_seqlens and have one B and T")

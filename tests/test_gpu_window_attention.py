@@ -112,11 +112,11 @@ def test_a_window_over_everything_is_none(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("d", [64, 128])
-def test_what_a_row_does_not_see_may_be_no_number(d, dtype):
+@pytest.mark.parametrize("d,heads", [(64, 4), (128, 4), (64, 60), (128, 60), (64, 160), (128, 160)])
+def test_what_a_row_does_not_see_may_be_no_number(d, heads, dtype):
     """Keys and values that lie before a row's window and behind the sinks: NaN and infinities there leave the row as it was."""
     n, window, sinks = 300, 50, 3
-    q, k, v, _, cu, _ = make([n], [n], 4, 2, d, dtype)
+    q, k, v, _, cu, _ = make([n], [n], heads, heads // 2, d, dtype)
     clean = anchor.attention(*(t.to(DEV) for t in (q, k, v, cu)), window=window, sinks=sinks).cpu()
     k[100], v[100], v[20, :, 7], v[150, 0, 9] = float("nan"), float("inf"), float("-inf"), float("nan")
     got = anchor.attention(*(t.to(DEV) for t in (q, k, v, cu)), window=window, sinks=sinks).cpu()

@@ -11,10 +11,10 @@
 // What bounds them: few rows, HBM (one token of 224 streams, contexts of 512 to 16384, 16 heads of 128 over 4: 2.07 GB in 373 us,
 // 5.5 TB/s; a large copy 4.9, a read 4.0); many, a wave's own chain of copies, products and softmax for each tile, two to a SIMD where
 // 160 rows are five waves on two workgroups, and the unequal chunks' tail (16 trees of 40 drafts, contexts of 1500 to 16384, 32 heads
-// over 8: 0.53 GB in 158 us, of which the join 14; matrix cores busy 16 %, CUs 75 %).
+// over 8: 0.53 GB in 153 us, of which the join 9; matrix cores busy 16 %, CUs 75 %).
 //   Under a window (WIN) a context is what its sinks' and its window's tiles hold, one behind the other, and contexts come to the same
 // length: chunks that share it evenly, 224 streams of up to 32768 keys in a window of 2048 158 us for 0.79 GB (5.0 TB/s), with chunks of
-// 2048 and a rest 176.  The 16 trees in a window of 4096: 81 us, 0.24 GB, bound as without one.
+// 2048 and a rest 176.  The 16 trees in a window of 4096: 77 us, 0.24 GB, bound as without one.
 //   Weights (SCORES): a row's sum is known when its walk is over, so the walk leaves its scores, 4 bytes a row and key, and tree_weights
 // adds up their exponentials.  64 streams of 512 to 16384 keys, 32 heads of 128 over 8: 286 + 20 us, without weights 247 + 6; of the walk's
 // 39 more as many remain with a quarter of the scores written, or in other layouts, or nontemporal.  A second pass over the keys
@@ -651,11 +651,16 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) tr
   }
 }
 
-// The chunks of one row joined in their order: a wave a row, D / 64 values a lane.
+// The chunks of one row joined in their order: half a wave a row, D / 32 values a lane (with a wave a row 16 trees of 40 drafts 12.0 us, so
+// 8.7).
+constexpr int JOIN_LANES = 32, JOIN_ROWS = 256 / JOIN_LANES;
 template <class E, int D, bool WIN>
 __device__ __forceinline__ void tree_join(const TreeParams& p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int L = JOIN_LANES, V = D / L, AHEAD = 4;  // chunks whose sums are on their way at a time
+  typedef float Sums __attribute__((ext_vector_type(V)));
+  typedef E Out __attribute__((ext_vector_type(V)));
+  const int lane = threadIdx.x % L;
+  const int64_t id = (int64_t)blockIdx.x * JOIN_ROWS + threadIdx.x / L;
   const int most = p.max_new * p.G, r = (int)(id % most);
   const int64_t be = id / most;
   if (be >= (int64_t)p.nseq * p.KV) return;
@@ -663,46 +668,44 @@ __device__ __forceinline__ void tree_join(const TreeParams& p) {
   const TreeWork t = tree_seq<WIN>(p, b);
   if (r >= t.n * p.G || t.chunks == 1) return;
   const int64_t first = be * p.max_chunks * most + r;
-  constexpr int V = D / 64, AHEAD = 4;  // chunks whose sums are on their way at a time
-  auto load = [&](int x0, float (&v)[AHEAD][V]) {
+  Sums v[AHEAD];
+  auto load = [&](int x0) {
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[j][i] = p.po[(first + (int64_t)min(x0 + j, t.chunks - 1) * most) * D + V * lane + i];
+    for (int j = 0; j < AHEAD; ++j) v[j] = *reinterpret_cast<const Sums*>(p.po + (first + (int64_t)min(x0 + j, t.chunks - 1) * most) * D + V * lane);
   };
-  float v[AHEAD][V], top = -INFINITY, ms = -INFINITY, ls = 0.f;  // the maxima and sums of 64 chunks, one a lane
-  load(0, v);
+  float top = -INFINITY, m = -INFINITY, l = 0.f;  // the maxima and sums of L chunks, one a lane
+  load(0);
   auto stats = [&](int x) {
-    const bool there = x + lane < t.chunks;
     const float* at = p.pml + 2 * (first + (int64_t)min(x + lane, t.chunks - 1) * most);
-    ms = there ? at[0] : -INFINITY;
-    ls = at[1];
+    m = x + lane < t.chunks ? at[0] : -INFINITY;
+    l = at[1];
   };
-  for (int x = (t.chunks - 1) / 64 * 64; x >= 0; x -= 64) {
+  for (int x = (t.chunks - 1) / L * L; x >= 0; x -= L) {
     stats(x);
-    top = fmaxf(top, ms);
+    top = fmaxf(top, m);
   }
 #pragma unroll
-  for (int s = 1; s < 64; s *= 2) top = fmaxf(top, __shfl_xor(top, s));
-  float sum = 0.f, o[V] = {};
+  for (int s = 1; s < L; s *= 2) top = fmaxf(top, __shfl_xor(top, s, L));
+  float sum = 0.f, f = 0.f;
+  Sums o = 0.f;
   for (int x0 = 0; x0 < t.chunks; x0 += AHEAD) {
-    if (x0 > 0) load(x0, v);
-    if (x0 > 0 && x0 % 64 == 0) stats(x0);
+    if (x0 > 0) load(x0);
+    if (x0 > 0 && x0 % L == 0) stats(x0);
+    if (x0 % L == 0) f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    float fs[AHEAD], ls[AHEAD];
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j) {
-      if (x0 + j >= t.chunks) break;
-      const float m = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ms), (x0 + j) % 64));
-      const float l = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ls), (x0 + j) % 64));
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-      sum += l * f;
+    for (int j = 0; j < AHEAD; ++j) fs[j] = __shfl(f, (x0 + j) % L, L), ls[j] = __shfl(l, (x0 + j) % L, L);
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = __builtin_fmaf(v[j][i], f, o[i]);
-    }
+    for (int j = 0; j < AHEAD; ++j)
+      if (x0 + j < t.chunks) {
+        sum = __builtin_fmaf(ls[j], fs[j], sum);
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = __builtin_fmaf(v[j][i], fs[j], o[i]);
+      }
   }
   const float g = sum == 0.f ? 0.f : 1.f / sum;
   E* dst = reinterpret_cast<E*>(p.y) + (t.lo + r / p.G) * p.ys[0] + (int64_t)(e * p.G + r % p.G) * p.ys[1] + V * lane;
-#pragma unroll
-  for (int i = 0; i < V; ++i) dst[i] = (E)(o[i] * g);
+  *reinterpret_cast<Out*>(dst) = __builtin_convertvector(o * g, Out);
 }
 
 template <class E, int D, bool WIN>
@@ -860,7 +863,7 @@ static int launch_tree(TreeParams& p, hipStream_t st) {
     p.zero_from = (int)((units + 7) / 8 * 8 * blocks);
     hipLaunchKernelGGL((tree_many_kernel<P, WIN>), dim3((unsigned)p.zero_from + ZERO_GROUPS), dim3(256), 0, st, p, blocks);
   }
-  const int64_t joins = p.max_chunks > 1 ? ((int64_t)p.nseq * p.KV * rows + 3) / 4 : 0;
+  const int64_t joins = p.max_chunks > 1 ? ((int64_t)p.nseq * p.KV * rows + JOIN_ROWS - 1) / JOIN_ROWS : 0;
   if (p.weights && p.nseq > 0) {
     const int64_t parts = (p.room + WEIGHT_KEYS - 1) / WEIGHT_KEYS * p.nseq * p.KV;
     hipLaunchKernelGGL((tree_finish_kernel<typename P::elem, P::D, WIN>), dim3((unsigned)(joins + parts)), dim3(256), 0, st, p, (int)joins);

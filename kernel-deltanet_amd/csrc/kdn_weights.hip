@@ -371,7 +371,8 @@ struct WeightsPlan {
     // 25; 256 rows 28, 18, 30; all rows 538, 159, 103.  Nine of 3000, 32 heads of 128 over 8: 256 rows 90, 105, 206; all rows 431, 417, 551.
     const int64_t walk = ((win ? std::min<int64_t>(each, window + keys) : each) + rows - 1) / rows * G;
     const int64_t st = (sinks + keys - 1) / keys;
-    const int64_t busy = win ? std::min(tiles, (((each + window) / keys + 2 + st) * a->num_seqs) * a->H_kv) : tiles;  // tiles that have rows
+    // tiles that have rows
+    const int64_t busy = win ? (int64_t)std::min((double)tiles, (double)((each + window) / keys + 2 + st) * (double)a->num_seqs * (double)a->H_kv) : tiles;
     for (int n = 2; n <= 16 && each >= (bf16 ? 32 : 1); ++n)
       if ((busy * n <= 288 && walk >= (tiles * n <= 2304 ? n : 4 * n)) || (busy * n <= 576 && walk >= 2 * n) || (busy * n <= 2048 && walk >= 8 * n)) parts = n;
     if (win && sinks > 0 && each > (int64_t)window + 2 * keys && st <= 512 && a->num_seqs <= 512 && a->H_kv <= 512 && st * a->num_seqs * a->H_kv <= 512) {

@@ -141,6 +141,7 @@ def test_weights_arguments():
     sinks = size(args(window=64, sinks=9, **long)) - size(args(window=64, **long))  # partial sums of the rows far behind the sinks
     assert sinks > 0 and sinks % (2 * 9 * 4) == 0 and size(args(window=64, sinks=4032, **long)) == size(args(**long))
     for kw in (dict(window=64, sinks=9, num_seqs=1 << 30, num_slots=1 << 30, H=1 << 20, H_kv=1 << 20), dict(window=1, sinks=1 << 29, total_k=1 << 30, total_q=1 << 30),
+               dict(window=1, sinks=1 << 29, total_k=1 << 30, total_q=1 << 30, num_seqs=1 << 30, num_slots=1 << 30, H=1 << 20, H_kv=1 << 20),
                dict(window=2 ** 62, sinks=2 ** 62)):
         assert size(args(**kw)) > 0
     assert call(args(num_seqs=0, num_slots=0), None) == 0 and call(args(total_k=0, total_q=0), None) == 0

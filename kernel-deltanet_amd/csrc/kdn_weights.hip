@@ -195,19 +195,19 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
 }
 
 // Few rows over many keys (the last rows of prompts): a sequence's rows of all heads of a key head stay in LDS while the workgroup
-// goes along the keys, `per` tiles of them one after another, each wave's next K fragments on their way as it works on the present
-// ones.  What is read is K, once.  More rows than LDS holds come in batches, for each tile of keys anew.  The last 64 rows of five prompts
-// of up to 32768 keys, 32 heads of 128 over 8, bf16: 72 us, 0.19 GB at 2.6 TB/s, 0.33 PFLOP/s: the products and exponentials of a tile come
-// after its keys rather than beside the next one's (matrix cores busy 26 %, CUs 73 %).  By the kernel above, whose workgroups stage the
-// rows anew for every 256 keys: 88.
+// goes along the keys, `per` tiles of them one after another, 32 keys a wave.  What is read is K, once.  More rows than LDS holds come in
+// batches, for each tile of keys anew.  Four waves a SIMD have each other's loads, products and exponentials to wait beside: the last 64
+// rows of five prompts of up to 32768 keys, 32 heads of 128 over 8, bf16: 64 us, 0.19 GB at 2.9 TB/s, 0.36 PFLOP/s; with 64 keys a wave,
+// the next ones loaded ahead and two waves a SIMD 71.  Without the products 35 (5.4 TB/s), of which half is what starts and ends it;
+// by the kernel above, whose workgroups stage the rows anew for every 256 keys, 88.
 template <class P>
 struct WeightsFew {
-  static constexpr int BLOCKS = WeightsTile<P>::BLOCKS, KEYS = 128 * BLOCKS, ROWS = 64, TILE = ROWS * P::ROW;
+  static constexpr int WAVES = 8, BLOCKS = 1, KEYS = 32 * WAVES * BLOCKS, ROWS = 64, TILE = ROWS * P::ROW;
   static constexpr int TILES = 65536 / TILE, LDS = TILES * (TILE + ROWS * 4);  // two workgroups a CU
 };
 
 template <class P>
-__global__ void __launch_bounds__(256, 2) attn_weights_few_kernel(WeightsParams wp, int64_t slots, int64_t per) {
+__global__ void __launch_bounds__(64 * WeightsFew<P>::WAVES, 4) attn_weights_few_kernel(WeightsParams wp, int64_t slots, int64_t per) {
   typedef typename P::elem E;
   typedef WeightsFew<P> S;
   constexpr int KS = P::D / 16, BLOCKS = S::BLOCKS, KEYS = S::KEYS, ROWS = S::ROWS, TILES = S::TILES;
@@ -215,8 +215,10 @@ __global__ void __launch_bounds__(256, 2) attn_weights_few_kernel(WeightsParams 
   const AttnParams& p = wp.a;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int e = blockIdx.x % p.KV;
-  int64_t slot = blockIdx.x / p.KV * per - 1;
+  // A workgroup's number mod 8 is its XCD, and an XCD has all heads of its keys: whole rows of them come through its cache (1 % less time
+  // than with a head to an XCD).
+  const int e = blockIdx.x / 8 % p.KV;
+  int64_t slot = ((int64_t)(blockIdx.x / 8 / p.KV) * 8 + blockIdx.x % 8) * per - 1;
   const int64_t end = min(slot + 1 + per, slots);
   SeqTile now;
   now.row0 = -1;
@@ -234,22 +236,22 @@ __global__ void __launch_bounds__(256, 2) attn_weights_few_kernel(WeightsParams 
     t.row0 = -1;
     return t;
   };
-  typename P::frag k[BLOCKS][KS], next[BLOCKS][KS];
-  auto load = [&](const SeqTile& t, typename P::frag (&to)[BLOCKS][KS]) {
+  typename P::frag k[BLOCKS][KS];
+  auto load = [&](const SeqTile& t) {
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) {
       const int64_t key = t.lo + min(t.row0 + 32 * (BLOCKS * w + b) + (lane & 31), t.len - 1);
       const E* src = reinterpret_cast<const E*>(p.k) + key * p.ks[0] + (int64_t)e * p.ks[1];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) to[b][ks] = P::load(src + 16 * ks + 8 * half);
+      for (int ks = 0; ks < KS; ++ks) k[b][ks] = P::load(src + 16 * ks + 8 * half);
     }
     asm volatile("" ::: "memory");  // they are issued here, not where they are used
   };
   const float c = p.scale * LOG2E;
-  const Stager<P, ROWS, 4> stage_q(p.qs[0], w, lane);
+  const Stager<P, ROWS, S::WAVES> stage_q(p.qs[0], w, lane);
   now = after(now);
   if (now.row0 < 0) return;
-  load(now, k);
+  load(now);
   int staged = -2, known = -2;  // the sequences whose rows are in LDS, all of them, and whose offsets are here
   int64_t qlo = 0;
   int lenq = 0;
@@ -263,7 +265,6 @@ __global__ void __launch_bounds__(256, 2) attn_weights_few_kernel(WeightsParams 
     float sum[BLOCKS];
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) sum[b] = 0.f;
-    bool loaded = false;
     for (int64_t j0 = 0; j0 < tiles; j0 += TILES) {
       const int n = (int)min((int64_t)TILES, tiles - j0);
       int r0 = (int)(j0 % each) * ROWS;  // the batch's first tile's first row
@@ -273,15 +274,13 @@ __global__ void __launch_bounds__(256, 2) attn_weights_few_kernel(WeightsParams 
         for (int j = 0; j < n; ++j) {
           const int last = min(lenq - 1 - r, ROWS - 1);
           stage_q(reinterpret_cast<const E*>(p.q) + (qlo + r) * p.qs[0] + (int64_t)h * p.qs[1], last, lds + j * S::TILE);
-          if (w == j % 4) reinterpret_cast<float*>(lds + TILES * S::TILE)[j * ROWS + lane] = p.lse[(int64_t)h * p.total_q + qlo + r + min(lane, last)] * -LOG2E;
+          if (w == j % S::WAVES) reinterpret_cast<float*>(lds + TILES * S::TILE)[j * ROWS + lane] = p.lse[(int64_t)h * p.total_q + qlo + r + min(lane, last)] * -LOG2E;
           r += ROWS;
           if (r >= lenq) r = 0, ++h;
         }
         staged_barrier();
         staged = now.seq;
       }
-      if (!loaded && then.row0 >= 0) load(then, next);
-      loaded = true;
       for (int j = 0; j < n; ++j) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -294,14 +293,12 @@ __global__ void __launch_bounds__(256, 2) attn_weights_few_kernel(WeightsParams 
         if (r0 >= lenq) r0 = 0;
       }
     }
-    if (!loaded && then.row0 >= 0) load(then, next);  // (a sequence without rows)
+    if (then.row0 >= 0) load(then);
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) {
       const int key = first_key + 32 * b + (lane & 31);
       const float x = half_sum(sum[b]);
       if (half == 0 && key < now.len) put_weight(wp, now.seq, e, key, off, x);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) k[b][ks] = next[b][ks];
     }
     now = then;
   }
@@ -359,11 +356,12 @@ struct WeightsPlan {
     const int row = a->d * (int)dtype_size(a->dtype), keys = row <= 256 ? 256 : 128, rows = row <= 128 ? 128 : 64;
     const int64_t tiles = tile_slots(a->total_k, keys, a->num_seqs) * a->H_kv, G = a->H / a->H_kv;
     const int64_t each = a->total_q / std::max<int64_t>(a->num_seqs, 1);  // an average sequence's rows
-    // Few rows: as long as reading K, not the products, is most of it, and there is a tile for every CU.  bf16, us by that kernel and the
-    // other: 128 features, four heads to a key head, four prompts of 16000, their last 1, 64, 256, 512 rows 44 (54), 51 (62), 157 (163),
-    // 299 (293); 64 features 21 (23), 25 (27), 65 (60).  One prompt of 8000, 64 rows: 15 (15).  One of 500, 64 features, 256 rows: 28 (13).
-    // Never fp32 (four prompts of 16000, 64 rows 49 and 54, the other 48 and 52), and no window, which leaves most keys fewer rows.
-    few = bf16 && !win && tiles >= 256 && (each + 63) / 64 * G <= (a->d == 64 ? 4 : 16);
+    // Few rows: as long as reading K, not the products, is most of it, and there are tiles for half the CUs.  bf16, us by that kernel and
+    // the other: 128 features, four heads to a key head, four prompts of 16000, their last 1, 64, 256, 512 rows 35 (54), 47 (62), 157 (163),
+    // 300 (293); 64 features 18 (23), 20 (27), 59 (60).  One prompt of 8000, 64 features, 64 rows: 9 (12).  One of 500, 256 rows: 28 (13).
+    // Never fp32, which waits for its products (four prompts of 16000, 64 rows 49 and 54, the other 48 and 52), and no window, which
+    // leaves most keys fewer rows.
+    few = bf16 && !win && tiles >= 128 && (each + 63) / 64 * G <= (a->d == 64 ? 8 : 16);
     if (few) return;
     // Parts: a part costs a workgroup's start, and all of them a launch, so that there are as many as fill the CUs once, twice if each
     // has two tiles of rows left, eight times if eight (and an eighth more);
@@ -386,9 +384,10 @@ template <class P>
 static int launch_weights_few(const WeightsParams& p, hipStream_t st) {
   // as many workgroups as there is room for at a time, each as many tiles (twice or four times as many: 84 and 83 us for 81)
   const int64_t slots = tile_slots(p.a.total_k, WeightsFew<P>::KEYS, p.a.nseq), groups = std::max<int64_t>(1, 512 / p.a.KV);
-  const int64_t per = (slots + groups - 1) / groups, grid = (slots + per - 1) / per * p.a.KV;
+  const int64_t per = (slots + groups - 1) / groups;
+  const int64_t grid = ((slots + per - 1) / per + 7) / 8 * 8 * p.a.KV;
   if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(attn_weights_few_kernel<P>, dim3((unsigned)grid), dim3(256), 0, st, p, slots, per);
+  hipLaunchKernelGGL(attn_weights_few_kernel<P>, dim3((unsigned)grid), dim3(64 * WeightsFew<P>::WAVES), 0, st, p, slots, per);
   return launch_status();
 }
 

@@ -34,7 +34,11 @@ struct Fwd {
 // 49 %, at 1.7 to 1.8 GHz).  The shorter the window, the more its edges weigh: 16384 rows, 1024 keys 420 us, 0.62 PFLOP/s seen; a workgroup's 45 us
 // are 18.4 tiles of 1.94 for the 16 that it sees, 5.3 before the second one, 4.3 for the end.  Seven prompts of 33 to 2048 rows, 16 heads
 // of 64, 256 keys: 23 us, one workgroup's walk of six tiles and what starts and ends it.
-template <class P, int SPLIT, bool WIN>
+//   EXACT: with what rounding took from the weights, for training where a row sees few keys: one of them may have nearly all the weight,
+// and then ds = p (dp - delta) is what is left of two nearly equal numbers, so that delta = dy.y needs a y of more than the weights' eight
+// bits (dq and dk of windows of 1 to 6 keys and up to four sinks 1.50 to 1.52 times as far from 64 bits as gradients rounded once, so
+// 1.40 to 1.43; from 30 keys on 1.46 at most without it).
+template <class P, int SPLIT, bool WIN, bool EXACT = false>
 __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) attn_fwd_kernel(AttnParams p, int64_t slots) {
   typedef typename P::elem E;
   typedef Fwd<P, SPLIT> S;
@@ -147,6 +151,18 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) at
       for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, r0 + 16 * kk, ct, lane), pf);
     }
     sched_products<P, 2 * S::BLOCKS * CT, P::COL_READS>();
+    if constexpr (EXACT) {
+#pragma unroll
+      for (int b = 0; b < S::BLOCKS; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] -= (float)(E)s[b][i];
+#pragma unroll
+      for (int kk = 0; kk < 2 * S::BLOCKS; ++kk) {
+        const typename P::frag pf = P::from_acc(s[kk >> 1], kk & 1);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) o[ct] = P::mma(o[ct], P::col_frag(vt, r0 + 16 * kk, ct, lane), pf);
+      }
+    }
   };
   if (S::BUFS == 2 && ntiles > 0) stage(0, lds);
   for (int j = 0; j < ntiles; ++j) {
@@ -339,17 +355,23 @@ using namespace kdn;
 extern "C" int kdn_anchor_version(void) { return 1 << 16; }
 extern "C" int kdn_bounded_version(void) { return 1 << 16; }
 
-template <class P, int SPLIT, bool WIN>
+template <class P, int SPLIT, bool WIN, bool EXACT = false>
 static int launch_fwd(const AttnParams& p, hipStream_t st) {
   const int64_t slots = tile_slots(p.total_q, Fwd<P, SPLIT>::ROWS, p.nseq), grid = slots * p.H;
   if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((attn_fwd_kernel<P, SPLIT, WIN>), dim3((unsigned)grid), dim3(256), 0, st, p, slots);
+  hipLaunchKernelGGL((attn_fwd_kernel<P, SPLIT, WIN, EXACT>), dim3((unsigned)grid), dim3(256), 0, st, p, slots);
   return launch_status();
 }
 
 template <class P, bool WIN>
 static int launch_fwd(const AttnParams& p, hipStream_t st) {
   const int split = WIN ? window_split(p.total_q, p.H, WINDOW_FOUR<P>) : attn_split(p.total_q, p.H);
+  if constexpr (WIN && sizeof(typename P::elem) == 2)
+    if (p.low && p.window <= 32 && p.sinks <= 32 - p.window) {  // (never one wave: its registers)
+      if constexpr (P::D == 64)
+        if (split == 4) return launch_fwd<P, 4, true, true>(p, st);
+      return launch_fwd<P, 2, true, true>(p, st);
+    }
   if constexpr (!WIN || WINDOW_FOUR<P>)
     if (split == 4) return launch_fwd<P, 4, WIN>(p, st);
   // fp32 with 64 features always shares them: so two workgroups' registers fit on a CU (2240 tiles, 256 keys 328 us, so 258)

@@ -23,6 +23,7 @@ struct WeightsParams {
   float* part;         // [part][key head][total_k], or NULL: the sums go to their places at once
   float* far_part;     // [far][sequence][key head][sink]: of the rows behind a window, which see the sinks alone
   int parts, far, far_tiles, add;  // shares of a tile's rows; of the far ones', and tiles of the keys that have some
+  int long_rows;       // few rows: a sequence with more has its tiles dealt out; INT_MAX where none has
 };
 
 template <class P>
@@ -206,7 +207,46 @@ struct WeightsFew {
   static constexpr int TILES = 65536 / TILE, LDS = TILES * (TILE + ROWS * 4);  // two workgroups a CU
 };
 
-template <class P>
+// The host knows the sequences' rows together, not apart: a prompt's piece beside decoding streams has many, and the tiles of its keys would be
+// the walks of a few workgroups.  LONG: the tiles of the sequences that have more than long_rows, dealt out one by one; without it
+// those are left out.  128 features, 32 heads over 8, 63 streams with one row and one with 4096, 4096 keys each: 3350 us, so 470; with
+// 256 rows 369, so 173 (one launch for both, with dealt workgroups first, 357 and 178, and its registers cost even batches a tenth).
+//
+// The i-th tile of keys of those sequences, in order; past their last one a negative first row.
+template <int KEYS>
+__device__ __forceinline__ SeqTile long_tile(const WeightsParams& wp, int64_t i, int lane) {
+  const AttnParams& p = wp.a;
+  SeqTile t;
+  t.row0 = -1;
+  for (int64_t b0 = 0; b0 < p.nseq; b0 += 64) {
+    int64_t lo, from;
+    int len, rows;
+    const int b = (int)min(b0 + lane, p.nseq);  // (the number past the last has no rows)
+    other_rows(p.cu_k, p.nseq, p.total_k, b, lo, len);
+    other_rows(p.cu_q, p.nseq, p.total_q, b, from, rows);
+    const int n = rows > wp.long_rows ? (len + KEYS - 1) / KEYS : 0;
+    int upto = n;
+#pragma unroll
+    for (int s = 1; s < 64; s *= 2) {
+      const int x = __shfl_up(upto, s);
+      if (lane >= s) upto += x;
+    }
+    const int all = __builtin_amdgcn_readlane(upto, 63);
+    if (i >= all) {
+      i -= all;
+      continue;
+    }
+    const int at = __builtin_amdgcn_readfirstlane(__popcll(__ballot(upto <= i)));
+    t.seq = (int)b0 + at;
+    t.lo = (int64_t)__builtin_amdgcn_readlane((int)(lo >> 32), at) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, at);
+    t.len = __builtin_amdgcn_readlane(len, at);
+    t.row0 = ((int)i - __builtin_amdgcn_readlane(upto - n, at)) * KEYS;
+    return t;
+  }
+  return t;
+}
+
+template <class P, bool LONG>
 __global__ void __launch_bounds__(64 * WeightsFew<P>::WAVES, 4) attn_weights_few_kernel(WeightsParams wp, int64_t slots, int64_t per) {
   typedef typename P::elem E;
   typedef WeightsFew<P> S;
@@ -218,13 +258,15 @@ __global__ void __launch_bounds__(64 * WeightsFew<P>::WAVES, 4) attn_weights_few
   // A workgroup's number mod 8 is its XCD, and an XCD has all heads of its keys: whole rows of them come through its cache (1 % less time
   // than with a head to an XCD).
   const int e = blockIdx.x / 8 % p.KV;
-  int64_t slot = ((int64_t)(blockIdx.x / 8 / p.KV) * 8 + blockIdx.x % 8) * per - 1;
+  const int64_t group = (int64_t)(blockIdx.x / 8 / p.KV) * 8 + blockIdx.x % 8;
+  int64_t slot = (LONG ? group : group * per) - (LONG ? gridDim.x / p.KV : 1);
   const int64_t end = min(slot + 1 + per, slots);
   SeqTile now;
   now.row0 = -1;
   now.len = 0;
   // the tile after `t`, one with keys, or with a negative first row the end
   auto after = [&](SeqTile t) {
+    if constexpr (LONG) return long_tile<KEYS>(wp, slot += gridDim.x / p.KV, lane);
     while (++slot < end) {
       if (t.row0 >= 0 && t.row0 + KEYS < t.len) {
         t.row0 += KEYS;
@@ -261,7 +303,8 @@ __global__ void __launch_bounds__(64 * WeightsFew<P>::WAVES, 4) attn_weights_few
     known = now.seq;
     const int off = now.len - lenq, first_key = now.row0 + 32 * BLOCKS * w;
     const int each = (lenq + ROWS - 1) / ROWS;
-    const int64_t tiles = (int64_t)each * p.G;
+    const bool others = !LONG && lenq > wp.long_rows;  // the other launch's
+    const int64_t tiles = others ? 0 : (int64_t)each * p.G;
     float sum[BLOCKS];
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) sum[b] = 0.f;
@@ -298,7 +341,7 @@ __global__ void __launch_bounds__(64 * WeightsFew<P>::WAVES, 4) attn_weights_few
     for (int b = 0; b < BLOCKS; ++b) {
       const int key = first_key + 32 * b + (lane & 31);
       const float x = half_sum(sum[b]);
-      if (half == 0 && key < now.len) put_weight(wp, now.seq, e, key, off, x);
+      if (half == 0 && key < now.len && !others) put_weight(wp, now.seq, e, key, off, x);
     }
     now = then;
   }
@@ -345,9 +388,9 @@ static int weights_check(const kdn_attn_weights_args* a) {
 // many more to a tile with sinks.
 struct WeightsPlan {
   bool few;
-  int parts, far, far_tiles;
+  int parts, far, far_tiles, long_rows;
   int window, sinks;
-  explicit WeightsPlan(const kdn_attn_weights_args* a) : parts(1), far(0), far_tiles(0) {
+  explicit WeightsPlan(const kdn_attn_weights_args* a) : parts(1), far(0), far_tiles(0), long_rows(INT32_MAX) {
     AttnParams p = {};
     p.total_k = a->total_k;
     attn_window(p, a->window > 0 ? a->window : NO_WINDOW, a->sinks);
@@ -362,7 +405,10 @@ struct WeightsPlan {
     // Never fp32, which waits for its products (four prompts of 16000, 64 rows 49 and 54, the other 48 and 52), and no window, which
     // leaves most keys fewer rows.
     few = bf16 && !win && tiles >= 128 && (each + 63) / 64 * G <= (a->d == 64 ? 8 : 16);
-    if (few) return;
+    if (few) {  // twice the average's tiles of rows
+      long_rows = (int)std::min<int64_t>(128 * ((std::max<int64_t>(each, 1) + 63) / 64), INT32_MAX);
+      return;
+    }
     // Parts: a part costs a workgroup's start, and all of them a launch, so that there are as many as fill the CUs once, twice if each
     // has two tiles of rows left, eight times if eight (and an eighth more);
     // in bf16 a tile of a few rows is too little.  One prompt of 8000, 16 heads of 64 over 4, with 1, 4 and 16 parts: 1 row 11, 12,
@@ -381,13 +427,18 @@ struct WeightsPlan {
 };
 
 template <class P>
-static int launch_weights_few(const WeightsParams& p, hipStream_t st) {
+static int launch_weights_few(WeightsParams p, hipStream_t st) {
   // as many workgroups as there is room for at a time, each as many tiles (twice or four times as many: 84 and 83 us for 81)
   const int64_t slots = tile_slots(p.a.total_k, WeightsFew<P>::KEYS, p.a.nseq), groups = std::max<int64_t>(1, 512 / p.a.KV);
   const int64_t per = (slots + groups - 1) / groups;
   const int64_t grid = ((slots + per - 1) / per + 7) / 8 * 8 * p.a.KV;
   if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(attn_weights_few_kernel<P>, dim3((unsigned)grid), dim3(64 * WeightsFew<P>::WAVES), 0, st, p, slots, per);
+  // A launch of the long sequences' own takes 2.7 us where there are none; without it the longest walk is that of a stretch whose rows
+  // are all the call's, about a microsecond for each of its tiles of rows.
+  const bool deal = p.a.total_q > p.long_rows && per * ((p.a.total_q + 63) / 64 * p.a.G) > 128;
+  if (deal) hipLaunchKernelGGL((attn_weights_few_kernel<P, true>), dim3((unsigned)((groups + 7) / 8 * 8 * p.a.KV)), dim3(64 * WeightsFew<P>::WAVES), 0, st, p, slots, per);
+  else p.long_rows = INT32_MAX;
+  hipLaunchKernelGGL((attn_weights_few_kernel<P, false>), dim3((unsigned)grid), dim3(64 * WeightsFew<P>::WAVES), 0, st, p, slots, per);
   return launch_status();
 }
 
@@ -427,7 +478,7 @@ extern "C" int kdn_attn_weights(const kdn_attn_weights_args* a, void* stream) {
   if (!stage_reach(a->q_stride[0], a->dtype)) return KDN_ERR_UNSUPPORTED;
   WeightsParams p = {};
   const WeightsPlan plan(a);
-  p.parts = plan.parts, p.far = plan.far, p.far_tiles = plan.far_tiles;
+  p.parts = plan.parts, p.far = plan.far, p.far_tiles = plan.far_tiles, p.long_rows = plan.long_rows;
   const bool join = plan.parts > 1 || plan.far > 0;
   if (join && (!a->workspace || a->workspace_bytes < kdn_attn_weights_workspace_bytes(a))) return KDN_ERR_WORKSPACE_TOO_SMALL;
   p.a.q = a->q; p.a.k = a->k;

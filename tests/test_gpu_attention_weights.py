@@ -174,3 +174,41 @@ def test_refusals():
         with pytest.raises((ValueError, RuntimeError)):
             attention_weights(**{**ok, **bad})
     assert not w.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("add", [False, True])
+def test_long_pieces_among_single_rows(d, add):
+    """A few sequences with far more rows than the others, one of them behind the 64th, one without keys and one that is the last."""
+    lens_k = [(91 * i) % 500 + 60 for i in range(80)]
+    lens_q = [min(1, n) for n in lens_k]
+    for b, rows, keys in ((3, 400, 520), (9, 300, 0), (70, 700, 700), (79, 130, 900)):
+        lens_q[b], lens_k[b] = rows, keys
+    check(lens_q, lens_k, H=32 if d == 128 else 64, KV=32, d=d, add=add)
+
+
+@pytest.mark.gpu
+def test_long_pieces_are_walked_by_many_workgroups():
+    """One piece of a prompt among decoding streams: in one call at most four times as long as the two kinds in calls of their own
+    (when its keys' tiles were the stretch of two workgroups a head, thirteen times)."""
+    H, KV, d, keys, rows, streams = 32, 8, 128, 4096, 4096, 63
+    g = torch.Generator(device=DEV).manual_seed(0)
+    make_bf16 = lambda n, h: torch.randn(n, h, d, generator=g, device=DEV).to(torch.bfloat16)  # noqa: E731
+
+    def took(lens_q):
+        q, k = make_bf16(sum(lens_q), H), make_bf16(keys * len(lens_q), KV)
+        lse = torch.full((H, sum(lens_q)), 9.0, device=DEV)
+        cq, ck = (torch.tensor([0, *n], device=DEV).cumsum(0) for n in (lens_q, [keys] * len(lens_q)))
+        w = torch.zeros(len(lens_q), KV, keys, device=DEV)
+        times = []
+        for _ in range(6):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            attention_weights(q, k, lse, w, cq, ck, add=True)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+
+    assert took([1] * 20 + [rows] + [1] * (streams - 20)) < 4 * (took([1] * streams) + took([rows]))

@@ -75,7 +75,7 @@ int kdn_attn_weights(const kdn_attn_weights_args* a, void* stream);
  * stream holds the token at position positions[slot][layer][head][j] if j < settled[b], else j + evicted[b] (what a stream's
  * tokens so far are more than its places).  Of the places stay: those of positions below `sinks`, then those of the last `recent` of
  * the L + evicted[b] positions, then those of largest weight (a weight that is no positive number counts as 0); of equals the
- * lowest.  The kept places from N on move, in order, to the given-up ones before it, in order: key, value, weight and position;
+ * lowest (of the last `recent`, too, where they and the sinks are more than N: give at most N - sinks to have the latest).  The kept places from N on move, in order, to the given-up ones before it, in order: key, value, weight and position;
  * afterwards positions[0 .. N) are all there (settled is N, evicted L - N more).  What lies from N on is left as it is.
  * The pages of places below N are the stream's own: no other stream has them.  Slots out of range are skipped; slots and pages are
  * distinct.  Needs max_len >= every lens[b] (longer ones are cut), `places` and the page table's room for it. */

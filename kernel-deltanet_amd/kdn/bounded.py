@@ -118,7 +118,8 @@ def evict(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor
     j < settled[b] (none given: 0), else j + evicted[b] (0; how many of a stream's tokens have no place any more).
 
     What stays: the positions below `sinks`, then the last `recent` of the stream's, then those of largest weight (one that is
-    no positive number counts as 0), of equals the lowest places.  The kept places behind the new length go, in order, to the
+    no positive number counts as 0), of equals the lowest places.  That goes for the last `recent`, too: with a `recent` of at most
+    keep - sinks all of them stay, with a larger one the latest may be those that go.  The kept places behind the new length go, in order, to the
     given-up ones before it, in order, with key, value, weight and position; attention does not ask for an order of its keys.
     Afterwards positions of all places below the new length are there: settled is then the new length, evicted greater by what
     went.  What lies behind stays as it is.  The pages of places below the new length have to be the stream's own

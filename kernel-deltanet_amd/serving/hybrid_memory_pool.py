@@ -238,13 +238,15 @@ class HybridMemoryPool:
 
     def anchor_evict(self, streams: Sequence[int], keep: int, sinks: int = 0, recent: int = 0) -> None:
         """Cuts each of the streams to `keep` places, in every layer and head to the positions below `sinks`, the last `recent` and,
-        of the others, the keys of largest weight.  If the pages do not suffice (a stream whose pages others share gets its own),
-        RuntimeError, and no stream is cut.  Plans made before are void."""
+        of the others, the keys of largest weight.  Where those are more than `keep`, the sinks and the latest keep - sinks stay.  If the pages
+        do not suffice (a stream whose pages others share gets its own), RuntimeError, and no stream is cut.  Plans made before are
+        void."""
         if self._weights is None:
             raise ValueError("HybridMemoryPool: weights need anchor_queries")
         keep = operator.index(keep)
         if keep < 0 or operator.index(sinks) < 0 or operator.index(recent) < 0:
             raise ValueError(f"anchor_evict: keep, sinks and recent are 0 or more, got {keep}, {sinks}, {recent}")
+        recent = min(recent, max(keep - sinks, 0))  # of more than there is room for the lowest places would stay, the oldest tokens
         if len(set(streams)) != len(streams):
             raise ValueError("anchor_evict: a stream twice")
         long = [s for s in streams if self._anchor.length(self._anchor_stream[s]) > keep]

@@ -230,3 +230,24 @@ def test_many_query_heads_to_a_key_head():
     w = pool.anchor_weights(0)
     assert float((w[s] - w[t]).abs().max()) < 41 * 36 * 2.0 ** -18
     assert abs(float(w[s].double().sum()) - 41 * 36) < 41 * 36 * 2.0 ** -16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("keep,sinks,recent", [(12, 2, 64), (12, 0, 12), (20, 4, 2 ** 40), (3, 5, 8), (12, 2, 11)])
+def test_a_budget_below_sinks_and_recent_keeps_the_latest(keep, sinks, recent):
+    """Cut after every token, whatever the weights: the sinks, then the latest tokens, the one just written among them."""
+    _, pool = make(layers=2, queries=4)
+    s = pool.allocate_stream(0)
+    total = 50
+    pool.anchor_plan([s], [total])
+    pool._weights[s] = torch.rand(pool._weights[s].shape, device=DEV).sort(-1, descending=True).values  # the oldest the largest
+    for _ in range(6):
+        pool.anchor_evict([s], keep, sinks=sinks, recent=recent)
+        first = min(sinks, keep)
+        want = [*range(first), *range(total - (keep - first), total)]
+        for pos in pool._positions[s, :, :, :keep].flatten(0, 1).tolist():
+            assert sorted(pos) == want
+        assert pool.anchor_tokens(s) == keep
+        pool.anchor_plan([s], [1])
+        pool._weights[s, :, :, keep] = 0.1
+        total += 1

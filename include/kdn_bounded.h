@@ -78,7 +78,7 @@ int kdn_attn_weights(const kdn_attn_weights_args* a, void* stream);
  * lowest (of the last `recent`, too, where they and the sinks are more than N: give at most N - sinks to have the latest).  The kept places from N on move, in order, to the given-up ones before it, in order: key, value, weight and position;
  * afterwards positions[0 .. N) are all there (settled is N, evicted L - N more).  What lies from N on is left as it is.
  * The pages of places below N are the stream's own: no other stream has them.  Slots out of range are skipped; slots and pages are
- * distinct.  Needs max_len >= every lens[b] (longer ones are cut), `places` and the page table's room for it. */
+ * distinct, and no stride over several pages, layers, heads, tokens or slots is 0 (KDN_ERR_INVALID_ARGUMENT).  Needs max_len >= every lens[b] (longer ones are cut), `places` and the page table's room for it. */
 typedef struct kdn_evict_args {
   int64_t num_seqs, layers, H_kv;
   int d, dtype;

@@ -275,6 +275,12 @@ extern "C" int kdn_evict(const kdn_evict_args* a, void* stream) {
     fits = fits && p.kps[i] % 16 == 0 && p.vps[i] % 16 == 0;
   }
   if (!fits) return KDN_ERR_MISALIGNED;
+  // rows, weights and positions that lie on one another would be written more than once, in no order
+  const int64_t sizes[4] = {a->num_pages, a->layers, a->H_kv, a->page_tokens}, slots[3] = {a->num_slots, a->layers, a->H_kv};
+  for (int i = 0; i < 4; ++i)
+    if (sizes[i] > 1 && (a->k_pages_stride[i] == 0 || a->v_pages_stride[i] == 0)) return KDN_ERR_INVALID_ARGUMENT;
+  for (int i = 0; i < 3; ++i)
+    if (slots[i] > 1 && (a->weights_stride[i] == 0 || a->positions_stride[i] == 0)) return KDN_ERR_INVALID_ARGUMENT;
   p.kp = (unsigned char*)a->k_pages; p.vp = (unsigned char*)a->v_pages;
   p.table = a->page_table; p.lens = a->lens; p.keep = a->keep; p.settled = a->settled; p.evicted = a->evicted; p.slots = a->slots;
   p.weights = a->weights; p.positions = a->positions;

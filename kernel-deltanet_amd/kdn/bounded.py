@@ -96,6 +96,9 @@ def _layers(t: torch.Tensor, what: str):
         steps = (steps[0], 0, *steps[1:]) if dim == 4 else steps
     if last != 1 or p & 15 or (steps[0] | steps[1] | steps[2] | steps[3]) & odd:
         raise ValueError(f"{what}: needs contiguous rows that start on 16 bytes (a cache is used where it is, never copied)")
+    if 0 in rest or a == 0:
+        if any(x == 0 and n > 1 for x, n in zip((a, *rest), t.shape)):
+            raise ValueError(f"{what}: rows are written where they are, and these lie on one another (an expanded tensor)")
     return p, *steps
 
 

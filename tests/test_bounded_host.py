@@ -169,6 +169,20 @@ def test_evict_arguments():
     assert call(args(num_seqs=0), None) == 0 and call(args(max_len=0), None) == 0
 
 
+def test_evict_refuses_rows_that_lie_on_one_another():
+    a = N.EvictArgs()
+    a.num_seqs, a.layers, a.H_kv, a.d, a.dtype, a.page_tokens, a.num_pages, a.table_width, a.max_len = 1, 2, 2, 64, 1, 16, 9, 4, 64
+    a.page_table = a.lens = a.keep = a.k_pages = a.v_pages = a.weights = a.positions = a.workspace = 1 << 12
+    a.places, a.num_slots, a.workspace_bytes = 64, 2, 1 << 20
+    strides = dict(k_pages=(8192, 4096, 1024, 64), v_pages=(8192, 4096, 1024, 64), weights=(256, 128, 64), positions=(256, 128, 64))
+    for name in strides:
+        for i in range(len(strides[name])):
+            for n, s in strides.items():
+                for j, x in enumerate(s):
+                    getattr(a, n + "_stride")[j] = 0 if (n, j) == (name, i) else x
+            assert N.lib().kdn_evict(ctypes.byref(a), None) == -1
+
+
 def test_pages_of_ones_own_and_dropped_ones():
     pool = anchor.PagePool(12, 16, 8)
     a = pool.open()

@@ -209,3 +209,22 @@ def test_refusals():
         with pytest.raises((ValueError, RuntimeError)):
             evict(**{**ok, **bad})
     assert torch.equal(slab, before)
+
+
+@pytest.mark.gpu
+def test_rows_that_lie_on_one_another_are_refused():
+    """Expanded pages: a move into one would be a move into several, in no order."""
+    slab, table, w, _ = (t.to(DEV) if isinstance(t, torch.Tensor) else t for t in make([40, 30], layers=2))
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    pos = torch.zeros(w.shape, dtype=torch.int32, device=DEV)
+    k, v = slab[:, :, 0], slab[:, :, 1]
+    before = slab.clone()
+    for one in (k[:1], k[:, :1], k[:, :, :1], k[:, :, :, :1]):
+        for pages in ((one.expand(k.shape), v), (v, one.expand(k.shape))):
+            with pytest.raises(ValueError, match="lie on one another"):
+                evict(*pages, table, ints(40, 30), ints(20, 20), w, pos)
+    with pytest.raises(ValueError, match="lie on one another"):
+        evict(k[:, 0, :1].expand(k[:, 0].shape), v[:, 0], table, ints(40, 30), ints(20, 20), w[:, 0], pos[:, 0])
+    assert torch.equal(slab, before) and not pos.any()
+    one = slab[:, :1, 0], slab[:, :1, 1]  # a single entry's stride may be any
+    evict(*(t.as_strided(t.shape, (t.stride(0), 0, *t.stride()[2:]), t.storage_offset()) for t in one), table, ints(40, 30), ints(20, 20), w[:, :1], pos[:, :1])

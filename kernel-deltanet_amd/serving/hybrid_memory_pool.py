@@ -213,11 +213,12 @@ class HybridMemoryPool:
         if 0 < tokens < self._least[stream_id]:
             raise ValueError(f"anchor_truncate: stream {stream_id} goes back to {self._least[stream_id]} places at the least (an eviction filled those "
                              "before, or a window's pages are freed), or to none")
+        had = self._anchor.length(self._anchor_stream[stream_id])
         self._anchor.truncate(self._anchor_stream[stream_id], tokens)
         if tokens == 0:
             self._gone[stream_id] = self._settled[stream_id] = self._least[stream_id] = 0
-        if self._weights is not None:
-            self._weights[stream_id, :, :, tokens:] = 0
+        if self._weights is not None and tokens < had:
+            self._weights[stream_id, :, :, tokens:had] = 0  # (those behind a stream's last place are 0)
 
     def anchor_slide(self, streams: Sequence[int], window: int, sinks: int = 0) -> int:
         """Frees the pages that no token from now on sees in layers that all have this window and sinks (or smaller ones): those
@@ -270,7 +271,7 @@ class HybridMemoryPool:
             n, k, settled, gone, slots = rest
             bounded.evict(self.anchor_slab[:, :, 0], self.anchor_slab[:, :, 1], tab.view(table.shape), n, k, self._weights, self._positions, settled,
                           gone, sinks=sinks, recent=recent, slots=slots, max_len=max(lens))
-            self._weights[..., keep:].index_fill_(0, slots.long(), 0)
+            self._weights[..., keep:max(lens)].index_fill_(0, slots.long(), 0)
         for s, i, L in zip(long, ids, lens):
             self._anchor.truncate(i, keep)
             self._gone[s] += L - keep

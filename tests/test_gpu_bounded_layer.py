@@ -251,3 +251,23 @@ def test_a_budget_below_sinks_and_recent_keeps_the_latest(keep, sinks, recent):
         pool.anchor_plan([s], [1])
         pool._weights[s, :, :, keep] = 0.1
         total += 1
+
+
+@pytest.mark.gpu
+def test_cutting_clears_the_places_that_streams_had():
+    """Those and no others: what a cut costs goes by what it takes away, not by the longest stream that the pool has room for."""
+    _, pool = make(layers=2, queries=4)
+    a, b, c = (pool.allocate_stream(0) for _ in range(3))
+    pool.anchor_plan([a, b, c], [90, 70, 60])
+    pool._weights.fill_(5.0)
+    w = pool._weights
+    pool.anchor_evict([a, b], 50)
+    assert not w[a, :, :, 50:90].any() and not w[b, :, :, 50:70].any() and bool((w[[a, b]][..., :50] == 5).all())
+    assert bool((w[[a, b]][..., 90:] == 5).all()) and bool((w[c] == 5).all())
+    pool.anchor_truncate(c, 20)
+    assert not w[c, :, :, 20:60].any() and bool((w[c, :, :, :20] == 5).all()) and bool((w[c, :, :, 60:] == 5).all())
+    pool.anchor_truncate(c, 20)
+    with pytest.raises(RuntimeError):
+        pool.anchor_truncate(c, 21)
+    pool.anchor_truncate(c, 0)
+    assert not w[c, :, :, :60].any()

@@ -204,3 +204,25 @@ def test_refusals():
     before = w._version
     anchor.tree_attention(*dev, weights=w, max_new=2)
     assert w._version > before
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", [1, 8])
+@pytest.mark.parametrize("window,sinks", [(2000, 70), (1200, 900), (130, 2000)])
+def test_weights_in_a_window_over_many_chunks(window, sinks, new, d, dtype):
+    """Contexts longer than the window and not; where the window's keys follow the sinks', inside the first chunk and inside later ones."""
+    check([5000, 2100, 900, 3], [new, max(1, new - 3), new, 1], d=d, dtype=dtype, weights=True, window=window, sinks=sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("streams,KV,window", [(70, 8, 900), (100, 8, 900), (97, 8, 5000)])
+def test_large_batches_in_a_window(streams, KV, window, dtype):
+    """More workgroups than run at a time, in one chunk a context and in several; with weights, and a token more for some streams."""
+    g = torch.Generator().manual_seed(streams)
+    lens = torch.randint(0, 2 * window, (streams,), generator=g).tolist()
+    lens[3] = 2 * window
+    for weights in (False, True):
+        check(lens, [1 + (b % 5 == 0) for b in range(streams)], H=KV, KV=KV, dtype=dtype, weights=weights, window=window, sinks=4)

@@ -811,7 +811,8 @@ static int tree_chunk(const kdn_tree_attn_args* a, int64_t longest) {
 static int64_t tree_chunks(int64_t longest, int64_t chunk) { return longest > 0 ? (longest + chunk - 1) / chunk : 1; }
 // Under a window most contexts come to the longest one: even chunks, in bf16 as many as fill the GPU once, two workgroups a CU, by the
 // rows that there are rather than the most that a stream may have; where there are more workgroups than that anyway, of 2600 keys, which
-// evens out shorter contexts.  us with as many as the rule above says, and so: 32 heads of 128 over 8, a window of 4000, one token of 16
+// evens out shorter contexts and a last round of few workgroups (32 heads of 128 over 8, a window of 16000, one token of 65 streams with
+// one chunk each 1034, so 761; of 80 1054, 906; contexts of 200 to 32000, 832, 673).  us with as many as the rule above says, and so: 32 heads of 128 over 8, a window of 4000, one token of 16
 // streams 44, 38, eight of 16 54, 40, eight of 64 158, 144, up to 64 of four 55, 47, of 16 112, 107 (but up to 33 of 16 74, 78); a window of
 // 1000, eight of 64 67, 54, up to 64 of 16 69, 50.  Short chunks of many rows do not pay for their partial sums.  fp32, whose products
 // take the time, is the slower for it (64 streams, eight heads of 64 over two, a window of 4000, up to 33 tokens 174, 223).
@@ -823,7 +824,7 @@ static int tree_chunk(const kdn_tree_attn_args* a, const TreePlan& plan) {
   }
   const int64_t heads = a->num_seqs * a->H_kv, blocks = tree_blocks(a), rows = times(a->total_new, a->H / a->H_kv);  // rows of all streams to a key head
   const int64_t units = std::max<int64_t>(1, blocks == 1 ? heads : std::min(std::max(times(rows / 64 + a->num_seqs, a->H_kv) / 2, heads), times(heads, blocks)));
-  const int64_t most = units >= 768 ? (plan.longest + 1300) / 2600 : (512 + units / 2) / units;
+  const int64_t most = units > 512 ? (plan.longest + 1300) / 2600 : (512 + units / 2) / units;
   const int64_t fit = tree_rows(a) <= 32 ? (plan.longest + 32) / 128
                       : units >= 200    ? plan.longest / 800
                                         : std::max(plan.longest / 256, std::min(256 / units, plan.longest / 128));

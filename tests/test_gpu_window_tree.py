@@ -226,3 +226,28 @@ def test_large_batches_in_a_window(streams, KV, window, dtype):
     lens[3] = 2 * window
     for weights in (False, True):
         check(lens, [1 + (b % 5 == 0) for b in range(streams)], H=KV, KV=KV, dtype=dtype, weights=weights, window=window, sinks=4)
+
+
+@pytest.mark.gpu
+def test_a_stream_more_than_the_gpu_has_room_for_is_no_second_round():
+    """65 streams of eight key heads, a window of 16000, at most a quarter longer than 64, whose workgroups run all at once (in chunks of a
+    whole window half as long again)."""
+    H, KV, d, P, window = 32, 8, 128, 64, 16000
+
+    def took(streams):
+        each = -(-(window + 2000) // P)
+        kp, vp = (torch.zeros(streams * each, KV, P, d, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        table = torch.arange(streams * each, dtype=torch.int32, device=DEV).view(streams, each)
+        q, k = (torch.ones(streams, h, d, dtype=torch.bfloat16, device=DEV) for h in (H, KV))
+        lens = torch.full((streams,), window + 2000, dtype=torch.int32, device=DEV)
+        times = []
+        for _ in range(8):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            anchor.tree_attention(q, k, k, kp, vp, table, lens, max_context=window + 2000, window=window, sinks=4)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+
+    assert took(65) < 1.25 * took(64)

@@ -101,7 +101,9 @@ class AnchorAttentionLayer(nn.Module):
              weights: Optional[torch.Tensor] = None):
         """x (tokens, d_model), the new tokens of plan's streams, against this layer's pages.  Returns the layer's output; for
         a plan of drafts (`keep` false) (output, k, v), of which the caller puts the accepted ones into the pages
-        (anchor.page_append at the rows of a plan made for them).  `weights`: this layer's, to be added to (drafts add nothing)."""
+        (anchor.page_append at the rows of a plan made for them).  `weights`: this layer's, to be added to.  Drafts add nothing, since
+        they may be refused: where a pool keeps weights, the accepted ones' rows of x go through step once more, as a run of the plan made for
+        them, which puts them into the pages and adds what the cached keys got from them."""
         if self.window is not None and not plan.in_order:
             raise ValueError("AnchorAttentionLayer: a window has no meaning over places that an eviction has filled out of order")
         weights = weights if plan.keep else None

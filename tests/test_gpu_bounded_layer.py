@@ -271,3 +271,34 @@ def test_cutting_clears_the_places_that_streams_had():
         pool.anchor_truncate(c, 21)
     pool.anchor_truncate(c, 0)
     assert not w[c, :, :, :60].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_accepted_drafts_weigh_as_tokens_do(dtype):
+    """A tree verified without weights, its accepted path as a run with them: the weights, positions and pages of tokens one by one."""
+    net, pool = make(dtype, queries=4)
+    n, path, tree = 50, [0, 1, 3], [-1, 0, 0, 1]  # draft 2 is refused
+    x = torch.randn(n + 4, 256, device=DEV).to(dtype)
+    with torch.no_grad():
+        a, b = pool.allocate_stream(0), pool.allocate_stream(0)
+        for s in (a, b):
+            step(net, pool, pool.anchor_plan([s], [n]), x[:n], True)
+        pool.anchor_evict([a, b], 40, sinks=2, recent=4)
+        one = torch.cat([step(net, pool, pool.anchor_plan([a], [1]), x[n + t:n + t + 1], True) for t in path])
+        drafts, y, before = pool.anchor_plan([b], [4], depths=[0, 1, 1, 2]), x[n:], []
+        for i, layer in enumerate(net):
+            before.append(y)
+            y = y + layer.step(y, drafts, *pool.anchor_pages(i), parents=torch.tensor(tree, dtype=torch.int32, device=DEV), weights=pool.anchor_weights(i))[0]
+        same(y[path], one, dtype)
+        assert not pool.anchor_weights(0)[b, :, 40:].any()
+        plan = pool.anchor_plan([b], [3])
+        for i, layer in enumerate(net):
+            layer.step(before[i][path], plan, *pool.anchor_pages(i), weights=pool.anchor_weights(i))
+        for i in range(2):
+            w = pool.anchor_weights(i)
+            same(w[b], w[a], dtype)
+            assert bool((w[b, :, 40:43] > 0).all())
+            rows = [pool._anchor.rows(pool._anchor_stream[s], 0, 43) for s in (a, b)]
+            for pages in pool.anchor_pages(i):
+                same(*(pages[r // 16, :, r % 16] for r in rows), dtype)

@@ -7,6 +7,9 @@
 // transposed, S^T = K Q^T and Y^T = V^T P^T: a query is a lane, its scores are 32 of the lane's registers, so the row
 // maximum and sum are register arithmetic and one exchange between the halves of the wave, and P^T is the B operand of
 // the second product as it lies (kdn_attn_tile.hpp).
+//   bf16: the second product takes the weights in bf16, each off by 2^-8 of itself at most, so that y is 0.0020 to 0.0024 of its size from 64
+// bits where its own rounding alone is 0.0016.  What that took, as a product of its own, would be half as many products again on a
+// kernel that products bound (EXACT below has it and what it costs).  Maxima, sums, lse and y's sum are fp32.
 #include <cmath>
 #include "kdn_attn_tile.hpp"
 
@@ -30,14 +33,17 @@ struct Fwd {
 
 //   WIN: a row sees the last p.window keys and the first p.sinks.  The walk skips the tiles between (KeyWalk); tiles that the
 // window's edge or the sinks' end passes through select their scores as those on the diagonal do.  One sequence of 32768 rows, 32 heads of
-// 128, bf16, a window of 4096 and four sinks: 2.0 to 2.2 ms by card, 0.94 to 1.03 PFLOP/s of the pairs that are seen (matrix cores busy
-// 49 %, at 1.7 to 1.8 GHz).  The shorter the window, the more its edges weigh: 16384 rows, 1024 keys 420 us, 0.62 PFLOP/s seen; a workgroup's 45 us
+// 128, bf16, a window of 4096 and four sinks: 2.0 to 2.35 ms by card, 0.88 to 1.03 PFLOP/s of the pairs that are seen (matrix cores busy
+// 49 %, at 1.7 to 1.8 GHz).  The shorter the window, the more its edges weigh: 16384 rows, 1024 keys 420 to 445 us, 0.60 to 0.63 PFLOP/s seen; a workgroup's 45 us
 // are 18.4 tiles of 1.94 for the 16 that it sees, 5.3 before the second one, 4.3 for the end.  Seven prompts of 33 to 2048 rows, 16 heads
 // of 64, 256 keys: 23 us, one workgroup's walk of six tiles and what starts and ends it.
 //   EXACT: with what rounding took from the weights, for training where a row sees few keys: one of them may have nearly all the weight,
 // and then ds = p (dp - delta) is what is left of two nearly equal numbers, so that delta = dy.y needs a y of more than the weights' eight
 // bits (dq and dk of windows of 1 to 6 keys and up to four sinks 1.50 to 1.52 times as far from 64 bits as gradients rounded once, so
-// 1.40 to 1.43; from 30 keys on 1.46 at most without it).
+// 1.40 to 1.43; from 30 keys on 1.46 at most without it: the limit of 32 is where that is no more than longer rows have).  It takes a quarter to
+// two fifths of such a forward, with the waves that then share a row (16384 rows in a window of 32, 32 heads of 128, 146 us, so 184; 16
+// heads of 64 42, 48; a prompt of 2048 22.2, 27.5); forwards without gradients do without it, and their y is another
+// rounding of the same sums.
 template <class P, int SPLIT, bool WIN, bool EXACT = false>
 __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1) attn_fwd_kernel(AttnParams p, int64_t slots) {
   typedef typename P::elem E;

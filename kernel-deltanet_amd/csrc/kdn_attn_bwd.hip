@@ -8,7 +8,8 @@
 // workgroup per 128 query rows of a head walking its keys.  The scores are formed twice (seven products for the five that
 // one pass with atomic sums of dq would take; eight with 128 features, see Dkdv): every sum then has one owner and one order,
 // so that the gradients are the same bits every time.  As in the forward a product's accumulator is the next one's B
-// operand in registers.
+// operand in registers: in bf16 p and ds are rounded to its eight bits there, and dq and dk come 1.40 to 1.46 times as far from 64 bits
+// as sums in fp32 of unrounded ones, rounded once, do; in two parts each, three of the eight products would be six.
 //   What bounds it: as in the forward, products and exponentials that overlap in part.  One sequence of 8192 rows, 32 heads
 // of 128 over 8, bf16: the forward 0.56 ms, the gradients 2.1 to 2.4 (2.20 TFLOP in eight products: 0.9 to 1.0 PFLOP/s; five of
 // them, those that the formulas need, 0.6), at 1.7 to 1.9 GHz.  fp32, 4096 rows, 32 heads of 128: 5.0 ms, matrix cores busy 71 %
@@ -66,11 +67,10 @@ __device__ __forceinline__ const AttnParams& params_here() {
 // Under a window (WIN) the rows that see a tile of keys end `window` behind it, but for the first `sinks` keys, which all later
 // rows see: one workgroup that walked them all would run on when the others are done (a sequence of 65536 rows and a window of
 // 1024: fifty times as long).  So those rows are cut into segments of FAR_ROWS, a workgroup each and 32 sinks, whose waves share the
-// rows (one wave with all of them: the gradients of 16384 rows in a window of 1024, four sinks, 32 heads of 128 over 8, bf16, 1448 us, so
-// 1429).  Their sums of the sinks' dk and dv come to lie apart in fp32, as the near rows' do a second time; attn_sinks_kernel adds them
+// rows (one wave with all of them: the gradients of 16384 rows in a window of 1024, four sinks, 32 heads of 128 over 8, bf16, 1 % more).  Their sums of the sinks' dk and dv come to lie apart in fp32, as the near rows' do a second time; attn_sinks_kernel adds them
 // in a fixed order.
-//   Of those 1429 us dv takes a quarter, dk and dq a third each, the far rows a twentieth; matrix cores busy 39 %, at 2.0 GHz.  With the
-// products that the formulas need, 0.47 PFLOP/s: eight are formed for five, and a tile of 128 keys walks 1152 rows for 1024.
+//   Of their 1430 to 1500 us by card dv takes a quarter, dk and dq a third each, the far rows a twentieth; matrix cores busy 39 %, at 2.0 GHz.  With the
+// products that the formulas need, 0.45 to 0.47 PFLOP/s: eight are formed for five, and a tile of 128 keys walks 1152 rows for 1024.
 constexpr int FAR_ROWS = 1024;
 constexpr int FAR_SINKS = 256;  // with more, their tiles are many themselves, and walked by one workgroup each: no segments
 // The query rows [from, to) of a sequence that see keys of the tile row0 .. row0 + keys - 1 for nearness, in whole tiles of `rows`.

@@ -14,11 +14,14 @@
 // over 8: 0.53 GB in 153 us, of which the join 9; matrix cores busy 16 %, CUs 75 %).
 //   Under a window (WIN) a context is what its sinks' and its window's tiles hold, one behind the other, and contexts come to the same
 // length: chunks that share it evenly, 224 streams of up to 32768 keys in a window of 2048 158 us for 0.79 GB (5.0 TB/s), with chunks of
-// 2048 and a rest 176.  The 16 trees in a window of 4096: 77 us, 0.24 GB, bound as without one.
+// 2048 and a rest 176.  The 16 trees in a window of 4096: 78 us (74 and the join's 9 in a trace), 0.24 GB, bound as without one.
 //   Weights (SCORES): a row's sum is known when its walk is over, so the walk leaves its scores, 4 bytes a row and key, and tree_weights
-// adds up their exponentials.  64 streams of 512 to 16384 keys, 32 heads of 128 over 8: 286 + 20 us, without weights 247 + 6; of the walk's
+// adds up their exponentials.  64 streams of 512 to 16384 keys, 32 heads of 128 over 8: 287 + 22 us, without weights 247 + 6; of the walk's
 // 39 more as many remain with a quarter of the scores written, or in other layouts, or nontemporal.  A second pass over the keys
 // instead would read twice what is read now.
+//   bf16 takes the weights rounded once, as the prompts' kernel does, so that a token's output does not go by which kernel formed it: y is
+// 0.0023 of its size from 64 bits, its own rounding alone 0.0017.  (In two parts, where few rows wait for HBM, that would be 0.0017; the
+// 224 streams in a window 159 us, so 161.5, the 64 with weights 320, 321.  Many rows would have half as many products again.)
 // One token of three streams, contexts of 700 to 2500, fp32: 14 us, and 5 for the join.  Of these the products take 3.4 (a wave has
 // two tiles in turn, 64 products of 64 cycles each, 4 of their 32 columns in use), the rest is the chain from the chunk's number
 // over its page's to the copies.  fp32 of larger sizes is bound by its products: one token of 64 streams, contexts of 512 to 16384,

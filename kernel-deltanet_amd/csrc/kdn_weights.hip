@@ -5,7 +5,7 @@
 // registers, and the query rows of the heads pass through LDS in tiles of 64 or 128; S = Q K^T has a key a lane and its rows in the lane's
 // registers, so that a column's sum is register arithmetic and one exchange between the halves of the wave.
 //   What bounds it: the exponential of each pair and the multiplication and the addition around it, at 64 features more than the
-// products.  Three prompts of 1000 to 8192 rows, 16 heads of 64 over 4, bf16: 116 us, of which the join 5, 0.73 PFLOP/s; 14.6 vector
+// products.  Three prompts of 1000 to 8192 rows, 16 heads of 64 over 4, bf16: 116 to 128 us by card, of which the join 5, 0.65 to 0.72 PFLOP/s; 14.6 vector
 // instructions for each of the matrix cores' (12 are the arithmetic's), which are busy 30 %.  With 32 keys a wave it was 150,
 // with the comparisons of the cut tiles formed for every block 150 too, with 64 rows a tile 133.  The products of one block beside the
 // exponentials of the one before, in one wave, took 147 for 128 (230 registers).

@@ -207,8 +207,8 @@ __global__ void __launch_bounds__(EVICT_THREADS) evict_select_kernel(EvictParams
 // nontemporal.  Of 32 streams' 16 heads of 4096 to 16384 places half kept, 256-byte rows, 1.29 GB read and written: 315 us, 4.1 TB/s
 // (a large copy 4.9); with four rows at a time 354, eight 793, with plain loads and stores two 331.
 constexpr int MOVE_ROWS = 2;
-__global__ void __launch_bounds__(256) evict_move_kernel(EvictParams p, int blocks) {
-  const int unit = blockIdx.x / blocks, block = blockIdx.x % blocks;
+__global__ void __launch_bounds__(256) evict_move_kernel(EvictParams p, int blocks, int first_unit) {
+  const int unit = first_unit + blockIdx.x / blocks, block = blockIdx.x % blocks;
   const int lanes = 1 << p.pieces, piece = threadIdx.x & (lanes - 1), row = threadIdx.x >> p.pieces, rows = 256 >> p.pieces;
   const int n = 2 * p.count[unit], first = block * rows * MOVE_ROWS + row;
   if (block * rows * MOVE_ROWS >= n) return;
@@ -244,7 +244,7 @@ static int evict_check(const kdn_evict_args* a) {
     return KDN_ERR_INVALID_ARGUMENT;
   if (!a->slots && a->num_slots < a->num_seqs) return KDN_ERR_INVALID_ARGUMENT;
   int64_t units;
-  if (__builtin_mul_overflow(a->layers * a->H_kv, a->num_seqs, &units) || units > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  if (__builtin_mul_overflow(a->layers * a->H_kv, a->num_seqs, &units) || units > max_groups(EVICT_THREADS)) return KDN_ERR_UNSUPPORTED;
   return KDN_OK;
 }
 
@@ -299,10 +299,15 @@ extern "C" int kdn_evict(const kdn_evict_args* a, void* stream) {
   p.pieces = __builtin_ctz((unsigned)(a->d * size / 16));
   const int rows = (256 >> p.pieces) * MOVE_ROWS;
   const int64_t blocks = (2 * (a->max_len / 2) + rows - 1) / rows;
-  if (blocks * units > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  const int64_t most = max_groups(256);
+  if (blocks > most) return KDN_ERR_UNSUPPORTED;
   hipStream_t st = as_stream(stream);
   hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)units), dim3(EVICT_THREADS), 0, st, p);
   if ((rc = launch_status()) != KDN_OK || blocks == 0) return rc;
-  hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)(blocks * units)), dim3(256), 0, st, p, (int)blocks);
-  return launch_status();
+  for (int64_t first = 0, n; first < units && rc == KDN_OK; first += n) {  // 64 streams of 32 layers, eight heads and 32768 places are more than one grid
+    n = std::min(most / blocks, units - first);
+    hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)(blocks * n)), dim3(256), 0, st, p, (int)blocks, (int)first);
+    rc = launch_status();
+  }
+  return rc;
 }

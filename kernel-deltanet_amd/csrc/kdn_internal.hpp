@@ -14,6 +14,10 @@ inline int launch_status() {
   return e == hipSuccess ? KDN_OK : KDN_ERR_DEVICE;
 }
 
+// The most workgroups of a launch in one dimension: its work-items are counted in 32 bits, and the runtime takes a larger grid without an
+// error and leaves the rest of it out.
+constexpr int64_t max_groups(int64_t threads) { return (int64_t)UINT32_MAX / threads; }
+
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 inline bool valid_dtype(int dt) { return dt == KDN_DTYPE_F32 || dt == KDN_DTYPE_BF16; }

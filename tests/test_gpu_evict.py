@@ -228,3 +228,22 @@ def test_rows_that_lie_on_one_another_are_refused():
     assert torch.equal(slab, before) and not pos.any()
     one = slab[:, :1, 0], slab[:, :1, 1]  # a single entry's stride may be any
     evict(*(t.as_strided(t.shape, (t.stride(0), 0, *t.stride()[2:]), t.storage_offset()) for t in one), table, ints(40, 30), ints(20, 20), w[:, :1], pos[:, :1])
+
+
+@pytest.mark.gpu
+def test_more_moves_than_one_grid_counts():
+    """65 streams, 32 layers, eight heads, room for 32768 places: 17 million workgroups, whose work-items are past 32 bits; the places that
+    there are, 40 of each head, are few."""
+    streams, layers, KV, d, P, L, keep, room = 65, 32, 8, 128, 16, 40, 20, 32768
+    slab = torch.randn(3 * streams, layers, 2, KV, P, d, device=DEV).to(torch.bfloat16)
+    table = torch.zeros(streams, room // P, dtype=torch.int32, device=DEV)
+    table[:, :3] = torch.arange(3 * streams, device=DEV).view(streams, 3)
+    w = torch.zeros(streams, layers, KV, room, device=DEV)
+    w[..., :L] = torch.arange(L, device=DEV) + 1.0  # the latest stay
+    pos = torch.zeros(w.shape, dtype=torch.int32, device=DEV)
+    rows = lambda: slab[table[:, :3].long()].permute(0, 2, 3, 4, 1, 5, 6).reshape(streams, layers, 2, KV, 3 * P, d)  # noqa: E731
+    before = rows().clone()
+    ints = lambda x: torch.full((streams,), x, dtype=torch.int32, device=DEV)  # noqa: E731
+    evict(slab[:, :, 0], slab[:, :, 1], table, ints(L), ints(keep), w, pos, max_len=room)
+    assert torch.equal(rows()[..., :keep, :], before[..., L - keep:L, :])
+    assert bool((w[..., :keep] == w[0, 0, 0, L - keep:L]).all()) and bool((pos[..., :keep] == torch.arange(L - keep, L, device=DEV)).all())

@@ -23,9 +23,9 @@ namespace kdn {
 // Minus delta, and minus lse / scale: what dkdv's products start from.  Sixteen lanes a row, eight values each; 8192 rows of
 // 32 heads, 128 features, bf16: 35 us, 5.7 TB/s of y, its low part and dy.
 template <class P>
-__global__ void __launch_bounds__(256) attn_delta_kernel(AttnParams p, float* stat, float* delta) {
+__global__ void __launch_bounds__(256) attn_delta_kernel(AttnParams p, float* stat, float* delta, int64_t first) {
   typedef typename P::elem E;
-  const int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (row, head), heads fastest
+  const int64_t at = first + (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (row, head), heads fastest
   const int j = threadIdx.x & 15;
   if (at >= p.total_q * p.H) return;
   const int64_t row = at / p.H, h = at % p.H;
@@ -477,6 +477,18 @@ __global__ void __launch_bounds__(256, sizeof(typename P::elem) == 2 ? 2 : 1)
   }
 }
 
+template <class P>
+static int launch_delta(const AttnParams& p, hipStream_t st) {
+  const int64_t blocks = (p.total_q * p.H + 15) / 16, most = max_groups(256);
+  int rc = KDN_OK;
+  for (int64_t first = 0; first < blocks && rc == KDN_OK; first += most) {  // 8 million rows of 32 heads are more than one grid
+    hipLaunchKernelGGL(attn_delta_kernel<P>, dim3((unsigned)std::min(most, blocks - first)), dim3(256), 0, st, p, const_cast<float*>(p.stat), const_cast<float*>(p.delta),
+                       16 * first);
+    rc = launch_status();
+  }
+  return rc;
+}
+
 template <class P, int SPLIT, bool WIN>
 static int launch_grads(const AttnParams& p, hipStream_t st) {
   const int64_t slots_k = p.total_k > 0 ? tile_slots(p.total_k, Dkdv<P, SPLIT>::KEYS, p.nseq) : 0;
@@ -485,13 +497,14 @@ static int launch_grads(const AttnParams& p, hipStream_t st) {
   const int64_t far_blocks = far > 0 ? (p.nseq * p.sinks * p.KV * (P::D / 4) + 255) / 256 : 0;
   const int64_t nk = slots_k * p.KV * p.subsets + far, part = (nk + 7) / 8 * 8;  // a workgroup's number mod 8 is its XCD
   const int64_t grid = part * (P::D == 64 ? 1 : 2) + slots_q * p.H;
-  if (grid > INT32_MAX || far_blocks > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  const int64_t blocks = p.subsets > 1 && p.total_k > 0 ? (p.total_k * p.KV * (P::D / 4) + 255) / 256 : 0;
+  if (std::max({grid, far_blocks, blocks}) > max_groups(256)) return KDN_ERR_UNSUPPORTED;
+  int rc = launch_delta<P>(p, st);
+  if (rc != KDN_OK) return rc;
   hipLaunchKernelGGL((attn_grads_kernel<P, SPLIT, WIN>), dim3((unsigned)grid), dim3(256), 0, st, p, (int)slots_k, (int)slots_q, (int)part, (int)nk,
                      (int)far);
-  int rc = launch_status();
-  if (rc == KDN_OK && p.subsets > 1 && p.total_k > 0) {
-    const int64_t blocks = (p.total_k * p.KV * (P::D / 4) + 255) / 256;
-    if (blocks > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  rc = launch_status();
+  if (rc == KDN_OK && blocks > 0) {
     hipLaunchKernelGGL(attn_subsets_kernel<P>, dim3((unsigned)blocks), dim3(256), 0, st, p);
     rc = launch_status();
   }
@@ -516,14 +529,7 @@ static int launch_grads(const AttnParams& p, hipStream_t st) {
 }
 
 template <class P>
-static int launch_bwd(const AttnParams& p, float* stat, float* delta, hipStream_t st) {
-  int rc = KDN_OK;
-  if (p.total_q > 0) {
-    const int64_t rows = p.total_q * p.H;
-    if ((rows + 15) / 16 > INT32_MAX) return KDN_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL(attn_delta_kernel<P>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, p, stat, delta);
-    if ((rc = launch_status()) != KDN_OK) return rc;
-  }
+static int launch_bwd(const AttnParams& p, hipStream_t st) {
   return p.window < NO_WINDOW ? launch_grads<P, true>(p, st) : launch_grads<P, false>(p, st);
 }
 
@@ -602,8 +608,8 @@ static int attn_bwd(const kdn_attn_bwd_args* a, int64_t window, int64_t sinks, v
   }
   hipStream_t st = as_stream(stream);
   if (f->dtype == KDN_DTYPE_BF16)
-    return f->d == 64 ? launch_bwd<AttnBF16<64>>(p, stat, delta, st) : launch_bwd<AttnBF16<128>>(p, stat, delta, st);
-  return f->d == 64 ? launch_bwd<AttnF32<64>>(p, stat, delta, st) : launch_bwd<AttnF32<128>>(p, stat, delta, st);
+    return f->d == 64 ? launch_bwd<AttnBF16<64>>(p, st) : launch_bwd<AttnBF16<128>>(p, st);
+  return f->d == 64 ? launch_bwd<AttnF32<64>>(p, st) : launch_bwd<AttnF32<128>>(p, st);
 }
 
 extern "C" size_t kdn_attn_bwd_workspace_bytes(const kdn_attn_bwd_args* a) { return bwd_workspace_bytes(a, NO_WINDOW, 0); }

@@ -654,8 +654,17 @@ extern "C" int kdn_fwht(const void* x, int64_t rows, int64_t x_row_stride, int n
   if (x_row_stride < n || out_row_stride < n) return KDN_ERR_INVALID_ARGUMENT;
   if (rows == 0) return KDN_OK;
   hipStream_t st = as_stream(stream);
+  const int64_t most = 4 * max_groups(256);
+  if (rows > most) {  // more rows than one grid counts
+    const size_t size = dtype_size(dtype);
+    for (int64_t r = 0; r < rows; r += most) {
+      const int rc = kdn_fwht((const char*)x + (size_t)(r * x_row_stride) * size, rows - r < most ? rows - r : most, x_row_stride, n, dtype,
+                              (char*)out + (size_t)(r * out_row_stride) * size, out_row_stride, stream);
+      if (rc != KDN_OK) return rc;
+    }
+    return KDN_OK;
+  }
   const int64_t wgs = (rows + 3) / 4;
-  if (wgs > 0x7fffffff) return KDN_ERR_UNSUPPORTED;
 #define KDN_FWHT_CASE(T, N)                                                                                   \
   case N:                                                                                                     \
     hipLaunchKernelGGL((fwht_rows_kernel<T, N>), dim3((unsigned)wgs), dim3(256), 0, st, (const T*)x, rows, \
@@ -896,14 +905,19 @@ extern "C" int kdn_fwht_lift_factored(const void* x, int64_t rows, int64_t x_row
                      phase2, 64, 512, inv_tau, static_cast<unsigned char*>(out) + 512 * osz, out_row_stride, out_dtype,
                      stream);
   if (rc != KDN_OK || rows == 0) return rc;
-  const dim3 grid((unsigned)((rows + 3) / 4));
-  if (out_dtype == KDN_DTYPE_BF16)
-    hipLaunchKernelGGL(renorm_rows_kernel<__bf16>, grid, dim3(256), 0, as_stream(stream), static_cast<__bf16*>(out),
-                       rows, out_row_stride, 1e-7f);
-  else
-    hipLaunchKernelGGL(renorm_rows_kernel<float>, grid, dim3(256), 0, as_stream(stream), static_cast<float*>(out), rows,
-                       out_row_stride, 1e-7f);
-  return launch_status();
+  const int64_t most = 4 * max_groups(256);  // rows of a grid
+  for (int64_t r = 0; r < rows && rc == KDN_OK; r += most) {
+    const int64_t n = rows - r < most ? rows - r : most;
+    const dim3 grid((unsigned)((n + 3) / 4));
+    if (out_dtype == KDN_DTYPE_BF16)
+      hipLaunchKernelGGL(renorm_rows_kernel<__bf16>, grid, dim3(256), 0, as_stream(stream),
+                         static_cast<__bf16*>(out) + r * out_row_stride, n, out_row_stride, 1e-7f);
+    else
+      hipLaunchKernelGGL(renorm_rows_kernel<float>, grid, dim3(256), 0, as_stream(stream),
+                         static_cast<float*>(out) + r * out_row_stride, n, out_row_stride, 1e-7f);
+    rc = launch_status();
+  }
+  return rc;
 }
 
 namespace kdn {

@@ -100,7 +100,7 @@ extern "C" int kdn_page_copy(void* slab, int64_t num_pages, int64_t page_bytes, 
   if (!slab || !pairs) return KDN_ERR_INVALID_ARGUMENT;
   if (!aligned(slab, 16)) return KDN_ERR_MISALIGNED;
   const int64_t blocks = (page_bytes / 16 + 256 * COPY_UNITS - 1) / (256 * COPY_UNITS);
-  if (n > num_pages || num_pages > INT32_MAX || blocks > INT32_MAX) return KDN_ERR_INVALID_ARGUMENT;
+  if (n > num_pages || num_pages > INT32_MAX || blocks > max_groups(256)) return KDN_ERR_INVALID_ARGUMENT;
   const int rc = guarded([&]() -> int {
     std::vector<int32_t> to((size_t)n);
     for (int64_t i = 0; i < n; ++i) {
@@ -156,7 +156,7 @@ extern "C" int kdn_page_append(const kdn_page_append_args* a, void* stream) {
   p.pieces = __builtin_ctz((unsigned)(a->d * size / 16));
   p.shift = __builtin_ctz((unsigned)a->page_tokens);
   const int64_t blocks = (((a->tokens * 2 * a->H_kv) << p.pieces) + 255) / 256;
-  if (blocks > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  if (blocks > max_groups(256)) return KDN_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(page_append_kernel, dim3((unsigned)blocks), dim3(256), 0, as_stream(stream), p);
   return launch_status();
 }

@@ -143,6 +143,7 @@ extern "C" int kdn_rotary(const kdn_rotary_args* a, void* stream) {
   p.H = (int)a->H; p.heads = (int)(a->H + a->H_kv); p.rot = a->rotary_dim; p.inverse = a->inverse != 0;
   p.mag = a->magnitude;
   p.per = a->tokens >= 8192 ? 4 : 1;
+  if ((a->tokens + p.per - 1) / p.per > max_groups(256)) return KDN_ERR_UNSUPPORTED;
   const bool il = a->interleaved != 0;
   const bool wide = il ? a->rotary_dim % per == 0 : a->rotary_dim % (2 * per) == 0;
   hipStream_t st = as_stream(stream);

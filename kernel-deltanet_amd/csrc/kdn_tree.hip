@@ -858,18 +858,20 @@ template <class P, bool WIN>
 static int launch_tree(TreeParams& p, hipStream_t st) {
   const int rows = p.max_new * p.G;
   const int64_t units = (int64_t)p.nseq * p.KV * p.max_chunks;
+  const int64_t joins = p.max_chunks > 1 ? ((int64_t)p.nseq * p.KV * rows + JOIN_ROWS - 1) / JOIN_ROWS : 0;
+  const int64_t parts = p.weights ? (p.room + WEIGHT_KEYS - 1) / WEIGHT_KEYS * p.nseq * p.KV : 0;
+  const int64_t grid = rows <= 32 ? units : (units + 7) / 8 * 8 * TreeMany<P>::blocks(rows);
+  if (grid + ZERO_GROUPS > max_groups(rows <= 32 ? 64 * TreeFew<P>::WAVES : 256) || joins + parts > max_groups(256)) return KDN_ERR_UNSUPPORTED;
   if (rows <= 32) {
-    p.zero_from = (int)units;
-    if (p.weights) hipLaunchKernelGGL((tree_few_kernel<P, WIN, true>), dim3((unsigned)units + ZERO_GROUPS), dim3(64 * TreeFew<P>::WAVES), 0, st, p);
-    else hipLaunchKernelGGL((tree_few_kernel<P, WIN, false>), dim3((unsigned)units + ZERO_GROUPS), dim3(64 * TreeFew<P>::WAVES), 0, st, p);
+    p.zero_from = (int)grid;
+    if (p.weights) hipLaunchKernelGGL((tree_few_kernel<P, WIN, true>), dim3((unsigned)grid + ZERO_GROUPS), dim3(64 * TreeFew<P>::WAVES), 0, st, p);
+    else hipLaunchKernelGGL((tree_few_kernel<P, WIN, false>), dim3((unsigned)grid + ZERO_GROUPS), dim3(64 * TreeFew<P>::WAVES), 0, st, p);
   } else {
     const int blocks = TreeMany<P>::blocks(rows);
-    p.zero_from = (int)((units + 7) / 8 * 8 * blocks);
-    hipLaunchKernelGGL((tree_many_kernel<P, WIN>), dim3((unsigned)p.zero_from + ZERO_GROUPS), dim3(256), 0, st, p, blocks);
+    p.zero_from = (int)grid;
+    hipLaunchKernelGGL((tree_many_kernel<P, WIN>), dim3((unsigned)grid + ZERO_GROUPS), dim3(256), 0, st, p, blocks);
   }
-  const int64_t joins = p.max_chunks > 1 ? ((int64_t)p.nseq * p.KV * rows + JOIN_ROWS - 1) / JOIN_ROWS : 0;
-  if (p.weights && p.nseq > 0) {
-    const int64_t parts = (p.room + WEIGHT_KEYS - 1) / WEIGHT_KEYS * p.nseq * p.KV;
+  if (parts > 0) {
     hipLaunchKernelGGL((tree_finish_kernel<typename P::elem, P::D, WIN>), dim3((unsigned)(joins + parts)), dim3(256), 0, st, p, (int)joins);
   } else if (joins > 0) {
     hipLaunchKernelGGL((tree_join_kernel<typename P::elem, P::D, WIN>), dim3((unsigned)joins), dim3(256), 0, st, p);

@@ -432,11 +432,12 @@ static int launch_weights_few(WeightsParams p, hipStream_t st) {
   const int64_t slots = tile_slots(p.a.total_k, WeightsFew<P>::KEYS, p.a.nseq), groups = std::max<int64_t>(1, 512 / p.a.KV);
   const int64_t per = (slots + groups - 1) / groups;
   const int64_t grid = ((slots + per - 1) / per + 7) / 8 * 8 * p.a.KV;
-  if (grid > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  const int64_t dealt = (groups + 7) / 8 * 8 * p.a.KV;
+  if (std::max(grid, dealt) > max_groups(64 * WeightsFew<P>::WAVES)) return KDN_ERR_UNSUPPORTED;
   // A launch of the long sequences' own takes 2.7 us where there are none; without it the longest walk is that of a stretch whose rows
   // are all the call's, about a microsecond for each of its tiles of rows.
   const bool deal = p.a.total_q > p.long_rows && per * ((p.a.total_q + 63) / 64 * p.a.G) > 128;
-  if (deal) hipLaunchKernelGGL((attn_weights_few_kernel<P, true>), dim3((unsigned)((groups + 7) / 8 * 8 * p.a.KV)), dim3(64 * WeightsFew<P>::WAVES), 0, st, p, slots, per);
+  if (deal) hipLaunchKernelGGL((attn_weights_few_kernel<P, true>), dim3((unsigned)dealt), dim3(64 * WeightsFew<P>::WAVES), 0, st, p, slots, per);
   else p.long_rows = INT32_MAX;
   hipLaunchKernelGGL((attn_weights_few_kernel<P, false>), dim3((unsigned)grid), dim3(64 * WeightsFew<P>::WAVES), 0, st, p, slots, per);
   return launch_status();
@@ -449,7 +450,7 @@ static int launch_weights(const WeightsParams& p, bool few, hipStream_t st) {
   const int64_t slots = tile_slots(p.a.total_k, WeightsTile<P>::KEYS, p.a.nseq);
   const int64_t grid = (slots * p.parts + (p.far > 0 ? p.a.nseq * p.far_tiles * p.far : 0)) * p.a.KV;
   const int64_t joins = p.part ? tile_slots(p.a.total_k, 256, p.a.nseq) * p.a.KV : 0;
-  if (grid > INT32_MAX || joins > INT32_MAX) return KDN_ERR_UNSUPPORTED;
+  if (std::max(grid, joins) > max_groups(256)) return KDN_ERR_UNSUPPORTED;
   if (p.a.window < NO_WINDOW) hipLaunchKernelGGL((attn_weights_kernel<P, true>), dim3((unsigned)grid), dim3(256), 0, st, p, slots);
   else hipLaunchKernelGGL((attn_weights_kernel<P, false>), dim3((unsigned)grid), dim3(256), 0, st, p, slots);
   if (joins > 0) hipLaunchKernelGGL(attn_weights_join_kernel, dim3((unsigned)joins), dim3(256), 0, st, p);

@@ -169,6 +169,48 @@ def test_evict_arguments():
     assert call(args(num_seqs=0), None) == 0 and call(args(max_len=0), None) == 0
 
 
+def test_grids_past_32_bits_of_work_items_are_refused():
+    """Before anything is launched: such a grid would be cut short without an error."""
+    L, none = N.lib(), ctypes.c_void_p(None)
+    many = dict(num_seqs=1 << 20, H=32, H_kv=32)  # a tile slot a sequence and head: 33 million workgroups of 256
+    for kw in (many, dict(many, dtype=0), dict(many, d=128)):
+        assert L.kdn_attn_fwd(ctypes.byref(_attn(**kw)), none) == -2
+        assert L.kdn_attn_window_fwd(ctypes.byref(_attn(**kw)), 4, 1, none) == -2
+        fwd = _attn(lse=1 << 12, **kw)
+        b = N.AttnBwdArgs()
+        b.fwd = ctypes.addressof(fwd)
+        b.dy = b.dq = b.dk = b.dv = b.workspace = 1 << 12
+        b.workspace_bytes = 1 << 50
+        for s in ("dy", "dq", "dk", "dv"):
+            getattr(b, s + "_stride")[0], getattr(b, s + "_stride")[1] = 256, 64
+        assert L.kdn_attn_bwd(ctypes.byref(b), none) == -2 and L.kdn_attn_window_bwd(ctypes.byref(b), 4, 1, none) == -2
+    t = _tree(num_seqs=1 << 20, total_new=1 << 20, H=32, H_kv=32, max_context=128)
+    t.cu_new = t.context_lens = t.page_table = t.q = t.k = t.v = t.y = t.k_pages = t.v_pages = t.workspace = 1 << 12
+    for s in ("q", "k", "v", "y"):
+        getattr(t, s + "_stride")[0], getattr(t, s + "_stride")[1] = 4096, 128
+    t.workspace_bytes = 1 << 50
+    for d, dtype in ((64, 1), (128, 1), (64, 0)):
+        t.d, t.dtype, t.num_seqs = d, dtype, 1 << 21
+        assert L.kdn_tree_attn(ctypes.byref(t), none) == -2 and L.kdn_tree_attn_bounded(ctypes.byref(t), ctypes.byref(_bound(window=4)), none) == -2
+    t.max_new = 64  # more than 32 rows
+    assert L.kdn_tree_attn(ctypes.byref(t), none) == -2
+    w = N.AttnWeightsArgs()
+    w.num_seqs, w.total_q, w.total_k, w.H, w.H_kv, w.d, w.dtype, w.scale = 1 << 20, 8, 8, 32, 32, 64, 0, 0.125
+    w.cu_q = w.q = w.k = w.lse = w.weights = w.workspace = 1 << 12
+    w.places, w.num_slots, w.workspace_bytes = 8, 1 << 20, 1 << 50
+    assert L.kdn_attn_weights(ctypes.byref(w), none) == -2
+    r = N.RotaryArgs()
+    r.tokens, r.H, r.H_kv, r.d, r.rotary_dim, r.dtype, r.magnitude = 1 << 27, 4, 2, 64, 64, 1, 1.0
+    r.positions = r.inv_freq = r.q = r.k = r.q_out = r.k_out = 1 << 12
+    for s in ("q", "k", "q_out", "k_out"):
+        getattr(r, s + "_stride")[0], getattr(r, s + "_stride")[1] = 256, 64
+    assert L.kdn_rotary(ctypes.byref(r), none) == -2
+    p = N.PageAppendArgs()
+    p.tokens, p.H_kv, p.d, p.dtype, p.page_tokens, p.num_pages = 1 << 26, 8, 64, 1, 16, 4
+    p.rows = p.k = p.v = p.k_pages = p.v_pages = 1 << 12
+    assert L.kdn_page_append(ctypes.byref(p), none) == -2
+
+
 def test_evict_refuses_rows_that_lie_on_one_another():
     a = N.EvictArgs()
     a.num_seqs, a.layers, a.H_kv, a.d, a.dtype, a.page_tokens, a.num_pages, a.table_width, a.max_len = 1, 2, 2, 64, 1, 16, 9, 4, 64

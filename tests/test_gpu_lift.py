@@ -258,3 +258,12 @@ def test_lift_bits_butterfly_matches_oracle(D, dtype, normalize):
     ref = ol.lift(xr.numpy(), op)
     assert rel_l2(a.float().cpu().numpy(), ref) < tol
     assert rel_l2(a.float().cpu().numpy(), b.float().cpu().numpy()) < tol
+
+
+@pytest.mark.gpu
+def test_fwht_of_more_rows_than_a_grid_counts():
+    """2^26 rows are 2^32 work-items."""
+    x = torch.randn(2 ** 26 + 5, 2, device="cuda:0").to(torch.bfloat16)
+    y = ops.fwht(x)
+    assert torch.equal(y[:, 0], (x[:, 0].float() + x[:, 1].float()).to(torch.bfloat16))
+    assert torch.equal(y[:, 1], (x[:, 0].float() - x[:, 1].float()).to(torch.bfloat16))

@@ -227,3 +227,22 @@ def test_refusals():
         leaf = q.clone().requires_grad_(True)
         g, = torch.autograd.grad(anchor.attention(leaf, k, v, cu, window=4).float().sum(), leaf, create_graph=True)
         g.float().sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", [dict(), dict(window=9, sinks=2)])
+def test_gradients_of_more_rows_than_a_grid_counts(how):
+    """8.4 million rows of 32 heads, sixteen to a workgroup, are past 32 bits of work-items: sequences alike have gradients alike."""
+    n, seqs, H, d = 64, 2 ** 17 + 64, 32, 64
+    g = torch.Generator(device=DEV).manual_seed(0)
+    one = [torch.randn(n, 1, d, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2)]
+    k, v = (t.repeat(seqs, 1, 1) for t in one)
+    q, dy = (torch.randn(1, H, d, generator=g, device=DEV).to(torch.bfloat16).expand(n * seqs, H, d) for _ in range(2))
+    cu = torch.arange(seqs + 1, device=DEV) * n
+    y, lse = anchor.attention_forward(q, k, v, cu, return_lse=True, **how)
+    few = anchor.attention_backward(q[:8 * n], k[:8 * n], v[:8 * n], y[:8 * n], lse[:, :8 * n], dy[:8 * n], cu[:9], **how)
+    got = anchor.attention_backward(q, k, v, y, lse, dy, cu, **how)
+    for a, b in zip(got, few):
+        part = a.view(seqs, n, *a.shape[1:])
+        assert float(b.float().norm()) > 0 and bool((part[-1] == part[0]).all()) and bool((part[2 ** 16:2 ** 16 + 64] == part[:1]).all())
+        assert float((part[:8].float() - b.view(8, n, *b.shape[1:]).float()).norm()) < 2.0 ** -6 * float(b.float().norm())  # roundings of bf16

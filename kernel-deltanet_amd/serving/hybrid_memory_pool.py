@@ -68,8 +68,9 @@ class HybridMemoryPool:
                 if anchor_queries < 1 or anchor_queries % anchor_heads:
                     raise ValueError(f"HybridMemoryPool: anchor_queries is a multiple of anchor_heads, got {anchor_queries} and {anchor_heads}")
                 shape = (max_streams, anchor_layers, anchor_heads, -(-max_seq_len // page_tokens) * page_tokens)
-                self._weights = torch.zeros(shape, dtype=torch.float32, device=device)
-                self._positions = torch.zeros(shape, dtype=torch.int32, device=device)
+                with torch.inference_mode(False):  # torch writes them too: wherever the pool is made, they can be written everywhere
+                    self._weights = torch.zeros(shape, dtype=torch.float32, device=device)
+                    self._positions = torch.zeros(shape, dtype=torch.int32, device=device)
                 self._run = min(64, 32 // (anchor_queries // anchor_heads))
 
     @property

@@ -320,6 +320,19 @@ def test_a_cut_stream_keeps_its_positions():
         make_pool(anchor_queries=3)
 
 
+@pytest.mark.parametrize("made", [False, True])
+def test_a_pool_is_used_in_another_mode_than_it_was_made_in(made):
+    with torch.inference_mode(made):
+        pool = make_pool(anchor_pages=16, anchor_queries=8)
+    with torch.inference_mode(not made):
+        s = pool.allocate_stream(0)
+        pool.anchor_plan([s], [30])
+        f = pool.fork_stream(s)
+        pool.anchor_evict([f], 20)
+        pool.anchor_truncate(s, 10)
+        assert [pool.anchor_tokens(x) for x in (s, f)] == [10, 20] and not pool.anchor_weights(1).any()
+
+
 def test_layer_arguments():
     for bad in (dict(window=0), dict(window=4, sinks=-1)):
         with pytest.raises(ValueError):
